@@ -363,6 +363,157 @@ typedef struct NnopsQdqArgs {
 int nnops_hip_quantize_linear(const NnopsQdqArgs* args, void* stream);
 int nnops_hip_dequantize_linear(const NnopsQdqArgs* args, void* stream);
 
+/* Root-mean-square norm with the residual's addition, and its output as s8
+ * codes with one scale per row: the step between two int8 products of a
+ * decoder layer (no counterpart in nnops). Per row, in f32:
+ *   h = x + residual;  sum = h in x's type;
+ *   rstd = 1 / sqrt(mean(h^2) + epsilon);  u = h * weight;
+ *   f16 / f32 (x's type):  y = u * rstd;
+ *   s8:  a = max |u|,  q = rint(u * (127 / a)),  scale = a * rstd / 127,
+ * so that q * scale is u * rstd within half a step (rstd cancels in q: the
+ * codes do not depend on the order in which the squares are summed). A row
+ * with a < 2^-119 has codes 0; a row with an infinity or a NaN in u has codes
+ * 0 and the scale NaN. The codes and scales are what nnops_hip_gemm_i8 takes
+ * as A and s_a.
+ * sum may be x's or residual's buffer, y (f16 / f32) x's or residual's where
+ * that is not sum's; otherwise no output may overlap another buffer.
+ * Stream-ordered, no allocation, no workspace. */
+typedef struct NnopsRmsNormArgs {
+    const void* x;              /* [rows][ld_x] f16 (in_f16) or f32 */
+    const void* weight;         /* [cols], x's type */
+    const void* residual;       /* [rows][ld_residual], x's type, or NULL */
+    void* y;                    /* [rows][ld_y] */
+    float* scale;               /* [rows], s8 only */
+    void* sum;                  /* [rows][ld_sum], x's type: with a residual only */
+    int64_t rows, cols;
+    int64_t ld_x, ld_residual, ld_y, ld_sum; /* elements */
+    int32_t in_f16;
+    int32_t out_kind;           /* NNOPS_OUT_S8, or x's type */
+    float epsilon;              /* >= 0 */
+} NnopsRmsNormArgs;
+
+int nnops_hip_rms_norm(const NnopsRmsNormArgs* args, void* stream);
+
+/* Rotary positions (no counterpart in nnops). Each row of x holds `heads`
+ * heads of head_dim values; the first rotary_dim values of each head are
+ * rotated in pairs by the row's position, the others are copied:
+ *   (y_a, y_b) = (x_a c - x_b s, x_b c + x_a s)
+ * with (a, b) = (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when interleaved,
+ * and c, s = table[position][i], table[position][rotary_dim / 2 + i], each
+ * product and sum rounded in f32, y to x's type. A position outside [0,
+ * max_pos) gives NaN in the rotated values. y may be x (in place); otherwise
+ * they may not overlap. */
+typedef struct NnopsRotaryArgs {
+    const void* x;              /* [tokens][ld_x] f16 (in_f16) or f32 */
+    void* y;                    /* [tokens][ld_y], x's type */
+    const int32_t* positions;   /* [tokens] */
+    const float* table;         /* [max_pos][ld_table]: cosines, then sines */
+    int64_t tokens, heads, head_dim, rotary_dim, max_pos;
+    int64_t ld_x, ld_y, ld_table; /* elements */
+    int32_t in_f16, interleaved;
+} NnopsRotaryArgs;
+
+int nnops_hip_rotary(const NnopsRotaryArgs* args, void* stream);
+
+/* Fills a rotary table: row p, column i: cos(p f_i) * attention_factor, column
+ * rotary_dim / 2 + i the sine, with f_i = base^(-2 i / rotary_dim), angles in
+ * f64. Scaled for long contexts: with factor != 1 a frequency becomes
+ *   g f + (1 - g) f / factor,
+ * g = 0 everywhere when original_context is 0 (every position divided by
+ * factor); otherwise g = clamp((t - low_turns) / (high_turns - low_turns), 0,
+ * 1) of the turns t = original_context f / (2 pi) that the pair made over the
+ * context that the model was trained on: fast pairs keep their frequency, slow
+ * ones are stretched. */
+typedef struct NnopsRotaryTableArgs {
+    float* table;
+    int64_t max_pos, rotary_dim, ld_table; /* ld_table: elements */
+    double base, factor, original_context, low_turns, high_turns, attention_factor;
+} NnopsRotaryTableArgs;
+
+int nnops_hip_rotary_table(const NnopsRotaryTableArgs* args, void* stream);
+
+/* A key / value cache held in 8 bits, in pages (no counterpart in nnops).
+ * A page holds page_tokens consecutive tokens of one sequence, for every KV
+ * head head_dim codes of the key and of the value per token, with one scale
+ * per page and head on each side (value = code * scale):
+ *   k        [pages][heads][page_tokens][head_dim]
+ *   v        [pages][heads][head_dim][page_tokens]   (a channel's tokens side
+ *            by side: what the product with the probabilities reads)
+ *   k_scale, v_scale   [pages][heads], finite and >= 0
+ * Token p of sequence b lies in slot p % page_tokens of page
+ * page_table[b][p / page_tokens].
+ * A call's rows are the LAST tokens of each sequence: sequence b has rows
+ * row_starts[b] .. row_starts[b + 1] - 1 (row_starts NULL: rows / sequences
+ * each), its last row stands for token lengths[b] - 1.
+ * page_tokens: 16, 32, 64, 128 or 256; head_dim: a multiple of 16 up to 256;
+ * k and v 16-byte aligned, dense.
+ * The tables are device memory that the host does not see. What they should
+ * not hold does not fault: lengths are taken into [0, table_pages *
+ * page_tokens] and row_starts into [0, rows]; a row that would stand for a
+ * token before the first is not written, reads as 0 and attends to nothing; a
+ * page number outside [0, pages) is not written and reads as NaN. */
+typedef struct NnopsKvPages {
+    int8_t* k;
+    int8_t* v;
+    float* k_scale;
+    float* v_scale;
+    int64_t pages, heads, page_tokens, head_dim;
+    const int32_t* page_table;  /* [sequences][ld_table], table_pages columns */
+    int64_t sequences, table_pages, ld_table; /* ld_table: elements */
+    const int32_t* lengths;     /* [sequences] */
+    const int32_t* row_starts;  /* [sequences + 1], or NULL */
+} NnopsKvPages;
+
+/* Key and value rows of a call, `heads` * head_dim values each. */
+typedef struct NnopsKvRowsArgs {
+    NnopsKvPages cache;
+    void* k_rows;               /* [rows][ld_k] f16 (f16) or f32; write: only read */
+    void* v_rows;               /* [rows][ld_v] */
+    int64_t rows, ld_k, ld_v;   /* elements */
+    int32_t f16;
+} NnopsKvRowsArgs;
+
+/* Write: the rows become codes in the sequences' pages. For each page and head
+ * that gets rows, with a the largest magnitude among them:
+ *   scale = max(old scale, a / 127, 2^-100)   (the old one only if the page
+ *           holds tokens of the sequence before the call's first),
+ *   new code = rint(x / scale) (as x * (1 / scale)),
+ *   code of an older token = rint(code * (old scale / scale)) where it grew.
+ * An infinity or a NaN among them makes the page's scale NaN (until the page
+ * is begun anew), so that whatever reads the page shows it. No atomics, no
+ * order: the same inputs give the same bits. Pages that get rows may not be
+ * shared between sequences.
+ * Read: the rows' codes times their scales, in f32, rounded to the rows' type.
+ * Stream-ordered, no allocation, no workspace. */
+int nnops_hip_kv_cache_write(const NnopsKvRowsArgs* args, void* stream);
+int nnops_hip_kv_cache_read(const NnopsKvRowsArgs* args, void* stream);
+
+/* Causal attention of query rows over that cache (no counterpart in nnops).
+ * Row r of q holds q_heads heads of head_dim values, head m attends to KV head
+ * m / (q_heads / heads). For a query at position p:
+ *   out = sum_j softmax_j(scale * q . k_j) v_j over the tokens
+ *   j <= p  and  (window == 0  or  p - j < window  or  j < sinks),
+ * 0 where there are none. (The call's own rows are in the cache already.)
+ * Scores, softmax statistics and sums are f32. f16: q and the codes enter the
+ * matrix products exactly, the probabilities as f16 (of 14 bits more range);
+ * f32: both exactly, as three bf16 parts.
+ * nnops_hip_cache_attention_workspace_size bytes of workspace (16-byte
+ * aligned) hold the partial results of long sequences that are split over the
+ * chip. */
+typedef struct NnopsCacheAttentionArgs {
+    NnopsKvPages cache;
+    const void* q;              /* [rows][ld_q] f16 (f16) or f32 */
+    void* out;                  /* [rows][ld_out], q's type */
+    int64_t rows, q_heads, ld_q, ld_out; /* ld: elements */
+    int32_t f16;
+    float scale;                /* 0: 1 / sqrt(head_dim) */
+    int64_t window, sinks;      /* >= 0 */
+} NnopsCacheAttentionArgs;
+
+size_t nnops_hip_cache_attention_workspace_size(const NnopsCacheAttentionArgs* args);
+int nnops_hip_cache_attention(const NnopsCacheAttentionArgs* args, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
 /* What the kernel selection of a call comes to (no counterpart in nnops; for
  * tests and for callers that tune shapes). Host code: the arguments' pointers
  * are looked at for their alignment only, and nothing is launched. */

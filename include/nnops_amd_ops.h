@@ -1,5 +1,6 @@
 /* nnops_amd_ops.h -- C ABI over the MatMul / Linear / QuantizeLinear /
- * DequantizeLinear front end.
+ * DequantizeLinear front end, and over RmsNorm / Rotary / KvCacheWrite /
+ * KvCacheRead / CacheAttention.
  *
  * For callers that cannot bind C++ (ctypes, cgo, JNI, N-API): each call maps
  * one-to-one onto the C++ operator contract of nnops
@@ -89,6 +90,24 @@ typedef struct NnopsQuantLinearAttrs {
     int32_t output_dtype;   /* quantize: NNOPS_S8 / NNOPS_U8; dequantize: NNOPS_F32 / NNOPS_F16 */
 } NnopsQuantLinearAttrs;
 
+/* The operators between the products of a decoder layer (no counterparts in
+ * nnops; nnops/ops/rms_norm.hpp, rotary.hpp and kv_cache.hpp of the C++ headers
+ * state inputs and outputs, nnops_amd.h the arithmetic). */
+typedef struct NnopsRmsNormAttrs {
+    float epsilon;
+    int32_t output_dtype;   /* x's type, or NNOPS_S8 (then outputs y, scale) */
+} NnopsRmsNormAttrs;
+
+typedef struct NnopsRotaryAttrs {
+    int64_t head_dim, rotary_dim;   /* rotary_dim 0: head_dim */
+    int32_t interleaved;
+} NnopsRotaryAttrs;
+
+typedef struct NnopsCacheAttentionAttrs {
+    float scale;            /* 0: 1 / sqrt(head_dim) */
+    int64_t window, sinks;  /* window 0: none */
+} NnopsCacheAttentionAttrs;
+
 typedef struct NnopsOp NnopsOp;
 
 /* Attribute defaults matching the C++ structs (epilogue clip +-inf etc.). */
@@ -102,6 +121,22 @@ NnopsOp* nnops_linear_create(const NnopsLinearAttrs* attrs, int32_t backend);
 void nnops_quant_linear_attrs_init(NnopsQuantLinearAttrs* attrs);
 NnopsOp* nnops_quantize_linear_create(const NnopsQuantLinearAttrs* attrs, int32_t backend);
 NnopsOp* nnops_dequantize_linear_create(const NnopsQuantLinearAttrs* attrs, int32_t backend);
+/* RmsNorm: inputs x, weight [, residual]; outputs y [, scale] [, sum].
+ * Rotary: inputs x, positions, table; output y.
+ * KvCacheWrite: inputs k, v, page_table, lengths [, row_starts]; outputs
+ * k_cache, v_cache, k_scale, v_scale (updated in place).
+ * KvCacheRead: inputs k_cache, v_cache, k_scale, v_scale, page_table, lengths
+ * [, row_starts]; outputs k, v (output_dtype NNOPS_F32 / NNOPS_F16).
+ * CacheAttention: inputs q, k_cache, v_cache, k_scale, v_scale, page_table,
+ * lengths [, row_starts]; output q's shape and type. */
+void nnops_rms_norm_attrs_init(NnopsRmsNormAttrs* attrs);
+NnopsOp* nnops_rms_norm_create(const NnopsRmsNormAttrs* attrs, int32_t backend);
+void nnops_rotary_attrs_init(NnopsRotaryAttrs* attrs);
+NnopsOp* nnops_rotary_create(const NnopsRotaryAttrs* attrs, int32_t backend);
+NnopsOp* nnops_kv_cache_write_create(int32_t backend);
+NnopsOp* nnops_kv_cache_read_create(int32_t output_dtype, int32_t backend);
+void nnops_cache_attention_attrs_init(NnopsCacheAttentionAttrs* attrs);
+NnopsOp* nnops_cache_attention_create(const NnopsCacheAttentionAttrs* attrs, int32_t backend);
 void nnops_op_destroy(NnopsOp* op);
 
 /* OpBase::prepackWeights (include/nnops/core/op_base.hpp:72-78) for MatMul /
@@ -116,6 +151,11 @@ int nnops_op_prepack_weights(NnopsOp* op, const NnopsTensor* inputs, int32_t n_i
 /* Fills out_desc (dims, rank, dtype; data NULL). Returns 0 on success. */
 int nnops_op_output_desc(const NnopsOp* op, const NnopsTensor* inputs, int32_t n_inputs,
                          NnopsTensor* out_desc);
+/* The same for every output of the call, in order, into outs[0 .. n_outs):
+ * returns their number, or a negative Status (too little room; an operator
+ * whose outputs are the caller's, such as KvCacheWrite). */
+int nnops_op_output_descs(const NnopsOp* op, const NnopsTensor* inputs, int32_t n_inputs,
+                          NnopsTensor* outs, int32_t n_outs);
 int nnops_op_validate(const NnopsOp* op, const NnopsTensor* inputs, int32_t n_inputs,
                       const NnopsTensor* outputs, int32_t n_outputs);
 size_t nnops_op_workspace_size(const NnopsOp* op, const NnopsTensor* inputs, int32_t n_inputs,

@@ -67,6 +67,57 @@ class GemmFpArgs(C.Structure):
     ]
 
 
+class RmsNormArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("weight", C.c_void_p), ("residual", C.c_void_p),
+        ("y", C.c_void_p), ("scale", C.c_void_p), ("sum", C.c_void_p),
+        ("rows", C.c_int64), ("cols", C.c_int64),
+        ("ld_x", C.c_int64), ("ld_residual", C.c_int64), ("ld_y", C.c_int64), ("ld_sum", C.c_int64),
+        ("in_f16", C.c_int32), ("out_kind", C.c_int32), ("epsilon", C.c_float),
+    ]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("y", C.c_void_p), ("positions", C.c_void_p), ("table", C.c_void_p),
+        ("tokens", C.c_int64), ("heads", C.c_int64), ("head_dim", C.c_int64), ("rotary_dim", C.c_int64),
+        ("max_pos", C.c_int64), ("ld_x", C.c_int64), ("ld_y", C.c_int64), ("ld_table", C.c_int64),
+        ("in_f16", C.c_int32), ("interleaved", C.c_int32),
+    ]
+
+
+class RotaryTableArgs(C.Structure):
+    _fields_ = [
+        ("table", C.c_void_p), ("max_pos", C.c_int64), ("rotary_dim", C.c_int64), ("ld_table", C.c_int64),
+        ("base", C.c_double), ("factor", C.c_double), ("original_context", C.c_double),
+        ("low_turns", C.c_double), ("high_turns", C.c_double), ("attention_factor", C.c_double),
+    ]
+
+
+class KvPages(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("pages", C.c_int64), ("heads", C.c_int64), ("page_tokens", C.c_int64), ("head_dim", C.c_int64),
+        ("page_table", C.c_void_p), ("sequences", C.c_int64), ("table_pages", C.c_int64), ("ld_table", C.c_int64),
+        ("lengths", C.c_void_p), ("row_starts", C.c_void_p),
+    ]
+
+
+class KvRowsArgs(C.Structure):
+    _fields_ = [
+        ("cache", KvPages), ("k_rows", C.c_void_p), ("v_rows", C.c_void_p),
+        ("rows", C.c_int64), ("ld_k", C.c_int64), ("ld_v", C.c_int64), ("f16", C.c_int32),
+    ]
+
+
+class CacheAttentionArgs(C.Structure):
+    _fields_ = [
+        ("cache", KvPages), ("q", C.c_void_p), ("out", C.c_void_p),
+        ("rows", C.c_int64), ("q_heads", C.c_int64), ("ld_q", C.c_int64), ("ld_out", C.c_int64),
+        ("f16", C.c_int32), ("scale", C.c_float), ("window", C.c_int64), ("sinks", C.c_int64),
+    ]
+
+
 class Tensor(C.Structure):
     _fields_ = [
         ("rank", C.c_int64), ("dims", C.c_int64 * 8), ("dtype", C.c_int32),
@@ -111,6 +162,18 @@ class LinearAttrs(C.Structure):
         ("gate_limit", C.c_float),
         ("matmul_order", C.c_int32), ("alpha", C.c_float), ("beta", C.c_float),
     ]
+
+
+class RmsNormAttrs(C.Structure):
+    _fields_ = [("epsilon", C.c_float), ("output_dtype", C.c_int32)]
+
+
+class RotaryAttrs(C.Structure):
+    _fields_ = [("head_dim", C.c_int64), ("rotary_dim", C.c_int64), ("interleaved", C.c_int32)]
+
+
+class CacheAttentionAttrs(C.Structure):
+    _fields_ = [("scale", C.c_float), ("window", C.c_int64), ("sinks", C.c_int64)]
 
 
 class FpOutArgs(C.Structure):
@@ -161,6 +224,13 @@ SIGNATURES = {
                                             C.c_int64, C.c_void_p]),
     "nnops_hip_quantize_linear": (C.c_int, [C.POINTER(QdqArgs), C.c_void_p]),
     "nnops_hip_dequantize_linear": (C.c_int, [C.POINTER(QdqArgs), C.c_void_p]),
+    "nnops_hip_rms_norm": (C.c_int, [C.POINTER(RmsNormArgs), C.c_void_p]),
+    "nnops_hip_rotary": (C.c_int, [C.POINTER(RotaryArgs), C.c_void_p]),
+    "nnops_hip_rotary_table": (C.c_int, [C.POINTER(RotaryTableArgs), C.c_void_p]),
+    "nnops_hip_kv_cache_write": (C.c_int, [C.POINTER(KvRowsArgs), C.c_void_p]),
+    "nnops_hip_kv_cache_read": (C.c_int, [C.POINTER(KvRowsArgs), C.c_void_p]),
+    "nnops_hip_cache_attention_workspace_size": (C.c_size_t, [C.POINTER(CacheAttentionArgs)]),
+    "nnops_hip_cache_attention": (C.c_int, [C.POINTER(CacheAttentionArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
     "nnops_matmul_attrs_init": (None, [C.POINTER(MatMulAttrs)]),
     "nnops_linear_attrs_init": (None, [C.POINTER(LinearAttrs)]),
     "nnops_matmul_create": (C.c_void_p, [C.POINTER(MatMulAttrs), C.c_int32]),
@@ -168,10 +238,19 @@ SIGNATURES = {
     "nnops_quant_linear_attrs_init": (None, [C.POINTER(QuantLinearAttrs)]),
     "nnops_quantize_linear_create": (C.c_void_p, [C.POINTER(QuantLinearAttrs), C.c_int32]),
     "nnops_dequantize_linear_create": (C.c_void_p, [C.POINTER(QuantLinearAttrs), C.c_int32]),
+    "nnops_rms_norm_attrs_init": (None, [C.POINTER(RmsNormAttrs)]),
+    "nnops_rms_norm_create": (C.c_void_p, [C.POINTER(RmsNormAttrs), C.c_int32]),
+    "nnops_rotary_attrs_init": (None, [C.POINTER(RotaryAttrs)]),
+    "nnops_rotary_create": (C.c_void_p, [C.POINTER(RotaryAttrs), C.c_int32]),
+    "nnops_kv_cache_write_create": (C.c_void_p, [C.c_int32]),
+    "nnops_kv_cache_read_create": (C.c_void_p, [C.c_int32, C.c_int32]),
+    "nnops_cache_attention_attrs_init": (None, [C.POINTER(CacheAttentionAttrs)]),
+    "nnops_cache_attention_create": (C.c_void_p, [C.POINTER(CacheAttentionAttrs), C.c_int32]),
     "nnops_op_destroy": (None, [C.c_void_p]),
     "nnops_op_prepack_weights": (C.c_int, [C.c_void_p, C.POINTER(Tensor), C.c_int32, C.POINTER(Tensor), C.c_int32,
                                            C.c_void_p]),
     "nnops_op_output_desc": (C.c_int, [C.c_void_p, C.POINTER(Tensor), C.c_int32, C.POINTER(Tensor)]),
+    "nnops_op_output_descs": (C.c_int, [C.c_void_p, C.POINTER(Tensor), C.c_int32, C.POINTER(Tensor), C.c_int32]),
     "nnops_op_validate": (C.c_int, [C.c_void_p, C.POINTER(Tensor), C.c_int32, C.POINTER(Tensor), C.c_int32]),
     "nnops_op_workspace_size": (C.c_size_t, [C.c_void_p, C.POINTER(Tensor), C.c_int32,
                                              C.POINTER(Tensor), C.c_int32]),

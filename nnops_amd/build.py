@@ -37,8 +37,14 @@ SOURCES = [
     "csrc/kernels/quant.hip",
     "csrc/kernels/fp_out.hip",
     "csrc/kernels/fp_gemm.hip",
+    "csrc/kernels/rms_norm.hip",
+    "csrc/kernels/rotary.hip",
+    "csrc/kernels/kv_cache.hip",
+    "csrc/kernels/cache_attention.hip",
     "csrc/host/ops.cpp",
     "csrc/host/quant_linear.cpp",
+    "csrc/host/rms_norm.cpp",
+    "csrc/host/kv_cache.cpp",
     "csrc/host/capi_ops.cpp",
 ]
 

@@ -1,8 +1,11 @@
-// C facade over the MatMul / Linear classes (include/nnops_amd_ops.h): turns
+// C facade over the operator classes (include/nnops_amd_ops.h): turns
 // NnopsTensor records into TensorDesc / TensorView and forwards each call.
+#include "nnops/ops/kv_cache.hpp"
 #include "nnops/ops/linear.hpp"
 #include "nnops/ops/matmul.hpp"
 #include "nnops/ops/quant_linear.hpp"
+#include "nnops/ops/rms_norm.hpp"
+#include "nnops/ops/rotary.hpp"
 #include "nnops_amd_ops.h"
 
 #include <limits>
@@ -71,6 +74,18 @@ QuantLinearAttributes to_qlinear(const NnopsQuantLinearAttrs* a)
         attrs.output_dtype = static_cast<DataType>(a->output_dtype);
     }
     return attrs;
+}
+
+NnopsTensor from_desc(const TensorDesc& d)
+{
+    NnopsTensor t{};
+    t.rank = d.rank;
+    for (int64_t i = 0; i < d.rank; ++i) {
+        t.dims[i] = d.dims[static_cast<size_t>(i)];
+    }
+    t.dtype = static_cast<int32_t>(d.dtype);
+    t.scale = 1.0f;
+    return t;
 }
 
 std::vector<TensorDesc> descs(const NnopsTensor* t, int32_t n)
@@ -182,6 +197,84 @@ NnopsOp* nnops_dequantize_linear_create(const NnopsQuantLinearAttrs* a, int32_t 
     return h;
 }
 
+void nnops_rms_norm_attrs_init(NnopsRmsNormAttrs* a)
+{
+    if (a == nullptr) {
+        return;
+    }
+    const RmsNormAttributes d;
+    a->epsilon = d.epsilon;
+    a->output_dtype = static_cast<int32_t>(d.output_dtype);
+}
+
+NnopsOp* nnops_rms_norm_create(const NnopsRmsNormAttrs* a, int32_t backend)
+{
+    RmsNormAttributes attrs;
+    if (a != nullptr) {
+        attrs.epsilon = a->epsilon;
+        attrs.output_dtype = static_cast<DataType>(a->output_dtype);
+    }
+    auto* h = new NnopsOp;
+    h->op = RmsNorm::create(attrs, static_cast<Backend>(backend));
+    return h;
+}
+
+void nnops_rotary_attrs_init(NnopsRotaryAttrs* a)
+{
+    if (a != nullptr) {
+        *a = NnopsRotaryAttrs{};
+    }
+}
+
+NnopsOp* nnops_rotary_create(const NnopsRotaryAttrs* a, int32_t backend)
+{
+    RotaryAttributes attrs;
+    if (a != nullptr) {
+        attrs.head_dim = a->head_dim;
+        attrs.rotary_dim = a->rotary_dim;
+        attrs.interleaved = a->interleaved != 0;
+    }
+    auto* h = new NnopsOp;
+    h->op = Rotary::create(attrs, static_cast<Backend>(backend));
+    return h;
+}
+
+NnopsOp* nnops_kv_cache_write_create(int32_t backend)
+{
+    auto* h = new NnopsOp;
+    h->op = KvCacheWrite::create(static_cast<Backend>(backend));
+    return h;
+}
+
+NnopsOp* nnops_kv_cache_read_create(int32_t output_dtype, int32_t backend)
+{
+    KvCacheReadAttributes attrs;
+    attrs.output_dtype = static_cast<DataType>(output_dtype);
+    auto* h = new NnopsOp;
+    h->op = KvCacheRead::create(attrs, static_cast<Backend>(backend));
+    return h;
+}
+
+void nnops_cache_attention_attrs_init(NnopsCacheAttentionAttrs* a)
+{
+    if (a != nullptr) {
+        *a = NnopsCacheAttentionAttrs{};
+    }
+}
+
+NnopsOp* nnops_cache_attention_create(const NnopsCacheAttentionAttrs* a, int32_t backend)
+{
+    CacheAttentionAttributes attrs;
+    if (a != nullptr) {
+        attrs.scale = a->scale;
+        attrs.window = a->window;
+        attrs.sinks = a->sinks;
+    }
+    auto* h = new NnopsOp;
+    h->op = CacheAttention::create(attrs, static_cast<Backend>(backend));
+    return h;
+}
+
 void nnops_op_destroy(NnopsOp* op)
 {
     delete op;
@@ -198,14 +291,24 @@ int nnops_op_output_desc(const NnopsOp* op, const NnopsTensor* inputs, int32_t n
     if (o.empty()) {
         return static_cast<int>(Status::invalid_argument);
     }
-    *out = NnopsTensor{};
-    out->rank = o[0].rank;
-    for (int64_t i = 0; i < o[0].rank; ++i) {
-        out->dims[i] = o[0].dims[static_cast<size_t>(i)];
-    }
-    out->dtype = static_cast<int32_t>(o[0].dtype);
-    out->scale = 1.0f;
+    *out = from_desc(o[0]);
     return 0;
+}
+
+int nnops_op_output_descs(const NnopsOp* op, const NnopsTensor* inputs, int32_t n_inputs, NnopsTensor* outs,
+                          int32_t n_outs)
+{
+    if (op == nullptr || inputs == nullptr || outs == nullptr || n_inputs < 1) {
+        return -static_cast<int>(Status::invalid_argument);
+    }
+    const std::vector<TensorDesc> o = op->op->getOutputTensorDesc(descs(inputs, n_inputs));
+    if (o.empty() || static_cast<size_t>(n_outs < 0 ? 0 : n_outs) < o.size()) {
+        return -static_cast<int>(Status::invalid_argument);
+    }
+    for (size_t i = 0; i < o.size(); ++i) {
+        outs[i] = from_desc(o[i]);
+    }
+    return static_cast<int>(o.size());
 }
 
 int nnops_op_prepack_weights(NnopsOp* op, const NnopsTensor* inputs, int32_t n_inputs, NnopsTensor* outputs,
@@ -269,10 +372,10 @@ size_t nnops_op_workspace_size(const NnopsOp* op, const NnopsTensor* inputs, int
 int nnops_op_compute(NnopsOp* op, const NnopsTensor* outputs, int32_t n_outputs,
                      const NnopsTensor* inputs, int32_t n_inputs, void* hip_stream, void* workspace)
 {
-    if (op == nullptr || n_inputs < 0 || n_outputs < 0 || n_inputs > 3 || n_outputs > 1) {
+    if (op == nullptr || n_inputs < 0 || n_outputs < 0 || n_inputs > 8 || n_outputs > 4) {
         return static_cast<int>(Status::invalid_argument);
     }
-    TensorView in[3], out[1];
+    TensorView in[8], out[4];
     for (int32_t i = 0; i < n_inputs; ++i) {
         in[i] = to_view(inputs[i]);
     }

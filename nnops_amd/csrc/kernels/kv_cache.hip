@@ -1,0 +1,419 @@
+// The 8-bit key / value cache: rows quantized into pages as they are written,
+// and read back. A page has one scale per KV head and side (keys, values):
+//   scale = max(old scale, max |new| / 127, 2^-100)
+//   new code = rint(x (1 / scale)),  older code = rint(code (old / scale))
+// so a page whose scale grows is rewritten; it can grow only as long as the
+// page fills.
+//
+// Bound: HBM: the new rows and their codes; reading back, the codes and the
+// values. One workgroup owns one page of a sequence, one head and one side, so
+// that a page's maximum needs no atomics and every run gives the same bits.
+// Writing, the rows are read twice, the second time from the CU's caches.
+// Values lie transposed in a page (a channel's tokens side by side): a thread
+// takes two channels by 16 tokens, so that its lanes read and write whole rows
+// and its codes are 16-byte pieces.
+#include "paged.hpp"
+
+namespace nnops_amd {
+
+int check_pages(const NnopsKvPages& c, int64_t rows)
+{
+    if (rows < 0 || c.sequences < 0 || c.pages < 0 || c.heads < 0 || c.table_pages < 0) {
+        return NNOPS_INVALID_ARGUMENT;
+    }
+    const int64_t t = c.page_tokens, d = c.head_dim;
+    if (t != 16 && t != 32 && t != 64 && t != 128 && t != 256) {
+        return NNOPS_UNSUPPORTED;
+    }
+    if (d < 16 || d > 256 || d % 16 != 0) {
+        return NNOPS_UNSUPPORTED;
+    }
+    if (rows == 0 || c.heads == 0) {
+        return NNOPS_OK;
+    }
+    if (rows > INT32_MAX / 2 || c.sequences > INT32_MAX / 2 || c.pages > INT32_MAX || c.heads > (1 << 16) ||
+        c.table_pages > INT32_MAX / t) {
+        return NNOPS_UNSUPPORTED;
+    }
+    if (c.sequences == 0 || (c.row_starts == nullptr && rows % c.sequences != 0)) {
+        return NNOPS_INVALID_ARGUMENT;
+    }
+    if (c.page_table == nullptr || c.lengths == nullptr || c.ld_table < c.table_pages) {
+        return NNOPS_INVALID_ARGUMENT;
+    }
+    if (c.pages > 0 && (c.k == nullptr || c.v == nullptr || c.k_scale == nullptr || c.v_scale == nullptr ||
+                        (uintptr_t)c.k % 16 != 0 || (uintptr_t)c.v % 16 != 0)) {
+        return NNOPS_INVALID_ARGUMENT;
+    }
+    return -1;
+}
+
+Paged paged(const NnopsKvPages& c, int64_t rows)
+{
+    Paged p{};
+    p.k = c.k;
+    p.v = c.v;
+    p.k_scale = c.k_scale;
+    p.v_scale = c.v_scale;
+    p.table = c.page_table;
+    p.lengths = c.lengths;
+    p.row_starts = c.row_starts;
+    p.ld_table = c.ld_table;
+    p.pages = (int32_t)c.pages;
+    p.heads = (int32_t)c.heads;
+    p.page = (int32_t)c.page_tokens;
+    p.page_log2 = __builtin_ctzll((unsigned long long)c.page_tokens);
+    p.d = (int32_t)c.head_dim;
+    p.seqs = (int32_t)c.sequences;
+    p.table_pages = (int32_t)c.table_pages;
+    p.rows = (int32_t)rows;
+    p.uniform = (int32_t)(rows / c.sequences);
+    return p;
+}
+
+namespace {
+
+struct RowsKern {
+    Paged c;
+    void* k;
+    void* v;
+    int64_t ld_k, ld_v;
+    int32_t per_seq;      // items of a sequence, equal rows each (0: found by search)
+};
+
+// Items of a sequence: the pages that its rows of the call fall in; one, of no
+// slots, where it has rows but holds no tokens.
+__device__ __forceinline__ int touched(const Paged& p, const SeqRows& s)
+{
+    const int first = max(s.len - s.n, 0);
+    return s.n <= 0 ? 0 : s.len <= first ? 1 : ((s.len - 1) >> p.page_log2) - (first >> p.page_log2) + 1;
+}
+
+// The part of a page that a workgroup has: slots [from, to) are rows of the
+// call, row `row` + slot - from; slots before `from` are older tokens. `absent`
+// rows before it (of a sequence's first item) stand for no token.
+struct PagePart {
+    int id, from, to, absent;
+    int64_t row;
+};
+
+__device__ __forceinline__ bool page_part(const RowsKern& p, int64_t item, PagePart& t)
+{
+    int b, j;
+    SeqRows s;
+    if (p.per_seq > 0) {
+        b = (int)(item / p.per_seq);
+        j = (int)(item - (int64_t)b * p.per_seq);
+        s = seq_rows(p.c, b);
+        if (j >= touched(p.c, s)) {
+            return false;
+        }
+    } else if (!find_item(p.c, item, [&](const SeqRows& q) { return touched(p.c, q); }, b, j, s)) {
+        return false;
+    }
+    const int first = max(s.len - s.n, 0);
+    const int page = (first >> p.c.page_log2) + j, base = page << p.c.page_log2;
+    t.from = max(first - base, 0);
+    t.to = min(s.len - base, p.c.page);
+    t.id = t.to > t.from ? page_of(p.c, b, page) : -1;
+    t.absent = j == 0 ? max(s.n - s.len, 0) : 0;
+    t.row = (int64_t)s.start + (base + t.from) - (s.len - s.n);
+    return true;
+}
+
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+__device__ __forceinline__ uint32_t code_byte(float x, float inv)
+{
+    const int q = (int)__builtin_rintf(__fmul_rn(x, inv));
+    return (uint32_t)min(max(q, -127), 127) & 0xffu;
+}
+
+// Byte e of a dword as a signed code, scaled to the grown step.
+__device__ __forceinline__ uint32_t rescaled(uint32_t d, float ratio)
+{
+    uint32_t o = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        o |= code_byte((float)(int8_t)(d >> (8 * e)), ratio) << (8 * e);
+    }
+    return o;
+}
+
+// blockIdx.x: item * heads + head; blockIdx.y: keys or values.
+template <typename T>
+__global__ __launch_bounds__(256) void kv_write_kernel(const RowsKern p)
+{
+    __shared__ uint32_t s_max[4];
+    const Paged& c = p.c;
+    const int64_t item = blockIdx.x / (unsigned)c.heads;
+    const int head = (int)(blockIdx.x - item * c.heads);
+    const bool values = blockIdx.y != 0;
+    PagePart t;
+    if (!page_part(p, item, t) || t.id < 0) {
+        return;                                    // the whole workgroup
+    }
+    const int d = c.d, n = t.to - t.from;
+    const int64_t ld = values ? p.ld_v : p.ld_k;
+    const T* rows = static_cast<const T*>(values ? p.v : p.k) + t.row * ld + (int64_t)head * d;
+    float* scale = (values ? c.v_scale : c.k_scale) + (int64_t)t.id * c.heads + head;
+    int8_t* page = (values ? c.v : c.k) + ((int64_t)t.id * c.heads + head) * ((int64_t)c.page * d);
+    const float old = t.from > 0 ? *scale : 0.0f;
+
+    uint32_t a = 0;
+    const int per_row = d / 8;
+    for (int i = threadIdx.x; i < n * per_row; i += 256) {
+        const int r = i / per_row, at = (i - r * per_row) * 8;
+        T x[8];
+        __builtin_memcpy(x, rows + r * ld + at, sizeof x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            a = max(a, magnitude((float)x[e]));
+        }
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+        a = max(a, (uint32_t)__shfl_xor((int)a, m));
+    }
+    if (threadIdx.x % 64 == 0) {
+        s_max[threadIdx.x / 64] = a;
+    }
+    __syncthreads();                               // every thread has read the old scale, too
+    a = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
+    // a NaN (of the rows or of the page before) stays one; fmaxf would drop it
+    const bool bad = a >= 0x7f800000u || !(old == old);
+    const float s = bad ? __uint_as_float(0x7fc00000u)
+                        : fmaxf(fmaxf(old, __fmul_rn(__uint_as_float(a), 1.0f / 127.0f)), kLeastScale);
+    const float inv = bad ? 0.0f : __fdiv_rn(1.0f, s);
+    const bool grew = !bad && t.from > 0 && s > old;
+    const float ratio = grew ? __fdiv_rn(old, s) : 1.0f;
+    if (threadIdx.x == 0) {
+        *scale = s;
+    }
+
+    if (!values) {
+        // a thread: 16 codes of a token
+        const int per_tok = d / 16;
+        const int begin = grew ? 0 : t.from;
+        for (int i = threadIdx.x; i < (t.to - begin) * per_tok; i += 256) {
+            const int r = i / per_tok, at = (i - r * per_tok) * 16, slot = begin + r;
+            v4i* dst = reinterpret_cast<v4i*>(page + slot * d + at);
+            uint32_t o[4];
+            if (slot < t.from) {
+                const v4i w = *dst;
+                const uint32_t wd[4] = {(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    o[e] = rescaled(wd[e], ratio);
+                }
+            } else {
+                T x[16];
+                __builtin_memcpy(x, rows + (slot - t.from) * ld + at, sizeof x);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const uint32_t q = bad ? 0u : code_byte((float)x[e], inv);
+                    o[e / 4] = (e % 4 ? o[e / 4] : 0u) | q << (8 * (e % 4));
+                }
+            }
+            *dst = v4i{(int)o[0], (int)o[1], (int)o[2], (int)o[3]};
+        }
+        return;
+    }
+    // a thread: two channels by a group of 16 tokens; groups with nothing to
+    // write are left out, older codes of a group kept or rescaled
+    const int g0 = grew ? 0 : t.from / 16, groups = (t.to + 15) / 16 - g0, pairs = d / 2;
+    for (int i = threadIdx.x; i < groups * pairs; i += 256) {
+        const int g = i / pairs, ch = (i - g * pairs) * 2, slot0 = (g0 + g) * 16;
+        v4i* dst[2] = {reinterpret_cast<v4i*>(page + ch * c.page + slot0),
+                       reinterpret_cast<v4i*>(page + (ch + 1) * c.page + slot0)};
+        uint32_t o[2][4] = {};
+        if (slot0 < t.from || slot0 + 16 > t.to) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const v4i w = *dst[h];
+                const uint32_t wd[4] = {(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    o[h][e] = grew ? rescaled(wd[e], ratio) : wd[e];
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int slot = slot0 + e;
+            if (slot >= t.from && slot < t.to) {
+                T x[2];
+                __builtin_memcpy(x, rows + (slot - t.from) * ld + ch, sizeof x);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t q = bad ? 0u : code_byte((float)x[h], inv);
+                    o[h][e / 4] = (o[h][e / 4] & ~(0xffu << (8 * (e % 4)))) | q << (8 * (e % 4));
+                }
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            *dst[h] = v4i{(int)o[h][0], (int)o[h][1], (int)o[h][2], (int)o[h][3]};
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void kv_read_kernel(const RowsKern p)
+{
+    const Paged& c = p.c;
+    const int64_t item = blockIdx.x / (unsigned)c.heads;
+    const int head = (int)(blockIdx.x - item * c.heads);
+    const bool values = blockIdx.y != 0;
+    PagePart t;
+    if (!page_part(p, item, t)) {
+        return;
+    }
+    const int d = c.d;
+    const int64_t ld = values ? p.ld_v : p.ld_k;
+    T* rows = static_cast<T*>(values ? p.v : p.k) + t.row * ld + (int64_t)head * d;
+    for (int64_t i = threadIdx.x; i < (int64_t)t.absent * d; i += 256) {
+        const int64_t r = i / d;
+        rows[(r - t.absent) * ld + (i - r * d)] = (T)0.0f;
+    }
+    const bool there = t.id >= 0;
+    const int64_t at_page = there ? (int64_t)t.id * c.heads + head : 0;
+    const float s = there ? (values ? c.v_scale : c.k_scale)[at_page] : __uint_as_float(0x7fc00000u);
+    const int8_t* page = (values ? c.v : c.k) + at_page * ((int64_t)c.page * d);
+    if (!values) {
+        const int per_tok = d / 16;
+        for (int i = threadIdx.x; i < (t.to - t.from) * per_tok; i += 256) {
+            const int r = i / per_tok, at = (i - r * per_tok) * 16;
+            const v4i w = there ? *reinterpret_cast<const v4i*>(page + (t.from + r) * d + at) : v4i{0, 0, 0, 0};
+            const uint32_t wd[4] = {(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w};
+            T y[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                y[e] = (T)__fmul_rn((float)(int8_t)(wd[e / 4] >> (8 * (e % 4))), s);
+            }
+            __builtin_memcpy(rows + r * ld + at, y, sizeof y);
+        }
+        return;
+    }
+    const int g0 = t.from / 16, groups = (t.to + 15) / 16 - g0, pairs = d / 2;
+    for (int i = threadIdx.x; i < groups * pairs; i += 256) {
+        const int g = i / pairs, ch = (i - g * pairs) * 2, slot0 = (g0 + g) * 16;
+        uint32_t wd[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const v4i w = there ? *reinterpret_cast<const v4i*>(page + (ch + h) * c.page + slot0) : v4i{0, 0, 0, 0};
+            wd[h][0] = (uint32_t)w.x, wd[h][1] = (uint32_t)w.y, wd[h][2] = (uint32_t)w.z, wd[h][3] = (uint32_t)w.w;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int slot = slot0 + e;
+            if (slot >= t.from && slot < t.to) {
+                T y[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    y[h] = (T)__fmul_rn((float)(int8_t)(wd[h][e / 4] >> (8 * (e % 4))), s);
+                }
+                __builtin_memcpy(rows + (slot - t.from) * ld + ch, y, sizeof y);
+            }
+        }
+    }
+}
+
+// Workgroups along x: pages that the rows can fall in, by heads.
+int64_t items(const NnopsKvRowsArgs* g, int32_t& per_seq)
+{
+    const int64_t t = g->cache.page_tokens, b = g->cache.sequences;
+    if (g->cache.row_starts == nullptr) {
+        const int64_t n = g->rows / b;
+        per_seq = (int32_t)((n + t - 2) / t + 1);
+        const int64_t held = g->cache.table_pages > 0 ? g->cache.table_pages : 1;
+        per_seq = (int32_t)(per_seq < held ? per_seq : held);
+        return b * per_seq;
+    }
+    per_seq = 0;
+    // sum over the sequences that have rows of (n + t - 2) / t + 1
+    const int64_t most = g->rows / t + 2 * (b < g->rows ? b : g->rows);
+    return most;
+}
+
+int check_rows(const NnopsKvRowsArgs* g)
+{
+    if (g == nullptr) {
+        return NNOPS_INVALID_ARGUMENT;
+    }
+    const int rc = check_pages(g->cache, g->rows);
+    if (rc >= 0) {
+        return rc;
+    }
+    const int64_t width = g->cache.heads * g->cache.head_dim;
+    if (g->k_rows == nullptr || g->v_rows == nullptr || g->ld_k < width || g->ld_v < width) {
+        return NNOPS_INVALID_ARGUMENT;
+    }
+    return -1;
+}
+
+RowsKern rows_kern(const NnopsKvRowsArgs* g, int32_t per_seq)
+{
+    RowsKern k{};
+    k.c = paged(g->cache, g->rows);
+    k.k = g->k_rows;
+    k.v = g->v_rows;
+    k.ld_k = g->ld_k;
+    k.ld_v = g->ld_v;
+    k.per_seq = per_seq;
+    return k;
+}
+
+}  // namespace
+}  // namespace nnops_amd
+
+using namespace nnops_amd;
+
+extern "C" int nnops_hip_kv_cache_write(const NnopsKvRowsArgs* g, void* stream)
+{
+    const TimingDisarm disarm;
+    const int rc = check_rows(g);
+    if (rc >= 0) {
+        return rc;
+    }
+    int32_t per_seq = 0;
+    const int64_t n = items(g, per_seq) * g->cache.heads;
+    if (n == 0 || g->cache.pages == 0) {
+        return NNOPS_OK;                          // no page to write to
+    }
+    if (n > INT32_MAX / 256) {
+        return NNOPS_UNSUPPORTED;
+    }
+    const RowsKern k = rows_kern(g, per_seq);
+    const dim3 grid((unsigned)n, 2);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (g->f16) {
+        NNOPS_LAUNCH(kv_write_kernel<_Float16>, grid, dim3(256), 0, s, k);
+    } else {
+        NNOPS_LAUNCH(kv_write_kernel<float>, grid, dim3(256), 0, s, k);
+    }
+    return hipGetLastError() == hipSuccess ? NNOPS_OK : NNOPS_INTERNAL;
+}
+
+extern "C" int nnops_hip_kv_cache_read(const NnopsKvRowsArgs* g, void* stream)
+{
+    const TimingDisarm disarm;
+    const int rc = check_rows(g);
+    if (rc >= 0) {
+        return rc;
+    }
+    int32_t per_seq = 0;
+    const int64_t n = items(g, per_seq) * g->cache.heads;
+    if (n > INT32_MAX / 256) {
+        return NNOPS_UNSUPPORTED;
+    }
+    const RowsKern k = rows_kern(g, per_seq);
+    const dim3 grid((unsigned)n, 2);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (g->f16) {
+        NNOPS_LAUNCH(kv_read_kernel<_Float16>, grid, dim3(256), 0, s, k);
+    } else {
+        NNOPS_LAUNCH(kv_read_kernel<float>, grid, dim3(256), 0, s, k);
+    }
+    return hipGetLastError() == hipSuccess ? NNOPS_OK : NNOPS_INTERNAL;
+}

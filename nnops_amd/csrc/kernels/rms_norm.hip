@@ -1,0 +1,362 @@
+// Root-mean-square norm with the residual's addition, its output in the input's
+// type or as s8 codes with one scale per row. Per row, in f32:
+//   h = x + residual;  rstd = 1 / sqrt(mean(h^2) + eps);  u = h w;
+//   y = u rstd,  or  a = max |u|, q = rint(u (127 / a)), scale = a rstd / 127.
+// The code needs no rstd: u rstd / (a rstd / 127) = 127 u / a, so codes depend
+// on a maximum only, which no order of evaluation changes.
+//
+// Bound: HBM; x and the residual are read once, the sum and the codes written
+// once. A row stays in its threads' registers between the two sums and the
+// output: lane l of a row's RW waves holds the NC chunks of 8 elements l, l +
+// 64 RW, ..; chunks are 16-byte loads (two for f32) from any alignment, the
+// last chunk of a row whose width is no multiple of 8 goes element by element.
+// Rows wider than 16 waves x 2 chunks (16384) are read twice.
+#include "common.hpp"
+
+namespace nnops_amd {
+namespace {
+
+struct NormKern {
+    const void* x;
+    const void* w;
+    const void* r;
+    void* y;
+    float* scale;
+    void* sum;
+    int64_t rows, cols, ld_x, ld_r, ld_y, ld_sum;
+    float eps;
+};
+
+// |v|'s bits order like |v|, infinities and NaNs above every finite value, so
+// an integer maximum keeps them where fmaxf would drop a NaN.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&f)[8])
+{
+    T t[8];
+    __builtin_memcpy(t, p, sizeof t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        f[e] = (float)t[e];
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_upto(const T* p, int n, float (&f)[8])
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        f[e] = e < n ? (float)p[e] : 0.0f;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_upto(T* p, int n, const float (&f)[8])
+{
+    T t[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        t[e] = (T)f[e];
+    }
+    if (n >= 8) {
+        __builtin_memcpy(p, t, sizeof t);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if (e < n) {
+            p[e] = t[e];
+        }
+    }
+}
+
+__device__ __forceinline__ void store_codes(int8_t* p, int n, const float (&u)[8], float inv)
+{
+    uint32_t d[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        // |u inv| <= 127 (1 + 2^-22): the rounding ends at +-127
+        const int q = (int)__builtin_rintf(__fmul_rn(u[e], inv));
+        d[e / 4] |= ((uint32_t)q & 0xffu) << (8 * (e % 4));
+    }
+    if (n >= 8) {
+        __builtin_memcpy(p, d, 8);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if (e < n) {
+            p[e] = (int8_t)(d[e / 4] >> (8 * (e % 4)));
+        }
+    }
+}
+
+// Sum and maximum over a row's RW waves, the same value in each of its lanes.
+template <int RW>
+__device__ __forceinline__ void row_reduce(float& ss, uint32_t& a)
+{
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+        ss += __shfl_xor(ss, m);
+        a = max(a, (uint32_t)__shfl_xor((int)a, m));
+    }
+    if constexpr (RW > 1) {
+        __shared__ float s_ss[RW];
+        __shared__ uint32_t s_a[RW];
+        const int wave = threadIdx.x / 64;
+        if (threadIdx.x % 64 == 0) {
+            s_ss[wave] = ss;
+            s_a[wave] = a;
+        }
+        __syncthreads();
+        ss = s_ss[0];
+        a = s_a[0];
+#pragma unroll
+        for (int i = 1; i < RW; ++i) {
+            ss += s_ss[i];
+            a = max(a, s_a[i]);
+        }
+    }
+}
+
+// The factor of u in the codes; 0 gives codes 0 (rows of next to nothing, and
+// rows that hold an infinity or a NaN, whose scale then says so).
+__device__ __forceinline__ float code_factor(uint32_t a)
+{
+    constexpr uint32_t kLeast = (127 - 119) << 23, kInf = 0x7f800000u;
+    return a >= kLeast && a < kInf ? __fmul_rn(__fdiv_rn(1.0f, __uint_as_float(a)), 127.0f) : 0.0f;
+}
+
+__device__ __forceinline__ float row_scale(uint32_t a, float rstd)
+{
+    return a < 0x7f800000u ? __fmul_rn(__fmul_rn(__uint_as_float(a), rstd), 1.0f / 127.0f) : __uint_as_float(0x7fc00000u);
+}
+
+template <typename T, int RW, int NC, bool S8, bool RES>
+__global__ __launch_bounds__(64 * (RW > 4 ? RW : 4)) void rms_norm_kernel(const NormKern p)
+{
+    constexpr int kRows = RW >= 4 ? 1 : 4 / RW;   // rows of a workgroup
+    static_assert(RW == 1 || RW >= 4, "a row has one wave, or the workgroup");
+    const int64_t row = kRows == 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * kRows + threadIdx.x / 64;
+    const int lane = kRows == 1 ? threadIdx.x : threadIdx.x % 64;
+    if (row >= p.rows) {
+        return;                                    // one wave per row: no barrier below
+    }
+    const T* x = static_cast<const T*>(p.x) + row * p.ld_x;
+    const T* r = RES ? static_cast<const T*>(p.r) + row * p.ld_r : nullptr;
+    const T* w = static_cast<const T*>(p.w);
+    T* sum = RES ? static_cast<T*>(p.sum) + row * p.ld_sum : nullptr;
+    const int cols = (int)p.cols;
+    float h[NC][8], u[NC][8];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int at = (lane + c * 64 * RW) * 8, n = cols - at;
+        float f[8];
+        if (n >= 8) {
+            load8(x + at, h[c]);
+            load8(w + at, u[c]);
+            if constexpr (RES) {
+                load8(r + at, f);
+            }
+        } else {
+            load_upto(x + at, n, h[c]);
+            load_upto(w + at, n, u[c]);
+            if constexpr (RES) {
+                load_upto(r + at, n, f);
+            }
+        }
+        if constexpr (RES) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                h[c][e] = __fadd_rn(h[c][e], f[e]);
+            }
+        }
+    }
+    float ss = 0.0f;
+    uint32_t a = 0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        if constexpr (RES) {
+            const int at = (lane + c * 64 * RW) * 8;
+            store_upto(sum + at, cols - at, h[c]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            ss = __builtin_fmaf(h[c][e], h[c][e], ss);
+            u[c][e] = __fmul_rn(h[c][e], u[c][e]);
+            if constexpr (S8) {
+                a = max(a, magnitude(u[c][e]));
+            }
+        }
+    }
+    row_reduce<RW>(ss, a);
+    const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, (float)cols) + p.eps));
+    if constexpr (S8) {
+        const float inv = code_factor(a);
+        int8_t* y = static_cast<int8_t*>(p.y) + row * p.ld_y;
+        if (lane == 0) {
+            p.scale[row] = row_scale(a, rstd);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int at = (lane + c * 64 * RW) * 8;
+            if (inv == 0.0f) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    u[c][e] = 0.0f;                // inf * 0 is no 0
+                }
+            }
+            store_codes(y + at, cols - at, u[c], inv);
+        }
+    } else {
+        T* y = static_cast<T*>(p.y) + row * p.ld_y;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int at = (lane + c * 64 * RW) * 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                u[c][e] = __fmul_rn(u[c][e], rstd);
+            }
+            store_upto(y + at, cols - at, u[c]);
+        }
+    }
+}
+
+// Rows of any width: one pass for the sum and the maximum, one for the output.
+// Nothing is written before the last, so that sum may lie over x or the residual.
+template <typename T, bool S8, bool RES>
+__global__ __launch_bounds__(1024) void rms_norm_wide(const NormKern p)
+{
+    const int64_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(p.x) + row * p.ld_x;
+    const T* r = RES ? static_cast<const T*>(p.r) + row * p.ld_r : nullptr;
+    const T* w = static_cast<const T*>(p.w);
+    auto chunk = [&](int64_t at, int n, float (&h)[8], float (&u)[8]) {
+        float f[8];
+        if (n >= 8) {
+            load8(x + at, h);
+            load8(w + at, u);
+            if constexpr (RES) {
+                load8(r + at, f);
+            }
+        } else {
+            load_upto(x + at, n, h);
+            load_upto(w + at, n, u);
+            if constexpr (RES) {
+                load_upto(r + at, n, f);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (RES) {
+                h[e] = __fadd_rn(h[e], f[e]);
+            }
+            u[e] = __fmul_rn(h[e], u[e]);
+        }
+    };
+    float ss = 0.0f;
+    uint32_t a = 0;
+    for (int64_t at = (int64_t)threadIdx.x * 8; at < p.cols; at += 8192) {
+        float h[8], u[8];
+        chunk(at, (int)min((int64_t)8, p.cols - at), h, u);
+        float part = 0.0f;                         // a sum of sums: no long chain of one rounding each
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            part = __builtin_fmaf(h[e], h[e], part);
+            a = max(a, magnitude(u[e]));
+        }
+        ss += part;
+    }
+    row_reduce<16>(ss, a);
+    const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, (float)p.cols) + p.eps));
+    const float inv = code_factor(a);
+    if (S8 && threadIdx.x == 0) {
+        p.scale[row] = row_scale(a, rstd);
+    }
+    for (int64_t at = (int64_t)threadIdx.x * 8; at < p.cols; at += 8192) {
+        const int n = (int)min((int64_t)8, p.cols - at);
+        float h[8], u[8];
+        chunk(at, n, h, u);
+        if constexpr (RES) {
+            store_upto(static_cast<T*>(p.sum) + row * p.ld_sum + at, n, h);
+        }
+        if constexpr (S8) {
+            if (inv == 0.0f) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    u[e] = 0.0f;
+                }
+            }
+            store_codes(static_cast<int8_t*>(p.y) + row * p.ld_y + at, n, u, inv);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                u[e] = __fmul_rn(u[e], rstd);
+            }
+            store_upto(static_cast<T*>(p.y) + row * p.ld_y + at, n, u);
+        }
+    }
+}
+
+template <typename T, bool S8, bool RES>
+void launch_norm(const NormKern& k, hipStream_t s)
+{
+    const int64_t chunks = (k.cols + 7) / 8;
+    const unsigned one = (unsigned)k.rows, four = (unsigned)((k.rows + 3) / 4);
+    if (chunks <= 64) {
+        NNOPS_LAUNCH((rms_norm_kernel<T, 1, 1, S8, RES>), dim3(four), dim3(256), 0, s, k);
+    } else if (chunks <= 128) {
+        NNOPS_LAUNCH((rms_norm_kernel<T, 1, 2, S8, RES>), dim3(four), dim3(256), 0, s, k);
+    } else if (chunks <= 256) {
+        NNOPS_LAUNCH((rms_norm_kernel<T, 4, 1, S8, RES>), dim3(one), dim3(256), 0, s, k);
+    } else if (chunks <= 512) {
+        NNOPS_LAUNCH((rms_norm_kernel<T, 4, 2, S8, RES>), dim3(one), dim3(256), 0, s, k);
+    } else if (chunks <= 1024) {
+        NNOPS_LAUNCH((rms_norm_kernel<T, 8, 2, S8, RES>), dim3(one), dim3(512), 0, s, k);
+    } else if (chunks <= 2048) {
+        NNOPS_LAUNCH((rms_norm_kernel<T, 16, 2, S8, RES>), dim3(one), dim3(1024), 0, s, k);
+    } else {
+        NNOPS_LAUNCH((rms_norm_wide<T, S8, RES>), dim3(one), dim3(1024), 0, s, k);
+    }
+}
+
+}  // namespace
+}  // namespace nnops_amd
+
+using namespace nnops_amd;
+
+extern "C" int nnops_hip_rms_norm(const NnopsRmsNormArgs* g, void* stream)
+{
+    const TimingDisarm disarm;
+    if (g == nullptr || g->rows < 0 || g->cols < 0) {
+        return NNOPS_INVALID_ARGUMENT;
+    }
+    if (g->rows == 0 || g->cols == 0) {
+        return NNOPS_OK;
+    }
+    const bool s8 = g->out_kind == NNOPS_OUT_S8;
+    if (!s8 && g->out_kind != (g->in_f16 ? NNOPS_OUT_F16 : NNOPS_OUT_F32)) {
+        return NNOPS_UNSUPPORTED;
+    }
+    if (g->rows > INT32_MAX || g->cols > INT32_MAX) {
+        return NNOPS_UNSUPPORTED;
+    }
+    const bool res = g->residual != nullptr;
+    if (g->x == nullptr || g->weight == nullptr || g->y == nullptr || g->ld_x < g->cols || g->ld_y < g->cols ||
+        (s8 != (g->scale != nullptr)) || (res != (g->sum != nullptr)) ||
+        (res && (g->ld_residual < g->cols || g->ld_sum < g->cols)) || !(g->epsilon >= 0.0f)) {
+        return NNOPS_INVALID_ARGUMENT;
+    }
+    const NormKern k{g->x,    g->weight, g->residual,    g->y,    g->scale,  g->sum,    g->rows,
+                     g->cols, g->ld_x,   g->ld_residual, g->ld_y, g->ld_sum, g->epsilon};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (g->in_f16) {
+        s8 ? (res ? launch_norm<_Float16, true, true>(k, s) : launch_norm<_Float16, true, false>(k, s))
+           : (res ? launch_norm<_Float16, false, true>(k, s) : launch_norm<_Float16, false, false>(k, s));
+    } else {
+        s8 ? (res ? launch_norm<float, true, true>(k, s) : launch_norm<float, true, false>(k, s))
+           : (res ? launch_norm<float, false, true>(k, s) : launch_norm<float, false, false>(k, s));
+    }
+    return hipGetLastError() == hipSuccess ? NNOPS_OK : NNOPS_INTERNAL;
+}

@@ -49,7 +49,7 @@ def tensor(t, *, dtype=None, shape=None, scale=1.0, zero_point=0, scale_data=Non
     x.data = t.data_ptr() if t is not None else None
     if pitch is not None:
         x.pitch = int(pitch)
-    elif t is not None and t.dim() >= 2:
+    elif t is not None and t.dim() >= 2 and t.numel() > 0:   # (an empty one's strides mean nothing)
         assert t.stride(-1) == 1, "innermost dim must be contiguous"
         x.pitch = t.stride(-2) * t.element_size()
     x.scale = float(scale)
@@ -128,7 +128,7 @@ def _host_tables(scales, zps):
 
 
 # array types for a call's tensors (an empty list still has an address)
-_ARRAYS = [L.Tensor * max(1, n) for n in range(5)]
+_ARRAYS = [L.Tensor * max(1, n) for n in range(9)]
 
 
 class _Op:
@@ -156,6 +156,15 @@ class _Op:
         if rc != 0:
             raise ValueError(f"output_desc failed: status {rc}")
         return [out.dims[i] for i in range(out.rank)], out.dtype
+
+    def output_descs(self, inputs):
+        """(shape, dtype code) of every output, in order."""
+        arr, n = self._arr(inputs)
+        outs = (L.Tensor * 8)()
+        got = L.lib().nnops_op_output_descs(self._h, arr, n, outs, 8)
+        if got < 0:
+            raise ValueError(f"output_descs failed: status {-got}")
+        return [([o.dims[i] for i in range(o.rank)], o.dtype) for o in outs[:got]]
 
     def validate(self, inputs, outputs):
         ai, ni = self._arr(inputs)
@@ -268,6 +277,93 @@ class DequantizeLinear(_Op):
         L.lib().nnops_quant_linear_attrs_init(C.byref(a))
         a.axis, a.output_dtype = axis, output_dtype
         super().__init__(L.lib().nnops_dequantize_linear_create(C.byref(a), backend))
+
+
+class RmsNorm(_Op):
+    """inputs: x [.., C] (f16/f32), weight [C] (, residual of x's shape);
+    outputs: y of x's shape (, scale f32 [rows] with an s8 y) (, sum = x +
+    residual, with a residual; may be x's or the residual's buffer). An s8 y and
+    its scales are the per-token activation that Linear and MatMul take:
+    ``tensor(y, scale_data=scale, granularity=1)``."""
+
+    def __init__(self, *, epsilon=1e-6, output_dtype=L.DT_F16, backend=L.BACKEND_HIP):
+        a = L.RmsNormAttrs()
+        L.lib().nnops_rms_norm_attrs_init(C.byref(a))
+        a.epsilon, a.output_dtype = epsilon, output_dtype
+        super().__init__(L.lib().nnops_rms_norm_create(C.byref(a), backend))
+
+
+class Rotary(_Op):
+    """inputs: x [tokens, heads * head_dim] (f16/f32, any row pitch), positions
+    s32 [tokens], table f32 [max_pos, rotary_dim] (:func:`rotary_table`);
+    output: x's shape and type, x itself if wanted."""
+
+    def __init__(self, *, head_dim, rotary_dim=0, interleaved=False, backend=L.BACKEND_HIP):
+        a = L.RotaryAttrs()
+        L.lib().nnops_rotary_attrs_init(C.byref(a))
+        a.head_dim, a.rotary_dim, a.interleaved = head_dim, rotary_dim, int(interleaved)
+        super().__init__(L.lib().nnops_rotary_create(C.byref(a), backend))
+
+
+class KvCacheWrite(_Op):
+    """inputs: k, v [rows, heads * head_dim] (f16/f32), page_table s32
+    [sequences, table_pages], lengths s32 [sequences] (, row_starts s32
+    [sequences + 1]); outputs, updated in place: k_cache s8 [pages, heads,
+    page_tokens, head_dim], v_cache s8 [pages, heads, head_dim, page_tokens],
+    k_scale and v_scale f32 [pages, heads]. :func:`kv_cache` makes one."""
+
+    def __init__(self, *, backend=L.BACKEND_HIP):
+        super().__init__(L.lib().nnops_kv_cache_write_create(backend))
+
+
+class KvCacheRead(_Op):
+    """inputs: k_cache, v_cache, k_scale, v_scale, page_table, lengths
+    (, row_starts); outputs: k, v [rows, heads * head_dim], the last tokens of
+    each sequence."""
+
+    def __init__(self, *, output_dtype=L.DT_F16, backend=L.BACKEND_HIP):
+        super().__init__(L.lib().nnops_kv_cache_read_create(output_dtype, backend))
+
+
+class CacheAttention(_Op):
+    """inputs: q [rows, q_heads * head_dim] (f16/f32), k_cache, v_cache, k_scale,
+    v_scale, page_table, lengths (, row_starts); output: q's shape and type.
+    ``scale`` 0: 1 / sqrt(head_dim); ``window`` 0: no window; ``sinks``: first
+    tokens that a window leaves visible."""
+
+    def __init__(self, *, scale=0.0, window=0, sinks=0, backend=L.BACKEND_HIP):
+        a = L.CacheAttentionAttrs()
+        L.lib().nnops_cache_attention_attrs_init(C.byref(a))
+        a.scale, a.window, a.sinks = scale, window, sinks
+        super().__init__(L.lib().nnops_cache_attention_create(C.byref(a), backend))
+
+
+def rotary_table(max_pos, rotary_dim, *, base=10000.0, factor=1.0, original_context=0, low_turns=1.0,
+                 high_turns=32.0, attention_factor=1.0, out=None, stream=None, device="cuda"):
+    """The cosines and sines that :class:`Rotary` takes, f32 [max_pos,
+    rotary_dim] (``out`` if given). ``factor``: positions divided by it; with
+    ``original_context`` only as far as a pair made fewer than ``high_turns``
+    turns over that context, and wholly below ``low_turns``."""
+    import torch
+    if out is None:
+        out = torch.empty((max_pos, rotary_dim), dtype=torch.float32, device=device)
+    a = L.RotaryTableArgs()
+    a.table, a.max_pos, a.rotary_dim, a.ld_table = out.data_ptr(), max_pos, rotary_dim, out.stride(0)
+    a.base, a.factor, a.original_context = base, factor, original_context
+    a.low_turns, a.high_turns, a.attention_factor = low_turns, high_turns, attention_factor
+    rc = L.lib().nnops_hip_rotary_table(C.byref(a), _stream_ptr(stream))
+    if rc != 0:
+        raise RuntimeError(f"nnops_hip_rotary_table failed: status {rc}")
+    return out
+
+
+def kv_cache(pages, heads, page_tokens, head_dim, *, device="cuda"):
+    """k_cache, v_cache, k_scale, v_scale of an empty cache (torch tensors)."""
+    import torch
+    return (torch.zeros((pages, heads, page_tokens, head_dim), dtype=torch.int8, device=device),
+            torch.zeros((pages, heads, head_dim, page_tokens), dtype=torch.int8, device=device),
+            torch.zeros((pages, heads), dtype=torch.float32, device=device),
+            torch.zeros((pages, heads), dtype=torch.float32, device=device))
 
 
 def gemm_i8(a, b, c, *, trans_a=False, trans_b=False, bias=None, out_kind=L.OUT_S32,

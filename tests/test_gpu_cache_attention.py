@@ -1,0 +1,339 @@
+"""CacheAttention against attention in 64 bits over the dequantized cache: head
+sizes, pages and groups, one token and prompts, ragged mixtures, windows and
+sinks, sequences that are split and joined, rows that see nothing, pages that
+do not exist, NaN and infinite values where the masks hide them, strides,
+streams and graphs."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import datagen as dg
+import decoder_ref as ref
+import nnops_amd as na
+from gpu_util import dev, host, pitched, announce
+
+pytestmark = pytest.mark.gpu
+
+
+def _cache(seqs, tokens, heads, page, d, seed=1, spare=2):
+    """codes and scales (numpy), pages shuffled, and the table."""
+    per = max(1, -(-tokens // page))
+    n = seqs * per + spare
+    kc, vc = dg.ints(seed, (n, heads, page, d), -127, 127), dg.ints(seed + 1, (n, heads, d, page), -127, 127)
+    ks = (0.01 * np.exp(0.5 * dg.normal(seed + 2, (n, heads)))).astype(np.float32)
+    vs = (0.02 * np.exp(0.7 * dg.normal(seed + 3, (n, heads)))).astype(np.float32)
+    table = np.argsort(dg.unit(seed + 4, n))[:seqs * per].reshape(seqs, per).astype(np.int32)
+    return kc, vc, ks, vs, table
+
+
+def _run(q, cache, lens, rows, *, ragged, window=0, sinks=0, scale=0.0, pad=0, stream=None, workspace=None):
+    import torch
+    kc, vc, ks, vs, table = cache
+    starts = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+    dq = pitched(q, q.shape[1] + pad)
+    out = pitched(np.full(q.shape, 7, q.dtype), q.shape[1] + 2 * pad)
+    ins = [na.tensor(dq)] + [na.tensor(dev(x)) for x in (kc, vc, ks, vs, table, np.array(lens, np.int32))]
+    ins += [na.tensor(dev(starts))] if ragged else []
+    op = na.CacheAttention(window=window, sinks=sinks, scale=scale)
+    outs = [na.tensor(out)]
+    assert op.validate(ins, outs) == na.OK
+    assert op.compute(outs, ins, stream=stream, workspace=workspace) == na.OK
+    torch.cuda.synchronize()
+    return host(out)
+
+
+def _check(q, cache, lens, rows, *, window=0, sinks=0, scale=0.0, **kw):
+    got = _run(q, cache, lens, rows, window=window, sinks=sinks, scale=scale, **kw).astype(np.float64)
+    want, weight, spread = ref.attention(q, *cache, lens, rows, window=window, sinks=sinks,
+                                         scale=scale or None)
+    tol = ref.attention_tolerance(q.dtype == np.float16, want, weight, spread, cache[3])
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    ok = ~np.isnan(want)
+    worst = np.max((abs(got - want) / tol)[ok]) if ok.any() else 0.0
+    assert worst <= 1.0, worst
+    return got
+
+
+def _q(seed, t, width, f16):
+    return dg.normal(seed, (t, width)).astype(np.float16 if f16 else np.float32)
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("d,page,heads,group", [(128, 64, 2, 4), (128, 16, 1, 1), (64, 32, 2, 8), (80, 16, 2, 5),
+                                                (96, 128, 1, 16), (256, 64, 1, 2), (16, 256, 3, 1), (112, 64, 2, 7),
+                                                (64, 16, 1, 71), (192, 32, 1, 3)])
+def test_single_tokens(d, page, heads, group, f16):
+    """One query each: lengths of one, around pages and tiles of 64."""
+    announce(f"attention d={d} page={page} heads={heads} group={group} f16={f16}")
+    lens = [1, 15, 16, 17, 63, 64, 65, 300]
+    cache = _cache(len(lens), 300, heads, page, d)
+    q = _q(3, len(lens), heads * group * d, f16)
+    rows = [1] * len(lens)
+    a = _check(q, cache, lens, rows, ragged=False)
+    b = _check(q, cache, lens, rows, ragged=True, pad=3)
+    assert np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("d,page,heads,group", [(128, 16, 1, 4), (64, 64, 2, 1), (80, 128, 1, 3), (256, 32, 1, 1)])
+def test_prompts(d, page, heads, group, f16):
+    """Ragged prompts behind prefixes of different lengths, a sequence without
+    rows, a whole prompt, a single token."""
+    announce(f"attention prompts d={d} page={page} group={group} f16={f16}")
+    lens, rows = [130, 70, 9, 200, 64], [130, 5, 0, 1, 64]
+    cache = _cache(len(lens), 200, heads, page, d)
+    _check(_q(4, sum(rows), heads * group * d, f16), cache, lens, rows, ragged=True)
+    # as many rows each
+    _check(_q(5, 5 * 9, heads * group * d, f16), cache, lens, [9] * 5, ragged=False, pad=5)
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (64, 0), (100, 70), (100, 200), (300, 5),
+                                          (1 << 40, 3), (7, 1 << 40)])
+def test_windows(window, sinks, f16):
+    announce(f"attention window={window} sinks={sinks} f16={f16}")
+    heads, group, d, page = 2, 3, 64, 16
+    lens, rows = [400, 1, 333, 90], [1, 1, 70, 90]
+    cache = _cache(4, 400, heads, page, d)
+    _check(_q(6, sum(rows), heads * group * d, f16), cache, lens, rows, ragged=True, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("tokens,page,group,n", [(5000, 64, 4, 1), (5000, 16, 1, 1), (3001, 128, 8, 3), (2000, 32, 2, 40)])
+def test_long(tokens, page, group, n):
+    """Long sequences, split over workgroups and joined, beside short ones."""
+    announce(f"attention long {tokens} page={page} group={group} n={n}")
+    heads, d = 2, 64
+    lens = [tokens, n, 900]
+    cache = _cache(3, tokens, heads, page, d)
+    q = _q(7, 3 * n, heads * group * d, True)
+    a = _check(q, cache, lens, [n] * 3, ragged=False)
+    b = _check(q, cache, lens, [n] * 3, ragged=True)
+    assert np.max(abs(a - b)) <= 2.0 ** -9 * np.max(abs(a))
+    _check(q.astype(np.float32), cache, lens, [n] * 3, ragged=True, window=1500, sinks=100)
+
+
+def test_scales_far_apart():
+    """Pages whose value scales differ by powers of ten, pages of zeros, the
+    smallest scale; a scale of 0 reads as zeros."""
+    heads, d, page, n = 1, 64, 16, 200
+    for f16 in (True, False):
+        announce(f"attention scales far apart f16={f16}")
+        kc, vc, ks, vs, table = _cache(1, n, heads, page, d)
+        vs[table[0], 0] = (10.0 ** (np.arange(table.shape[1]) % 7 - 4.0)).astype(np.float32)
+        vs[table[0, 2], 0] = ref.LEAST_SCALE
+        vs[table[0, 3], 0] = 0
+        vc[table[0, 2]] = 0
+        ks[table[0, 4], 0] = 0
+        cache = (kc, vc, ks, vs, table)
+        _check(_q(8, 3, 2 * d, f16), cache, [n], [3], ragged=False)
+        # nothing but zeros
+        vs[:], vc[:] = ref.LEAST_SCALE, 0
+        assert np.all(_run(_q(9, 1, d, f16), cache, [n], [1], ragged=False) == 0)
+
+
+def test_sharp_and_flat():
+    """Scores of hundreds (one token takes all) and of nothing (an average), rows
+    far from 1, a scale of the caller's."""
+    heads, d, page, n = 2, 128, 64, 500
+    cache = _cache(1, n, heads, page, d)
+    for f16 in (True, False):
+        for size in (60.0, 1e-4, 0.0) if f16 else (60.0, 1e-30, 0.0, 1e30):
+            announce(f"attention size {size} f16={f16}")
+            q = (size * dg.normal(10, (2, heads * d))).astype(np.float16 if f16 else np.float32)
+            _check(q, cache, [n], [2], ragged=False, scale=0.0 if size < 1e20 else 1e-30)
+        _check(_q(11, 2, heads * d, f16), cache, [n], [2], ragged=False, scale=0.3)
+
+
+def test_hidden_values_do_not_show():
+    """Pages past a row's position hold NaN scales and any codes; unwritten page
+    table entries are garbage; a query that is NaN or infinite shows in its own
+    row alone."""
+    heads, d, page = 1, 64, 16
+    for f16 in (True, False):
+        announce(f"attention hidden f16={f16}")
+        kc, vc, ks, vs, table = _cache(2, 160, heads, page, d)
+        clean = [x.copy() for x in (kc, vc, ks, vs, table)]
+        q = _q(12, 40, 2 * d, f16)
+        lens, rows = [100, 40], [20, 20]
+        want = _check(q, (kc, vc, ks, vs, table), lens, rows, ragged=False)
+        # rows at positions 80 .. 99 of the first: its pages of tokens 96 on hold
+        # a NaN from row 16 on; past the length the table holds garbage
+        ks[table[0, 6]], vs[table[0, 6]] = np.nan, np.nan
+        table[0, 7:], table[1, 3:] = -5, 1 << 30
+        got = _run(q, (kc, vc, ks, vs, table), lens, rows, ragged=False).astype(np.float64)
+        assert np.array_equal(got[:16], want[:16]) and np.array_equal(got[20:], want[20:])
+        assert np.isnan(got[16:20]).all()
+        # a window that has moved past them
+        kc, vc, ks, vs, table = [x.copy() for x in clean]
+        want = _run(q, (kc, vc, ks, vs, table), lens, rows, ragged=False, window=30)
+        ks[table[0, :3]], vs[table[0, :3]] = np.nan, np.inf
+        table[0, 0] = -1
+        assert np.array_equal(want, _run(q, (kc, vc, ks, vs, table), lens, rows, ragged=False, window=30))
+        q[3, 5], q[25, d + 1] = np.nan, np.inf
+        want = _run(_q(12, 40, 2 * d, f16), tuple(clean), lens, rows, ragged=False).astype(np.float64)
+        got = _run(q, tuple(clean), lens, rows, ragged=False).astype(np.float64)
+        hit = np.zeros_like(got, bool)
+        hit[3, :d], hit[25, d:] = True, True
+        assert np.isnan(got[hit]).all() and np.array_equal(got[~hit], want[~hit])
+
+
+def test_rows_that_see_nothing():
+    """More rows than tokens, sequences without tokens: zeros; a page number
+    outside the cache: NaN in the rows that see it."""
+    announce("attention empty rows")
+    heads, d, page = 2, 32, 16
+    cache = _cache(3, 64, heads, page, d)
+    lens, rows = [4, 0, 64], [10, 3, 7]
+    for f16 in (True, False):
+        q = _q(13, 20, heads * d, f16)
+        got = _check(q, cache, lens, rows, ragged=True)
+        assert np.all(got[:6] == 0) and np.all(got[10:13] == 0) and np.all(np.any(got[6:10] != 0, axis=1))
+        _check(q[:9], cache, [0, 0, 2], [3, 3, 3], ragged=False)
+        table = cache[4].copy()
+        table[2, 1] = 99999
+        got = _check(q, cache[:4] + (table,), lens, rows, ragged=True)
+        assert np.isnan(got[13:]).all()
+
+
+def test_rows_without_a_sequence_stay():
+    """Rows past the last start belong to nobody and are left as they are."""
+    import torch
+    announce("attention rows without a sequence")
+    heads, d, page = 1, 32, 16
+    cache = _cache(1, 40, heads, page, d)
+    q = _q(14, 6, d, True)
+    out = torch.full((6, d), 7.0, dtype=torch.float16, device="cuda")
+    ins = [na.tensor(dev(x)) for x in (q,) + cache + (np.array([40], np.int32), np.array([1, 4], np.int32))]
+    assert na.CacheAttention().compute([na.tensor(out)], ins) == na.OK
+    torch.cuda.synchronize()
+    want = _run(q[1:4], cache, [40], [3], ragged=False)
+    assert np.array_equal(host(out)[1:4], want) and np.all(host(out)[[0, 4, 5]] == 7)
+
+
+@pytest.mark.parametrize("seqs", [65, 130])
+def test_many_sequences(seqs):
+    announce(f"attention {seqs} sequences")
+    heads, group, d, page = 1, 2, 32, 16
+    cache = _cache(seqs, 90, heads, page, d)
+    lens = 1 + dg.ints(15, (seqs,), 0, 80).astype(np.int64)
+    rows = np.minimum(dg.ints(16, (seqs,), 0, 12), lens)
+    _check(_q(17, int(rows.sum()), group * d, True), cache, lens, rows, ragged=True)
+
+
+def test_cache_past_2_gib():
+    import torch
+    announce("attention past 2^32 bytes")
+    page, heads, d = 128, 8, 128
+    n = (1 << 32) // (heads * page * d) + 40
+    small = _cache(1, 3 * page, heads, page, d, spare=0)
+    kc, vc = (torch.zeros((n,) + x.shape[1:], dtype=torch.int8, device="cuda") for x in small[:2])
+    ks, vs = (torch.zeros((n, heads), device="cuda") for _ in range(2))
+    places = [n - 1, n // 2 + 1, n - 7]
+    for i, at in enumerate(places):
+        for big, x in zip((kc, vc, ks, vs), small):
+            big[at] = torch.from_numpy(x[i]).cuda()
+    table = np.array([[places[i] for i in small[4][0]]], np.int32)
+    q = _q(18, 2, heads * 2 * d, True)
+    out = torch.zeros((2, heads * 2 * d), dtype=torch.float16, device="cuda")
+    op = na.CacheAttention()
+    assert op.compute([na.tensor(out)], [na.tensor(dev(q))] + [na.tensor(x) for x in (kc, vc, ks, vs)] +
+                      [na.tensor(dev(table)), na.tensor(dev(np.array([370], np.int32)))]) == na.OK
+    torch.cuda.synchronize()
+    assert np.array_equal(host(out), _run(q, small, [370], [2], ragged=False))
+
+
+def test_streams_and_workspace():
+    """A stream of the caller's, a workspace of the caller's that holds anything,
+    the same bits every time; too little workspace is refused."""
+    import ctypes
+    import torch
+    announce("attention stream and workspace")
+    heads, d, page, n = 2, 128, 64, 3000
+    cache = _cache(1, n, heads, page, d)
+    q = _q(19, 1, heads * 4 * d, True)
+    want = _run(q, cache, [n], [1], ragged=False)
+    side = torch.cuda.Stream()
+    ws = torch.full((64 << 20,), 0xFF, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(3):
+        assert np.array_equal(want, _run(q, cache, [n], [1], ragged=False, stream=side, workspace=ws))
+    dq, t = dev(q), [dev(x) for x in cache] + [dev(np.array([n], np.int32))]
+    out = torch.full(q.shape, 7.0, dtype=torch.float16, device="cuda")
+    a = na.CacheAttentionArgs()
+    a.q, a.out, a.rows, a.q_heads, a.ld_q, a.ld_out, a.f16 = dq.data_ptr(), out.data_ptr(), 1, 8, 1024, 1024, 1
+    c = a.cache
+    c.k, c.v, c.k_scale, c.v_scale, c.page_table, c.lengths = (x.data_ptr() for x in t)
+    c.pages, c.heads, c.page_tokens, c.head_dim = cache[0].shape
+    c.sequences, c.table_pages, c.ld_table = 1, cache[4].shape[1], cache[4].shape[1]
+    lib = na.lib()
+    need = lib.nnops_hip_cache_attention_workspace_size(ctypes.byref(a))
+    assert need > 0
+    assert lib.nnops_hip_cache_attention(ctypes.byref(a), ws.data_ptr(), need - 1, None) == na.NOT_INITIALIZED
+    assert lib.nnops_hip_cache_attention(ctypes.byref(a), None, 0, None) == na.NOT_INITIALIZED
+    torch.cuda.synchronize()
+    assert np.all(host(out) == 7)
+    assert lib.nnops_hip_cache_attention(ctypes.byref(a), ws.data_ptr(), need, None) == na.OK
+    torch.cuda.synchronize()
+    assert np.array_equal(host(out), want)
+
+
+def test_graph_replays():
+    """The operators of a step captured into one graph: the norm, the rotation,
+    the cache's write and the attention, replayed with other inputs between."""
+    import torch
+    announce("decoder step under graph replay")
+    heads, group, d, page, b = 2, 2, 64, 16, 3
+    hq = heads * group
+    width = (hq + 2 * heads) * d
+    lens = np.array([40, 1, 700], np.int32)
+    kc, vc, ks, vs, table = _cache(b, 700, heads, page, d)
+    dt, dl = dev(table), dev(lens)
+    cache = [dev(x) for x in (kc, vc, ks, vs)]
+    keep = [x.clone() for x in cache]
+    x = dev(dg.normal(20, (b, width)).astype(np.float16))
+    w = dev(np.ones(width, np.float16))
+    y = torch.zeros_like(x)
+    out = torch.zeros((b, hq * d), dtype=torch.float16, device="cuda")
+    pos = dev((lens - 1).astype(np.int32))
+    tab = na.rotary_table(1000, d)
+    norm, rot, wr, at = na.RmsNorm(), na.Rotary(head_dim=d), na.KvCacheWrite(), na.CacheAttention()
+    qk = y[:, :(hq + heads) * d]
+    pages = [na.tensor(z) for z in cache]
+    where = [na.tensor(dt), na.tensor(dl)]
+    ains, aouts = [na.tensor(y[:, :hq * d])] + pages + where, [na.tensor(out)]
+    ws = torch.empty(max(1, at.workspace_size(ains, aouts)), dtype=torch.uint8, device="cuda")
+
+    def step(s):
+        assert norm.compute([na.tensor(y)], [na.tensor(x), na.tensor(w)], stream=s) == na.OK
+        assert rot.compute([na.tensor(qk)], [na.tensor(qk), na.tensor(pos), na.tensor(tab)], stream=s) == na.OK
+        assert wr.compute(pages, [na.tensor(y[:, hq * d:(hq + heads) * d]), na.tensor(y[:, (hq + heads) * d:])] + where,
+                          stream=s) == na.OK
+        assert at.compute(aouts, ains, stream=s, workspace=ws) == na.OK
+
+    def reset():
+        for z, k in zip(cache, keep):
+            z.copy_(k)
+
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        step(s)
+    torch.cuda.synchronize()
+    reset()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        step(s)
+    for r in range(4):
+        x.copy_(dev(dg.normal(30 + r, (b, width)).astype(np.float16)))
+        reset()
+        step(None)
+        torch.cuda.synchronize()
+        want = [host(z).copy() for z in [out] + cache]
+        reset()
+        out.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        for a, z in zip(want, [out] + cache):
+            assert np.array_equal(a, host(z), equal_nan=True), r
