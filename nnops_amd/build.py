@@ -41,6 +41,7 @@ SOURCES = [
     "csrc/kernels/rotary.hip",
     "csrc/kernels/kv_cache.hip",
     "csrc/kernels/cache_attention.hip",
+    "csrc/kernels/cache_attention_tiled.hip",
     "csrc/host/ops.cpp",
     "csrc/host/quant_linear.cpp",
     "csrc/host/rms_norm.cpp",

@@ -17,163 +17,19 @@
 //
 // Scales: with ks, vs the scales of a token's page,
 //   x = scale log2(e) (q . code) ks + log2(vs),  M = running max of x,
-//   P = 2^(x - M + 14),  O += P code,  l += P 2^-14 / vs,  out = 2^-14 O / l:
-// the value scale rides in the exponent (one fma), P's largest weight is 2^14
-// whatever the scales are, and f16's range below it is 2^-38.
+//   P = 2^(x - M + 6),  O += P code,  l += P 2^-6 / vs,  out = 2^-6 O / l:
+// the value scale rides in the exponent (one fma), and P's largest weight is
+// the same whatever the scales are.
 //
 // Bound: HBM for few rows, the codes read once per KV head. Long sequences are
 // split over workgroups (partial O, M, l in the workspace, joined by a second
 // kernel); a workgroup's 4 waves take every fourth tile and join in LDS.
-#include <limits>
-
-#include "paged.hpp"
+#include "cache_attention.hpp"
 
 namespace nnops_amd {
 namespace {
 
-constexpr int kRows = 16;           // rows of a wave's tile
-constexpr int kTile = 64;           // tokens of a step
-constexpr float kPShift = 14.0f;    // log2 of the largest weight
-
-struct AttnKern {
-    Paged c;
-    const void* q;
-    void* out;
-    int64_t ld_q, ld_out;
-    float* part;          // [splits][rows][q_heads][d + 2]: O, M, l
-    float scale_log2;
-    int32_t q_heads, group, window, sinks;
-    int32_t per_seq;      // row tiles of a sequence, equal rows each (0: found by search)
-    int32_t chunk;        // tiles of 64 tokens that a split takes
-};
-
-// The tiles of 64 tokens that rows at positions pmin .. pmax look at: the
-// first `sink_tiles`, then those from `first` on, `tiles` in all.
-struct Span {
-    int sink_tiles, first, tiles;
-};
-
-__host__ __device__ __forceinline__ Span span_of(int pmin, int pmax, int window, int sinks)
-{
-    Span s{0, 0, pmax < 0 ? 0 : pmax / kTile + 1};
-    if (window > 0 && pmax >= 0) {
-        const int lo = (pmin > window - 1 ? pmin - window + 1 : 0) / kTile;
-        const int kept = sinks < pmax + 1 ? sinks : pmax + 1;
-        const int st = (kept + kTile - 1) / kTile;
-        if (st < lo) {
-            s.sink_tiles = st;
-            s.first = lo;
-            s.tiles += st - lo;
-        }
-    }
-    return s;
-}
-
-// The operands of the two products, by the rows' type.
-//   f16: the rows as they are, the probabilities rounded to f16, codes as f16.
-//   f32: each value as three bf16 parts that hold it exactly (8 bits each, by
-//        truncation, the last difference having no more), codes as bf16 (7 bits
-//        and a sign: exact), three products into one f32 accumulator. Two f16
-//        parts would be one product fewer, but their range ends 2^-38 below the
-//        largest probability.
-typedef __bf16 v8b __attribute__((ext_vector_type(8)));
-typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-
-template <typename T>
-struct Operand {
-    static constexpr int kParts = 1;
-    typedef v8h Vec;
-    static __device__ __forceinline__ Vec codes(uint32_t a, uint32_t b)
-    {
-        // a byte u of 0x64uu is 1024 + u; u = code ^ 0x80 is code + 128
-        a ^= 0x80808080u;
-        b ^= 0x80808080u;
-        const v4u w{__builtin_amdgcn_perm(0x64646464u, a, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u),
-                    __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)};
-        Vec h;
-        __builtin_memcpy(&h, &w, 16);
-        return h - (_Float16)1152.0f;
-    }
-    template <typename S>
-    static __device__ __forceinline__ void split(const S (&x)[8], Vec (&v)[1])
-    {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            v[0][e] = (_Float16)x[e];
-        }
-    }
-    static __device__ __forceinline__ v4f mfma(Vec a, Vec b, v4f c)
-    {
-#if __HIP_DEVICE_COMPILE__
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-#else
-        (void)a, (void)b;
-        return c;
-#endif
-    }
-};
-
-template <>
-struct Operand<float> {
-    static constexpr int kParts = 3;
-    typedef v8b Vec;
-    // the upper halves of two f32
-    static __device__ __forceinline__ uint32_t uppers(float lo, float hi)
-    {
-        return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
-    }
-    static __device__ __forceinline__ Vec codes(uint32_t a, uint32_t b)
-    {
-        const uint32_t d[2] = {a ^ 0x80808080u, b ^ 0x80808080u};
-        v4u w;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t u = d[i / 2] >> (16 * (i % 2));
-            w[i] = uppers((float)(u & 0xffu) - 128.0f, (float)((u >> 8) & 0xffu) - 128.0f);
-        }
-        Vec h;
-        __builtin_memcpy(&h, &w, 16);
-        return h;
-    }
-    static __device__ __forceinline__ void split(const float (&x)[8], Vec (&v)[3])
-    {
-        float r[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            r[e] = x[e];
-        }
-#pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            const v4u w{uppers(r[0], r[1]), uppers(r[2], r[3]), uppers(r[4], r[5]), uppers(r[6], r[7])};
-            __builtin_memcpy(&v[i], &w, 16);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                r[e] = __fsub_rn(r[e], __uint_as_float(__float_as_uint(r[e]) & 0xffff0000u));
-            }
-        }
-    }
-    static __device__ __forceinline__ v4f mfma(Vec a, Vec b, v4f c)
-    {
-#if __HIP_DEVICE_COMPILE__
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-#else
-        (void)a, (void)b;
-        return c;
-#endif
-    }
-};
-
-// c + a (b's parts)
-template <typename T>
-__device__ __forceinline__ v4f product(typename Operand<T>::Vec a, const typename Operand<T>::Vec (&b)[Operand<T>::kParts],
-                                       v4f c)
-{
-#pragma unroll
-    for (int i = 0; i < Operand<T>::kParts; ++i) {
-        c = Operand<T>::mfma(a, b[i], c);
-    }
-    return c;
-}
+constexpr int kRows = 16;           // rows of a wave
 
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const AttnKern p)
@@ -187,22 +43,15 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
     const Paged& c = p.c;
     const int64_t item = blockIdx.x / (unsigned)c.heads;
     const int kvh = (int)(blockIdx.x - item * c.heads);
-    int b, rt;
-    SeqRows seq;
-    if (p.per_seq > 0) {
-        b = (int)(item / p.per_seq);
-        rt = (int)(item - (int64_t)b * p.per_seq);
-        seq = seq_rows(c, b);
-    } else if (!find_item(c, item, [&](const SeqRows& s) { return (int)(((int64_t)s.n * p.group + kRows - 1) / kRows); },
-                          b, rt, seq)) {
+    RowTile rt;
+    if (!find_tile(p, item, false, rt)) {
         return;
     }
-    const int64_t row0 = (int64_t)rt * kRows, rows = (int64_t)seq.n * p.group;
-    const int tok_first = (int)(row0 / p.group);
-    const int tok_last = (int)(min(row0 + kRows, rows) - 1) / p.group;
-    const int pmin = seq.len - seq.n + tok_first, pmax = seq.len - seq.n + tok_last;
-    const Span span = span_of(pmin, pmax, p.window, p.sinks);
-    const int active = (span.tiles + p.chunk - 1) / p.chunk;
+    const SeqRows& seq = rt.seq;
+    const Span& span = rt.span;
+    const int b = rt.b, pmin = rt.pmin, pmax = rt.pmax, active = rt.active;
+    const int64_t row0 = rt.row0, rows = rt.rows;
+    const int tok_last = pmax - (seq.len - seq.n);
     const int split = blockIdx.y;
     if (split > 0 && split >= active) {
         return;
@@ -236,13 +85,13 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
     for (int t = 0; t < kT; ++t) {
         o[t] = v4f{0, 0, 0, 0};
     }
-    float m_run = -std::numeric_limits<float>::infinity(), l_run = 0.0f;
+    float m_run = kNone, l_run = 0.0f;
     const int64_t page_bytes = (int64_t)c.page * d;
     const int kb = n / 4;                          // the token group of a lane's keys
     const int ktok = 16 * kb + n % 4;              // + 4 t: its token in the tile
 
     for (int v = v0 + wave; v < v1; v += 4) {
-        const int base = kTile * (v < span.sink_tiles ? v : span.first + v - span.sink_tiles);
+        const int base = tile_base(span, v);
         // pages of the lane's key group and value group; past the last
         // position there is none, any page's codes do (they are masked)
         const int kt0 = base + 16 * kb, vt0 = base + 16 * g;
@@ -260,10 +109,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
                 kr[t][i] = 64 * i + 16 * g < d ? *reinterpret_cast<const v4i*>(kp + 4 * t * d + 64 * i) : v4i{0, 0, 0, 0};
             }
         }
-        const bool any = vt0 <= pmax;
-        const float nan = __uint_as_float(0x7fc00000u);
-        const float ks = !any ? 0.0f : vid < 0 ? nan : c.k_scale[vpage];
-        const float vs = !any ? 1.0f : vid < 0 ? nan : c.v_scale[vpage];
+        const Scales sc = vt0 <= pmax ? scales_of(p, vid, vpage) : Scales{0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int t = 0; t < kT; ++t) {
             vr[t] = 16 * t < d ? *reinterpret_cast<const v4i*>(vp + (int64_t)16 * t * c.page) : v4i{0, 0, 0, 0};
@@ -280,20 +126,18 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
             }
         }
 
-        const float vs_eff = vs < kLeastScale ? kLeastScale : vs;
-        const float mul = p.scale_log2 * ks, add = __builtin_amdgcn_logf(vs_eff);
         float x[4][4];
-        float top = -std::numeric_limits<float>::infinity();
+        float top = kNone;
         const bool open = base + kTile - 1 <= pmin && (p.window == 0 || pmax - base < p.window);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float y = __builtin_fmaf(s[t][i], mul, add);
+                float y = __builtin_fmaf(s[t][i], sc.mul, sc.add);
                 if (!open) {
                     const int at = vt0 + 4 * t + i;
                     const bool seen = at <= pos && (p.window == 0 || pos - at < p.window || at < p.sinks);
-                    y = seen ? y : -std::numeric_limits<float>::infinity();
+                    y = seen ? y : kNone;
                 }
                 x[t][i] = y;
                 top = fmaxf(top, y);
@@ -301,18 +145,17 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
         }
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float m_new = fmaxf(m_run, top);
-        if (__any(m_new > m_run)) {
-            // (0 where nothing was seen before, and where nothing is seen yet)
-            const float f = m_new > m_run ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+        if (__any(top > m_run + kLazy)) {
+            // (0 where nothing was seen before)
+            const float f = top > m_run ? __builtin_amdgcn_exp2f(m_run - top) : 1.0f;
             l_run *= f;
 #pragma unroll
             for (int t = 0; t < kT; ++t) {
                 o[t] *= f;
             }
-            m_run = m_new;
+            m_run = fmaxf(m_run, top);
         }
-        const float shift = m_run > -std::numeric_limits<float>::infinity() ? kPShift - m_run : 0.0f;
+        const float shift = m_run > kNone ? kLift - m_run : 0.0f;
         float sum = 0.0f, w[2][8];
         typename Op::Vec pf[2][Op::kParts];
 #pragma unroll
@@ -326,7 +169,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
         Op::split(w[0], pf[0]);
         Op::split(w[1], pf[1]);
         // a page of which the row sees nothing adds nothing, whatever its scale
-        l_run += sum != 0.0f ? sum * (0x1p-14f / vs_eff) : 0.0f;
+        l_run += sum != 0.0f ? sum * sc.inv : 0.0f;
 #pragma unroll
         for (int t = 0; t < kT; ++t) {
             if (16 * t < d) {
@@ -374,7 +217,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
             }
         } else {
             static_cast<T*>(p.out)[token * p.ld_out + (int64_t)qh * d + ch] =
-                (T)(l == 0.0f ? 0.0f : sum * 0x1p-14f / l);
+                (T)(l == 0.0f ? 0.0f : sum * kDrop / l);
         }
     }
 }
@@ -406,18 +249,17 @@ __global__ __launch_bounds__(256) void attention_join(const AttnKern p)
     if (tok < 0 || tok >= seq.n) {
         return;
     }
-    const int64_t rows = (int64_t)seq.n * p.group;
-    const int64_t row0 = ((int64_t)tok * p.group + qh % p.group) / kRows * kRows;
-    const int pmin = seq.len - seq.n + (int)(row0 / p.group);
-    const int pmax = seq.len - seq.n + (int)((min(row0 + kRows, rows) - 1) / p.group);
-    const int active = (span_of(pmin, pmax, p.window, p.sinks).tiles + p.chunk - 1) / p.chunk;
+    RowTile rt;
+    rt.seq = seq;
+    place_tile(p, (int)(((int64_t)tok * p.group + qh % p.group) / p.tile_rows), rt);
+    const int active = rt.active;
     if (active <= 1) {
         return;
     }
     const int d = c.d;
     const int64_t step = (int64_t)c.rows * p.q_heads * (d + 2);
     const float* part = p.part + (token * p.q_heads + qh) * (d + 2);
-    float m = -std::numeric_limits<float>::infinity();
+    float m = kNone;
     for (int s = 0; s < active; ++s) {
         m = fmaxf(m, part[s * step + d]);
     }
@@ -437,36 +279,44 @@ __global__ __launch_bounds__(256) void attention_join(const AttnKern p)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         if (lane + 64 * e < d) {
-            out[lane + 64 * e] = (T)(l == 0.0f ? 0.0f : o[e] * 0x1p-14f / l);
+            out[lane + 64 * e] = (T)(l == 0.0f ? 0.0f : o[e] * kDrop / l);
         }
     }
 }
 
 struct AttnPlan {
     int64_t items;        // row tiles, all KV heads
-    int32_t per_seq, chunk, splits;
+    int32_t tile_rows, per_seq, chunk, splits;
+    bool tiled;           // attention_rows_tiled, else attention_rows16
     size_t workspace;
 };
 
-// Splits of the longest sequence that the page table has room for: enough
-// workgroups to fill the chip twice, no fewer than 4 tiles each (one per wave).
+// Rows of a sequence past kRows go to the kernel whose waves share their tiles
+// (ragged calls: by their mean). Splits of the longest sequence that the page
+// table has room for: enough workgroups to fill the chip, no fewer than 4 tiles
+// each.
 AttnPlan attn_plan(const NnopsCacheAttentionArgs* g)
 {
     AttnPlan a{};
     const int64_t group = g->q_heads / g->cache.heads, b = g->cache.sequences;
+    const int64_t mean = (g->rows * group + b - 1) / b;
+    const int tiled = mean > kRows ? tiled_rows(g->cache.head_dim, g->f16, mean) : 0;
+    a.tiled = tiled > 0;
+    a.tile_rows = a.tiled ? tiled : kRows;
     if (g->cache.row_starts == nullptr) {
-        a.per_seq = (int32_t)((g->rows / b * group + kRows - 1) / kRows);
+        a.per_seq = (int32_t)((g->rows / b * group + a.tile_rows - 1) / a.tile_rows);
         a.items = b * a.per_seq * g->cache.heads;
     } else {
-        a.items = (g->rows * group / kRows + (b < g->rows ? b : g->rows)) * g->cache.heads;
+        a.items = (g->rows * group / a.tile_rows + (b < g->rows ? b : g->rows)) * g->cache.heads;
     }
     int64_t tiles = (g->cache.table_pages * g->cache.page_tokens + kTile - 1) / kTile;
     if (g->window > 0) {
-        // a tile's rows see the window, up to 15 tokens more, and the sinks
-        const int64_t seen = (g->window + kRows) / kTile + 2 + (g->sinks + kTile - 1) / kTile;
+        // a tile's rows see the window, up to tile_rows - 1 tokens more, and the sinks
+        const int64_t seen = (g->window + a.tile_rows) / kTile + 2 + (g->sinks + kTile - 1) / kTile;
         tiles = tiles < seen ? tiles : seen;
     }
-    int64_t splits = (512 + a.items - 1) / a.items;
+    const int64_t full = a.tiled ? 256 : 512;
+    int64_t splits = (full + a.items - 1) / a.items;
     const int64_t most = (tiles + 3) / 4;
     splits = splits < most ? splits : most;
     splits = splits > 1 ? splits : 1;
@@ -499,7 +349,9 @@ template <typename T>
 void launch_attention(const AttnKern& k, const AttnPlan& a, hipStream_t s)
 {
     const dim3 grid((unsigned)a.items, (unsigned)a.splits);
-    if (k.c.d <= 64) {
+    if (a.tiled) {
+        launch_tiled(k, grid, sizeof(T) == 2, s);
+    } else if (k.c.d <= 64) {
         NNOPS_LAUNCH((attention_rows16<T, 64>), grid, dim3(256), 0, s, k);
     } else if (k.c.d <= 128) {
         NNOPS_LAUNCH((attention_rows16<T, 128>), grid, dim3(256), 0, s, k);
@@ -541,7 +393,7 @@ extern "C" int nnops_hip_cache_attention(const NnopsCacheAttentionArgs* g, void*
         return NNOPS_INVALID_ARGUMENT;
     }
     const AttnPlan a = attn_plan(g);
-    if (a.items > INT32_MAX / 256 || a.splits > 65535) {
+    if (a.items > INT32_MAX / 512 || a.splits > 65535) {
         return NNOPS_UNSUPPORTED;
     }
     if (a.workspace > 0 && (workspace == nullptr || workspace_bytes < a.workspace || (uintptr_t)workspace % 16 != 0)) {
@@ -560,6 +412,7 @@ extern "C" int nnops_hip_cache_attention(const NnopsCacheAttentionArgs* g, void*
     k.group = (int32_t)(g->q_heads / g->cache.heads);
     k.window = g->window > INT32_MAX ? 0 : (int32_t)g->window;   // longer than any sequence: none
     k.sinks = g->sinks > INT32_MAX ? INT32_MAX : (int32_t)g->sinks;
+    k.tile_rows = a.tile_rows;
     k.per_seq = a.per_seq;
     k.chunk = a.chunk;
     hipStream_t s = static_cast<hipStream_t>(stream);

@@ -1,0 +1,255 @@
+// What the kernels of attention over the paged cache share: their parameters,
+// which tokens a tile of rows looks at, and the operands of the two products.
+#pragma once
+
+#include <limits>
+
+#include "paged.hpp"
+
+namespace nnops_amd {
+
+constexpr int kTile = 64;           // tokens of a step
+
+// Weights are 2^(x - M + kLift) for a reference M that is the running maximum,
+// or up to kLazy below it: O and l are brought to a new reference only when the
+// maximum has passed the old one by more, which is rare after the first tiles.
+// The largest weight is then 2^14, and f16's range ends 2^-30 below the maximum.
+constexpr float kLift = 6.0f, kLazy = 8.0f;
+constexpr float kDrop = 0x1p-6f;    // 2^-kLift
+
+constexpr float kNone = -std::numeric_limits<float>::infinity();
+
+struct AttnKern {
+    Paged c;
+    const void* q;
+    void* out;
+    int64_t ld_q, ld_out;
+    float* part;          // [splits][rows][q_heads][d + 2]: O, M, l
+    float scale_log2;
+    int32_t q_heads, group, window, sinks;
+    int32_t tile_rows;    // rows (tokens x heads of a group) of a workgroup
+    int32_t per_seq;      // row tiles of a sequence, equal rows each (0: found by search)
+    int32_t chunk;        // tiles of 64 tokens that a split takes
+};
+
+// The tiles of 64 tokens that rows at positions pmin .. pmax look at: the
+// first `sink_tiles`, then those from `first` on, `tiles` in all.
+struct Span {
+    int sink_tiles, first, tiles;
+};
+
+__host__ __device__ __forceinline__ Span span_of(int pmin, int pmax, int window, int sinks)
+{
+    Span s{0, 0, pmax < 0 ? 0 : pmax / kTile + 1};
+    if (window > 0 && pmax >= 0) {
+        const int lo = (pmin > window - 1 ? pmin - window + 1 : 0) / kTile;
+        const int kept = sinks < pmax + 1 ? sinks : pmax + 1;
+        const int st = (kept + kTile - 1) / kTile;
+        if (st < lo) {
+            s.sink_tiles = st;
+            s.first = lo;
+            s.tiles += st - lo;
+        }
+    }
+    return s;
+}
+
+__device__ __forceinline__ int tile_base(const Span& s, int v)
+{
+    return kTile * (v < s.sink_tiles ? v : s.first + v - s.sink_tiles);
+}
+
+// A tile of rows of one sequence: row r is head r % group of token r / group
+// among the sequence's rows.
+struct RowTile {
+    int b;
+    SeqRows seq;
+    int64_t row0, rows;       // first row; rows of the sequence
+    int pmin, pmax;           // positions of the first and the last row
+    Span span;
+    int active;               // splits that have tiles
+};
+
+__device__ __forceinline__ void place_tile(const AttnKern& p, int rt, RowTile& t)
+{
+    t.row0 = (int64_t)rt * p.tile_rows;
+    t.rows = (int64_t)t.seq.n * p.group;
+    const int64_t last = (t.row0 + p.tile_rows < t.rows ? t.row0 + p.tile_rows : t.rows) - 1;
+    t.pmin = t.seq.len - t.seq.n + (int)(t.row0 / p.group);
+    t.pmax = t.seq.len - t.seq.n + (int)(last / p.group);
+    t.span = span_of(t.pmin, t.pmax, p.window, p.sinks);
+    t.active = (t.span.tiles + p.chunk - 1) / p.chunk;
+}
+
+// The item-th tile. Later tiles of a sequence look at more tokens: `from_last`
+// numbers them from the last, so that the longest work begins first.
+__device__ __forceinline__ bool find_tile(const AttnKern& p, int64_t item, bool from_last, RowTile& t)
+{
+    int rt;
+    if (p.per_seq > 0) {
+        if (from_last) {
+            const int back = (int)(item / p.c.seqs);
+            t.b = (int)(item - (int64_t)back * p.c.seqs);
+            rt = p.per_seq - 1 - back;
+        } else {
+            t.b = (int)(item / p.per_seq);
+            rt = (int)(item - (int64_t)t.b * p.per_seq);
+        }
+        t.seq = seq_rows(p.c, t.b);
+    } else {
+        const auto count = [&](const SeqRows& s) {
+            return (int)(((int64_t)s.n * p.group + p.tile_rows - 1) / p.tile_rows);
+        };
+        if (!find_item(p.c, item, count, t.b, rt, t.seq)) {
+            return false;
+        }
+        rt = from_last ? count(t.seq) - 1 - rt : rt;
+    }
+    place_tile(p, rt, t);
+    return true;
+}
+
+// A page's scales as the softmax takes them: x = s mul + add, l += w inv.
+struct Scales {
+    float mul, add, inv;
+};
+
+__device__ __forceinline__ Scales scales_of(const AttnKern& p, int page, int64_t at)
+{
+    const float nan = __uint_as_float(0x7fc00000u);
+    const float ks = page < 0 ? nan : p.c.k_scale[at], vs = page < 0 ? nan : p.c.v_scale[at];
+    // (codes of a page whose scale is less count for nothing beside any other)
+    const float v = vs < kLeastScale ? kLeastScale : vs;
+    return Scales{p.scale_log2 * ks, __builtin_amdgcn_logf(v), kDrop / v};
+}
+
+// The operands of the two products, by the rows' type.
+//   f16: the rows as they are, the probabilities rounded to f16, codes as f16.
+//   f32: each value as three bf16 parts that hold it exactly (8 bits each, by
+//        truncation, the last difference having no more), codes as bf16 (7 bits
+//        and a sign: exact), three products into one f32 accumulator. Two f16
+//        parts would be one product fewer, but their range ends 2^-38 below the
+//        largest probability.
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+
+template <typename T>
+struct Operand {
+    static constexpr int kParts = 1;
+    typedef v8h Vec;
+    static __device__ __forceinline__ Vec codes(uint32_t a, uint32_t b)
+    {
+        // a byte u of 0x64uu is 1024 + u; u = code ^ 0x80 is code + 128
+        a ^= 0x80808080u;
+        b ^= 0x80808080u;
+        const v4u w{__builtin_amdgcn_perm(0x64646464u, a, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u),
+                    __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)};
+        Vec h;
+        __builtin_memcpy(&h, &w, 16);
+        return h - (_Float16)1152.0f;
+    }
+    template <typename S>
+    static __device__ __forceinline__ void split(const S (&x)[8], Vec (&v)[1])
+    {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            v[0][e] = (_Float16)x[e];   // (in pairs: v_cvt_pk_f16_f32, to nearest)
+        }
+    }
+    static __device__ __forceinline__ v4f mfma(Vec a, Vec b, v4f c)
+    {
+#if __HIP_DEVICE_COMPILE__
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+#else
+        (void)a, (void)b;
+        return c;
+#endif
+    }
+    static __device__ __forceinline__ v16f mfma(Vec a, Vec b, v16f c)
+    {
+#if __HIP_DEVICE_COMPILE__
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+#else
+        (void)a, (void)b;
+        return c;
+#endif
+    }
+};
+
+template <>
+struct Operand<float> {
+    static constexpr int kParts = 3;
+    typedef v8b Vec;
+    // the upper halves of two f32
+    static __device__ __forceinline__ uint32_t uppers(float lo, float hi)
+    {
+        return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+    }
+    static __device__ __forceinline__ Vec codes(uint32_t a, uint32_t b)
+    {
+        const uint32_t d[2] = {a ^ 0x80808080u, b ^ 0x80808080u};
+        v4u w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t u = d[i / 2] >> (16 * (i % 2));
+            w[i] = uppers((float)(u & 0xffu) - 128.0f, (float)((u >> 8) & 0xffu) - 128.0f);
+        }
+        Vec h;
+        __builtin_memcpy(&h, &w, 16);
+        return h;
+    }
+    static __device__ __forceinline__ void split(const float (&x)[8], Vec (&v)[3])
+    {
+        float r[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            r[e] = x[e];
+        }
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            const v4u w{uppers(r[0], r[1]), uppers(r[2], r[3]), uppers(r[4], r[5]), uppers(r[6], r[7])};
+            __builtin_memcpy(&v[i], &w, 16);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                r[e] = __fsub_rn(r[e], __uint_as_float(__float_as_uint(r[e]) & 0xffff0000u));
+            }
+        }
+    }
+    static __device__ __forceinline__ v4f mfma(Vec a, Vec b, v4f c)
+    {
+#if __HIP_DEVICE_COMPILE__
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+#else
+        (void)a, (void)b;
+        return c;
+#endif
+    }
+    static __device__ __forceinline__ v16f mfma(Vec a, Vec b, v16f c)
+    {
+#if __HIP_DEVICE_COMPILE__
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+#else
+        (void)a, (void)b;
+        return c;
+#endif
+    }
+};
+
+// c + a (b's parts)
+template <typename T, typename Acc>
+__device__ __forceinline__ Acc product(typename Operand<T>::Vec a, const typename Operand<T>::Vec (&b)[Operand<T>::kParts],
+                                       Acc c)
+{
+#pragma unroll
+    for (int i = 0; i < Operand<T>::kParts; ++i) {
+        c = Operand<T>::mfma(a, b[i], c);
+    }
+    return c;
+}
+
+// attention_rows_tiled's launch (cache_attention_tiled.hip): d, type and rows
+// of a workgroup that it has a kernel for.
+int tiled_rows(int64_t d, bool f16, int64_t rows);
+void launch_tiled(const AttnKern& k, const dim3& grid, bool f16, hipStream_t s);
+
+}  // namespace nnops_amd
