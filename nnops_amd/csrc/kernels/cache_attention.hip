@@ -24,6 +24,7 @@
 // Bound: HBM for few rows, the codes read once per KV head. Long sequences are
 // split over workgroups (partial O, M, l in the workspace, joined by a second
 // kernel); a workgroup's 4 waves take every fourth tile and join in LDS.
+#include <cstdlib>
 #include "cache_attention.hpp"
 
 namespace nnops_amd {
@@ -32,7 +33,7 @@ namespace {
 constexpr int kRows = 16;           // rows of a wave
 
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const AttnKern p)
+__global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 ? 3 : 2) : 1) void attention_rows16(const AttnKern p)
 {
     constexpr int kC = DP / 64;                    // 64-channel pieces of a key
     constexpr int kT = DP / 16;                    // 16-channel tiles of O
@@ -41,7 +42,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
     __shared__ float s_o[4][kRows][kPitch];
     __shared__ float s_m[4][kRows], s_l[4][kRows];
     const Paged& c = p.c;
-    const int64_t item = blockIdx.x / (unsigned)c.heads;
+    const uint32_t item = blockIdx.x / (uint32_t)c.heads;
     const int kvh = (int)(blockIdx.x - item * c.heads);
     RowTile rt;
     if (!find_tile(p, item, false, rt)) {
@@ -50,7 +51,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
     const SeqRows& seq = rt.seq;
     const Span& span = rt.span;
     const int b = rt.b, pmin = rt.pmin, pmax = rt.pmax, active = rt.active;
-    const int64_t row0 = rt.row0, rows = rt.rows;
+    const int row0 = rt.row0, rows = rt.rows;
     const int tok_last = pmax - (seq.len - seq.n);
     const int split = blockIdx.y;
     if (split > 0 && split >= active) {
@@ -58,12 +59,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
     }
     const int v0 = split * p.chunk, v1 = min(span.tiles, v0 + p.chunk);
 
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int n = lane % 16, g = lane / 16;
-    const int64_t row = row0 + n;
+    const int row = row0 + n;
     const bool is_row = row < rows;
-    const int tok = is_row ? (int)(row / p.group) : tok_last;
-    const int head = kvh * p.group + (is_row ? (int)(row - (int64_t)tok * p.group) : 0);
+    const int tok = is_row ? (int)((uint32_t)row / (uint32_t)p.group) : tok_last;
+    const int head = kvh * p.group + (is_row ? row - tok * p.group : 0);
     const int pos = seq.len - seq.n + tok;
     const int d = c.d;
 
@@ -90,29 +91,54 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
     const int kb = n / 4;                          // the token group of a lane's keys
     const int ktok = 16 * kb + n % 4;              // + 4 t: its token in the tile
 
-    for (int v = v0 + wave; v < v1; v += 4) {
+    // The codes of a wave's next tile are in flight while it works on this one:
+    // its keys from the scores on, its values from the second product on, its
+    // page numbers a tile earlier still.
+    const int32_t* table = c.table + (int64_t)b * c.ld_table;
+    const int64_t page_step = page_bytes * c.heads;
+    const int8_t* k_at = c.k + kvh * page_bytes + 16 * g;
+    const int8_t* v_at = c.v + kvh * page_bytes + n * c.page;
+    v4i kr[4][kC], vr[kT];
+    int kid, vid;
+    PageScales scale_next{0.0f, 0.0f, 0.0f};
+    // (a group past the last position has the last page's codes: they are masked)
+    // (page numbers as they lie in the table: looked at when they are used)
+    const auto ids = [&](int v) {
         const int base = tile_base(span, v);
-        // pages of the lane's key group and value group; past the last
-        // position there is none, any page's codes do (they are masked)
-        const int kt0 = base + 16 * kb, vt0 = base + 16 * g;
-        const int kid = kt0 <= pmax ? page_of(c, b, kt0 >> c.page_log2) : 0;
-        const int vid = vt0 <= pmax ? page_of(c, b, vt0 >> c.page_log2) : 0;
-        const int8_t* kp = c.k + ((int64_t)max(kid, 0) * c.heads + kvh) * page_bytes +
-                           (int64_t)((base + ktok) & (c.page - 1)) * d + 16 * g;
-        const int64_t vpage = (int64_t)max(vid, 0) * c.heads + kvh;
-        const int8_t* vp = c.v + vpage * page_bytes + (int64_t)n * c.page + (vt0 & (c.page - 1));
-        v4i kr[4][kC], vr[kT];
+        kid = table[min(base + 16 * kb, pmax) >> c.page_log2];
+        vid = table[min(base + 16 * g, pmax) >> c.page_log2];
+    };
+    const auto load_k = [&](int v) {
+        const int base = tile_base(span, v);
+        const int8_t* at = k_at + readable(c, kid) * page_step + ((base + ktok) & (c.page - 1)) * d;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
             for (int i = 0; i < kC; ++i) {
-                kr[t][i] = 64 * i + 16 * g < d ? *reinterpret_cast<const v4i*>(kp + 4 * t * d + 64 * i) : v4i{0, 0, 0, 0};
+                kr[t][i] = 64 * i + 16 * g < d ? *reinterpret_cast<const v4i*>(at + 4 * t * d + 64 * i) : v4i{0, 0, 0, 0};
             }
         }
-        const Scales sc = vt0 <= pmax ? scales_of(p, vid, vpage) : Scales{0.0f, 0.0f, 0.0f};
+        scale_next = page_scales(c, vid, kvh);
+    };
+    const auto load_v = [&](int v) {
+        const int base = tile_base(span, v);
+        const int8_t* at = v_at + readable(c, vid) * page_step + ((base + 16 * g) & (c.page - 1));
 #pragma unroll
         for (int t = 0; t < kT; ++t) {
-            vr[t] = 16 * t < d ? *reinterpret_cast<const v4i*>(vp + (int64_t)16 * t * c.page) : v4i{0, 0, 0, 0};
+            vr[t] = 16 * t < d ? *reinterpret_cast<const v4i*>(at + 16 * t * c.page) : v4i{0, 0, 0, 0};
+        }
+    };
+    if (v0 + wave < v1) {
+        ids(v0 + wave);
+        load_k(v0 + wave);
+        load_v(v0 + wave);
+    }
+    for (int v = v0 + wave; v < v1; v += 4) {
+        const int base = tile_base(span, v), vt0 = base + 16 * g;
+        const bool more = v + 4 < v1;
+        const PageScales scale = scale_next;
+        if (more) {
+            ids(v + 4);
         }
 
         v4f s[4];
@@ -124,6 +150,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
                 s[t] = product<T>(Op::codes((uint32_t)kr[t][i].x, (uint32_t)kr[t][i].y), qf[2 * i], s[t]);
                 s[t] = product<T>(Op::codes((uint32_t)kr[t][i].z, (uint32_t)kr[t][i].w), qf[2 * i + 1], s[t]);
             }
+        }
+
+        const Scales sc = softmax_scales(p, scale);
+        if (more) {
+            load_k(v + 4);
         }
 
         float x[4][4];
@@ -177,6 +208,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
                 o[t] = product<T>(Op::codes((uint32_t)vr[t].z, (uint32_t)vr[t].w), pf[1], o[t]);
             }
         }
+        if (more) {
+            load_v(v + 4);
+        }
     }
 
     // the waves' parts, brought to one maximum and summed
@@ -191,51 +225,60 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
         *reinterpret_cast<v4f*>(&s_o[wave][n][16 * t + 4 * g]) = o[t];
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < kRows * d; i += 256) {
-        const int r = i / d, ch = i - r * d;
-        if (row0 + r >= rows) {
+    // 16 threads a row, 4 channels each at a time
+    const int r = threadIdx.x / 16, ch0 = threadIdx.x % 16 * 4;
+    if (row0 + r >= rows) {
+        return;
+    }
+    const float m = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+    float f[4], l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        // a wave that saw nothing has m = -inf and nothing to add
+        f[w] = s_m[w][r] < m ? __builtin_amdgcn_exp2f(s_m[w][r] - m) : 1.0f;
+        l += f[w] * s_l[w][r];
+    }
+    const int rtok = (int)((uint32_t)(row0 + r) / (uint32_t)p.group);
+    const int64_t token = seq.start + rtok;
+    const int qh = kvh * p.group + (row0 + r - rtok * p.group);
+    const int64_t at_part = ((int64_t)split * c.rows + token) * p.q_heads + qh;
+    const float scale = active > 1 ? 1.0f : l == 0.0f ? 0.0f : kDrop / l;
+#pragma unroll
+    for (int i = 0; i < DP / 64; ++i) {
+        const int ch = ch0 + 64 * i;
+        if (ch >= d) {
             break;
         }
-        const float m = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-        float sum = 0.0f, l = 0.0f;
+        v4f sum = v4f{0, 0, 0, 0};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            // a wave that saw nothing has m = -inf and nothing to add
-            const float f = s_m[w][r] < m ? __builtin_amdgcn_exp2f(s_m[w][r] - m) : 1.0f;
-            sum += f * s_o[w][r][ch];
-            l += f * s_l[w][r];
+            sum += f[w] * *reinterpret_cast<const v4f*>(&s_o[w][r][ch]);
         }
-        const int64_t at = row0 + r;
-        const int64_t token = seq.start + at / p.group;
-        const int qh = kvh * p.group + (int)(at % p.group);
         if (active > 1) {
-            float* dst = p.part + (((int64_t)split * c.rows + token) * p.q_heads + qh) * (d + 2);
-            dst[ch] = sum;
-            if (ch == 0) {
-                dst[d] = m;
-                dst[d + 1] = l;
-            }
+            *reinterpret_cast<v4f*>(&p.part[at_part * d + ch]) = sum;
         } else {
-            static_cast<T*>(p.out)[token * p.ld_out + (int64_t)qh * d + ch] =
-                (T)(l == 0.0f ? 0.0f : sum * kDrop / l);
+            T y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                y[e] = (T)(sum[e] * scale);
+            }
+            __builtin_memcpy(static_cast<T*>(p.out) + token * p.ld_out + (int64_t)qh * d + ch, y, sizeof y);
         }
+    }
+    if (active > 1 && ch0 == 0) {
+        p.part_ml[2 * at_part] = m;
+        p.part_ml[2 * at_part + 1] = l;
     }
 }
 
-// Joins the splits of the rows that have more than one. A wave per row.
-template <typename T>
-__global__ __launch_bounds__(256) void attention_join(const AttnKern p)
+// The splits of a row that have something: 0 or 1 where there is nothing to
+// join (or the row is no sequence's).
+__device__ __forceinline__ int splits_of(const AttnKern& p, int token, int qh)
 {
     const Paged& c = p.c;
-    const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
-    const int64_t token = i / p.q_heads;
-    if (token >= c.rows) {
-        return;
-    }
-    const int qh = (int)(i - token * p.q_heads), lane = threadIdx.x % 64;
     int b;
     if (c.row_starts == nullptr) {
-        b = (int)(token / c.uniform);
+        b = (int)((uint32_t)token / (uint32_t)c.uniform);
     } else {
         int lo = 0, hi = c.seqs;                   // the last sequence that starts at or before the row
         while (hi - lo > 1) {
@@ -244,43 +287,138 @@ __global__ __launch_bounds__(256) void attention_join(const AttnKern p)
         }
         b = lo;
     }
-    const SeqRows seq = seq_rows(c, b);
-    const int tok = (int)(token - seq.start);
-    if (tok < 0 || tok >= seq.n) {
+    RowTile rt;
+    rt.seq = seq_rows(c, b);
+    const int tok = token - rt.seq.start;
+    if (tok < 0 || tok >= rt.seq.n) {
+        return 0;
+    }
+    const uint32_t row = (uint32_t)(tok * p.group) + (uint32_t)qh % (uint32_t)p.group;
+    place_tile(p, (int)(row / (uint32_t)p.tile_rows), rt);
+    return rt.active;
+}
+
+// Joins the splits of the rows that have more than one. Few splits: a wave per
+// row, 4 channels a lane.
+constexpr int kFewSplits = 8;
+
+template <typename T>
+__global__ __launch_bounds__(256) void attention_join_few(const AttnKern p)
+{
+    const uint32_t i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int token = (int)(i / (uint32_t)p.q_heads), qh = (int)(i - (uint32_t)token * p.q_heads);
+    if (token >= p.c.rows) {
         return;
     }
-    RowTile rt;
-    rt.seq = seq;
-    place_tile(p, (int)(((int64_t)tok * p.group + qh % p.group) / p.tile_rows), rt);
-    const int active = rt.active;
+    const int active = splits_of(p, token, qh);
+    const int d = p.c.d, ch = threadIdx.x % 64 * 4;
+    if (active <= 1 || ch >= d) {
+        return;
+    }
+    const int64_t rows = (int64_t)p.c.rows * p.q_heads, at = (int64_t)token * p.q_heads + qh;
+    float ms[kFewSplits], ls[kFewSplits], m = kNone, l = 0.0f;
+    v4f os[kFewSplits], o = v4f{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < kFewSplits; ++s) {
+        if (s < active) {
+            ms[s] = p.part_ml[2 * (s * rows + at)];
+            ls[s] = p.part_ml[2 * (s * rows + at) + 1];
+            os[s] = *reinterpret_cast<const v4f*>(p.part + (s * rows + at) * d + ch);
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < kFewSplits; ++s) {
+        m = s < active ? fmaxf(m, ms[s]) : m;
+    }
+#pragma unroll
+    for (int s = 0; s < kFewSplits; ++s) {
+        if (s < active) {
+            const float w = ms[s] < m ? __builtin_amdgcn_exp2f(ms[s] - m) : 1.0f;
+            l += w * ls[s];
+            o += w * os[s];
+        }
+    }
+    const float f = l == 0.0f ? 0.0f : kDrop / l;
+    T y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        y[e] = (T)(o[e] * f);
+    }
+    __builtin_memcpy(static_cast<T*>(p.out) + token * p.ld_out + (int64_t)qh * d + ch, y, sizeof y);
+}
+
+// Many: a workgroup per row, its weights 2^(M - max) in LDS, every 8th split by
+// 32 lanes of 4 channels.
+constexpr int kMostSplits = 512;
+
+template <typename T>
+__global__ __launch_bounds__(256) void attention_join(const AttnKern p)
+{
+    __shared__ float s_w[kMostSplits];
+    __shared__ float s_red[8];
+    __shared__ __attribute__((aligned(16))) float s_o[8][256];
+    const Paged& c = p.c;
+    const int token = (int)(blockIdx.x / (uint32_t)p.q_heads), tid = threadIdx.x;
+    const int qh = (int)(blockIdx.x - (uint32_t)token * p.q_heads);
+    const int active = splits_of(p, token, qh);
     if (active <= 1) {
         return;
     }
     const int d = c.d;
-    const int64_t step = (int64_t)c.rows * p.q_heads * (d + 2);
-    const float* part = p.part + (token * p.q_heads + qh) * (d + 2);
+    const int64_t rows = (int64_t)c.rows * p.q_heads, at = (int64_t)token * p.q_heads + qh;
     float m = kNone;
-    for (int s = 0; s < active; ++s) {
-        m = fmaxf(m, part[s * step + d]);
+    for (int s = tid; s < active; s += 256) {
+        s_w[s] = p.part_ml[2 * (s * rows + at)];
+        m = fmaxf(m, s_w[s]);
     }
-    float l = 0.0f, o[4] = {0, 0, 0, 0};
-    for (int s = 0; s < active; ++s) {
-        const float ms = part[s * step + d];
-        const float f = ms < m ? __builtin_amdgcn_exp2f(ms - m) : 1.0f;
-        l += f * part[s * step + d + 1];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (lane + 64 * e < d) {
-                o[e] += f * part[s * step + lane + 64 * e];
+    for (int i = 1; i < 64; i *= 2) {
+        m = fmaxf(m, __shfl_xor(m, i));
+    }
+    if (tid % 64 == 0) {
+        s_red[tid / 64] = m;
+    }
+    __syncthreads();
+    m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+    float l = 0.0f;
+    for (int s = tid; s < active; s += 256) {
+        const float w = s_w[s] < m ? __builtin_amdgcn_exp2f(s_w[s] - m) : 1.0f;
+        s_w[s] = w;
+        l += w * p.part_ml[2 * (s * rows + at) + 1];
+    }
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) {
+        l += __shfl_xor(l, i);
+    }
+    if (tid % 64 == 0) {
+        s_red[4 + tid / 64] = l;
+    }
+    __syncthreads();
+    l = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
+    const int g = tid / 32, i = tid % 32;
+    v4f o[2] = {v4f{0, 0, 0, 0}, v4f{0, 0, 0, 0}};
+#pragma unroll 4
+    for (int s = g; s < active; s += 8) {
+        const float* src = p.part + (s * rows + at) * d;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (4 * i + 128 * h < d) {
+                o[h] += s_w[s] * *reinterpret_cast<const v4f*>(src + 4 * i + 128 * h);
             }
         }
     }
-    T* out = static_cast<T*>(p.out) + token * p.ld_out + (int64_t)qh * d;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if (lane + 64 * e < d) {
-            out[lane + 64 * e] = (T)(l == 0.0f ? 0.0f : o[e] * kDrop / l);
+    for (int h = 0; h < 2; ++h) {
+        *reinterpret_cast<v4f*>(&s_o[g][4 * i + 128 * h]) = o[h];
+    }
+    __syncthreads();
+    if (tid < d) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            sum += s_o[e][tid];
         }
+        static_cast<T*>(p.out)[token * p.ld_out + (int64_t)qh * d + tid] = (T)(l == 0.0f ? 0.0f : sum * kDrop / l);
     }
 }
 
@@ -315,9 +453,10 @@ AttnPlan attn_plan(const NnopsCacheAttentionArgs* g)
         const int64_t seen = (g->window + a.tile_rows) / kTile + 2 + (g->sinks + kTile - 1) / kTile;
         tiles = tiles < seen ? tiles : seen;
     }
-    const int64_t full = a.tiled ? 256 : 512;
+    static const int ev=getenv("NN_FULL")?atoi(getenv("NN_FULL")):512, em=getenv("NN_MIN")?atoi(getenv("NN_MIN")):4, et=getenv("NN_TFULL")?atoi(getenv("NN_TFULL")):256;
+    const int64_t full = a.tiled ? et : ev;
     int64_t splits = (full + a.items - 1) / a.items;
-    const int64_t most = (tiles + 3) / 4;
+    const int64_t mn = a.tiled ? 4 : em; const int64_t most = (tiles + mn - 1) / mn;
     splits = splits < most ? splits : most;
     splits = splits > 1 ? splits : 1;
     const int64_t chunk = ((tiles + splits - 1) / splits + 3) / 4 * 4;
@@ -339,7 +478,7 @@ int check_attention(const NnopsCacheAttentionArgs* g)
     if (g->q_heads == 0 || g->q_heads % g->cache.heads != 0 || g->cache.pages == 0) {
         return NNOPS_INVALID_ARGUMENT;
     }
-    if (g->q_heads > (1 << 16) || g->rows * g->q_heads > INT32_MAX) {
+    if (g->q_heads > (1 << 16) || g->rows * g->q_heads > INT32_MAX / 256) {
         return NNOPS_UNSUPPORTED;
     }
     return -1;
@@ -358,9 +497,10 @@ void launch_attention(const AttnKern& k, const AttnPlan& a, hipStream_t s)
     } else {
         NNOPS_LAUNCH((attention_rows16<T, 256>), grid, dim3(256), 0, s, k);
     }
-    if (a.splits > 1) {
-        const int64_t rows = (int64_t)k.c.rows * k.q_heads;
-        NNOPS_LAUNCH(attention_join<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, k);
+    if (a.splits > 1 && a.splits <= kFewSplits) {
+        NNOPS_LAUNCH(attention_join_few<T>, dim3((unsigned)((k.c.rows * k.q_heads + 3) / 4)), dim3(256), 0, s, k);
+    } else if (a.splits > 1) {
+        NNOPS_LAUNCH(attention_join<T>, dim3((unsigned)(k.c.rows * k.q_heads)), dim3(256), 0, s, k);
     }
 }
 
@@ -406,6 +546,7 @@ extern "C" int nnops_hip_cache_attention(const NnopsCacheAttentionArgs* g, void*
     k.ld_q = g->ld_q;
     k.ld_out = g->ld_out;
     k.part = static_cast<float*>(workspace);
+    k.part_ml = k.part + (size_t)a.splits * g->rows * g->q_heads * g->cache.head_dim;
     const float scale = g->scale > 0.0f ? g->scale : 1.0f / __builtin_sqrtf((float)g->cache.head_dim);
     k.scale_log2 = scale * 1.4426950408889634f;
     k.q_heads = (int32_t)g->q_heads;

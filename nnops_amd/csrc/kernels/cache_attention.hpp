@@ -24,7 +24,8 @@ struct AttnKern {
     const void* q;
     void* out;
     int64_t ld_q, ld_out;
-    float* part;          // [splits][rows][q_heads][d + 2]: O, M, l
+    float* part;          // partial O [splits][rows][q_heads][d]
+    float* part_ml;       // their M and l [splits][rows][q_heads][2]
     float scale_log2;
     int32_t q_heads, group, window, sinks;
     int32_t tile_rows;    // rows (tokens x heads of a group) of a workgroup
@@ -64,7 +65,7 @@ __device__ __forceinline__ int tile_base(const Span& s, int v)
 struct RowTile {
     int b;
     SeqRows seq;
-    int64_t row0, rows;       // first row; rows of the sequence
+    int row0, rows;           // first row; rows of the sequence (entry: rows x heads fit 31 bits)
     int pmin, pmax;           // positions of the first and the last row
     Span span;
     int active;               // splits that have tiles
@@ -72,33 +73,34 @@ struct RowTile {
 
 __device__ __forceinline__ void place_tile(const AttnKern& p, int rt, RowTile& t)
 {
-    t.row0 = (int64_t)rt * p.tile_rows;
-    t.rows = (int64_t)t.seq.n * p.group;
-    const int64_t last = (t.row0 + p.tile_rows < t.rows ? t.row0 + p.tile_rows : t.rows) - 1;
-    t.pmin = t.seq.len - t.seq.n + (int)(t.row0 / p.group);
-    t.pmax = t.seq.len - t.seq.n + (int)(last / p.group);
+    const uint32_t group = p.group;
+    t.row0 = rt * p.tile_rows;
+    t.rows = t.seq.n * p.group;
+    const uint32_t last = min(t.row0 + p.tile_rows, t.rows) - 1;
+    t.pmin = t.seq.len - t.seq.n + (int)((uint32_t)t.row0 / group);
+    t.pmax = t.seq.len - t.seq.n + (int)(last / group);
     t.span = span_of(t.pmin, t.pmax, p.window, p.sinks);
-    t.active = (t.span.tiles + p.chunk - 1) / p.chunk;
+    t.active = (int)((uint32_t)(t.span.tiles + p.chunk - 1) / (uint32_t)p.chunk);
 }
 
 // The item-th tile. Later tiles of a sequence look at more tokens: `from_last`
 // numbers them from the last, so that the longest work begins first.
-__device__ __forceinline__ bool find_tile(const AttnKern& p, int64_t item, bool from_last, RowTile& t)
+__device__ __forceinline__ bool find_tile(const AttnKern& p, uint32_t item, bool from_last, RowTile& t)
 {
     int rt;
     if (p.per_seq > 0) {
         if (from_last) {
-            const int back = (int)(item / p.c.seqs);
-            t.b = (int)(item - (int64_t)back * p.c.seqs);
-            rt = p.per_seq - 1 - back;
+            const uint32_t back = item / (uint32_t)p.c.seqs;
+            t.b = (int)(item - back * p.c.seqs);
+            rt = p.per_seq - 1 - (int)back;
         } else {
-            t.b = (int)(item / p.per_seq);
-            rt = (int)(item - (int64_t)t.b * p.per_seq);
+            t.b = (int)(item / (uint32_t)p.per_seq);
+            rt = (int)(item - (uint32_t)t.b * p.per_seq);
         }
         t.seq = seq_rows(p.c, t.b);
     } else {
         const auto count = [&](const SeqRows& s) {
-            return (int)(((int64_t)s.n * p.group + p.tile_rows - 1) / p.tile_rows);
+            return (int)((uint32_t)(s.n * p.group + p.tile_rows - 1) / (uint32_t)p.tile_rows);
         };
         if (!find_item(p.c, item, count, t.b, rt, t.seq)) {
             return false;
@@ -109,18 +111,32 @@ __device__ __forceinline__ bool find_tile(const AttnKern& p, int64_t item, bool 
     return true;
 }
 
-// A page's scales as the softmax takes them: x = s mul + add, l += w inv.
+// A page's scales as they lie in memory, and as the softmax takes them: x = s
+// mul + add, l += w inv. (Loaded with the codes, turned where they are used:
+// turning them at once would wait for the codes in flight.)
+struct PageScales {
+    float k, v, off;      // off: NaN where the page does not exist, else 0
+};
 struct Scales {
     float mul, add, inv;
 };
 
-__device__ __forceinline__ Scales scales_of(const AttnKern& p, int page, int64_t at)
+// The page to read for a page number of the table: the first one's codes stand
+// in for those of a page that does not exist, under scales that are NaN.
+__device__ __forceinline__ bool exists(const Paged& c, int page) { return (uint32_t)page < (uint32_t)c.pages; }
+__device__ __forceinline__ int64_t readable(const Paged& c, int page) { return exists(c, page) ? page : 0; }
+
+__device__ __forceinline__ PageScales page_scales(const Paged& c, int page, int kvh)
 {
-    const float nan = __uint_as_float(0x7fc00000u);
-    const float ks = page < 0 ? nan : p.c.k_scale[at], vs = page < 0 ? nan : p.c.v_scale[at];
+    const int64_t at = readable(c, page) * c.heads + kvh;
+    return PageScales{c.k_scale[at], c.v_scale[at], exists(c, page) ? 0.0f : __uint_as_float(0x7fc00000u)};
+}
+
+__device__ __forceinline__ Scales softmax_scales(const AttnKern& p, PageScales s)
+{
     // (codes of a page whose scale is less count for nothing beside any other)
-    const float v = vs < kLeastScale ? kLeastScale : vs;
-    return Scales{p.scale_log2 * ks, __builtin_amdgcn_logf(v), kDrop / v};
+    const float v = (s.v < kLeastScale ? kLeastScale : s.v) + s.off;
+    return Scales{p.scale_log2 * s.k + s.off, __builtin_amdgcn_logf(v), kDrop * __builtin_amdgcn_rcpf(v)};
 }
 
 // The operands of the two products, by the rows' type.

@@ -10,16 +10,16 @@
 // operand's k order.
 //
 // Bound: the matrix cores and, as long, the exponentials and the other steps of
-// the softmax. A wave alternates between a matrix phase (the last tile's
-// second product, the next tile's scores) and a vector phase (its softmax, its
-// share of the coming tiles' codes into LDS); of the two waves of a SIMD one is
-// a phase behind, so that one multiplies while the other computes weights. A
-// barrier ends each phase. Waves 4 to 7 stage a tile further ahead, since their
-// vector phase comes half a tile later: the keys of tile j + 1 and the values of
-// tile j are written in phases 2 j (waves 4 to 7) and 2 j + 1 (waves 0 to 3),
-// over those of j - 1 and j - 2, which phase 2 j - 1 read last. The global loads
-// of a piece are issued a period before it is written, its page number one
-// before that. Rows in LDS are 16 bytes longer than their data: 16 lanes' reads
+// the softmax. A wave alternates between a matrix phase (the last tile's second
+// product and the next tile's scores, with its share of the coming tiles' codes
+// turned and put into LDS between them: vector instructions beside a matrix
+// instruction are nearly free) and a vector phase (the softmax); of the two
+// waves of a SIMD one is a phase behind, so that one multiplies while the other
+// computes weights. A barrier ends each phase. The keys of tile j + 1 and the
+// values of tile j are written in phases 2 j (waves 0 to 3) and 2 j + 1 (waves 4
+// to 7), over those of j - 1 and j - 2, which phase 2 j - 1 read last. The loads
+// of a piece are issued a tile before it is written, its page number one before
+// that. Rows in LDS are 16 bytes longer than their data: 16 lanes' reads
 // of one column meet 16 bank groups, at constant offsets.
 #include <type_traits>
 
@@ -54,10 +54,10 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
 
     __shared__ __attribute__((aligned(16))) uint16_t s_k[2][kTile * kPitchK];
     __shared__ __attribute__((aligned(16))) uint16_t s_v[2][DP * kPitchV];
-    __shared__ __attribute__((aligned(16))) float s_scale[4][3][4];  // mul, add, inv of the groups of 16 tokens
+    __shared__ __attribute__((aligned(16))) v4f s_scale[4][4];       // mul, add, inv of the groups of 16 tokens
 
     const Paged& c = p.c;
-    const int64_t item = blockIdx.x / (unsigned)c.heads;
+    const uint32_t item = blockIdx.x / (uint32_t)c.heads;
     const int kvh = (int)(blockIdx.x - item * c.heads);
     RowTile rt;
     if (!find_tile(p, item, true, rt)) {
@@ -73,18 +73,19 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64);       // uniform: what hangs on it are scalar branches
     const int n = lane % 32, hh = lane / 32;
     const int d = c.d;
-    const int64_t page_bytes = (int64_t)c.page * d;
 
     // the wave's rows; a wave without any only helps to fill LDS
-    const int64_t wrow = rt.row0 + 32 * wave;
+    const uint32_t group = p.group;
+    const int wrow = rt.row0 + 32 * wave;
     const bool wave_live = wrow < rt.rows;
-    const int64_t wlast = min(wrow + 32, rt.rows) - 1;
+    const int wlast = min(wrow + 32, rt.rows) - 1;
     const int pos0 = seq.len - seq.n;
-    const int wmin = wave_live ? pos0 + (int)(wrow / p.group) : 0, wmax = wave_live ? pos0 + (int)(wlast / p.group) : -1;
-    const int64_t row = wrow + n;
+    const int wmin = wave_live ? pos0 + (int)((uint32_t)wrow / group) : 0;
+    const int wmax = wave_live ? pos0 + (int)((uint32_t)wlast / group) : -1;
+    const int row = wrow + n;
     const bool is_row = row < rt.rows;
-    const int tok = is_row ? (int)(row / p.group) : 0;
-    const int head = kvh * p.group + (is_row ? (int)(row - (int64_t)tok * p.group) : 0);
+    const int tok = is_row ? (int)((uint32_t)row / group) : 0;
+    const int head = kvh * p.group + (is_row ? row - tok * p.group : 0);
     const int pos = is_row ? pos0 + tok : -1;
 
     // Q's fragments: channels 16 i + 8 hh .. + 7 of the lane's row are k step i
@@ -102,92 +103,67 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
     }
 
     // --- codes: page number -> registers -> LDS -----------------------------
-    // (a page past the last position: any page's codes, they are masked)
+    // Without a branch, so that what is in flight stays in flight: tiles past the
+    // last one are the last again, tokens past the last position have its page
+    // (they are masked), channels past d are channel 0's codes (q is 0 there, and
+    // their output is not stored). Page numbers are looked at when they are used.
     const int32_t* table = c.table + (int64_t)rt.b * c.ld_table;
-    const auto page_at = [&](int token) {
-        const int id = table[min(token, rt.pmax) >> c.page_log2];
-        return id >= 0 && id < c.pages ? id : -1;
-    };
-    const int64_t page_step = page_bytes * c.heads;
-    const int8_t *k_at = c.k + kvh * page_bytes, *v_at = c.v + kvh * page_bytes;
+    const uint32_t page_step = (uint32_t)c.page * d * c.heads;      // (entry: fits 31 bits)
+    const int8_t *k_at = c.k + (uint32_t)(kvh * c.page * d), *v_at = c.v + (uint32_t)(kvh * c.page * d);
     v4i rk[kPer], rv[kPer];
-    int kid[kPer], vid[kPer], sid = 0;
-    Scales rs{0.0f, 0.0f, 0.0f};
+    int kid[kPer], vid, sid;
+    PageScales rs;
+    const auto base_of = [&](int v) { return tile_base(rt.span, min(v, v1 - 1)); };
+    const auto page_at = [&](int token) { return table[min(token, rt.pmax) >> c.page_log2]; };
     const auto ids_k = [&](int v) {
-        const int base = tile_base(rt.span, v);
+        const int base = base_of(v);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            kid[i] = page_at(base + (tid + i * kThreads) / kRowPieces);
-        }
-        if (tid < 4) {
-            sid = page_at(base + 16 * tid);
+            kid[i] = page_at(base + (tid + i * kThreads) / kRowPieces % kTile);
         }
     };
-    const auto ids_v = [&](int v) {
-        const int base = tile_base(rt.span, v);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            vid[i] = page_at(base + (tid + i * kThreads) % 4 * 16);
-        }
-    };
+    // (pieces of the values and scales: the thread's group of 16 tokens)
+    const auto id_v = [&](int v) { return page_at(base_of(v) + tid % 4 * 16); };
     const auto load_k = [&](int v) {
-        const int base = tile_base(rt.span, v);
+        const int base = base_of(v);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int piece = tid + i * kThreads, slot = (base + piece / kRowPieces) & (c.page - 1);
+            const int piece = tid + i * kThreads, slot = (base + piece / kRowPieces % kTile) & (c.page - 1);
             const int at = piece % kRowPieces * 16;
-            rk[i] = v4i{0, 0, 0, 0};
-            if ((kPieces % kThreads == 0 || piece < kPieces) && at < d) {
-                rk[i] = *reinterpret_cast<const v4i*>(k_at + max(kid[i], 0) * page_step + (slot * d + at));
-            }
-        }
-        if (tid < 4) {
-            rs = Scales{0.0f, 0.0f, 0.0f};
-            if (base + 16 * tid <= rt.pmax) {
-                rs = scales_of(p, sid, (int64_t)max(sid, 0) * c.heads + kvh);
-            }
+            rk[i] = *reinterpret_cast<const v4i*>(k_at + readable(c, kid[i]) * (uint64_t)page_step +
+                                                       (uint32_t)(slot * d + (at < d ? at : 0)));
         }
     };
+    const auto load_scales = [&](int page) { rs = page_scales(c, page, kvh); };
     const auto load_v = [&](int v) {
-        const int base = tile_base(rt.span, v);
+        const int slot = (base_of(v) + tid % 4 * 16) & (c.page - 1);
+        const int8_t* page = v_at + readable(c, vid) * (uint64_t)page_step + (uint32_t)slot;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int piece = tid + i * kThreads, ch = piece / 4, slot = (base + piece % 4 * 16) & (c.page - 1);
-            rv[i] = v4i{0, 0, 0, 0};
-            if ((kPieces % kThreads == 0 || piece < kPieces) && ch < d) {
-                rv[i] = *reinterpret_cast<const v4i*>(v_at + max(vid[i], 0) * page_step + (ch * c.page + slot));
-            }
+            const int ch = (tid + i * kThreads) / 4;
+            rv[i] = *reinterpret_cast<const v4i*>(page + (uint32_t)((ch < d ? ch : 0) * c.page));
         }
     };
-    const auto put = [&](uint16_t* at, const v4i& w) {
-        const Vec lo = Op::codes((uint32_t)w.x, (uint32_t)w.y), hi = Op::codes((uint32_t)w.z, (uint32_t)w.w);
-        __builtin_memcpy(__builtin_assume_aligned(at, 16), &lo, 16);
-        __builtin_memcpy(__builtin_assume_aligned(at + 8, 16), &hi, 16);
+    // (8 codes: half a piece)
+    const auto put = [&](uint16_t* at, const v4i& w, int half) {
+        const Vec x = half ? Op::codes((uint32_t)w.z, (uint32_t)w.w) : Op::codes((uint32_t)w.x, (uint32_t)w.y);
+        __builtin_memcpy(__builtin_assume_aligned(at + 8 * half, 16), &x, 16);
     };
-    const auto store_k = [&](int v) {
-        uint16_t* buf = s_k[v & 1];
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int piece = tid + i * kThreads;
-            if (kPieces % kThreads == 0 || piece < kPieces) {
-                put(buf + piece / kRowPieces * kPitchK + piece % kRowPieces * 16, rk[i]);
-            }
-        }
-        if (tid < 4) {
-            s_scale[v & 3][0][tid] = rs.mul;
-            s_scale[v & 3][1][tid] = rs.add;
-            s_scale[v & 3][2][tid] = rs.inv;
+    const auto store_k = [&](int v, int i, int half) {
+        const int piece = tid + i * kThreads;
+        if (kPieces % kThreads == 0 || piece < kPieces) {
+            put(s_k[v & 1] + piece / kRowPieces * kPitchK + piece % kRowPieces * 16, rk[i], half);
         }
     };
-    const auto store_v = [&](int v) {
-        uint16_t* buf = s_v[v & 1];
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int piece = tid + i * kThreads;
-            if (kPieces % kThreads == 0 || piece < kPieces) {
-                put(buf + piece / 4 * kPitchV + piece % 4 * 16, rv[i]);
-            }
+    const auto store_v = [&](int v, int i, int half) {
+        const int piece = tid + i * kThreads;
+        if (kPieces % kThreads == 0 || piece < kPieces) {
+            put(s_v[v & 1] + piece / 4 * kPitchV + piece % 4 * 16, rv[i], half);
         }
+    };
+    const auto store_scales = [&](int v) {
+        const Scales sc = softmax_scales(p, rs);
+        s_scale[v & 3][tid % 4] = v4f{sc.mul, sc.add, sc.inv, 0.0f};   // (the same from many threads)
     };
 
     // --- the two products and the softmax of a wave ------------------------
@@ -205,17 +181,6 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
         __builtin_memcpy(&a, __builtin_assume_aligned(at, 16), 16);
         return a;
     };
-    // LDS reads a few fragments ahead of the products, not all at once
-    const auto pace = [](auto fragments) {
-        constexpr int kN = decltype(fragments)::value, kAhead = kN < 6 ? kN : 6;
-        __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
-#pragma unroll
-        for (int i = 0; i < kN - kAhead; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, Op::kParts, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(0x008, Op::kParts * kAhead, 0);
-    };
     v16f s[2];
     Vec pf[4][Op::kParts];
     const auto scores = [&](int v) {
@@ -229,14 +194,17 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
                 s[u] = product<T>(lds_vec(buf + 32 * u * kPitchK + 16 * i), qf[i], s[u]);
             }
         }
-        pace(std::integral_constant<int, 2 * kSteps>{});
     };
     const auto soft = [&](auto masked, int v, int base) {
         constexpr bool kMasked = decltype(masked)::value;
         float mul[4], add[4], inv[4];
-        __builtin_memcpy(mul, s_scale[v & 3][0], 16);
-        __builtin_memcpy(add, s_scale[v & 3][1], 16);
-        __builtin_memcpy(inv, s_scale[v & 3][2], 16);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const v4f sc = s_scale[v & 3][g];
+            mul[g] = sc.x;
+            add[g] = sc.y;
+            inv[g] = sc.z;
+        }
         // bit i: the row sees token base + 8 hh + i
         uint32_t bits[2] = {~0u, ~0u};
         if (kMasked) {
@@ -294,7 +262,7 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
             Op::split(w, pf[g]);
         }
     };
-    const auto accumulate = [&](int v) {
+    const auto rescale = [&] {
         if (renew) {
 #pragma unroll
             for (int t = 0; t < kOut; ++t) {
@@ -302,6 +270,8 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
             }
             renew = false;
         }
+    };
+    const auto accumulate = [&](int v) {
         const uint16_t* buf = s_v[v & 1] + n * kPitchV + 8 * hh;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -310,7 +280,47 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
                 o[t] = product<T>(lds_vec(buf + 32 * t * kPitchV + 16 * g), pf[g], o[t]);
             }
         }
-        pace(std::integral_constant<int, 4 * kOut>{});
+    };
+    // accumulate(v - 1) and scores(v), each fragment read kAhead products before
+    // its own, other work in `parts` between them: the order of reads and products
+    // is fixed, vector instructions may move across.
+    const auto both = [&](int v, auto work, auto parts) {
+        constexpr int kFirst = 4 * kOut, kN = kFirst + 2 * kSteps, kAhead = 6;
+        constexpr int kEvery = kN / (decltype(parts)::value + 1) > 0 ? kN / (decltype(parts)::value + 1) : 1;
+        const uint16_t* bv = s_v[(v - 1) & 1] + n * kPitchV + 8 * hh;
+        const uint16_t* bk = s_k[v & 1] + krow * kPitchK + 8 * hh;
+        const auto fragment = [&](int i) {
+            return i < kFirst ? lds_vec(bv + 32 * (i % kOut) * kPitchV + 16 * (i / kOut))
+                              : lds_vec(bk + 32 * ((i - kFirst) % 2) * kPitchK + 16 * ((i - kFirst) / 2));
+        };
+        Vec f[kN];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            f[i] = fragment(i);
+        }
+        s[0] = v16f{};
+        s[1] = v16f{};
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            if (i + kAhead < kN) {
+                f[i + kAhead] = fragment(i + kAhead);
+            }
+            if (i < kFirst) {
+                o[i % kOut] = product<T>(f[i], pf[i / kOut], o[i % kOut]);
+            } else {
+                s[(i - kFirst) % 2] = product<T>(f[i], qf[(i - kFirst) / 2], s[(i - kFirst) % 2]);
+            }
+            // (loads stay where they are: above the last use of what they replace,
+            // they would need other registers, and a copy that waits for them)
+            __builtin_amdgcn_sched_barrier(0x2 | 0x4 | 0x200);
+            if (i % kEvery == kEvery - 1 && i / kEvery < decltype(parts)::value) {
+                work(i / kEvery);
+            }
+        }
+#pragma unroll
+        for (int i = kN / kEvery; i < decltype(parts)::value; ++i) {
+            work(i);
+        }
     };
     const auto live = [&](int base) {
         return wave_live && base <= wmax && (p.window == 0 || wmin - (base + kTile - 1) < p.window || base < p.sinks);
@@ -324,74 +334,91 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
     };
 
-    // Tiles in terms of 0 .. nt - 1. The group that is a phase behind writes
-    // what the other will in its next vector phase.
+    // Tiles in terms of 0 .. nt - 1.
     const int nt = v1 - v0, behind = kPair ? wave / 4 : 0;
     if (nt > 0) {
-        // written: keys 0, and by those behind keys 1 and values 0 (in phase 0);
-        // in flight: the first pieces of the loop
-        ids_k(v0);
-        ids_v(v0);
-        load_k(v0);
-        store_k(0);
-        if (nt > 1) {
-            ids_k(v0 + 1);
-            load_k(v0 + 1);
-        }
-        load_v(v0);
-        if (nt > 2) {
-            ids_k(v0 + 2);
-        }
-        if (nt > 1) {
-            ids_v(v0 + 1);
-        }
-        meet();
-        // a thread's pieces of the values of tile x and the keys of x + 1, and the loads after them
-        const auto pieces = [&](int x) {
-            if (x < nt) {
-                store_v(x);
-            }
-            if (x + 1 < nt) {
-                store_k(x + 1);
+        // Step x of a thread: its pieces of the values of tile x and the keys of x
+        // + 1 go into LDS, the next ones are asked for, then the page numbers of
+        // those after. (Scales go with the keys.)
+        constexpr int kParts = 4 * kPer + 4;
+        const auto part = [&](int x, int i) {
+            if (i < 2 * kPer) {
+                store_v(x, i / 2, i % 2);
+            } else if (i < 4 * kPer) {
+                store_k(x + 1, i / 2 - kPer, i % 2);
+            } else if (i == 4 * kPer) {
+                store_scales(x + 1);
                 load_v(v0 + x + 1);
-            }
-            if (x + 2 < nt) {
+            } else if (i == 4 * kPer + 1) {
                 load_k(v0 + x + 2);
-                ids_v(v0 + x + 2);
-            }
-            if (x + 3 < nt) {
+            } else if (i == 4 * kPer + 2) {
+                load_scales(sid);
+                vid = id_v(v0 + x + 2);
+                sid = id_v(v0 + x + 3);
+            } else {
                 ids_k(v0 + x + 3);
             }
         };
+        const auto step = [&](int x) {
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) {
+                part(x, i);
+            }
+        };
+        ids_k(v0);
+        load_scales(id_v(v0));
+        load_k(v0);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            store_k(0, i, 0);
+            store_k(0, i, 1);
+        }
+        store_scales(0);
+        vid = id_v(v0);
+        load_v(v0);
+        ids_k(v0 + 1);
+        load_k(v0 + 1);
+        load_scales(id_v(v0 + 1));
+        vid = id_v(v0 + 1);
+        sid = id_v(v0 + 2);
+        ids_k(v0 + 2);
+        meet();
         if (behind) {
-            pieces(0);
             meet();
         }
-        bool was = false;                          // the last tile has weights to multiply
-        for (int j = 0; j < nt; ++j) {
+        // A wave multiplies tiles that it does not look at too (the last ones of a
+        // tile of rows, and whole tiles outside a window): their weights are 0.
+        // Without a branch in the matrix phase, pieces in flight need no copies.
+        const auto weigh = [&](int j) {
             const int base = tile_base(rt.span, v0 + j);
-            const bool now = live(base);
-            if (was) {
-                accumulate(j - 1);
-            }
-            if (now) {
-                scores(j);
-            }
-            meet();
-            pieces(j + behind);
-            if (now) {
-                if (open(base)) {
-                    soft(std::false_type{}, j, base);
-                } else {
-                    soft(std::true_type{}, j, base);
+            if (!live(base)) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+#pragma unroll
+                    for (int i = 0; i < Op::kParts; ++i) {
+                        pf[g][i] = Vec{};
+                    }
                 }
+            } else if (open(base)) {
+                soft(std::false_type{}, j, base);
+            } else {
+                soft(std::true_type{}, j, base);
             }
-            was = now;
+        };
+        scores(0);
+        step(0);
+        meet();
+        for (int j = 1; j < nt; ++j) {
+            weigh(j - 1);
+            meet();
+            rescale();
+            both(j, [&](int i) { part(j, i); }, std::integral_constant<int, kParts>{});
             meet();
         }
-        if (was) {
-            accumulate(nt - 1);
-        }
+        weigh(nt - 1);
+        meet();
+        rescale();
+        accumulate(nt - 1);
         if (kPair && !behind) {
             meet();                                // as many as the others
         }
@@ -403,20 +430,21 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
     l_run += across(l_run);
     const int64_t token = seq.start + tok;
     if (rt.active > 1) {
-        float* dst = p.part + (((int64_t)split * c.rows + token) * p.q_heads + head) * (d + 2);
+        const int64_t at_part = ((int64_t)split * c.rows + token) * p.q_heads + head;
+        float* dst = p.part + at_part * d;
 #pragma unroll
         for (int t = 0; t < kOut; ++t) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int ch = 32 * t + 8 * (r / 4) + 4 * hh + r % 4;
+            for (int r = 0; r < 16; r += 4) {
+                const int ch = 32 * t + 8 * (r / 4) + 4 * hh;
                 if (ch < d) {
-                    dst[ch] = o[t][r];
+                    *reinterpret_cast<v4f*>(dst + ch) = v4f{o[t][r], o[t][r + 1], o[t][r + 2], o[t][r + 3]};
                 }
             }
         }
         if (hh == 0) {
-            dst[d] = m_run;
-            dst[d + 1] = l_run;
+            p.part_ml[2 * at_part] = m_run;
+            p.part_ml[2 * at_part + 1] = l_run;
         }
         return;
     }

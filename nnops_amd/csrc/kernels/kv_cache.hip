@@ -32,7 +32,7 @@ int check_pages(const NnopsKvPages& c, int64_t rows)
         return NNOPS_OK;
     }
     if (rows > INT32_MAX / 2 || c.sequences > INT32_MAX / 2 || c.pages > INT32_MAX || c.heads > (1 << 16) ||
-        c.table_pages > INT32_MAX / t) {
+        c.table_pages > INT32_MAX / t || c.heads * t * d > INT32_MAX) {
         return NNOPS_UNSUPPORTED;
     }
     if (c.sequences == 0 || (c.row_starts == nullptr && rows % c.sequences != 0)) {
