@@ -24,7 +24,6 @@
 // Bound: HBM for few rows, the codes read once per KV head. Long sequences are
 // split over workgroups (partial O, M, l in the workspace, joined by a second
 // kernel); a workgroup's 4 waves take every fourth tile and join in LDS.
-#include <cstdlib>
 #include "cache_attention.hpp"
 
 namespace nnops_amd {
@@ -429,34 +428,53 @@ struct AttnPlan {
     size_t workspace;
 };
 
-// Rows of a sequence past kRows go to the kernel whose waves share their tiles
+// The kernel: tiles of many rows that share their codes (attention_rows_tiled)
+// where a sequence has rows to fill one and the tiles, or the tiles by the
+// tokens they look at, fill the chip; 16 rows a workgroup, its waves sharing the
+// tokens, otherwise. Measured both ways (us, tiled / 16 rows; 32 query heads, 8
+// KV heads, d 128, f16, but where said):
+//   16 x 16 of 2048 tokens  41.0 / 34.2     64 x 33 of 300    29.6 / 51.9
+//   16 x 32 of 2048         48.3 / 49.4     64 x 64 of 64     32.2 / 70.0
+//   1 x 64 of 4096          24.6 / 24.8     16 x 128 of 2048  65.2 / 145
+//   1 x 256 of 4096         43.0 / 59.0     4 x 300 of 2500, 16 / 4 heads, d 64, f32  65.1 / 56.0
 // (ragged calls: by their mean). Splits of the longest sequence that the page
-// table has room for: enough workgroups to fill the chip, no fewer than 4 tiles
-// each.
+// table has room for: as many workgroups as the chip holds at once (more of
+// them were slower: one token over 126976, 58 us with 512, 67 with 768, 72 with
+// 1024), no fewer than 4 tiles each.
 AttnPlan attn_plan(const NnopsCacheAttentionArgs* g)
 {
     AttnPlan a{};
-    const int64_t group = g->q_heads / g->cache.heads, b = g->cache.sequences;
+    const int64_t heads = g->cache.heads, group = g->q_heads / heads, b = g->cache.sequences, d = g->cache.head_dim;
     const int64_t mean = (g->rows * group + b - 1) / b;
-    const int tiled = mean > kRows ? tiled_rows(g->cache.head_dim, g->f16, mean) : 0;
-    a.tiled = tiled > 0;
-    a.tile_rows = a.tiled ? tiled : kRows;
-    if (g->cache.row_starts == nullptr) {
-        a.per_seq = (int32_t)((g->rows / b * group + a.tile_rows - 1) / a.tile_rows);
-        a.items = b * a.per_seq * g->cache.heads;
-    } else {
-        a.items = (g->rows * group / a.tile_rows + (b < g->rows ? b : g->rows)) * g->cache.heads;
-    }
-    int64_t tiles = (g->cache.table_pages * g->cache.page_tokens + kTile - 1) / kTile;
-    if (g->window > 0) {
+    const auto items_of = [&](int64_t tile_rows) {
+        if (g->cache.row_starts == nullptr) {
+            return b * ((g->rows / b * group + tile_rows - 1) / tile_rows) * heads;
+        }
+        return (g->rows * group / tile_rows + (b < g->rows ? b : g->rows)) * heads;
+    };
+    const auto tiles_of = [&](int64_t tile_rows) {
+        const int64_t tiles = (g->cache.table_pages * g->cache.page_tokens + kTile - 1) / kTile;
+        if (g->window <= 0) {
+            return tiles;
+        }
         // a tile's rows see the window, up to tile_rows - 1 tokens more, and the sinks
-        const int64_t seen = (g->window + a.tile_rows) / kTile + 2 + (g->sinks + kTile - 1) / kTile;
-        tiles = tiles < seen ? tiles : seen;
+        const int64_t sinks = (g->sinks < INT32_MAX ? g->sinks : INT32_MAX) / kTile + 1;
+        const int64_t seen = (g->window < INT32_MAX ? g->window : INT32_MAX) / kTile + tile_rows / kTile + 3 + sinks;
+        return tiles < seen ? tiles : seen;
+    };
+    a.tile_rows = kRows;
+    if (const int rows = mean > 96 ? tiled_rows(d, g->f16, g->cache.page_tokens, mean) : 0; rows > 0) {
+        const int64_t items = items_of(rows);
+        if (items >= 128 || items * tiles_of(rows) * d >= 1 << 18) {
+            a.tiled = true;
+            a.tile_rows = rows;
+        }
     }
-    static const int ev=getenv("NN_FULL")?atoi(getenv("NN_FULL")):512, em=getenv("NN_MIN")?atoi(getenv("NN_MIN")):4, et=getenv("NN_TFULL")?atoi(getenv("NN_TFULL")):256;
-    const int64_t full = a.tiled ? et : ev;
-    int64_t splits = (full + a.items - 1) / a.items;
-    const int64_t mn = a.tiled ? 4 : em; const int64_t most = (tiles + mn - 1) / mn;
+    a.items = items_of(a.tile_rows);
+    a.per_seq = g->cache.row_starts == nullptr ? (int32_t)(a.items / (b * heads)) : 0;
+    const int64_t tiles = tiles_of(a.tile_rows);
+    int64_t splits = ((a.tiled ? 256 : 512) + a.items - 1) / a.items;
+    const int64_t most = (tiles + 3) / 4;
     splits = splits < most ? splits : most;
     splits = splits > 1 ? splits : 1;
     const int64_t chunk = ((tiles + splits - 1) / splits + 3) / 4 * 4;
@@ -478,7 +496,7 @@ int check_attention(const NnopsCacheAttentionArgs* g)
     if (g->q_heads == 0 || g->q_heads % g->cache.heads != 0 || g->cache.pages == 0) {
         return NNOPS_INVALID_ARGUMENT;
     }
-    if (g->q_heads > (1 << 16) || g->rows * g->q_heads > INT32_MAX / 256) {
+    if (g->q_heads > (1 << 16) || g->rows * g->q_heads > INT32_MAX / 2) {
         return NNOPS_UNSUPPORTED;
     }
     return -1;

@@ -265,7 +265,7 @@ __device__ __forceinline__ Acc product(typename Operand<T>::Vec a, const typenam
 
 // attention_rows_tiled's launch (cache_attention_tiled.hip): d, type and rows
 // of a workgroup that it has a kernel for.
-int tiled_rows(int64_t d, bool f16, int64_t rows);
+int tiled_rows(int64_t d, bool f16, int64_t page, int64_t rows);
 void launch_tiled(const AttnKern& k, const dim3& grid, bool f16, hipStream_t s);
 
 }  // namespace nnops_amd

@@ -38,7 +38,21 @@ __device__ __forceinline__ float across(float x)   // the other half-wave's valu
 #endif
 }
 
-template <typename T, int DP, int NW>
+// Memory that no kernel of the call writes, for addresses that are the same in
+// a whole wave: scalar loads, whatever barriers lie between.
+template <typename V>
+__device__ __forceinline__ V uniform_load(const V* p)
+{
+#if __HIP_DEVICE_COMPILE__
+    return *(const __attribute__((address_space(4))) V*)(uintptr_t)p;
+#else
+    return *p;
+#endif
+}
+
+// kOne: pages of 64 tokens and more, so that a tile lies in one: its number and
+// scales are scalars, its codes at a scalar base and fixed offsets.
+template <typename T, int DP, int NW, bool kOne>
 __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p)
 {
     typedef Operand<T> Op;
@@ -124,24 +138,51 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
     };
     // (pieces of the values and scales: the thread's group of 16 tokens)
     const auto id_v = [&](int v) { return page_at(base_of(v) + tid % 4 * 16); };
+    uint32_t koff[kPer], voff[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int piece = tid + i * kThreads, at = piece % kRowPieces * 16, ch = piece / 4;
+        koff[i] = (uint32_t)(piece / kRowPieces % kTile * d + (at < d ? at : 0));
+        voff[i] = (uint32_t)((ch < d ? ch : 0) * c.page + tid % 4 * 16);
+    }
+    int one_v = 0, one_k = 0;                      // kOne: page of the next values, of the next keys
+    float one_ks = 0.0f, one_vs = 0.0f;            //       scales of the next softmax
+    const auto one_page = [&](int v) { return uniform_load(table + (min(base_of(v), rt.pmax) >> c.page_log2)); };
     const auto load_k = [&](int v) {
         const int base = base_of(v);
+        if constexpr (kOne) {
+            const int8_t* page = k_at + readable(c, one_k) * (uint64_t)page_step + (uint32_t)((base & (c.page - 1)) * d);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int piece = tid + i * kThreads, slot = (base + piece / kRowPieces % kTile) & (c.page - 1);
-            const int at = piece % kRowPieces * 16;
-            rk[i] = *reinterpret_cast<const v4i*>(k_at + readable(c, kid[i]) * (uint64_t)page_step +
-                                                       (uint32_t)(slot * d + (at < d ? at : 0)));
+            for (int i = 0; i < kPer; ++i) {
+                rk[i] = *reinterpret_cast<const v4i*>(page + koff[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int piece = tid + i * kThreads, slot = (base + piece / kRowPieces % kTile) & (c.page - 1);
+                const int at = piece % kRowPieces * 16;
+                rk[i] = *reinterpret_cast<const v4i*>(k_at + readable(c, kid[i]) * (uint64_t)page_step +
+                                                      (uint32_t)(slot * d + (at < d ? at : 0)));
+            }
         }
     };
     const auto load_scales = [&](int page) { rs = page_scales(c, page, kvh); };
     const auto load_v = [&](int v) {
-        const int slot = (base_of(v) + tid % 4 * 16) & (c.page - 1);
-        const int8_t* page = v_at + readable(c, vid) * (uint64_t)page_step + (uint32_t)slot;
+        const int base = base_of(v);
+        if constexpr (kOne) {
+            const int8_t* page = v_at + readable(c, one_v) * (uint64_t)page_step + (uint32_t)(base & (c.page - 1));
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int ch = (tid + i * kThreads) / 4;
-            rv[i] = *reinterpret_cast<const v4i*>(page + (uint32_t)((ch < d ? ch : 0) * c.page));
+            for (int i = 0; i < kPer; ++i) {
+                rv[i] = *reinterpret_cast<const v4i*>(page + voff[i]);
+            }
+        } else {
+            const int slot = (base + tid % 4 * 16) & (c.page - 1);
+            const int8_t* page = v_at + readable(c, vid) * (uint64_t)page_step + (uint32_t)slot;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int ch = (tid + i * kThreads) / 4;
+                rv[i] = *reinterpret_cast<const v4i*>(page + (uint32_t)((ch < d ? ch : 0) * c.page));
+            }
         }
     };
     // (8 codes: half a piece)
@@ -197,13 +238,21 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
     };
     const auto soft = [&](auto masked, int v, int base) {
         constexpr bool kMasked = decltype(masked)::value;
-        float mul[4], add[4], inv[4];
+        constexpr int kGroups = kOne ? 1 : 4, kSize = 32 / kGroups;   // values of a lane under one scale
+        float mul[kGroups], add[kGroups], inv[kGroups];
+        if constexpr (kOne) {
+            const Scales sc = softmax_scales(p, PageScales{one_ks, one_vs, 0.0f});
+            mul[0] = sc.mul;
+            add[0] = sc.add;
+            inv[0] = sc.inv;
+        } else {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const v4f sc = s_scale[v & 3][g];
-            mul[g] = sc.x;
-            add[g] = sc.y;
-            inv[g] = sc.z;
+            for (int g = 0; g < 4; ++g) {
+                const v4f sc = s_scale[v & 3][g];
+                mul[g] = sc.x;
+                add[g] = sc.y;
+                inv[g] = sc.z;
+            }
         }
         // bit i: the row sees token base + 8 hh + i
         uint32_t bits[2] = {~0u, ~0u};
@@ -217,21 +266,22 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
             bits[0] = (uint32_t)m;
             bits[1] = (uint32_t)(m >> 32);
         }
-        const auto seen = [&](int g, int e) {      // all ones or none
-            return (uint32_t)((int32_t)(bits[g / 2] << (31 - 16 * (g % 2) - e)) >> 31);
+        // value i of a lane: token 16 (i / 8) + i % 8 of those. All ones or none
+        const auto seen = [&](int i) {
+            return (uint32_t)((int32_t)(bits[i / 16] << (31 - 16 * (i / 8 % 2) - i % 8)) >> 31);
         };
         float top = kNone;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
+        for (int g = 0; g < kGroups; ++g) {
             float t = kNone;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                float v = s[g / 2][8 * (g % 2) + e];
+            for (int i = kSize * g; i < kSize * g + kSize; ++i) {
+                float x = s[i / 16][i % 16];
                 if (kMasked) {
-                    const uint32_t m = seen(g, e);
-                    v = __uint_as_float((__float_as_uint(v) & m) | (0xff800000u & ~m));
+                    const uint32_t m = seen(i);
+                    x = __uint_as_float((__float_as_uint(x) & m) | (0xff800000u & ~m));
                 }
-                t = fmaxf(t, v);
+                t = fmaxf(t, x);
             }
             // (-inf times a scale of 0 or NaN is a NaN, which fmaxf drops)
             top = fmaxf(top, __builtin_fmaf(t, mul[g], add[g]));
@@ -246,20 +296,24 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
         }
         const float shift = m_run > kNone ? kLift - m_run : 0.0f;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            float w[8], sum = 0.0f;
+        for (int g = 0; g < kGroups; ++g) {
             const float a = add[g] + shift;
+            float sum = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g / 2][8 * (g % 2) + e], mul[g], a));
-                if (kMasked) {
-                    w[e] = __uint_as_float(__float_as_uint(w[e]) & seen(g, e));
+            for (int h = kSize / 8 * g; h < kSize / 8 * (g + 1); ++h) {
+                float w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h / 2][8 * (h % 2) + e], mul[g], a));
+                    if (kMasked) {
+                        w[e] = __uint_as_float(__float_as_uint(w[e]) & seen(8 * h + e));
+                    }
+                    sum += w[e];
                 }
-                sum += w[e];
+                Op::split(w, pf[h]);
             }
             // a page of which the row sees nothing adds nothing, whatever its scale
             l_run += !kMasked || sum != 0.0f ? sum * inv[g] : 0.0f;
-            Op::split(w, pf[g]);
         }
     };
     const auto rescale = [&] {
@@ -340,14 +394,16 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
         // Step x of a thread: its pieces of the values of tile x and the keys of x
         // + 1 go into LDS, the next ones are asked for, then the page numbers of
         // those after. (Scales go with the keys.)
-        constexpr int kParts = 4 * kPer + 4;
+        constexpr int kParts = 4 * kPer + (kOne ? 2 : 4);
         const auto part = [&](int x, int i) {
             if (i < 2 * kPer) {
                 store_v(x, i / 2, i % 2);
             } else if (i < 4 * kPer) {
                 store_k(x + 1, i / 2 - kPer, i % 2);
             } else if (i == 4 * kPer) {
-                store_scales(x + 1);
+                if constexpr (!kOne) {
+                    store_scales(x + 1);
+                }
                 load_v(v0 + x + 1);
             } else if (i == 4 * kPer + 1) {
                 load_k(v0 + x + 2);
@@ -359,29 +415,54 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
                 ids_k(v0 + x + 3);
             }
         };
+        // kOne, between steps x and x + 1 (in the vector phase, where no LDS read is
+        // in flight beside the scalar loads): the scales of tile x + 1, page numbers
+        const auto one_step = [&](int x) {
+            if constexpr (kOne) {
+                const float off = exists(c, one_v) ? 0.0f : __uint_as_float(0x7fc00000u);
+                const int64_t at = readable(c, one_v) * c.heads + kvh;
+                one_ks = uniform_load(c.k_scale + at) + off;
+                one_vs = uniform_load(c.v_scale + at) + off;
+                one_v = one_k;
+                one_k = one_page(v0 + x + 3);
+            }
+        };
         const auto step = [&](int x) {
 #pragma unroll
             for (int i = 0; i < kParts; ++i) {
                 part(x, i);
             }
         };
-        ids_k(v0);
-        load_scales(id_v(v0));
+        if constexpr (kOne) {
+            one_k = one_v = one_page(v0);
+        } else {
+            ids_k(v0);
+            load_scales(id_v(v0));
+            vid = id_v(v0);
+        }
         load_k(v0);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             store_k(0, i, 0);
             store_k(0, i, 1);
         }
-        store_scales(0);
-        vid = id_v(v0);
+        if constexpr (!kOne) {
+            store_scales(0);
+        }
         load_v(v0);
-        ids_k(v0 + 1);
-        load_k(v0 + 1);
-        load_scales(id_v(v0 + 1));
-        vid = id_v(v0 + 1);
-        sid = id_v(v0 + 2);
-        ids_k(v0 + 2);
+        if constexpr (kOne) {
+            one_step(-1);                          // scales of tile 0
+            one_v = one_k = one_page(v0 + 1);
+            load_k(v0 + 1);
+            one_k = one_page(v0 + 2);
+        } else {
+            ids_k(v0 + 1);
+            load_k(v0 + 1);
+            load_scales(id_v(v0 + 1));
+            vid = id_v(v0 + 1);
+            sid = id_v(v0 + 2);
+            ids_k(v0 + 2);
+        }
         meet();
         if (behind) {
             meet();
@@ -410,9 +491,12 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
         meet();
         for (int j = 1; j < nt; ++j) {
             weigh(j - 1);
+            one_step(j - 1);
             meet();
             rescale();
+            __builtin_amdgcn_s_setprio(2);         // before the other wave's vector phase: 168.7 -> 158.5 us (a prompt of 4096)
             both(j, [&](int i) { part(j, i); }, std::integral_constant<int, kParts>{});
+            __builtin_amdgcn_s_setprio(0);
             meet();
         }
         weigh(nt - 1);
@@ -469,38 +553,44 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
 
 }  // namespace
 
-int tiled_rows(int64_t d, bool f16, int64_t rows)
+int tiled_rows(int64_t d, bool f16, int64_t page, int64_t rows)
 {
-    if (d > 128 && !f16) {
+    if (d > 128 && (!f16 || page < kTile)) {
         return 0;                                  // three parts of 256 channels: more registers than there are
     }
-    if (d > 128 || !f16) {
+    if (d > (f16 ? 128 : 64)) {
         return 128;
     }
     return rows > 128 ? 256 : 128;
 }
 
+namespace {
+
+template <typename T, int DP, int NW>
+void launch_one(const AttnKern& k, const dim3& grid, hipStream_t s)
+{
+    if (k.c.page >= kTile) {
+        NNOPS_LAUNCH((attention_rows_tiled<T, DP, NW, true>), grid, dim3(64 * NW), 0, s, k);
+    } else {
+        NNOPS_LAUNCH((attention_rows_tiled<T, DP, NW, false>), grid, dim3(64 * NW), 0, s, k);
+    }
+}
+
+}  // namespace
+
 void launch_tiled(const AttnKern& k, const dim3& grid, bool f16, hipStream_t s)
 {
-    const int d = k.c.d, rows = k.tile_rows;
-    if (f16 && rows == 256) {
-        if (d <= 64) {
-            NNOPS_LAUNCH((attention_rows_tiled<_Float16, 64, 8>), grid, dim3(512), 0, s, k);
-        } else {
-            NNOPS_LAUNCH((attention_rows_tiled<_Float16, 128, 8>), grid, dim3(512), 0, s, k);
-        }
+    const int d = k.c.d;
+    if (f16 && k.tile_rows == 256) {
+        d <= 64 ? launch_one<_Float16, 64, 8>(k, grid, s) : launch_one<_Float16, 128, 8>(k, grid, s);
     } else if (f16) {
-        if (d <= 64) {
-            NNOPS_LAUNCH((attention_rows_tiled<_Float16, 64, 4>), grid, dim3(256), 0, s, k);
-        } else if (d <= 128) {
-            NNOPS_LAUNCH((attention_rows_tiled<_Float16, 128, 4>), grid, dim3(256), 0, s, k);
-        } else {
-            NNOPS_LAUNCH((attention_rows_tiled<_Float16, 256, 4>), grid, dim3(256), 0, s, k);
-        }
-    } else if (d <= 64) {
-        NNOPS_LAUNCH((attention_rows_tiled<float, 64, 4>), grid, dim3(256), 0, s, k);
+        d <= 64    ? launch_one<_Float16, 64, 4>(k, grid, s)
+        : d <= 128 ? launch_one<_Float16, 128, 4>(k, grid, s)
+                   : launch_one<_Float16, 256, 4>(k, grid, s);
+    } else if (k.tile_rows == 256) {
+        launch_one<float, 64, 8>(k, grid, s);
     } else {
-        NNOPS_LAUNCH((attention_rows_tiled<float, 128, 4>), grid, dim3(256), 0, s, k);
+        d <= 64 ? launch_one<float, 64, 4>(k, grid, s) : launch_one<float, 128, 4>(k, grid, s);
     }
 }
 
