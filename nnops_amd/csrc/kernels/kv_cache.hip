@@ -6,9 +6,11 @@
 // page fills.
 //
 // Bound: HBM: the new rows and their codes; reading back, the codes and the
-// values. One workgroup owns one page of a sequence, one head and one side, so
-// that a page's maximum needs no atomics and every run gives the same bits.
-// Writing, the rows are read twice, the second time from the CU's caches.
+// values; for few tokens the chain of loads (lengths, page table, codes). One
+// unit of waves owns one page of a sequence, one head and one side, so that a
+// page's maximum needs no atomics and every run gives the same bits: a single
+// wave where a page and head hold at most 4096 values, a workgroup of 4 waves
+// else. Rows stay in registers between the maximum and the codes.
 // Values lie transposed in a page (a channel's tokens side by side): a thread
 // takes two channels by 16 tokens, so that its lanes read and write whole rows
 // and its codes are 16-byte pieces.
@@ -79,6 +81,9 @@ struct RowsKern {
     void* v;
     int64_t ld_k, ld_v;
     int32_t per_seq;      // items of a sequence, equal rows each (0: found by search)
+    int32_t head_groups;  // groups of heads of an item, a workgroup (and side) each
+    int32_t group_heads;  // heads of a group
+    uint32_t row_magic;   // ceil(2^32 / x), x = group_heads d / 16 > 1: a division by x, reading
 };
 
 // Items of a sequence: the pages that its rows of the call fall in; one, of no
@@ -97,13 +102,13 @@ struct PagePart {
     int64_t row;
 };
 
-__device__ __forceinline__ bool page_part(const RowsKern& p, int64_t item, PagePart& t)
+__device__ __forceinline__ bool page_part(const RowsKern& p, uint32_t item, PagePart& t)
 {
     int b, j;
     SeqRows s;
     if (p.per_seq > 0) {
-        b = (int)(item / p.per_seq);
-        j = (int)(item - (int64_t)b * p.per_seq);
+        b = (int)(item / (uint32_t)p.per_seq);
+        j = (int)(item - (uint32_t)b * p.per_seq);
         s = seq_rows(p.c, b);
         if (j >= touched(p.c, s)) {
             return false;
@@ -140,19 +145,28 @@ __device__ __forceinline__ uint32_t rescaled(uint32_t d, float ratio)
     return o;
 }
 
-// blockIdx.x: item * heads + head; blockIdx.y: keys or values.
-template <typename T>
+// blockIdx.x: item, group of heads; blockIdx.y: keys or values. A unit of WAVES
+// waves has a head: 4 heads a workgroup, or one.
+template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void kv_write_kernel(const RowsKern p)
 {
+    constexpr int kLanes = 64 * WAVES;
+    constexpr int kHeldK = 4, kHeldV = 2;          // pieces of a thread that stay in registers
     __shared__ uint32_t s_max[4];
     const Paged& c = p.c;
-    const int64_t item = blockIdx.x / (unsigned)c.heads;
-    const int head = (int)(blockIdx.x - item * c.heads);
+    const uint32_t item = blockIdx.x / (uint32_t)p.head_groups;
+    const int group = (int)(blockIdx.x - item * p.head_groups);
     const bool values = blockIdx.y != 0;
     PagePart t;
     if (!page_part(p, item, t) || t.id < 0) {
         return;                                    // the whole workgroup
     }
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int head = WAVES == 1 ? group * 4 + wave : group;
+    if (head >= c.heads) {
+        return;                                    // (WAVES == 1: no barrier below)
+    }
+    const int lane = WAVES == 1 ? threadIdx.x % 64 : threadIdx.x;
     const int d = c.d, n = t.to - t.from;
     const int64_t ld = values ? p.ld_v : p.ld_k;
     const T* rows = static_cast<const T*>(values ? p.v : p.k) + t.row * ld + (int64_t)head * d;
@@ -160,26 +174,77 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const RowsKern p)
     int8_t* page = (values ? c.v : c.k) + ((int64_t)t.id * c.heads + head) * ((int64_t)c.page * d);
     const float old = t.from > 0 ? *scale : 0.0f;
 
-    uint32_t a = 0;
-    const int per_row = d / 8;
-    for (int i = threadIdx.x; i < n * per_row; i += 256) {
-        const int r = i / per_row, at = (i - r * per_row) * 8;
-        T x[8];
-        __builtin_memcpy(x, rows + r * ld + at, sizeof x);
+    // pieces: keys, 16 channels of a row; values, two channels of a group of 16 slots
+    const uint32_t per_row = d / 16, pairs = d / 2;
+    const int g0 = t.from / 16, groups = (t.to + 15) / 16 - g0;
+    const int pieces = values ? groups * (int)pairs : n * (int)per_row;
+    const auto load_k = [&](int i, T (&x)[16]) {
+        const uint32_t r = (uint32_t)i / per_row, at = ((uint32_t)i - r * per_row) * 16;
+        __builtin_memcpy(x, rows + (int64_t)r * ld + at, sizeof x);
+    };
+    const auto load_v = [&](int i, T (&x)[16][2]) {
+        const int g = (int)((uint32_t)i / pairs), ch = (i - g * (int)pairs) * 2, slot0 = (g0 + g) * 16;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            a = max(a, magnitude((float)x[e]));
+        for (int e = 0; e < 16; ++e) {
+            const int slot = slot0 + e;
+            x[e][0] = x[e][1] = (T)0.0f;
+            if (slot >= t.from && slot < t.to) {
+                __builtin_memcpy(x[e], rows + (int64_t)(slot - t.from) * ld + ch, sizeof x[e]);
+            }
+        }
+    };
+    T held_k[kHeldK][16], held_v[kHeldV][16][2];
+    uint32_t a = 0;
+    if (!values) {
+#pragma unroll
+        for (int h = 0; h < kHeldK; ++h) {
+            if (lane + h * kLanes < pieces) {
+                load_k(lane + h * kLanes, held_k[h]);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    a = max(a, magnitude((float)held_k[h][e]));
+                }
+            }
+        }
+        for (int i = lane + kHeldK * kLanes; i < pieces; i += kLanes) {
+            T x[16];
+            load_k(i, x);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                a = max(a, magnitude((float)x[e]));
+            }
+        }
+    } else {
+#pragma unroll
+        for (int h = 0; h < kHeldV; ++h) {
+            if (lane + h * kLanes < pieces) {
+                load_v(lane + h * kLanes, held_v[h]);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    a = max(a, max(magnitude((float)held_v[h][e][0]), magnitude((float)held_v[h][e][1])));
+                }
+            }
+        }
+        for (int i = lane + kHeldV * kLanes; i < pieces; i += kLanes) {
+            T x[16][2];
+            load_v(i, x);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                a = max(a, max(magnitude((float)x[e][0]), magnitude((float)x[e][1])));
+            }
         }
     }
 #pragma unroll
     for (int m = 1; m < 64; m *= 2) {
         a = max(a, (uint32_t)__shfl_xor((int)a, m));
     }
-    if (threadIdx.x % 64 == 0) {
-        s_max[threadIdx.x / 64] = a;
+    if constexpr (WAVES > 1) {
+        if (threadIdx.x % 64 == 0) {
+            s_max[wave] = a;
+        }
+        __syncthreads();                           // (every thread has read the old scale, too)
+        a = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
     }
-    __syncthreads();                               // every thread has read the old scale, too
-    a = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
     // a NaN (of the rows or of the page before) stays one; fmaxf would drop it
     const bool bad = a >= 0x7f800000u || !(old == old);
     const float s = bad ? __uint_as_float(0x7fc00000u)
@@ -187,83 +252,98 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const RowsKern p)
     const float inv = bad ? 0.0f : __fdiv_rn(1.0f, s);
     const bool grew = !bad && t.from > 0 && s > old;
     const float ratio = grew ? __fdiv_rn(old, s) : 1.0f;
-    if (threadIdx.x == 0) {
+    if (lane == 0) {
         *scale = s;
     }
 
     if (!values) {
-        // a thread: 16 codes of a token
-        const int per_tok = d / 16;
-        const int begin = grew ? 0 : t.from;
-        for (int i = threadIdx.x; i < (t.to - begin) * per_tok; i += 256) {
-            const int r = i / per_tok, at = (i - r * per_tok) * 16, slot = begin + r;
-            v4i* dst = reinterpret_cast<v4i*>(page + slot * d + at);
-            uint32_t o[4];
-            if (slot < t.from) {
+        const auto write = [&](int i, const T (&x)[16]) {
+            const uint32_t r = (uint32_t)i / per_row, at = ((uint32_t)i - r * per_row) * 16;
+            uint32_t o[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                o[e / 4] |= (bad ? 0u : code_byte((float)x[e], inv)) << (8 * (e % 4));
+            }
+            *reinterpret_cast<v4i*>(page + (t.from + r) * d + at) = v4i{(int)o[0], (int)o[1], (int)o[2], (int)o[3]};
+        };
+#pragma unroll
+        for (int h = 0; h < kHeldK; ++h) {
+            if (lane + h * kLanes < pieces) {
+                write(lane + h * kLanes, held_k[h]);
+            }
+        }
+        for (int i = lane + kHeldK * kLanes; i < pieces; i += kLanes) {
+            T x[16];
+            load_k(i, x);
+            write(i, x);
+        }
+        if (grew) {
+            for (int i = lane; i < t.from * (int)per_row; i += kLanes) {
+                v4i* at = reinterpret_cast<v4i*>(page) + i;            // rows of a page are dense
+                const v4i w = *at;
+                *at = v4i{(int)rescaled((uint32_t)w.x, ratio), (int)rescaled((uint32_t)w.y, ratio),
+                          (int)rescaled((uint32_t)w.z, ratio), (int)rescaled((uint32_t)w.w, ratio)};
+            }
+        }
+        return;
+    }
+    // groups that hold older tokens keep those, brought to the scale where it
+    // grew; whole groups of older tokens are touched only then
+    const auto write = [&](int i, const T (&x)[16][2]) {
+        const int g = (int)((uint32_t)i / pairs), ch = (i - g * (int)pairs) * 2, slot0 = (g0 + g) * 16;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            v4i* dst = reinterpret_cast<v4i*>(page + (ch + h) * c.page + slot0);
+            uint32_t o[4] = {0, 0, 0, 0};
+            if (slot0 < t.from || slot0 + 16 > t.to) {
                 const v4i w = *dst;
                 const uint32_t wd[4] = {(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    o[e] = rescaled(wd[e], ratio);
+                    o[e] = grew ? rescaled(wd[e], ratio) : wd[e];
                 }
-            } else {
-                T x[16];
-                __builtin_memcpy(x, rows + (slot - t.from) * ld + at, sizeof x);
+            }
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const uint32_t q = bad ? 0u : code_byte((float)x[e], inv);
-                    o[e / 4] = (e % 4 ? o[e / 4] : 0u) | q << (8 * (e % 4));
+            for (int e = 0; e < 16; ++e) {
+                if (slot0 + e >= t.from && slot0 + e < t.to) {
+                    const uint32_t q = bad ? 0u : code_byte((float)x[e][h], inv);
+                    o[e / 4] = (o[e / 4] & ~(0xffu << (8 * (e % 4)))) | q << (8 * (e % 4));
                 }
             }
             *dst = v4i{(int)o[0], (int)o[1], (int)o[2], (int)o[3]};
         }
-        return;
+    };
+#pragma unroll
+    for (int h = 0; h < kHeldV; ++h) {
+        if (lane + h * kLanes < pieces) {
+            write(lane + h * kLanes, held_v[h]);
+        }
     }
-    // a thread: two channels by a group of 16 tokens; groups with nothing to
-    // write are left out, older codes of a group kept or rescaled
-    const int g0 = grew ? 0 : t.from / 16, groups = (t.to + 15) / 16 - g0, pairs = d / 2;
-    for (int i = threadIdx.x; i < groups * pairs; i += 256) {
-        const int g = i / pairs, ch = (i - g * pairs) * 2, slot0 = (g0 + g) * 16;
-        v4i* dst[2] = {reinterpret_cast<v4i*>(page + ch * c.page + slot0),
-                       reinterpret_cast<v4i*>(page + (ch + 1) * c.page + slot0)};
-        uint32_t o[2][4] = {};
-        if (slot0 < t.from || slot0 + 16 > t.to) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const v4i w = *dst[h];
-                const uint32_t wd[4] = {(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    o[h][e] = grew ? rescaled(wd[e], ratio) : wd[e];
-                }
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int slot = slot0 + e;
-            if (slot >= t.from && slot < t.to) {
-                T x[2];
-                __builtin_memcpy(x, rows + (slot - t.from) * ld + ch, sizeof x);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t q = bad ? 0u : code_byte((float)x[h], inv);
-                    o[h][e / 4] = (o[h][e / 4] & ~(0xffu << (8 * (e % 4)))) | q << (8 * (e % 4));
-                }
-            }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            *dst[h] = v4i{(int)o[h][0], (int)o[h][1], (int)o[h][2], (int)o[h][3]};
+    for (int i = lane + kHeldV * kLanes; i < pieces; i += kLanes) {
+        T x[16][2];
+        load_v(i, x);
+        write(i, x);
+    }
+    if (grew) {
+        for (int i = lane; i < g0 * d; i += kLanes) {
+            const int g = (int)((uint32_t)i / (uint32_t)d), ch = i - g * d;
+            v4i* at = reinterpret_cast<v4i*>(page + ch * c.page + g * 16);
+            const v4i w = *at;
+            *at = v4i{(int)rescaled((uint32_t)w.x, ratio), (int)rescaled((uint32_t)w.y, ratio),
+                      (int)rescaled((uint32_t)w.z, ratio), (int)rescaled((uint32_t)w.w, ratio)};
         }
     }
 }
 
+// A workgroup reads one page of a group of heads, one side; the heads' pieces
+// side by side in a row, so that what it writes of a row is contiguous.
 template <typename T>
 __global__ __launch_bounds__(256) void kv_read_kernel(const RowsKern p)
 {
     const Paged& c = p.c;
-    const int64_t item = blockIdx.x / (unsigned)c.heads;
-    const int head = (int)(blockIdx.x - item * c.heads);
+    const uint32_t item = blockIdx.x / (uint32_t)p.head_groups;
+    const int head0 = (int)(blockIdx.x - item * p.head_groups) * p.group_heads;
+    const int heads = min(p.group_heads, c.heads - head0);
     const bool values = blockIdx.y != 0;
     PagePart t;
     if (!page_part(p, item, t)) {
@@ -271,49 +351,63 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const RowsKern p)
     }
     const int d = c.d;
     const int64_t ld = values ? p.ld_v : p.ld_k;
-    T* rows = static_cast<T*>(values ? p.v : p.k) + t.row * ld + (int64_t)head * d;
-    for (int64_t i = threadIdx.x; i < (int64_t)t.absent * d; i += 256) {
-        const int64_t r = i / d;
-        rows[(r - t.absent) * ld + (i - r * d)] = (T)0.0f;
+    T* rows = static_cast<T*>(values ? p.v : p.k) + t.row * ld + (int64_t)head0 * d;
+    const int width = heads * d;
+    for (int64_t i = threadIdx.x; i < (int64_t)t.absent * width; i += 256) {
+        const int64_t r = i / width;
+        rows[(r - t.absent) * ld + (i - r * width)] = (T)0.0f;
     }
     const bool there = t.id >= 0;
-    const int64_t at_page = there ? (int64_t)t.id * c.heads + head : 0;
-    const float s = there ? (values ? c.v_scale : c.k_scale)[at_page] : __uint_as_float(0x7fc00000u);
-    const int8_t* page = (values ? c.v : c.k) + at_page * ((int64_t)c.page * d);
+    const int64_t at_page = there ? (int64_t)t.id * c.heads + head0 : 0;
+    const float* scales = (values ? c.v_scale : c.k_scale) + at_page;
+    const uint32_t bytes = (uint32_t)c.page * d;
+    const int8_t* page = (values ? c.v : c.k) + at_page * (int64_t)bytes;
+    const float nan = __uint_as_float(0x7fc00000u);
     if (!values) {
-        const int per_tok = d / 16;
-        for (int i = threadIdx.x; i < (t.to - t.from) * per_tok; i += 256) {
-            const int r = i / per_tok, at = (i - r * per_tok) * 16;
-            const v4i w = there ? *reinterpret_cast<const v4i*>(page + (t.from + r) * d + at) : v4i{0, 0, 0, 0};
+        const uint32_t per_tok = d / 16, per_row = per_tok * p.group_heads;
+        const int n = (t.to - t.from) * (int)per_row;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < n; i += 256) {
+            const uint32_t r = per_row > 1 ? __umulhi((uint32_t)i, p.row_magic) : (uint32_t)i, in = (uint32_t)i - r * per_row;
+            const uint32_t h = in / per_tok, at = (in - h * per_tok) * 16;
+            if ((int)h >= heads) {
+                continue;
+            }
+            const v4i w = there ? *reinterpret_cast<const v4i*>(page + h * bytes + (t.from + r) * d + at) : v4i{0, 0, 0, 0};
+            const float s = there ? scales[h] : nan;
             const uint32_t wd[4] = {(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w};
             T y[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 y[e] = (T)__fmul_rn((float)(int8_t)(wd[e / 4] >> (8 * (e % 4))), s);
             }
-            __builtin_memcpy(rows + r * ld + at, y, sizeof y);
+            __builtin_memcpy(rows + (int64_t)r * ld + h * d + at, y, sizeof y);
         }
         return;
     }
-    const int g0 = t.from / 16, groups = (t.to + 15) / 16 - g0, pairs = d / 2;
-    for (int i = threadIdx.x; i < groups * pairs; i += 256) {
-        const int g = i / pairs, ch = (i - g * pairs) * 2, slot0 = (g0 + g) * 16;
+    const int g0 = t.from / 16, groups = (t.to + 15) / 16 - g0;
+    const uint32_t pairs = d / 2, all = pairs * heads;
+    for (int i = threadIdx.x; i < groups * (int)all; i += 256) {
+        const uint32_t g = (uint32_t)i / all, in = (uint32_t)i - g * all, h = in / pairs, ch = (in - h * pairs) * 2;
+        const int slot0 = (g0 + (int)g) * 16;
         uint32_t wd[2][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const v4i w = there ? *reinterpret_cast<const v4i*>(page + (ch + h) * c.page + slot0) : v4i{0, 0, 0, 0};
-            wd[h][0] = (uint32_t)w.x, wd[h][1] = (uint32_t)w.y, wd[h][2] = (uint32_t)w.z, wd[h][3] = (uint32_t)w.w;
+        for (int q = 0; q < 2; ++q) {
+            const v4i w = there ? *reinterpret_cast<const v4i*>(page + h * bytes + (ch + q) * c.page + slot0) : v4i{0, 0, 0, 0};
+            wd[q][0] = (uint32_t)w.x, wd[q][1] = (uint32_t)w.y, wd[q][2] = (uint32_t)w.z, wd[q][3] = (uint32_t)w.w;
         }
+        const float s = there ? scales[h] : nan;
+        T* dst = rows + (int64_t)(slot0 - t.from) * ld + (h * d + ch);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const int slot = slot0 + e;
             if (slot >= t.from && slot < t.to) {
                 T y[2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    y[h] = (T)__fmul_rn((float)(int8_t)(wd[h][e / 4] >> (8 * (e % 4))), s);
+                for (int q = 0; q < 2; ++q) {
+                    y[q] = (T)__fmul_rn((float)(int8_t)(wd[q][e / 4] >> (8 * (e % 4))), s);
                 }
-                __builtin_memcpy(rows + (slot - t.from) * ld + ch, y, sizeof y);
+                __builtin_memcpy(dst + e * ld, y, sizeof y);
             }
         }
     }
@@ -352,7 +446,7 @@ int check_rows(const NnopsKvRowsArgs* g)
     return -1;
 }
 
-RowsKern rows_kern(const NnopsKvRowsArgs* g, int32_t per_seq)
+RowsKern rows_kern(const NnopsKvRowsArgs* g, int32_t per_seq, int32_t group_heads)
 {
     RowsKern k{};
     k.c = paged(g->cache, g->rows);
@@ -361,6 +455,10 @@ RowsKern rows_kern(const NnopsKvRowsArgs* g, int32_t per_seq)
     k.ld_k = g->ld_k;
     k.ld_v = g->ld_v;
     k.per_seq = per_seq;
+    k.group_heads = group_heads;
+    k.head_groups = (k.c.heads + group_heads - 1) / group_heads;
+    const uint32_t per_row = (uint32_t)(group_heads * (k.c.d / 16));
+    k.row_magic = (uint32_t)(((1ull << 32) + per_row - 1) / per_row);
     return k;
 }
 
@@ -377,20 +475,27 @@ extern "C" int nnops_hip_kv_cache_write(const NnopsKvRowsArgs* g, void* stream)
         return rc;
     }
     int32_t per_seq = 0;
-    const int64_t n = items(g, per_seq) * g->cache.heads;
+    const int64_t n = items(g, per_seq);
     if (n == 0 || g->cache.pages == 0) {
         return NNOPS_OK;                          // no page to write to
     }
-    if (n > INT32_MAX / 256) {
+    const bool small = g->cache.page_tokens * g->cache.head_dim <= 4096;
+    const RowsKern k = rows_kern(g, per_seq, small ? 4 : 1);
+    if (n * k.head_groups > INT32_MAX / 256) {
         return NNOPS_UNSUPPORTED;
     }
-    const RowsKern k = rows_kern(g, per_seq);
-    const dim3 grid((unsigned)n, 2);
+    const dim3 grid((unsigned)(n * k.head_groups), 2);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (g->f16) {
-        NNOPS_LAUNCH(kv_write_kernel<_Float16>, grid, dim3(256), 0, s, k);
+        if (small) {
+            NNOPS_LAUNCH((kv_write_kernel<_Float16, 1>), grid, dim3(256), 0, s, k);
+        } else {
+            NNOPS_LAUNCH((kv_write_kernel<_Float16, 4>), grid, dim3(256), 0, s, k);
+        }
+    } else if (small) {
+        NNOPS_LAUNCH((kv_write_kernel<float, 1>), grid, dim3(256), 0, s, k);
     } else {
-        NNOPS_LAUNCH(kv_write_kernel<float>, grid, dim3(256), 0, s, k);
+        NNOPS_LAUNCH((kv_write_kernel<float, 4>), grid, dim3(256), 0, s, k);
     }
     return hipGetLastError() == hipSuccess ? NNOPS_OK : NNOPS_INTERNAL;
 }
@@ -403,12 +508,19 @@ extern "C" int nnops_hip_kv_cache_read(const NnopsKvRowsArgs* g, void* stream)
         return rc;
     }
     int32_t per_seq = 0;
-    const int64_t n = items(g, per_seq) * g->cache.heads;
-    if (n > INT32_MAX / 256) {
+    const int64_t n = items(g, per_seq);
+    // heads of a workgroup: 8192 codes, as long as there are workgroups to fill
+    // the chip (32 sequences of 1000: 26.1 us, 28.0 with 16384, 32.3 with 32768)
+    int32_t group = (int32_t)(8192 / (g->cache.page_tokens * g->cache.head_dim));
+    group = group < 1 ? 1 : group > g->cache.heads ? (int32_t)g->cache.heads : group;
+    while (group > 1 && n * 2 * ((g->cache.heads + group - 1) / group) < 2048) {
+        group /= 2;
+    }
+    const RowsKern k = rows_kern(g, per_seq, group);
+    if (n * k.head_groups > INT32_MAX / 256) {
         return NNOPS_UNSUPPORTED;
     }
-    const RowsKern k = rows_kern(g, per_seq);
-    const dim3 grid((unsigned)n, 2);
+    const dim3 grid((unsigned)(n * k.head_groups), 2);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (g->f16) {
         NNOPS_LAUNCH(kv_read_kernel<_Float16>, grid, dim3(256), 0, s, k);

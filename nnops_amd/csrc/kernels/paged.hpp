@@ -50,39 +50,38 @@ __device__ __forceinline__ int page_of(const Paged& p, int b, int page)
 }
 
 // Work item w of a launch that numbers count(sequence) items per sequence one
-// after another: its sequence and its number there; false past the last. Whole
-// waves call it (each wave searches for itself, 64 sequences a step); w is the
-// same in all lanes.
+// after another (fewer than 2^31 in all): its sequence and its number there;
+// false past the last. Whole waves call it (each wave searches for itself, 64
+// sequences a step); w is the same in all lanes.
 template <typename Count>
-__device__ __forceinline__ bool find_item(const Paged& p, int64_t w, Count count, int& b, int& j, SeqRows& seq)
+__device__ __forceinline__ bool find_item(const Paged& p, uint32_t w, Count count, int& b, int& j, SeqRows& seq)
 {
     const int lane = threadIdx.x % 64;
-    int64_t before = 0;
+    uint32_t before = 0;
     for (int base = 0; base < p.seqs; base += 64) {
         SeqRows s{0, 0, 0};
-        int c = 0;
+        uint32_t c = 0;
         if (base + lane < p.seqs) {
             s = seq_rows(p, base + lane);
-            c = count(s);
+            c = (uint32_t)count(s);
         }
-        int64_t upto = c;
+        uint32_t upto = c;
 #pragma unroll
         for (int m = 1; m < 64; m *= 2) {
-            const int64_t other = __shfl_up(upto, m);
-            upto += lane >= m ? other : 0;
+            const uint32_t other = (uint32_t)__shfl_up((int)upto, m);
+            upto += lane >= m ? other : 0u;
         }
         const uint64_t hit = __ballot(before + upto > w);
         if (hit != 0) {
             const int l = __builtin_ctzll(hit);
-            const int64_t first = before + __shfl(upto, l) - __shfl(c, l);
-            b = __builtin_amdgcn_readfirstlane(base + l);
-            j = __builtin_amdgcn_readfirstlane((int)(w - first));
-            seq.start = __builtin_amdgcn_readfirstlane(__shfl(s.start, l));
-            seq.n = __builtin_amdgcn_readfirstlane(__shfl(s.n, l));
-            seq.len = __builtin_amdgcn_readfirstlane(__shfl(s.len, l));
+            b = base + l;
+            j = (int)(w - before) - __builtin_amdgcn_readlane((int)(upto - c), l);
+            seq.start = __builtin_amdgcn_readlane(s.start, l);
+            seq.n = __builtin_amdgcn_readlane(s.n, l);
+            seq.len = __builtin_amdgcn_readlane(s.len, l);
             return true;
         }
-        before += __shfl(upto, 63);
+        before += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
     }
     return false;
 }
