@@ -569,9 +569,9 @@ namespace {
 template <typename T, int DP, int NW>
 void launch_one(const AttnKern& k, const dim3& grid, hipStream_t s)
 {
-    if (k.c.page >= kTile) {
+    if (DP > 128 || k.c.page >= kTile) {           // (wider heads come with such pages only)
         NNOPS_LAUNCH((attention_rows_tiled<T, DP, NW, true>), grid, dim3(64 * NW), 0, s, k);
-    } else {
+    } else if constexpr (DP <= 128) {
         NNOPS_LAUNCH((attention_rows_tiled<T, DP, NW, false>), grid, dim3(64 * NW), 0, s, k);
     }
 }

@@ -107,23 +107,24 @@ def attention(q, kc, vc, ks, vs, table, lens, rows, *, scale=None, window=0, sin
             k = (kc[ids, h].astype(np.float64) * ks[ids, h].astype(np.float64)[:, None, None] * bad).reshape(-1, d)[:length]
             v = (vc[ids, h].astype(np.float64) * vs[ids, h].astype(np.float64)[:, None, None]) * bad
             v = v.transpose(0, 2, 1).reshape(-1, d)[:length]
+            mine = slice(h * (qh // heads), (h + 1) * (qh // heads))
+            size_k, size_v = abs(k), abs(v)
             for i in range(n):
                 p = length - n + i
-                j = np.arange(length)
-                seen = j <= p
-                if window:
-                    seen &= (p - j < window) | (j < sinks)
-                if p < 0 or not seen.any():
+                if p < 0:
                     continue
-                for m in range(h * (qh // heads), (h + 1) * (qh // heads)):
-                    x = q[at + i, m] @ k[seen].T * scale
-                    with np.errstate(invalid="ignore"):
-                        e = np.exp(x - x.max())
-                    out[at + i, m] = e @ v[seen] / e.sum()
-                    weight[at + i, m] = e @ abs(v[seen]) / e.sum()
-                    with np.errstate(invalid="ignore"):
-                        top = np.max(abs(q[at + i, m]) @ abs(k[seen]).T * scale)
-                    spread = max(spread, 2.0 * top if np.isfinite(top) else 0.0)
+                seen = slice(0, p + 1)
+                if window:
+                    j = np.arange(p + 1)
+                    seen = np.flatnonzero((p - j < window) | (j < sinks))
+                x = q[at + i, mine] @ k[seen].T * scale
+                with np.errstate(invalid="ignore"):
+                    e = np.exp(x - x.max(axis=1, keepdims=True))
+                    e /= e.sum(axis=1, keepdims=True)
+                    top = (abs(q[at + i, mine]) @ size_k[seen].T).max() * scale
+                    out[at + i, mine] = e @ v[seen]
+                    weight[at + i, mine] = e @ size_v[seen]
+                spread = max(spread, 2.0 * top if np.isfinite(top) else 0.0)
         at += n
     return out.reshape(-1, qh * d), weight.reshape(-1, qh * d), spread
 
@@ -132,8 +133,8 @@ def attention_tolerance(f16, out, weight, spread, v_scale):
     """How far a result may be from the 64-bit one. A score x carries an error of
     a few roundings of what it is made of (its products, log2 of the value
     scale), so that a probability is off by the factor 1 + delta; the
-    probabilities enter the product as f16 (f32 rows: as two f16 parts, 22
-    bits); the result is rounded once."""
+    probabilities enter the product as f16 (f32 rows: as three bf16 parts, all
+    their 24 bits); the result is rounded once."""
     logs = np.abs(np.log2(v_scale[np.isfinite(v_scale) & (v_scale > 0)])).max() if v_scale.size else 0.0
     delta = 4.0 * 2.0 ** -24 * (1.45 * spread + logs + 16.0) + 2.0 ** -20
     part = 2.0 ** -11 if f16 else 2.0 ** -21

@@ -113,6 +113,111 @@ def test_long(tokens, page, group, n):
     _check(q.astype(np.float32), cache, lens, [n] * 3, ragged=True, window=1500, sinks=100)
 
 
+# Calls with rows enough for the tiles that share their codes: more than 96 rows
+# (tokens x heads of a group) a sequence at the mean and 128 tiles or more, of
+# 128 rows, or of 256 where the mean is past 128.
+TILES = [(128, 64, 16, 4, True), (128, 16, 16, 4, True), (64, 128, 32, 2, True), (80, 32, 16, 5, True),
+         (112, 256, 16, 8, True), (16, 16, 16, 4, True), (256, 64, 16, 4, True), (192, 128, 16, 3, True),
+         (128, 64, 16, 4, False), (96, 16, 16, 4, False), (64, 64, 16, 4, False), (48, 32, 16, 5, False)]
+
+
+def _mixed(total):
+    """Eight sequences, ragged: an empty one, one token, a whole prompt, rows
+    behind prefixes that end inside pages and tiles."""
+    lens, rows = [130, 70, 9, 200, 64, 33, 600, 1], [33, 70, 0, 40, 64, 33, 12, 1]
+    if total > 300:
+        rows[0], rows[3], rows[6] = 130, 101, 80
+    return lens, rows
+
+
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("d,page,heads,group,f16", TILES)
+def test_tiles(d, page, heads, group, f16, many):
+    announce(f"attention tiles d={d} page={page} heads={heads} group={group} f16={f16} many={many}")
+    lens, rows = _mixed(400 if many else 200)
+    cache = _cache(len(lens), 600, heads, page, d)
+    _check(_q(21, sum(rows), heads * group * d, f16), cache, lens, rows, ragged=True, pad=8 if many else 1)
+
+
+@pytest.mark.parametrize("d,page,heads,group,f16", TILES[:1] + TILES[3:4] + TILES[6:7] + TILES[8:11])
+def test_tiles_of_equal_rows(d, page, heads, group, f16):
+    """As many rows each, without starts; more rows than tokens among them."""
+    announce(f"attention equal tiles d={d} page={page} heads={heads} group={group} f16={f16}")
+    lens, n = [34, 12, 0, 64, 65, 300, 511, 513, 40], 34
+    cache = _cache(len(lens), 520, heads, page, d)
+    q = _q(22, n * len(lens), heads * group * d, f16)
+    got = _check(q, cache, lens, [n] * len(lens), ragged=False)
+    assert np.all(got[n:n + 22] == 0) and np.all(got[2 * n:3 * n] == 0)
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (16, 4), (64, 0), (100, 70), (300, 5), (7, 1 << 40)])
+@pytest.mark.parametrize("page,f16", [(16, True), (64, True), (128, False), (32, False)])
+def test_windows_in_tiles(window, sinks, page, f16):
+    announce(f"attention tiles window={window} sinks={sinks} page={page} f16={f16}")
+    heads, group, d = 16, 4, 64
+    lens, rows = _mixed(400)
+    cache = _cache(len(lens), 600, heads, page, d)
+    _check(_q(23, sum(rows), heads * group * d, f16), cache, lens, rows, ragged=True, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("page,f16", [(64, True), (16, True), (64, False)])
+def test_tiles_that_are_split(page, f16):
+    """Few tiles over a long sequence, so many splits that they are joined by a
+    workgroup a row; beside one that has a single tile of tokens."""
+    announce(f"attention split tiles page={page} f16={f16}")
+    heads, group, d, n, tokens = 4, 4, 128, 26, 33000
+    cache = _cache(2, tokens, heads, page, d)
+    q = _q(24, 2 * n, heads * group * d, f16)
+    _check(q, cache, [tokens, 50], [n, n], ragged=False)
+    _check(q, cache, [tokens, 50], [n, n], ragged=True, window=20000, sinks=100)
+
+
+@pytest.mark.parametrize("page,f16", [(64, True), (16, True), (128, False), (32, False)])
+def test_hidden_values_do_not_show_in_tiles(page, f16):
+    """The same bits whatever lies past the rows' positions or before their
+    window; a page that exists nowhere, a NaN scale and a NaN query show in the
+    rows and heads that see them alone."""
+    announce(f"attention hidden in tiles page={page} f16={f16}")
+    heads, group, d, n, seqs = 16, 4, 64, 40, 8
+    lens = [4 * page + 7] + [300] * (seqs - 1)
+    kc, vc, ks, vs, table = clean = _cache(seqs, 4 * page + 320, heads, page, d)
+    q = _q(25, seqs * n, heads * group * d, f16)
+    kw = dict(ragged=False)
+    want = _check(q, clean, lens, [n] * seqs, **kw)
+    table = table.copy()
+    for b in range(seqs):
+        table[b, -(-lens[b] // page):] = (-5, 1 << 30)[b % 2]
+    assert np.array_equal(want, _run(q, (kc, vc, ks, vs, table), lens, [n] * seqs, **kw))
+    # the last 7 tokens' page of the first sequence: a NaN in one head
+    k2, v2 = ks.copy(), vs.copy()
+    k2[table[0, 4], 3] = np.nan
+    v2[table[0, 4], 5] = np.nan
+    got = _run(q, (kc, vc, k2, v2, table), lens, [n] * seqs, **kw).reshape(-1, heads, group * d).astype(np.float64)
+    hit = np.zeros(got.shape, bool)
+    hit[n - 7:n, [3, 5]] = True
+    assert np.isnan(got[hit]).all() and np.array_equal(got[~hit], want.reshape(got.shape)[~hit])
+    t2 = table.copy()
+    t2[1, 299 // page] = 1 << 30
+    got = _run(q, (kc, vc, ks, vs, t2), lens, [n] * seqs, **kw)
+    first = max(0, 299 // page * page - (300 - n))          # the first row at or past the page
+    assert np.isnan(got[n + first:2 * n]).all()
+    assert np.array_equal(got[:n + first], want[:n + first]) and np.array_equal(got[2 * n:], want[2 * n:])
+    q2 = q.copy()
+    q2[n + 3, 5], q2[3 * n, d + 1] = np.nan, np.inf
+    got = _run(q2, (kc, vc, ks, vs, table), lens, [n] * seqs, **kw)
+    hit = np.zeros(got.shape, bool)
+    hit[n + 3, :d], hit[3 * n, d:2 * d] = True, True
+    assert np.isnan(got[hit]).all() and np.array_equal(got[~hit], want[~hit])
+    # a window that has moved past the first pages
+    kw = dict(ragged=False, window=60)
+    want = _run(q, clean, lens, [n] * seqs, **kw)
+    past = (300 - n - 60) // page
+    k2, v2, t2 = ks.copy(), vs.copy(), table.copy()
+    if past:
+        k2[table[1, :past]], v2[table[2, :past]], t2[3, 0] = np.nan, np.inf, -1
+        assert np.array_equal(want, _run(q, (kc, vc, k2, v2, t2), lens, [n] * seqs, **kw))
+
+
 def test_scales_far_apart():
     """Pages whose value scales differ by powers of ten, pages of zeros, the
     smallest scale; a scale of 0 reads as zeros."""
