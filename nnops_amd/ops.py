@@ -96,11 +96,18 @@ def _stream_ptr(stream):
     return raw(device())
 
 
-def _workspace(nbytes, device):
+def _workspace(nbytes, device, stream=None):
+    """A buffer of the stream that uses it: once the call has returned, its
+    memory goes to later work of that stream only."""
     import torch
     if nbytes == 0:
         return None
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    if stream is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream()
+    with torch.cuda.stream(stream):
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 def _epilogue(ep, act=None, min_clip=-math.inf, max_clip=math.inf, quant=L.EQ_NONE,
@@ -208,7 +215,7 @@ class _Op:
         ai, ni = self._arr(inputs)
         ao, no = self._arr(outputs)
         if workspace is None:
-            workspace = _workspace(L.lib().nnops_op_workspace_size(self._h, ai, ni, ao, no), device)
+            workspace = _workspace(L.lib().nnops_op_workspace_size(self._h, ai, ni, ao, no), device, stream)
         return L.lib().nnops_op_compute(self._h, ao, no, ai, ni, _stream_ptr(stream), _ptr(workspace))
 
 
@@ -409,7 +416,7 @@ def gemm_i8(a, b, c, *, trans_a=False, trans_b=False, bias=None, out_kind=L.OUT_
         return rc
     need = lib.nnops_hip_gemm_i8_workspace_size(C.byref(g))
     if workspace is None:
-        workspace = _workspace(need, a.device)
+        workspace = _workspace(need, a.device, stream)
     rc = lib.nnops_hip_gemm_i8(C.byref(g), _ptr(workspace), need, _stream_ptr(stream))
     if check and rc != 0:
         raise RuntimeError(f"nnops_hip_gemm_i8 failed: status {rc}")
@@ -430,7 +437,7 @@ def gemm_fp(a, b, c, *, trans_b=True, alpha=1.0, workspace=None, stream=None, ch
     lib = L.lib()
     need = lib.nnops_hip_gemm_fp_workspace_size(C.byref(g))
     if workspace is None:
-        workspace = _workspace(need, a.device)
+        workspace = _workspace(need, a.device, stream)
     rc = lib.nnops_hip_gemm_fp(C.byref(g), _ptr(workspace), need, _stream_ptr(stream))
     if check and rc != 0:
         raise RuntimeError(f"nnops_hip_gemm_fp failed: status {rc}")
@@ -452,7 +459,7 @@ def gemm_q4_1(a, b, c, *, n, trans_b=True, ldb_bytes=None, workspace=None, strea
     lib = L.lib()
     need = lib.nnops_hip_gemm_q4_1_workspace_size(C.byref(g))
     if workspace is None:
-        workspace = _workspace(need, a.device)
+        workspace = _workspace(need, a.device, stream)
     rc = lib.nnops_hip_gemm_q4_1(C.byref(g), _ptr(workspace), need, _stream_ptr(stream))
     if check and rc != 0:
         raise RuntimeError(f"nnops_hip_gemm_q4_1 failed: status {rc}")
