@@ -445,7 +445,12 @@ struct AttnPlan {
 // (ragged calls: by their mean). Splits of the longest sequence that the page
 // table has room for: as many workgroups as the chip holds at once (more of
 // them were slower: one token over 126976, 58 us with 512, 67 with 768, 72 with
-// 1024), no fewer than 4 tiles each.
+// 1024), no fewer than 4 tiles each, and none where a wave has no more than two
+// tiles without (f16 rows; split / not, one token of each, us: 8 x 300 9.8 / 8.6,
+// 32 x 300 11.6 / 8.9, 1 x 500 9.7 / 9.1, 1 x 777 9.8 / 11.6; f32 2 x 300 11.3 /
+// 11.8). Joining in the same launch, by the workgroup that is last to finish,
+// took as long as the second launch: its words go past the caches, one round
+// trip after another (1 x 777 10.2 us, 64 x 4096 75.1, 1 x 126976 66.0).
 AttnPlan attn_plan(const NnopsCacheAttentionArgs* g)
 {
     AttnPlan a{};
@@ -479,7 +484,7 @@ AttnPlan attn_plan(const NnopsCacheAttentionArgs* g)
     a.per_seq = g->cache.row_starts == nullptr ? (int32_t)(a.items / (b * heads)) : 0;
     const int64_t tiles = tiles_of(a.tile_rows);
     int64_t splits = ((a.tiled ? 256 : 512) + a.items - 1) / a.items;
-    const int64_t most = (tiles + 3) / 4;
+    const int64_t most = tiles <= 8 && g->f16 && d <= 128 && !a.tiled ? 1 : (tiles + 3) / 4;
     splits = splits < most ? splits : most;
     splits = splits > 1 ? splits : 1;
     const int64_t chunk = ((tiles + splits - 1) / splits + 3) / 4 * 4;
@@ -520,7 +525,9 @@ void launch_attention(const AttnKern& k, const AttnPlan& a, hipStream_t s)
     } else {
         NNOPS_LAUNCH((attention_rows16<T, 256>), grid, dim3(256), 0, s, k);
     }
-    if (a.splits > 1 && a.splits <= kFewSplits) {
+    // (a wave per row where few rows and 4 splits leave it waiting: 8 x 1 of 1500
+    // 13.8 us, 12.6 with a workgroup; 1 x 64 of 2000 16.9 and 19.5)
+    if (a.splits > 1 && a.splits <= kFewSplits && (a.splits <= 3 || k.c.rows * k.q_heads >= 1024)) {
         NNOPS_LAUNCH(attention_join_few<T>, dim3((unsigned)((k.c.rows * k.q_heads + 3) / 4)), dim3(256), 0, s, k);
     } else if (a.splits > 1) {
         NNOPS_LAUNCH(attention_join<T>, dim3((unsigned)(k.c.rows * k.q_heads)), dim3(256), 0, s, k);
