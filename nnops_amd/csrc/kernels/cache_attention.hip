@@ -441,7 +441,10 @@ struct AttnPlan {
 //   16 x 16 of 2048 tokens  41.0 / 34.2     64 x 33 of 300    29.6 / 51.9
 //   16 x 32 of 2048         48.3 / 49.4     64 x 64 of 64     32.2 / 70.0
 //   1 x 64 of 4096          24.6 / 24.8     16 x 128 of 2048  65.2 / 145
-//   1 x 256 of 4096         43.0 / 59.0     4 x 300 of 2500, 16 / 4 heads, d 64, f32  65.1 / 56.0
+//   1 x 256 of 4096         43.0 / 59.0     1 x 64 of 8000    28.8 / 36.2
+//   1 x 128 of 2500         28.2 / 27.1     1 x 256 of 1000   27.4 / 18.5
+//   1 x 64 of 8000, f32     41.7 / 56.1     1 x 256 of 1000, f32  32.6 / 29.4
+//   16 / 4 heads, d 64: 1 x 256 of 8000 37.7 / 39.9, f32 46.8 / 62.0; of 2500 24.3 / 19.5
 // (ragged calls: by their mean). Splits of the longest sequence that the page
 // table has room for: as many workgroups as the chip holds at once (more of
 // them were slower: one token over 126976, 58 us with 512, 67 with 768, 72 with
@@ -475,7 +478,7 @@ AttnPlan attn_plan(const NnopsCacheAttentionArgs* g)
     a.tile_rows = kRows;
     if (const int rows = mean > 96 ? tiled_rows(d, g->f16, g->cache.page_tokens, mean) : 0; rows > 0) {
         const int64_t items = items_of(rows);
-        if (items >= 128 || items * tiles_of(rows) * d >= 1 << 18) {
+        if (items >= 128 || items * tiles_of(rows) * d >= 7 << 14) {
             a.tiled = true;
             a.tile_rows = rows;
         }
