@@ -302,20 +302,23 @@ __device__ __forceinline__ int splits_of(const AttnKern& p, int token, int qh)
     return rt.active;
 }
 
-// Joins the splits of the rows that have more than one. Few splits: a wave per
-// row, 4 channels a lane.
+// Joins the splits of the rows that have more than one. Few splits: 4 channels
+// of a row by a lane, as many rows a wave as that gives.
 constexpr int kFewSplits = 8;
+
+__host__ __device__ __forceinline__ int join_lanes(int d) { return d <= 64 ? 16 : d <= 128 ? 32 : 64; }
 
 template <typename T>
 __global__ __launch_bounds__(256) void attention_join_few(const AttnKern p)
 {
-    const uint32_t i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int lanes = join_lanes(p.c.d);
+    const uint32_t i = (blockIdx.x * 256 + threadIdx.x) / (uint32_t)lanes;
     const int token = (int)(i / (uint32_t)p.q_heads), qh = (int)(i - (uint32_t)token * p.q_heads);
     if (token >= p.c.rows) {
         return;
     }
     const int active = splits_of(p, token, qh);
-    const int d = p.c.d, ch = threadIdx.x % 64 * 4;
+    const int d = p.c.d, ch = threadIdx.x % (uint32_t)lanes * 4;
     if (active <= 1 || ch >= d) {
         return;
     }
@@ -531,7 +534,8 @@ void launch_attention(const AttnKern& k, const AttnPlan& a, hipStream_t s)
     // (a wave per row where few rows and 4 splits leave it waiting: 8 x 1 of 1500
     // 13.8 us, 12.6 with a workgroup; 1 x 64 of 2000 16.9 and 19.5)
     if (a.splits > 1 && a.splits <= kFewSplits && (a.splits <= 3 || k.c.rows * k.q_heads >= 1024)) {
-        NNOPS_LAUNCH(attention_join_few<T>, dim3((unsigned)((k.c.rows * k.q_heads + 3) / 4)), dim3(256), 0, s, k);
+        const int rows = 256 / join_lanes(k.c.d);   // of a workgroup
+        NNOPS_LAUNCH(attention_join_few<T>, dim3((unsigned)((k.c.rows * k.q_heads + rows - 1) / rows)), dim3(256), 0, s, k);
     } else if (a.splits > 1) {
         NNOPS_LAUNCH(attention_join<T>, dim3((unsigned)(k.c.rows * k.q_heads)), dim3(256), 0, s, k);
     }
