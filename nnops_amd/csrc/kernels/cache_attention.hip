@@ -443,11 +443,13 @@ struct AttnPlan {
 // KV heads, d 128, f16, but where said):
 //   16 x 16 of 2048 tokens  41.0 / 34.2     64 x 33 of 300    29.6 / 51.9
 //   16 x 32 of 2048         48.3 / 49.4     64 x 64 of 64     32.2 / 70.0
-//   1 x 64 of 4096          24.6 / 24.8     16 x 128 of 2048  65.2 / 145
-//   1 x 256 of 4096         43.0 / 59.0     1 x 64 of 8000    28.8 / 36.2
-//   1 x 128 of 2500         28.2 / 27.1     1 x 256 of 1000   27.4 / 18.5
-//   1 x 64 of 8000, f32     41.7 / 56.1     1 x 256 of 1000, f32  32.6 / 29.4
-//   16 / 4 heads, d 64: 1 x 256 of 8000 37.7 / 39.9, f32 46.8 / 62.0; of 2500 24.3 / 19.5
+//   1 x 64 of 2500          25.1 / 19.7     1 x 64 of 8000    28.7 / 36.2
+//   1 x 128 of 2500         28.1 / 26.7     1 x 128 of 8000   38.0 / 60.0
+//   1 x 256 of 1000         25.9 / 18.4     1 x 256 of 8000   53.1 / 105
+//   f32 1 x 64 of 1000      25.1 / 19.1     f32 1 x 64 of 8000  41.7 / 55.8
+//   16 / 4 heads, d 64: 16 x 128 of 128 9.0 / 12.5, of 300 17.3 / 15.2; 1 x 256 of
+//   8000 37.8 / 38.1, f32 46.9 / 59.9; 24 sequences of 1 to 100 rows of 2500
+//   39.2 / 27.4, f32 58.9 / 44.2; of 1 to 300, f32, 94.4 / 108
 // (ragged calls: by their mean). Splits of the longest sequence that the page
 // table has room for: as many workgroups as the chip holds at once (more of
 // them were slower: one token over 126976, 58 us with 512, 67 with 768, 72 with
@@ -480,8 +482,11 @@ AttnPlan attn_plan(const NnopsCacheAttentionArgs* g)
     };
     a.tile_rows = kRows;
     if (const int rows = mean > 96 ? tiled_rows(d, g->f16, g->cache.page_tokens, mean) : 0; rows > 0) {
-        const int64_t items = items_of(rows);
-        if (items >= 128 || items * tiles_of(rows) * d >= 7 << 14) {
+        // (tiles that are sure to be full; heads of 64 channels and fewer gain less)
+        const bool ragged = g->cache.row_starts != nullptr;
+        const int64_t items = ragged ? g->rows * group / rows * heads : items_of(rows);
+        const int64_t least = d <= 64 && (g->f16 || ragged) ? 7 << 15 : 7 << 14;
+        if (items >= 128 || items * tiles_of(rows) * d >= least) {
             a.tiled = true;
             a.tile_rows = rows;
         }

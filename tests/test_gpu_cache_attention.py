@@ -114,11 +114,11 @@ def test_long(tokens, page, group, n):
 
 
 # Calls with rows enough for the tiles that share their codes: more than 96 rows
-# (tokens x heads of a group) a sequence at the mean and 128 tiles or more, of
-# 128 rows, or of 256 where the mean is past 128.
-TILES = [(128, 64, 16, 4, True), (128, 16, 16, 4, True), (64, 128, 32, 2, True), (80, 32, 16, 5, True),
-         (112, 256, 16, 8, True), (16, 16, 16, 4, True), (256, 64, 16, 4, True), (192, 128, 16, 3, True),
-         (128, 64, 16, 4, False), (96, 16, 16, 4, False), (64, 64, 16, 4, False), (48, 32, 16, 5, False)]
+# (tokens x heads of a group) a sequence at the mean and 128 full tiles or more,
+# of 128 rows, or of 256 where the mean is past 128.
+TILES = [(128, 64, 32, 4, True), (128, 16, 32, 4, True), (64, 128, 32, 4, True), (80, 32, 32, 5, True),
+         (112, 256, 24, 8, True), (16, 16, 32, 4, True), (256, 64, 32, 4, True), (192, 128, 32, 4, True),
+         (128, 64, 32, 4, False), (96, 16, 32, 4, False), (64, 64, 32, 4, False), (48, 32, 32, 5, False)]
 
 
 def _mixed(total):
@@ -154,7 +154,7 @@ def test_tiles_of_equal_rows(d, page, heads, group, f16):
 @pytest.mark.parametrize("page,f16", [(16, True), (64, True), (128, False), (32, False)])
 def test_windows_in_tiles(window, sinks, page, f16):
     announce(f"attention tiles window={window} sinks={sinks} page={page} f16={f16}")
-    heads, group, d = 16, 4, 64
+    heads, group, d = 32, 4, 64
     lens, rows = _mixed(400)
     cache = _cache(len(lens), 600, heads, page, d)
     _check(_q(23, sum(rows), heads * group * d, f16), cache, lens, rows, ragged=True, window=window, sinks=sinks)
