@@ -136,6 +136,45 @@ __device__ __forceinline__ uint32_t code_byte(float x, float inv)
     return (uint32_t)min(max(q, -127), 127) & 0xffu;
 }
 
+// The codes of four new values. Their magnitudes are a page's largest at most,
+// so that x inv is 127 (1 + 2^-22) at most and needs no clamp, and adding 1.5 2^23
+// leaves its nearest integer (ties to even) in the sum's lowest byte.
+template <typename T>
+__device__ __forceinline__ uint32_t new_codes(T x0, T x1, T x2, T x3, float inv)
+{
+    const float magic = 12582912.0f;
+    const uint32_t u0 = __float_as_uint(__fadd_rn(__fmul_rn((float)x0, inv), magic));
+    const uint32_t u1 = __float_as_uint(__fadd_rn(__fmul_rn((float)x1, inv), magic));
+    const uint32_t u2 = __float_as_uint(__fadd_rn(__fmul_rn((float)x2, inv), magic));
+    const uint32_t u3 = __float_as_uint(__fadd_rn(__fmul_rn((float)x3, inv), magic));
+    return __builtin_amdgcn_perm(u1, u0, 0x0c0c0400u) | __builtin_amdgcn_perm(u3, u2, 0x04000c0cu);
+}
+
+// The largest magnitude of N values, as the bits of an f32 (NaNs above all).
+template <int N>
+__device__ __forceinline__ uint32_t largest(const float (&x)[N])
+{
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        m = max(m, magnitude(x[e]));
+    }
+    return m;
+}
+
+template <int N>
+__device__ __forceinline__ uint32_t largest(const _Float16 (&x)[N])
+{
+    typedef uint16_t v2u16 __attribute__((ext_vector_type(2)));
+    v2u16 m{0, 0}, w[N / 2];
+    __builtin_memcpy(w, x, sizeof w);
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) {
+        m = __builtin_elementwise_max(m, w[e] & v2u16{0x7fff, 0x7fff});
+    }
+    return magnitude((float)__builtin_bit_cast(_Float16, max(m[0], m[1])));
+}
+
 // Byte e of a dword as a signed code, scaled to the grown step.
 __device__ __forceinline__ uint32_t rescaled(uint32_t d, float ratio)
 {
@@ -201,12 +240,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const RowsKern p)
         }
     };
     const auto most = [&](const T (&x)[4][8]) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-            m = max(m, magnitude((float)x[e / 8][e % 8]));
-        }
-        return m;
+        return max(max(largest(x[0]), largest(x[1])), max(largest(x[2]), largest(x[3])));
     };
     T held_k[kHeldK][16], held_v[kHeldV][4][8];
     uint32_t a = 0;
@@ -215,19 +249,13 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const RowsKern p)
         for (int h = 0; h < kHeldK; ++h) {
             if (lane + h * kLanes < pieces) {
                 load_k(lane + h * kLanes, held_k[h]);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    a = max(a, magnitude((float)held_k[h][e]));
-                }
+                a = max(a, largest(held_k[h]));
             }
         }
         for (int i = lane + kHeldK * kLanes; i < pieces; i += kLanes) {
             T x[16];
             load_k(i, x);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                a = max(a, magnitude((float)x[e]));
-            }
+            a = max(a, largest(x));
         }
     } else {
 #pragma unroll
@@ -259,6 +287,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const RowsKern p)
     const float s = bad ? __uint_as_float(0x7fc00000u)
                         : fmaxf(fmaxf(old, __fmul_rn(__uint_as_float(a), 1.0f / 127.0f)), kLeastScale);
     const float inv = bad ? 0.0f : __fdiv_rn(1.0f, s);
+    const uint32_t good = bad ? 0u : ~0u;          // codes of such pages are 0
     const bool grew = !bad && t.from > 0 && s > old;
     const float ratio = grew ? __fdiv_rn(old, s) : 1.0f;
     if (lane == 0) {
@@ -270,8 +299,8 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const RowsKern p)
             const uint32_t r = (uint32_t)i / per_row, at = ((uint32_t)i - r * per_row) * 16;
             uint32_t o[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                o[e / 4] |= (bad ? 0u : code_byte((float)x[e], inv)) << (8 * (e % 4));
+            for (int e = 0; e < 4; ++e) {
+                o[e] = good & new_codes(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3], inv);
             }
             *reinterpret_cast<v4i*>(page + (t.from + r) * d + at) = v4i{(int)o[0], (int)o[1], (int)o[2], (int)o[3]};
         };
@@ -316,11 +345,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const RowsKern p)
         }
 #pragma unroll
         for (int h = 0; h < 8; ++h) {
-            uint32_t o = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                o |= (bad ? 0u : code_byte((float)x[e][h], inv)) << (8 * e);
-            }
+            uint32_t o = good & new_codes(x[0][h], x[1][h], x[2][h], x[3][h], inv);
             if (mine != ~0u) {
                 o = (o & mine) | ((grew ? rescaled(old_dword[h], ratio) : old_dword[h]) & ~mine);
             }
