@@ -21,6 +21,9 @@
 // of a piece are issued a tile before it is written, its page number one before
 // that. Rows in LDS are 16 bytes longer than their data: 16 lanes' reads
 // of one column meet 16 bank groups, at constant offsets.
+// Measured: a prompt of 4096, 32 query and 8 KV heads of 128, f16, 137 GFLOP: 144 to
+// 152 us, 900 to 950 TFLOP/s, where a large f16 product reaches 1156 on this card;
+// with four waves (128 rows), none a phase behind, 249 us.
 #include <type_traits>
 
 #include "cache_attention.hpp"
@@ -553,6 +556,10 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
 
 }  // namespace
 
+// Eight waves where their registers allow it and the rows fill more than four's
+// (us, eight / four waves, 32 query and 8 KV heads; a prompt of 4096, d 128 150.7 /
+// 249, d 64 107 / 122; 64 x 33 rows of 300 29.5 / 50.0; 24 sequences of 1 to 300 rows
+// of 2500 121 / 177, d 64 99.6 / 97.9; f32, d 64, 64 x 64 of 300 38.5 / 54.4).
 int tiled_rows(int64_t d, bool f16, int64_t page, int64_t rows)
 {
     if (d > 128 && (!f16 || page < kTile)) {

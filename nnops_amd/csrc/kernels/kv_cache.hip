@@ -16,6 +16,12 @@
 // of 4 tokens per channel (two channels by 16 tokens, 4-byte loads and 16-byte
 // stores, ran 11.1 us where keys take 6.2: a prompt of 4096, pages of 16);
 // reading, two channels by 16 tokens, so that its lanes write whole rows.
+// Measured, 8 heads of 128, f16: a prompt of 4096 tokens, pages of 16, 25 MB each
+// way: written in 10.6 us, read in 9.7; 32 sequences of 1000, pages of 64: read in
+// 28.8 us (98 MB, 3.4 TB/s), a token appended to each in 5.0. All waves of such a
+// write are resident at once: it is one chain (lengths, table, rows, the page's
+// maximum, codes) long, in which 8 vector instructions a value counted (now 4:
+// 11.6 -> 10.6 us); asking for the rows before the page number is looked at did not.
 #include "paged.hpp"
 
 namespace nnops_amd {
@@ -524,6 +530,8 @@ extern "C" int nnops_hip_kv_cache_write(const NnopsKvRowsArgs* g, void* stream)
     if (n == 0 || g->cache.pages == 0) {
         return NNOPS_OK;                          // no page to write to
     }
+    // (written and read, us: 4096 tokens, pages of 16 x 128: a wave 17.2, four 22.6; of
+    // 64 x 128: a wave 22.4, four 16.6)
     const bool small = g->cache.page_tokens * g->cache.head_dim <= 4096;
     const RowsKern k = rows_kern(g, per_seq, small ? 4 : 1);
     if (n * k.head_groups > INT32_MAX / 256) {
