@@ -139,6 +139,8 @@ _ARRAYS = [L.Tensor * max(1, n) for n in range(9)]
 
 
 class _Op:
+    _takes_workspace = True
+
     def __init__(self, handle):
         if not handle:
             raise RuntimeError("nnops op creation failed")
@@ -214,7 +216,7 @@ class _Op:
         none is given. Returns the nnops Status code."""
         ai, ni = self._arr(inputs)
         ao, no = self._arr(outputs)
-        if workspace is None:
+        if workspace is None and self._takes_workspace:
             workspace = _workspace(L.lib().nnops_op_workspace_size(self._h, ai, ni, ao, no), device, stream)
         return L.lib().nnops_op_compute(self._h, ao, no, ai, ni, _stream_ptr(stream), _ptr(workspace))
 
@@ -292,6 +294,7 @@ class RmsNorm(_Op):
     residual, with a residual; may be x's or the residual's buffer). An s8 y and
     its scales are the per-token activation that Linear and MatMul take:
     ``tensor(y, scale_data=scale, granularity=1)``."""
+    _takes_workspace = False       # (asking costs a tenth of a small call)
 
     def __init__(self, *, epsilon=1e-6, output_dtype=L.DT_F16, backend=L.BACKEND_HIP):
         a = L.RmsNormAttrs()
@@ -304,6 +307,7 @@ class Rotary(_Op):
     """inputs: x [tokens, heads * head_dim] (f16/f32, any row pitch), positions
     s32 [tokens], table f32 [max_pos, rotary_dim] (:func:`rotary_table`);
     output: x's shape and type, x itself if wanted."""
+    _takes_workspace = False       # (asking costs a tenth of a small call)
 
     def __init__(self, *, head_dim, rotary_dim=0, interleaved=False, backend=L.BACKEND_HIP):
         a = L.RotaryAttrs()
@@ -318,6 +322,7 @@ class KvCacheWrite(_Op):
     [sequences + 1]); outputs, updated in place: k_cache s8 [pages, heads,
     page_tokens, head_dim], v_cache s8 [pages, heads, head_dim, page_tokens],
     k_scale and v_scale f32 [pages, heads]. :func:`kv_cache` makes one."""
+    _takes_workspace = False       # (asking costs a tenth of a small call)
 
     def __init__(self, *, backend=L.BACKEND_HIP):
         super().__init__(L.lib().nnops_kv_cache_write_create(backend))
@@ -327,6 +332,7 @@ class KvCacheRead(_Op):
     """inputs: k_cache, v_cache, k_scale, v_scale, page_table, lengths
     (, row_starts); outputs: k, v [rows, heads * head_dim], the last tokens of
     each sequence."""
+    _takes_workspace = False       # (asking costs a tenth of a small call)
 
     def __init__(self, *, output_dtype=L.DT_F16, backend=L.BACKEND_HIP):
         super().__init__(L.lib().nnops_kv_cache_read_create(output_dtype, backend))
