@@ -24,11 +24,15 @@
 // Bound: HBM for few rows, the codes read once per KV head. Long sequences are
 // split over workgroups (partial O, M, l in the workspace, joined by a second
 // kernel); a workgroup's 4 waves take every fourth tile and join in LDS. A wave
-// has a tile's 16 KB (d 128) of codes in flight and 177 registers, so that two
-// waves run on a SIMD; held to 168 for three it spilled and lost 5 %.
+// has a tile's 16 KB (d 128) of codes in flight and 168 registers, three waves a
+// SIMD. No branch stands around a tile's loads (channels past d are loaded as
+// channel 0's, the last tile is peeled off): the waits after one are for
+// everything (74 us for the batch below, and 42 against 35 at d 64).
 // One token of each of 64 sequences of up to 4096, 32 query and 8 KV heads, d 128:
-// 74.6 us, 4.16 TB/s; of one sequence of 126976: 57.5 us, 4.53 TB/s; of one of
-// 777: 9.8 us, two launches of which 7 us are the calls'.
+// 66.3 us, 4.68 TB/s; of one sequence of 126976: 55.0 us, 4.73 TB/s; of one of
+// 777: 9.0 us, two launches and the host's 5.
+#include <type_traits>
+
 #include "cache_attention.hpp"
 
 namespace nnops_amd {
@@ -48,6 +52,20 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
     const Paged& c = p.c;
     const uint32_t item = blockIdx.x / (uint32_t)c.heads;
     const int kvh = (int)(blockIdx.x - item * c.heads);
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int n = lane % 16, g = lane / 16;
+    const int kb = n / 4;                          // the token group of a lane's keys
+    // Without a window a wave's first tile is known before the sequence's length
+    // is: its page numbers are asked for beside it. (Past the sequence's end they
+    // may be anything; what is read through them is masked.)
+    const bool early = p.window == 0 && p.per_seq > 0 && c.table_pages > 0;
+    int kid = 0, vid = 0;
+    if (early) {
+        const int32_t* row = c.table + (int64_t)(item / (uint32_t)p.per_seq) * c.ld_table;
+        const int base = kTile * ((int)blockIdx.y * p.chunk + wave), last = c.table_pages - 1;
+        kid = row[min((base + 16 * kb) >> c.page_log2, last)];
+        vid = row[min((base + 16 * g) >> c.page_log2, last)];
+    }
     RowTile rt;
     if (!find_tile(p, item, false, rt)) {
         return;
@@ -63,8 +81,6 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
     }
     const int v0 = split * p.chunk, v1 = min(span.tiles, v0 + p.chunk);
 
-    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int n = lane % 16, g = lane / 16;
     const int row = row0 + n;
     const bool is_row = row < rows;
     const int tok = is_row ? (int)((uint32_t)row / (uint32_t)p.group) : tok_last;
@@ -92,18 +108,17 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
     }
     float m_run = kNone, l_run = 0.0f;
     const int64_t page_bytes = (int64_t)c.page * d;
-    const int kb = n / 4;                          // the token group of a lane's keys
     const int ktok = 16 * kb + n % 4;              // + 4 t: its token in the tile
 
     // The codes of a wave's next tile are in flight while it works on this one:
     // its keys from the scores on, its values from the second product on, its
-    // page numbers a tile earlier still.
+    // page numbers a tile earlier still. (Loads come back in order: page numbers
+    // asked for beside the keys they lead to would wait for this tile's values.)
     const int32_t* table = c.table + (int64_t)b * c.ld_table;
     const int64_t page_step = page_bytes * c.heads;
     const int8_t* k_at = c.k + kvh * page_bytes + 16 * g;
     const int8_t* v_at = c.v + kvh * page_bytes + n * c.page;
     v4i kr[4][kC], vr[kT];
-    int kid, vid;
     PageScales scale_next{0.0f, 0.0f, 0.0f};
     // (a group past the last position has the last page's codes: they are masked)
     // (page numbers as they lie in the table: looked at when they are used)
@@ -112,38 +127,49 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
         kid = table[min(base + 16 * kb, pmax) >> c.page_log2];
         vid = table[min(base + 16 * g, pmax) >> c.page_log2];
     };
-    const auto load_k = [&](int v) {
+    int koff[kC];                                  // channels past d: channel 0's codes (q is 0 there)
+#pragma unroll
+    for (int i = 0; i < kC; ++i) {
+        koff[i] = 64 * i + 16 * g < d ? 64 * i : -16 * g;
+    }
+    const auto load_k = [&](int v, int page_k, int page_v) {
         const int base = tile_base(span, v);
-        const int8_t* at = k_at + readable(c, kid) * page_step + ((base + ktok) & (c.page - 1)) * d;
+        const int8_t* at = k_at + readable(c, page_k) * page_step + ((base + ktok) & (c.page - 1)) * d;
+        int kstep = 4 * d;
+        if constexpr (DP <= 128) {
+            // (its multiples are computed here, not kept over the loop: 168 registers
+            // instead of 256 and spills)
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("" : "+s"(kstep));
+        }
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
             for (int i = 0; i < kC; ++i) {
-                kr[t][i] = 64 * i + 16 * g < d ? *reinterpret_cast<const v4i*>(at + 4 * t * d + 64 * i) : v4i{0, 0, 0, 0};
+                kr[t][i] = *reinterpret_cast<const v4i*>(at + koff[i] + (int64_t)(t * kstep));
             }
         }
-        scale_next = page_scales(c, vid, kvh);
+        scale_next = page_scales(c, page_v, kvh);
     };
-    const auto load_v = [&](int v) {
+    const auto load_v = [&](int v, int page_v) {
         const int base = tile_base(span, v);
-        const int8_t* at = v_at + readable(c, vid) * page_step + ((base + 16 * g) & (c.page - 1));
+        const int8_t* at = v_at + readable(c, page_v) * page_step + ((base + 16 * g) & (c.page - 1));
+        int vstep = 16 * c.page;
+        if constexpr (DP <= 128) {
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("" : "+s"(vstep));
+        }
 #pragma unroll
         for (int t = 0; t < kT; ++t) {
-            vr[t] = 16 * t < d ? *reinterpret_cast<const v4i*>(at + 16 * t * c.page) : v4i{0, 0, 0, 0};
+            vr[t] = *reinterpret_cast<const v4i*>(at + (int64_t)((16 * t < d ? t : 0) * vstep));
         }
     };
-    if (v0 + wave < v1) {
-        ids(v0 + wave);
-        load_k(v0 + wave);
-        load_v(v0 + wave);
-    }
-    for (int v = v0 + wave; v < v1; v += 4) {
+    // (no branch around the loads of a tile: it would wait for all of them)
+    const auto tile = [&](auto go_on, int v) {
+        constexpr bool more = decltype(go_on)::value;
+        const int next_v = vid;                    // the next tile's page
         const int base = tile_base(span, v), vt0 = base + 16 * g;
-        const bool more = v + 4 < v1;
         const PageScales scale = scale_next;
-        if (more) {
-            ids(v + 4);
-        }
 
         v4f s[4];
 #pragma unroll
@@ -157,8 +183,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
         }
 
         const Scales sc = softmax_scales(p, scale);
-        if (more) {
-            load_k(v + 4);
+        if constexpr (more) {
+            const int next_k = kid;
+            ids(min(v + 8, v1 - 1));
+            load_k(v + 4, next_k, next_v);
         }
 
         float x[4][4];
@@ -207,14 +235,26 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
         l_run += sum != 0.0f ? sum * sc.inv : 0.0f;
 #pragma unroll
         for (int t = 0; t < kT; ++t) {
-            if (16 * t < d) {
-                o[t] = product<T>(Op::codes((uint32_t)vr[t].x, (uint32_t)vr[t].y), pf[0], o[t]);
-                o[t] = product<T>(Op::codes((uint32_t)vr[t].z, (uint32_t)vr[t].w), pf[1], o[t]);
-            }
+            o[t] = product<T>(Op::codes((uint32_t)vr[t].x, (uint32_t)vr[t].y), pf[0], o[t]);
+            o[t] = product<T>(Op::codes((uint32_t)vr[t].z, (uint32_t)vr[t].w), pf[1], o[t]);
         }
-        if (more) {
-            load_v(v + 4);
+        if constexpr (more) {
+            load_v(v + 4, next_v);
         }
+    };
+    if (v0 + wave < v1) {
+        int v = v0 + wave;
+        if (!early) {
+            ids(v);
+        }
+        const int first_k = kid, first_v = vid;
+        ids(min(v + 4, v1 - 1));
+        load_k(v, first_k, first_v);
+        load_v(v, first_v);
+        for (; v + 4 < v1; v += 4) {
+            tile(std::true_type{}, v);
+        }
+        tile(std::false_type{}, v);
     }
 
     // the waves' parts, brought to one maximum and summed
@@ -441,15 +481,15 @@ struct AttnPlan {
 // tokens they look at, fill the chip; 16 rows a workgroup, its waves sharing the
 // tokens, otherwise. Measured both ways (us, tiled / 16 rows; 32 query heads, 8
 // KV heads, d 128, f16, but where said):
-//   16 x 16 of 2048 tokens  41.0 / 34.2     64 x 33 of 300    29.6 / 51.9
-//   16 x 32 of 2048         48.3 / 49.4     64 x 64 of 64     32.2 / 70.0
-//   1 x 64 of 2500          25.1 / 19.7     1 x 64 of 8000    28.7 / 36.2
-//   1 x 128 of 2500         28.1 / 26.7     1 x 128 of 8000   38.0 / 60.0
-//   1 x 256 of 1000         25.9 / 18.4     1 x 256 of 8000   53.1 / 105
-//   f32 1 x 64 of 1000      25.1 / 19.1     f32 1 x 64 of 8000  41.7 / 55.8
-//   16 / 4 heads, d 64: 16 x 128 of 128 9.0 / 12.5, of 300 17.3 / 15.2; 1 x 256 of
-//   8000 37.8 / 38.1, f32 46.9 / 59.9; 24 sequences of 1 to 100 rows of 2500
-//   39.2 / 27.4, f32 58.9 / 44.2; of 1 to 300, f32, 94.4 / 108
+//   64 x 33 of 300    29.5 / 46.9     64 x 64 of 64     32.2 / 63.0
+//   1 x 64 of 2500    25.1 / 18.1     1 x 64 of 8000    28.7 / 31.7
+//   1 x 256 of 1000   25.9 / 17.0     1 x 256 of 8000   53.1 / 92.0
+//   16 x 128 of 128   16.6 / 33.2     8 x 200 of 1200   40.9 / 69.0
+//   f32 1 x 64 of 2500 29.8 / 26.4, of 8000 41.6 / 49.4; 16 x 128 of 300 44.2 / 64.9
+//   16 / 4 heads, d 64: 16 x 128 of 128 8.9 / 12.1, of 300 17.3 / 14.6; 1 x 256 of
+//   8000 37.6 / 34.0, f32 47.3 / 54.1
+//   ragged, of 2500: 24 of 1 to 100 rows 82.2 / 69.0, f32 135 / 111; 24 of 1 to 300
+//   122 / 192, d 64 60.8 / 56.5, f32 94.7 / 98.0; 7 of 1 to 300 67.7 / 78.5
 // (ragged calls: by their mean). Splits of the longest sequence that the page
 // table has room for: as many workgroups as the chip holds at once (more of
 // them were slower: one token over 126976, 58 us with 512, 67 with 768, 72 with
@@ -481,9 +521,9 @@ AttnPlan attn_plan(const NnopsCacheAttentionArgs* g)
         return tiles < seen ? tiles : seen;
     };
     a.tile_rows = kRows;
-    if (const int rows = mean > 96 ? tiled_rows(d, g->f16, g->cache.page_tokens, mean) : 0; rows > 0) {
+    const bool ragged = g->cache.row_starts != nullptr;
+    if (const int rows = mean > (ragged ? 256 : 96) ? tiled_rows(d, g->f16, g->cache.page_tokens, mean) : 0; rows > 0) {
         // (tiles that are sure to be full; heads of 64 channels and fewer gain less)
-        const bool ragged = g->cache.row_starts != nullptr;
         const int64_t items = ragged ? g->rows * group / rows * heads : items_of(rows);
         const int64_t least = d <= 64 && (g->f16 || ragged) ? 7 << 15 : 7 << 14;
         if (items >= 128 || items * tiles_of(rows) * d >= least) {

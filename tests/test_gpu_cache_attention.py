@@ -113,12 +113,13 @@ def test_long(tokens, page, group, n):
     _check(q.astype(np.float32), cache, lens, [n] * 3, ragged=True, window=1500, sinks=100)
 
 
-# Calls with rows enough for the tiles that share their codes: more than 96 rows
-# (tokens x heads of a group) a sequence at the mean and 128 full tiles or more,
-# of 128 rows, or of 256 where the mean is past 128.
-TILES = [(128, 64, 32, 4, True), (128, 16, 32, 4, True), (64, 128, 32, 4, True), (80, 32, 32, 5, True),
-         (112, 256, 24, 8, True), (16, 16, 32, 4, True), (256, 64, 32, 4, True), (192, 128, 32, 4, True),
-         (128, 64, 32, 4, False), (96, 16, 32, 4, False), (64, 64, 32, 4, False), (48, 32, 32, 5, False)]
+# Calls with rows enough for the tiles that share their codes: at the mean more
+# than 256 rows (tokens x heads of a group) a sequence of ragged calls, 96 of
+# others, and 128 full tiles or more, of 256 rows or 128 (by type and head size;
+# equal rows also where they fill no more).
+TILES = [(128, 64, 16, 9, True), (128, 16, 16, 10, True), (64, 128, 20, 9, True), (80, 32, 16, 11, True),
+         (112, 256, 16, 9, True), (16, 16, 20, 9, True), (256, 64, 16, 9, True), (192, 128, 16, 10, True),
+         (128, 64, 16, 9, False), (96, 16, 16, 10, False), (64, 64, 16, 9, False), (48, 32, 16, 11, False)]
 
 
 def _mixed(total):
@@ -139,22 +140,23 @@ def test_tiles(d, page, heads, group, f16, many):
     _check(_q(21, sum(rows), heads * group * d, f16), cache, lens, rows, ragged=True, pad=8 if many else 1)
 
 
-@pytest.mark.parametrize("d,page,heads,group,f16", TILES[:1] + TILES[3:4] + TILES[6:7] + TILES[8:11])
-def test_tiles_of_equal_rows(d, page, heads, group, f16):
+@pytest.mark.parametrize("n", [13, 34])
+@pytest.mark.parametrize("d,page,heads,group,f16", TILES)
+def test_tiles_of_equal_rows(d, page, heads, group, f16, n):
     """As many rows each, without starts; more rows than tokens among them."""
-    announce(f"attention equal tiles d={d} page={page} heads={heads} group={group} f16={f16}")
-    lens, n = [34, 12, 0, 64, 65, 300, 511, 513, 40], 34
+    announce(f"attention equal tiles d={d} page={page} heads={heads} group={group} f16={f16} n={n}")
+    lens = [34, 12, 0, 64, 65, 300, 511, 513, 40]
     cache = _cache(len(lens), 520, heads, page, d)
     q = _q(22, n * len(lens), heads * group * d, f16)
     got = _check(q, cache, lens, [n] * len(lens), ragged=False)
-    assert np.all(got[n:n + 22] == 0) and np.all(got[2 * n:3 * n] == 0)
+    assert np.all(got[n:2 * n - 12] == 0) and np.all(got[2 * n:3 * n] == 0)
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (16, 4), (64, 0), (100, 70), (300, 5), (7, 1 << 40)])
 @pytest.mark.parametrize("page,f16", [(16, True), (64, True), (128, False), (32, False)])
 def test_windows_in_tiles(window, sinks, page, f16):
     announce(f"attention tiles window={window} sinks={sinks} page={page} f16={f16}")
-    heads, group, d = 32, 4, 64
+    heads, group, d = 20, 7, 64
     lens, rows = _mixed(400)
     cache = _cache(len(lens), 600, heads, page, d)
     _check(_q(23, sum(rows), heads * group * d, f16), cache, lens, rows, ragged=True, window=window, sinks=sinks)
@@ -169,7 +171,10 @@ def test_tiles_that_are_split(page, f16):
     cache = _cache(2, tokens, heads, page, d)
     q = _q(24, 2 * n, heads * group * d, f16)
     _check(q, cache, [tokens, 50], [n, n], ragged=False)
-    _check(q, cache, [tokens, 50], [n, n], ragged=True, window=20000, sinks=100)
+    _check(q, cache, [tokens, 50], [n, n], ragged=False, window=20000, sinks=100)
+    group = 11
+    q = _q(28, 2 * n, heads * group * d, f16)
+    _check(q, cache, [tokens, 50], [n, n], ragged=True)
 
 
 @pytest.mark.parametrize("page,f16", [(64, True), (16, True), (128, False), (32, False)])
