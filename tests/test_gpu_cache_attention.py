@@ -119,7 +119,7 @@ def test_long(tokens, page, group, n):
 # equal rows also where they fill no more).
 TILES = [(128, 64, 16, 9, True), (128, 16, 16, 10, True), (64, 128, 20, 9, True), (80, 32, 16, 11, True),
          (112, 256, 16, 9, True), (16, 16, 20, 9, True), (256, 64, 16, 9, True), (192, 128, 16, 10, True),
-         (128, 64, 16, 9, False), (96, 16, 16, 10, False), (64, 64, 16, 9, False), (48, 32, 16, 11, False)]
+         (128, 64, 16, 9, False), (96, 16, 16, 10, False), (64, 64, 16, 9, False), (48, 32, 16, 11, False), (32, 16, 16, 9, False)]
 
 
 def _mixed(total):
