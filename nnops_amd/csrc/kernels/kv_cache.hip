@@ -18,7 +18,7 @@
 // reading, two channels by 16 tokens, so that its lanes write whole rows.
 // Measured, 8 heads of 128, f16: a prompt of 4096 tokens, pages of 16, 25 MB each
 // way: written in 10.6 us, read in 9.7; 32 sequences of 1000, pages of 64: read in
-// 28.8 us (98 MB, 3.4 TB/s), a token appended to each in 5.0. All waves of such a
+// 20.4 us (98 MB, 4.8 TB/s), a token appended to each in 5.0. All waves of such a
 // write are resident at once: it is one chain (lengths, table, rows, the page's
 // maximum, codes) long, in which 8 vector instructions a value counted (now 4:
 // 11.6 -> 10.6 us); asking for the rows before the page number is looked at did not.
@@ -91,7 +91,7 @@ struct RowsKern {
     int32_t per_seq;      // items of a sequence, equal rows each (0: found by search)
     int32_t head_groups;  // groups of heads of an item, a workgroup (and side) each
     int32_t group_heads;  // heads of a group
-    uint32_t row_magic;   // ceil(2^32 / x), x = group_heads d / 16 > 1: a division by x, reading
+    uint32_t row_magic;   // ceil(2^32 / x), x the 16-byte pieces of group_heads heads' values: to divide by x
 };
 
 // Items of a sequence: the pages that its rows of the call fall in; one, of no
@@ -386,6 +386,19 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const RowsKern p)
     }
 }
 
+// Values that the kernel does not read again, stored past the caches as far as
+// they let it, whatever the row's alignment (32 sequences of 1000, 65 MB read back,
+// of six caches in turn: 28.9 us, 35.5 with plain stores; f32 35.5 and 52.1. Such
+// stores have to fill whole lines: 32 or 64 bytes a lane took 99 us).
+template <typename T, int N>
+__device__ __forceinline__ void put_once(T* to, const T (&y)[N])
+{
+    typedef int Word __attribute__((ext_vector_type(sizeof(T) * N / 4), aligned(sizeof(T))));
+    Word w;
+    __builtin_memcpy(&w, y, sizeof w);
+    __builtin_nontemporal_store(w, reinterpret_cast<Word*>(to));
+}
+
 // A workgroup reads one page of a group of heads, one side; the heads' pieces
 // side by side in a row, so that what it writes of a row is contiguous.
 template <typename T>
@@ -415,24 +428,28 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const RowsKern p)
     const int8_t* page = (values ? c.v : c.k) + at_page * (int64_t)bytes;
     const float nan = __uint_as_float(0x7fc00000u);
     if (!values) {
-        const uint32_t per_tok = d / 16, per_row = per_tok * p.group_heads;
+        // 16 bytes of a row a thread: side by side in a wave, whole lines
+        constexpr int kP = 16 / sizeof(T);
+        const uint32_t per_tok = d / kP, per_row = per_tok * p.group_heads;
         const int n = (t.to - t.from) * (int)per_row;
 #pragma unroll 4
         for (int i = threadIdx.x; i < n; i += 256) {
-            const uint32_t r = per_row > 1 ? __umulhi((uint32_t)i, p.row_magic) : (uint32_t)i, in = (uint32_t)i - r * per_row;
-            const uint32_t h = in / per_tok, at = (in - h * per_tok) * 16;
+            const uint32_t r = __umulhi((uint32_t)i, p.row_magic), in = (uint32_t)i - r * per_row;
+            const uint32_t h = in / per_tok, at = (in - h * per_tok) * kP;
             if ((int)h >= heads) {
                 continue;
             }
-            const v4i w = there ? *reinterpret_cast<const v4i*>(page + h * bytes + (t.from + r) * d + at) : v4i{0, 0, 0, 0};
+            uint32_t wd[kP / 4] = {};
+            if (there) {
+                __builtin_memcpy(wd, __builtin_assume_aligned(page + h * bytes + (t.from + r) * d + at, kP), kP);
+            }
             const float s = there ? scales[h] : nan;
-            const uint32_t wd[4] = {(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w};
-            T y[16];
+            T y[kP];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
+            for (int e = 0; e < kP; ++e) {
                 y[e] = (T)__fmul_rn((float)(int8_t)(wd[e / 4] >> (8 * (e % 4))), s);
             }
-            __builtin_memcpy(rows + (int64_t)r * ld + h * d + at, y, sizeof y);
+            put_once(rows + (int64_t)r * ld + h * d + at, y);
         }
         return;
     }
@@ -458,7 +475,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const RowsKern p)
                 for (int q = 0; q < 2; ++q) {
                     y[q] = (T)__fmul_rn((float)(int8_t)(wd[q][e / 4] >> (8 * (e % 4))), s);
                 }
-                __builtin_memcpy(dst + e * ld, y, sizeof y);
+                put_once(dst + e * ld, y);
             }
         }
     }
@@ -508,7 +525,7 @@ RowsKern rows_kern(const NnopsKvRowsArgs* g, int32_t per_seq, int32_t group_head
     k.per_seq = per_seq;
     k.group_heads = group_heads;
     k.head_groups = (k.c.heads + group_heads - 1) / group_heads;
-    const uint32_t per_row = (uint32_t)(group_heads * (k.c.d / 16));
+    const uint32_t per_row = (uint32_t)(group_heads * (k.c.d / (g->f16 ? 8 : 4)));
     k.row_magic = (uint32_t)(((1ull << 32) + per_row - 1) / per_row);
     return k;
 }
