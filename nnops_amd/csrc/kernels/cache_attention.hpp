@@ -203,12 +203,15 @@ struct Operand<float> {
     }
     static __device__ __forceinline__ Vec codes(uint32_t a, uint32_t b)
     {
-        const uint32_t d[2] = {a ^ 0x80808080u, b ^ 0x80808080u};
+        // (a signed byte to f32: one instruction that picks it. Unsigned bytes less
+        // 128 took two and more: vector instructions bound f32 rows, 7 ragged
+        // sequences of up to 2500, 16 heads of 64, window 1024: 31.6 -> 26.2 us)
+        const uint32_t d[2] = {a, b};
         v4u w;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t u = d[i / 2] >> (16 * (i % 2));
-            w[i] = uppers((float)(u & 0xffu) - 128.0f, (float)((u >> 8) & 0xffu) - 128.0f);
+            w[i] = uppers((float)(int8_t)u, (float)(int8_t)(u >> 8));
         }
         Vec h;
         __builtin_memcpy(&h, &w, 16);
