@@ -17,8 +17,8 @@
 // stores, ran 11.1 us where keys take 6.2: a prompt of 4096, pages of 16);
 // reading, two channels by 16 tokens, so that its lanes write whole rows.
 // Measured, 8 heads of 128, f16: a prompt of 4096 tokens, pages of 16, 25 MB each
-// way: written in 10.6 us, read in 9.7; 32 sequences of 1000, pages of 64: read in
-// 20.4 us (98 MB, 4.8 TB/s), a token appended to each in 5.0. All waves of such a
+// way: written in 10.6 us, read in 8.8; 32 sequences of 1000, pages of 64: read in
+// 20.6 us (98 MB, 4.8 TB/s), a token appended to each in 5.0. All waves of such a
 // write are resident at once: it is one chain (lengths, table, rows, the page's
 // maximum, codes) long, in which 8 vector instructions a value counted (now 4:
 // 11.6 -> 10.6 us); asking for the rows before the page number is looked at did not.
@@ -580,7 +580,8 @@ extern "C" int nnops_hip_kv_cache_read(const NnopsKvRowsArgs* g, void* stream)
     int32_t per_seq = 0;
     const int64_t n = items(g, per_seq);
     // heads of a workgroup: 8192 codes, as long as there are workgroups to fill
-    // the chip (32 sequences of 1000: 26.1 us, 28.0 with 16384, 32.3 with 32768)
+    // the chip (32 sequences of 1000, plain stores: 26.1 us, 28.0 with 16384, 32.3
+    // with 32768)
     int32_t group = (int32_t)(8192 / (g->cache.page_tokens * g->cache.head_dim));
     group = group < 1 ? 1 : group > g->cache.heads ? (int32_t)g->cache.heads : group;
     while (group > 1 && n * 2 * ((g->cache.heads + group - 1) / group) < 2048) {
