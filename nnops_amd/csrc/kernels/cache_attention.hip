@@ -490,7 +490,8 @@ struct AttnPlan {
 //   8000 37.6 / 34.0, f32 47.3 / 54.1
 //   ragged, of 2500: 24 of 1 to 100 rows 82.2 / 69.0, f32 135 / 111; 24 of 1 to 300
 //   122 / 192, d 64 60.8 / 56.5, f32 94.7 / 98.0; 7 of 1 to 300 67.7 / 78.5
-// (ragged calls: by their mean). Splits of the longest sequence that the page
+// (ragged calls: by their mean; f32 before its codes took one instruction each
+// instead of two and more, from which 16 rows gain the more). Splits of the longest sequence that the page
 // table has room for: as many workgroups as the chip holds at once (more of
 // them were slower: one token over 126976, 58 us with 512, 67 with 768, 72 with
 // 1024), no fewer than 4 tiles each, and none where a wave has no more than two
