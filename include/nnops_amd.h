@@ -444,7 +444,7 @@ int nnops_hip_rotary_table(const NnopsRotaryTableArgs* args, void* stream);
  * page_table[b][p / page_tokens].
  * A call's rows are the LAST tokens of each sequence: sequence b has rows
  * row_starts[b] .. row_starts[b + 1] - 1 (row_starts NULL: rows / sequences
- * each), its last row stands for token lengths[b] - 1.
+ * each, which has to be whole), its last row stands for token lengths[b] - 1.
  * page_tokens: 16, 32, 64, 128 or 256; head_dim: a multiple of 16 up to 256;
  * k and v 16-byte aligned, dense.
  * The tables are device memory that the host does not see. What they should
@@ -499,7 +499,8 @@ int nnops_hip_kv_cache_read(const NnopsKvRowsArgs* args, void* stream);
  * f32: both exactly, as three bf16 parts.
  * nnops_hip_cache_attention_workspace_size bytes of workspace (16-byte
  * aligned) hold the partial results of long sequences that are split over the
- * chip. */
+ * chip; the size goes by the sizes in args alone (no pointer is followed), and
+ * is 0 for a call that is refused. */
 typedef struct NnopsCacheAttentionArgs {
     NnopsKvPages cache;
     const void* q;              /* [rows][ld_q] f16 (f16) or f32 */

@@ -36,14 +36,19 @@ Status check_cache(std::span<const TensorDesc> c)
     return dense(k) && dense(v) && dense(ks) && dense(vs) ? Status::ok : Status::unsupported;
 }
 
-/// page_table, lengths [, row_starts].
-Status check_tables(std::span<const TensorDesc> t)
+/// page_table, lengths [, row_starts], for a call of `rows` rows.
+Status check_tables(std::span<const TensorDesc> t, int64_t rows)
 {
     if (t[0].rank != 2 || t[1].rank != 1 || t[0].dims[0] != t[1].dims[0] || t[0].dtype != DataType::s32 ||
         t[1].dtype != DataType::s32) {
         return Status::invalid_argument;
     }
     if (t.size() > 2 && (t[2].rank != 1 || t[2].dims[0] != t[1].dims[0] + 1 || t[2].dtype != DataType::s32)) {
+        return Status::invalid_argument;
+    }
+    // without starts, every sequence has as many rows
+    const int64_t seqs = t[1].dims[0];
+    if (rows > 0 && (seqs == 0 || (t.size() <= 2 && rows % seqs != 0))) {
         return Status::invalid_argument;
     }
     return Status::ok;
@@ -92,11 +97,11 @@ Status check_rw(std::span<const TensorDesc> rows, std::span<const TensorDesc> ca
     if (Status s = check_cache(cache); !is_ok(s)) {
         return s;
     }
-    if (Status s = check_tables(tables); !is_ok(s)) {
-        return s;
-    }
-    if (!same_shape(rows[0], rows[1]) || rows[0].dtype != rows[1].dtype) {
+    if (rows[0].rank != 2 || !same_shape(rows[0], rows[1]) || rows[0].dtype != rows[1].dtype) {
         return Status::invalid_argument;
+    }
+    if (Status s = check_tables(tables, rows[0].dims[0]); !is_ok(s)) {
+        return s;
     }
     return check_rows(rows[0], cache[0].dims[1], cache[0]);
 }
@@ -239,12 +244,15 @@ Status CacheAttention::validate(std::span<const TensorDesc> inputs, std::span<co
     if (Status s = check_cache(inputs.subspan(1, 4)); !is_ok(s)) {
         return s;
     }
-    if (Status s = check_tables(inputs.subspan(5)); !is_ok(s)) {
+    const TensorDesc& q = inputs[0];
+    if (q.rank != 2) {
+        return Status::invalid_argument;
+    }
+    if (Status s = check_tables(inputs.subspan(5), q.dims[0]); !is_ok(s)) {
         return s;
     }
-    const TensorDesc& q = inputs[0];
     const int64_t width = inputs[1].dims[1] * inputs[1].dims[3];
-    if (q.rank != 2 || width <= 0 || q.dims[1] <= 0 || q.dims[1] % width != 0 || !same_shape(q, outputs[0]) ||
+    if (width <= 0 || q.dims[1] <= 0 || q.dims[1] % width != 0 || !same_shape(q, outputs[0]) ||
         q.dtype != outputs[0].dtype) {
         return Status::invalid_argument;
     }

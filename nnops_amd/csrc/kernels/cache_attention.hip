@@ -546,13 +546,14 @@ AttnPlan attn_plan(const NnopsCacheAttentionArgs* g)
     return a;
 }
 
-int check_attention(const NnopsCacheAttentionArgs* g)
+// The rules on sizes: what attn_plan and the launch assume. (In particular,
+// rows that divide among the sequences: there is a tile of rows to plan for.)
+int check_shapes(const NnopsCacheAttentionArgs* g)
 {
     if (g == nullptr || g->q_heads < 0 || g->window < 0 || g->sinks < 0 || !(g->scale >= 0.0f)) {
         return NNOPS_INVALID_ARGUMENT;
     }
-    const int rc = check_pages(g->cache, g->rows);
-    if (rc >= 0) {
+    if (const int rc = check_page_shapes(g->cache, g->rows); rc >= 0) {
         return rc;
     }
     if (g->q_heads == 0 || g->q_heads % g->cache.heads != 0 || g->cache.pages == 0) {
@@ -594,21 +595,19 @@ using namespace nnops_amd;
 
 extern "C" size_t nnops_hip_cache_attention_workspace_size(const NnopsCacheAttentionArgs* g)
 {
-    // (the tables' contents and the pointers play no part)
-    if (g == nullptr || g->rows <= 0 || g->q_heads <= 0 || g->cache.heads <= 0 || g->cache.sequences <= 0 ||
-        g->cache.head_dim <= 0 || g->cache.page_tokens <= 0 || g->cache.table_pages < 0 ||
-        g->q_heads % g->cache.heads != 0 || g->window < 0 || g->sinks < 0) {
-        return 0;
-    }
-    return attn_plan(g).workspace;
+    // (the tables' contents and the pointers play no part; a call that is refused,
+    // or that has nothing to do, needs none)
+    return check_shapes(g) >= 0 ? 0 : attn_plan(g).workspace;
 }
 
 extern "C" int nnops_hip_cache_attention(const NnopsCacheAttentionArgs* g, void* workspace, size_t workspace_bytes,
                                          void* stream)
 {
     const TimingDisarm disarm;
-    const int rc = check_attention(g);
-    if (rc >= 0) {
+    if (const int rc = check_shapes(g); rc >= 0) {
+        return rc;
+    }
+    if (const int rc = check_page_memory(g->cache); rc >= 0) {
         return rc;
     }
     const int64_t width = g->q_heads * g->cache.head_dim;

@@ -26,7 +26,7 @@
 
 namespace nnops_amd {
 
-int check_pages(const NnopsKvPages& c, int64_t rows)
+int check_page_shapes(const NnopsKvPages& c, int64_t rows)
 {
     if (rows < 0 || c.sequences < 0 || c.pages < 0 || c.heads < 0 || c.table_pages < 0) {
         return NNOPS_INVALID_ARGUMENT;
@@ -48,6 +48,11 @@ int check_pages(const NnopsKvPages& c, int64_t rows)
     if (c.sequences == 0 || (c.row_starts == nullptr && rows % c.sequences != 0)) {
         return NNOPS_INVALID_ARGUMENT;
     }
+    return -1;
+}
+
+int check_page_memory(const NnopsKvPages& c)
+{
     if (c.page_table == nullptr || c.lengths == nullptr || c.ld_table < c.table_pages) {
         return NNOPS_INVALID_ARGUMENT;
     }
@@ -503,8 +508,10 @@ int check_rows(const NnopsKvRowsArgs* g)
     if (g == nullptr) {
         return NNOPS_INVALID_ARGUMENT;
     }
-    const int rc = check_pages(g->cache, g->rows);
-    if (rc >= 0) {
+    if (const int rc = check_page_shapes(g->cache, g->rows); rc >= 0) {
+        return rc;
+    }
+    if (const int rc = check_page_memory(g->cache); rc >= 0) {
         return rc;
     }
     const int64_t width = g->cache.heads * g->cache.head_dim;

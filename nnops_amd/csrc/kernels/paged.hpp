@@ -86,8 +86,10 @@ __device__ __forceinline__ bool find_item(const Paged& p, uint32_t w, Count coun
     return false;
 }
 
-// What every entry point checks of a cache. Returns -1 if the call is to run.
-int check_pages(const NnopsKvPages& c, int64_t rows);
+// What every entry point checks of a cache: its sizes, then what it points to.
+// They return -1 if the call is to run.
+int check_page_shapes(const NnopsKvPages& c, int64_t rows);
+int check_page_memory(const NnopsKvPages& c);
 Paged paged(const NnopsKvPages& c, int64_t rows);
 
 }  // namespace nnops_amd

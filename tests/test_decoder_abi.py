@@ -179,6 +179,37 @@ def test_compute_refusals():
                                        workspace=0) == na.NOT_INITIALIZED
 
 
+@pytest.mark.parametrize("rows,seqs", [(1, 3), (2, 3), (4, 3), (7, 3), (1, 64), (5, 2)])
+def test_rows_that_do_not_divide(rows, seqs):
+    """Without row starts every sequence has as many rows: fewer rows than
+    sequences, or rows that do not divide among them, are refused by validate(),
+    by compute() and by the query of the workspace, which returns."""
+    c, r, q = cache(pages=9000), desc([rows, 128], F16), desc([rows, 512], F16)
+    for d in c + [r, q]:
+        d.data = 4096
+    for per in (4, 3000):                                                # (a long table: splits, so a workspace)
+        t, with_starts = tables(seqs, per), tables(seqs, per, starts=True)
+        for d in t + with_starts:
+            d.data = 4096
+        for op, outs, ins in ((na.CacheAttention(), [q], [q] + c), (na.KvCacheWrite(), c, [r, r]),
+                              (na.KvCacheRead(), [r, r], c)):
+            assert op.validate(ins + t, outs) == na.INVALID_ARGUMENT
+            assert op.workspace_size(ins + t, outs) == 0
+            assert op.compute(outs, ins + t, stream=0, workspace=0) == na.INVALID_ARGUMENT
+            assert op.compute(outs, ins + t, stream=0) == na.INVALID_ARGUMENT        # (asks for the size)
+            assert op.validate(ins + with_starts, outs) == na.OK
+        assert (na.CacheAttention().workspace_size([q] + c + with_starts, [q]) > 0) == (per == 3000)
+
+
+def test_rows_of_no_sequence():
+    c, r, q = cache(), desc([2, 128], F16), desc([2, 512], F16)
+    for t in (tables(0), tables(0, starts=True)):
+        for op, outs, ins in ((na.CacheAttention(), [q], [q] + c), (na.KvCacheWrite(), c, [r, r]),
+                              (na.KvCacheRead(), [r, r], c)):
+            assert op.validate(ins + t, outs) == na.INVALID_ARGUMENT
+            assert op.workspace_size(ins + t, outs) == 0
+
+
 # --- the C ABI below -------------------------------------------------------------
 
 def test_abi_rms_norm():
@@ -298,3 +329,26 @@ def test_output_descs_room():
     assert L.lib().nnops_op_output_descs(op._h, ins, 2, outs, 1) == -na.INVALID_ARGUMENT
     assert L.lib().nnops_op_output_descs(op._h, ins, 2, outs, 2) == 2
     assert L.lib().nnops_op_output_descs(None, ins, 2, outs, 2) == -na.INVALID_ARGUMENT
+
+
+def test_abi_workspace_size_of_refused_calls():
+    """The query takes any argument that the call itself would refuse: 0, and it returns."""
+    lib = na.lib()
+    g = na.CacheAttentionArgs()
+    c = g.cache
+    c.pages, c.heads, c.page_tokens, c.head_dim, c.sequences, c.table_pages = 4000, 2, 16, 64, 3, 3000
+    g.rows, g.q_heads, g.f16 = 6, 8, 1                                   # (no pointers: they play no part)
+    f = lib.nnops_hip_cache_attention_workspace_size
+    need = f(C.byref(g))
+    assert need > 0
+    for obj, field, values in ((g, "rows", (0, -1, 1, 2, 7, 1 << 40)), (g, "q_heads", (0, -2, 7, 1 << 20)),
+                               (g, "window", (-1,)), (g, "sinks", (-1,)), (g, "scale", (-1.0, float("nan"))),
+                               (c, "heads", (0, -1, 3, 1 << 20)), (c, "page_tokens", (0, -16, 24, 1 << 40)),
+                               (c, "head_dim", (0, 8, 72, 1 << 40)), (c, "sequences", (0, -1, 4, 64, 1 << 40)),
+                               (c, "table_pages", (-1, 1 << 40, (1 << 63) - 1)), (c, "pages", (-1, 0, 1 << 40))):
+        old = getattr(obj, field)
+        for value in values:
+            setattr(obj, field, value)
+            assert f(C.byref(g)) == 0, (field, value)
+        setattr(obj, field, old)
+    assert f(C.byref(g)) == need
