@@ -394,8 +394,11 @@ extern "C" int nnops_hip_rms_norm(const NnopsRmsNormArgs* g, void* stream)
         (res && (g->ld_residual < g->cols || g->ld_sum < g->cols)) || !(g->epsilon >= 0.0f)) {
         return NNOPS_INVALID_ARGUMENT;
     }
+    // (no epsilon: the least that keeps the factor of a row of zeros finite, so that
+    // the row is zeros. Testing for it in the kernel took 3 % of 512 x 16384.)
+    const float eps = g->epsilon > 0.0f ? g->epsilon : 0x1p-149f;
     const NormKern k{g->x,    g->weight, g->residual,    g->y,    g->scale,  g->sum,    g->rows,
-                     g->cols, g->ld_x,   g->ld_residual, g->ld_y, g->ld_sum, g->epsilon};
+                     g->cols, g->ld_x,   g->ld_residual, g->ld_y, g->ld_sum, eps};
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (g->in_f16) {
         s8 ? (res ? launch_norm<_Float16, true, true>(k, s) : launch_norm<_Float16, true, false>(k, s))

@@ -170,3 +170,21 @@ def test_many_rows_and_empty():
     assert np.array_equal(y, np.tile(one, (10000, 1))) and np.array_equal(scale, np.tile(s1, 10000))
     e = torch.empty((0, 24), dtype=torch.float16, device="cuda")
     assert na.RmsNorm().compute([na.tensor(e)], [na.tensor(e), na.tensor(dev(w))]) == na.OK
+
+
+@pytest.mark.parametrize("cols", [40, 600, 4096, 16384, 20000])
+@pytest.mark.parametrize("f16", [True, False])
+def test_epsilon_of_zero(cols, f16):
+    """Rows of zeros (with a residual: x and -x) are zeros, their scale 0; the
+    rows beside them are what the formula says without an epsilon."""
+    announce(f"norm epsilon 0 {cols} f16={f16}")
+    x, r, w = _data(4, cols, f16)
+    r[1], x[2], r[2] = -x[1], 0, 0
+    for residual in (True, False):
+        for out in ("s8", "fp"):
+            y, scale, total = _run(x, r if residual else None, w, out, eps=0.0)
+            zero = [1, 2] if residual else [2]
+            rest = [i for i in range(4) if i not in zero]
+            assert np.all(y[zero] == 0) and (scale is None or np.all(scale[zero] == 0))
+            _check(x[rest], r[rest] if residual else None, w, out, y[rest], None if scale is None else scale[rest],
+                   None if total is None else total[rest], eps=0.0)
