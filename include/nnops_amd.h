@@ -374,7 +374,8 @@ int nnops_hip_dequantize_linear(const NnopsQdqArgs* args, void* stream);
  * codes do not depend on the order in which the squares are summed). A row
  * with a < 2^-119 has codes 0; a row with an infinity or a NaN in u has codes
  * 0 and the scale NaN. A row of zeros is 0 (codes, scale 0) whatever epsilon
- * is. The codes and scales are what nnops_hip_gemm_i8 takes
+ * is; f32 rows whose squares would leave f32's range are normed as multiples of
+ * a power of two. The codes and scales are what nnops_hip_gemm_i8 takes
  * as A and s_a.
  * sum may be x's or residual's buffer, y (f16 / f32) x's or residual's where
  * that is not sum's; otherwise no output may overlap another buffer.

@@ -29,7 +29,8 @@ struct NormKern {
     float* scale;
     void* sum;
     int64_t rows, cols, ld_x, ld_r, ld_y, ld_sum;
-    float eps;
+    float eps;            // no less than the smallest positive f32
+    float eps_given;
 };
 
 // |v|'s bits order like |v|, infinities and NaNs above every finite value, so
@@ -138,6 +139,30 @@ __device__ __forceinline__ float row_scale(uint32_t a, float rstd)
     return a < 0x7f800000u ? __fmul_rn(__fmul_rn(__uint_as_float(a), rstd), 1.0f / 127.0f) : __uint_as_float(0x7fc00000u);
 }
 
+__device__ __forceinline__ float row_rstd(float ss, float cols, float eps)
+{
+    return __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, cols) + eps));
+}
+
+// f32 rows whose squares leave f32's range: past 2^127 their sum is infinite and
+// the factor 0, below 2^-126 they lose their bits or are 0 (which shows where
+// epsilon is next to nothing). Such a row is normed as h times a power of two,
+// epsilon times its square: the same result. 1 where a row needs none, as every
+// row of f16 does (its squares are 0 or 2^-48 to 2^34).
+template <typename T>
+constexpr bool kRescales = sizeof(T) == 4;
+
+__device__ __forceinline__ float row_rescale(float ss, float cols, float eps)
+{
+    const float m = __fdiv_rn(ss, cols) + eps;
+    return m < 0x1p-100f ? 0x1p90f : m < __builtin_inff() ? 1.0f : 0x1p-80f;   // (a NaN stays one)
+}
+
+__device__ __forceinline__ float scaled_eps(const NormKern& p, float f)
+{
+    return fmaxf(__fmul_rn(__fmul_rn(p.eps_given, f), f), 0x1p-149f);
+}
+
 // A row's chunks as they lie in memory.
 template <typename T, int NC>
 struct RowChunks {
@@ -211,14 +236,44 @@ __global__ __launch_bounds__(64 * (RW > 4 ? RW : 4)) void rms_norm_kernel(const 
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 ss = __builtin_fmaf(h[c][e], h[c][e], ss);
-                h[c][e] = __fmul_rn(h[c][e], (float)ws.v[c][e]);
+                const float u = __fmul_rn(h[c][e], (float)ws.v[c][e]);
                 if constexpr (S8) {
-                    a = max(a, magnitude(h[c][e]));
+                    a = max(a, magnitude(u));
                 }
+                h[c][e] = kRescales<T> ? h[c][e] : u;
             }
         }
         row_reduce<RW>(ss, a);
-        const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, (float)cols) + p.eps));
+        float eps = p.eps;
+        if constexpr (kRescales<T>) {
+            const float f = row_rescale(ss, (float)cols, eps);
+            if (f != 1.0f) {                       // (the same in the whole row)
+                if constexpr (RW > 1) {
+                    __syncthreads();               // row_reduce's words are read
+                }
+                ss = 0.0f;
+                a = 0;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        h[c][e] = __fmul_rn(h[c][e], f);
+                        ss = __builtin_fmaf(h[c][e], h[c][e], ss);
+                        a = max(a, magnitude(__fmul_rn(h[c][e], (float)ws.v[c][e])));
+                    }
+                }
+                row_reduce<RW>(ss, a);
+                eps = scaled_eps(p, f);
+            }
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    h[c][e] = __fmul_rn(h[c][e], (float)ws.v[c][e]);
+                }
+            }
+        }
+        const float rstd = row_rstd(ss, (float)cols, eps);
         if constexpr (S8) {
             const float inv = code_factor(a);
             int8_t* y = static_cast<int8_t*>(p.y) + row * p.ld_y;
@@ -267,6 +322,7 @@ __global__ __launch_bounds__(1024) void rms_norm_wide(const NormKern p)
     const T* x = static_cast<const T*>(p.x) + row * p.ld_x;
     const T* r = RES ? static_cast<const T*>(p.r) + row * p.ld_r : nullptr;
     const T* w = static_cast<const T*>(p.w);
+    float factor = 1.0f;                           // of h in u and in the squares (row_rescale)
     auto chunk = [&](int64_t at, int n, float (&h)[8], float (&u)[8]) {
         float f[8];
         if (n >= 8) {
@@ -287,24 +343,38 @@ __global__ __launch_bounds__(1024) void rms_norm_wide(const NormKern p)
             if constexpr (RES) {
                 h[e] = __fadd_rn(h[e], f[e]);
             }
-            u[e] = __fmul_rn(h[e], u[e]);
+            u[e] = __fmul_rn(__fmul_rn(h[e], factor), u[e]);
         }
     };
-    float ss = 0.0f;
+    float ss = 0.0f, eps = p.eps;
     uint32_t a = 0;
-    for (int64_t at = (int64_t)threadIdx.x * 8; at < p.cols; at += 8192) {
-        float h[8], u[8];
-        chunk(at, (int)min((int64_t)8, p.cols - at), h, u);
-        float part = 0.0f;                         // a sum of sums: no long chain of one rounding each
+    const auto sums = [&] {
+        for (int64_t at = (int64_t)threadIdx.x * 8; at < p.cols; at += 8192) {
+            float h[8], u[8];
+            chunk(at, (int)min((int64_t)8, p.cols - at), h, u);
+            float part = 0.0f;                     // a sum of sums: no long chain of one rounding each
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            part = __builtin_fmaf(h[e], h[e], part);
-            a = max(a, magnitude(u[e]));
+            for (int e = 0; e < 8; ++e) {
+                const float x = __fmul_rn(h[e], factor);
+                part = __builtin_fmaf(x, x, part);
+                a = max(a, magnitude(u[e]));
+            }
+            ss += part;
         }
-        ss += part;
+        row_reduce<16>(ss, a);
+    };
+    sums();
+    if constexpr (kRescales<T>) {
+        factor = row_rescale(ss, (float)p.cols, eps);
+        if (factor != 1.0f) {                      // (the same in the whole workgroup)
+            __syncthreads();                       // row_reduce's words are read
+            ss = 0.0f;
+            a = 0;
+            sums();
+            eps = scaled_eps(p, factor);
+        }
     }
-    row_reduce<16>(ss, a);
-    const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, (float)p.cols) + p.eps));
+    const float rstd = row_rstd(ss, (float)p.cols, eps);
     const float inv = code_factor(a);
     if (S8 && threadIdx.x == 0) {
         p.scale[row] = row_scale(a, rstd);
@@ -398,7 +468,8 @@ extern "C" int nnops_hip_rms_norm(const NnopsRmsNormArgs* g, void* stream)
     // the row is zeros. Testing for it in the kernel took 3 % of 512 x 16384.)
     const float eps = g->epsilon > 0.0f ? g->epsilon : 0x1p-149f;
     const NormKern k{g->x,    g->weight, g->residual,    g->y,    g->scale,  g->sum,    g->rows,
-                     g->cols, g->ld_x,   g->ld_residual, g->ld_y, g->ld_sum, eps};
+                     g->cols, g->ld_x,   g->ld_residual, g->ld_y, g->ld_sum, eps,
+                     g->epsilon};
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (g->in_f16) {
         s8 ? (res ? launch_norm<_Float16, true, true>(k, s) : launch_norm<_Float16, true, false>(k, s))

@@ -188,3 +188,26 @@ def test_epsilon_of_zero(cols, f16):
             assert np.all(y[zero] == 0) and (scale is None or np.all(scale[zero] == 0))
             _check(x[rest], r[rest] if residual else None, w, out, y[rest], None if scale is None else scale[rest],
                    None if total is None else total[rest], eps=0.0)
+
+
+@pytest.mark.parametrize("cols", [40, 600, 1100, 4096, 5001, 8192, 16384, 20000])
+def test_f32_rows_whose_squares_leave_the_range(cols):
+    """f32 rows of 1e20 and 1e36, whose squares are infinite, and, without an
+    epsilon, of 1e-25 and 1e-41, whose squares are 0: what the formula says, as
+    for the ordinary row beside them; with an epsilon small rows stay small."""
+    announce(f"norm f32 range {cols}")
+    x, r, w = _data(6, cols, False)
+    size = np.array([1e20, 1.0, 1e36, 1e-25, 1e-41, 3e17])[:, None]
+    x, r = (x * size).astype(np.float32), (r * size).astype(np.float32)
+    for residual in (r, None):
+        for out in ("s8", "fp"):
+            _check(x, residual, w, out, *_run(x, residual, w, out, eps=0.0), eps=0.0)
+            rows = slice(0, 4) if out == "fp" else slice(0, 3)           # (u below 2^-119 has codes 0)
+            part = None if residual is None else r[rows]
+            _check(x[rows], part, w, out, *_run(x[rows], part, w, out))
+    # an infinity or a NaN in such a row still shows
+    x[0, cols // 3], x[2, cols - 1] = np.inf, np.nan
+    y, scale, _ = _run(x, None, w, "s8", eps=0.0)
+    assert np.all(y[[0, 2]] == 0) and np.isnan(scale[[0, 2]]).all() and np.isfinite(scale[[1, 3, 4, 5]]).all()
+    y, _, _ = _run(x, None, w, "fp", eps=0.0)
+    assert np.isnan(y[0, cols // 3]) and np.isnan(y[2]).all() and np.isfinite(y[[1, 3, 4, 5]]).all()
