@@ -378,7 +378,8 @@ int nnops_hip_dequantize_linear(const NnopsQdqArgs* args, void* stream);
  * a power of two. The codes and scales are what nnops_hip_gemm_i8 takes
  * as A and s_a.
  * sum may be x's or residual's buffer, y (f16 / f32) x's or residual's where
- * that is not sum's; otherwise no output may overlap another buffer.
+ * that is not sum's, with the same row pitch; otherwise no output may overlap
+ * another buffer.
  * Stream-ordered, no allocation, no workspace. */
 typedef struct NnopsRmsNormArgs {
     const void* x;              /* [rows][ld_x] f16 (in_f16) or f32 */

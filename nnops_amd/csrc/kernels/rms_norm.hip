@@ -464,6 +464,17 @@ extern "C" int nnops_hip_rms_norm(const NnopsRmsNormArgs* g, void* stream)
         (res && (g->ld_residual < g->cols || g->ld_sum < g->cols)) || !(g->epsilon >= 0.0f)) {
         return NNOPS_INVALID_ARGUMENT;
     }
+    // an output over an input: rows at the same places, or a row would be written
+    // that another has not read yet
+    const auto over = [&](const void* in, int64_t ld_in, const void* out, int64_t ld_out) {
+        return out == in && g->rows > 1 && ld_out != ld_in;
+    };
+    if (over(g->x, g->ld_x, g->y, g->ld_y) ||
+        (res && (over(g->residual, g->ld_residual, g->y, g->ld_y) || over(g->x, g->ld_x, g->sum, g->ld_sum) ||
+                 over(g->residual, g->ld_residual, g->sum, g->ld_sum) || g->y == g->sum)) ||
+        (s8 && (g->y == g->x || (res && g->y == g->residual)))) {
+        return NNOPS_INVALID_ARGUMENT;
+    }
     // (no epsilon: the least that keeps the factor of a row of zeros finite, so that
     // the row is zeros. Testing for it in the kernel took 3 % of 512 x 16384.)
     const float eps = g->epsilon > 0.0f ? g->epsilon : 0x1p-149f;

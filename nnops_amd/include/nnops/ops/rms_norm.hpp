@@ -12,7 +12,7 @@
 /// PerToken activation that Linear / MatMul take:
 ///   a = max |h weight|, code = rint(h weight (127 / a)),
 ///   scale = a / 127 / sqrt(mean(h^2) + epsilon).
-/// sum may be x's or the residual's buffer.
+/// sum may be x's or the residual's buffer, with its row pitch.
 
 #include "nnops/core/op_base.hpp"
 

@@ -291,7 +291,7 @@ class DequantizeLinear(_Op):
 class RmsNorm(_Op):
     """inputs: x [.., C] (f16/f32), weight [C] (, residual of x's shape);
     outputs: y of x's shape (, scale f32 [rows] with an s8 y) (, sum = x +
-    residual, with a residual; may be x's or the residual's buffer). An s8 y and
+    residual, with a residual; may be x's or the residual's view). An s8 y and
     its scales are the per-token activation that Linear and MatMul take:
     ``tensor(y, scale_data=scale, granularity=1)``."""
     _takes_workspace = False       # (asking costs a tenth of a small call)

@@ -236,6 +236,26 @@ def test_abi_rms_norm():
     assert f(C.byref(g), None) == na.UNSUPPORTED
 
 
+def test_abi_rms_norm_in_place():
+    """An output over an input needs the input's row pitch; codes lie over
+    neither, and the two outputs not over one another. (No call here is let
+    through: each names one refusal.)"""
+    f = na.lib().nnops_hip_rms_norm
+    X, R, Y, S = 1 << 20, 2 << 20, 3 << 20, 4 << 20
+
+    def args(**kw):
+        g = na.RmsNormArgs()
+        g.rows, g.cols, g.in_f16, g.out_kind, g.weight = 2, 8, 1, na.OUT_F16, 4096
+        g.x, g.residual, g.y, g.sum = X, R, Y, S
+        g.ld_x = g.ld_residual = g.ld_y = g.ld_sum = 16
+        for k, v in kw.items():
+            setattr(g, k, v)
+        return g
+    for kw in (dict(sum=X, ld_sum=8), dict(sum=R, ld_sum=24), dict(y=X, ld_y=8), dict(y=R, ld_y=24), dict(y=S),
+               dict(sum=X, y=X), dict(y=X, out_kind=na.OUT_S8, scale=4096), dict(y=R, out_kind=na.OUT_S8, scale=4096)):
+        assert f(C.byref(args(**kw)), None) == na.INVALID_ARGUMENT, kw
+
+
 def test_abi_rotary():
     f = na.lib().nnops_hip_rotary
     g = na.RotaryArgs()
