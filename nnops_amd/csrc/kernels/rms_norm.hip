@@ -433,7 +433,22 @@ void launch_norm(const NormKern& k, hipStream_t s)
     } else if (chunks <= 2048) {
         launch_rows<T, 16, 2, S8, RES>(k, s);
     } else {
-        NNOPS_LAUNCH((rms_norm_wide<T, S8, RES>), dim3((unsigned)k.rows), dim3(1024), 0, s, k);
+        // a launch has fewer than 2^32 threads: 2^22 workgroups of these are too many
+        constexpr int64_t kSlab = 1 << 20;
+        for (int64_t r0 = 0; r0 < k.rows; r0 += kSlab) {
+            NormKern part = k;
+            part.rows = k.rows - r0 < kSlab ? k.rows - r0 : kSlab;
+            part.x = static_cast<const T*>(k.x) + r0 * k.ld_x;
+            part.y = S8 ? (void*)(static_cast<int8_t*>(k.y) + r0 * k.ld_y) : (void*)(static_cast<T*>(k.y) + r0 * k.ld_y);
+            if constexpr (S8) {
+                part.scale = k.scale + r0;
+            }
+            if constexpr (RES) {
+                part.r = static_cast<const T*>(k.r) + r0 * k.ld_r;
+                part.sum = static_cast<T*>(k.sum) + r0 * k.ld_sum;
+            }
+            NNOPS_LAUNCH((rms_norm_wide<T, S8, RES>), dim3((unsigned)part.rows), dim3(1024), 0, s, part);
+        }
     }
 }
 

@@ -211,3 +211,59 @@ def test_f32_rows_whose_squares_leave_the_range(cols):
     assert np.all(y[[0, 2]] == 0) and np.isnan(scale[[0, 2]]).all() and np.isfinite(scale[[1, 3, 4, 5]]).all()
     y, _, _ = _run(x, None, w, "fp", eps=0.0)
     assert np.isnan(y[0, cols // 3]) and np.isnan(y[2]).all() and np.isfinite(y[[1, 3, 4, 5]]).all()
+
+
+def test_more_wide_rows_than_a_launch_holds():
+    """2^22 + 3 rows of 16385, a workgroup of 1024 threads each, in place: all
+    alike but for a few at the ends of the launches."""
+    import torch
+    rows, cols = (1 << 22) + 3, 16385
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < rows * cols * 2 + (24 << 30):
+        pytest.skip("needs half of the card's memory")
+    announce(f"norm {rows}x{cols}")
+    x, _, w = _data(2, cols, True)
+    want = dev(_run(x, None, w, "fp")[0])
+    big = torch.empty((rows, cols), dtype=torch.float16, device="cuda")
+    big[:] = dev(x[0])
+    odd = torch.tensor([1, (1 << 20) - 1, 1 << 20, (1 << 22) - 1, 1 << 22, rows - 1], device="cuda")
+    big[odd] = dev(x[1])
+    assert na.RmsNorm().compute([na.tensor(big)], [na.tensor(big), na.tensor(dev(w))]) == na.OK
+    torch.cuda.synchronize()
+    assert torch.equal(big[odd], want[1:].expand(len(odd), cols))
+    big[odd] = want[0]
+    for r0 in range(0, rows, 1 << 18):
+        part = big[r0:r0 + (1 << 18)]
+        assert torch.equal(part, want[:1].expand(len(part), cols)), r0
+    del big, part
+    torch.cuda.empty_cache()
+
+
+def test_wide_rows_of_the_second_launch():
+    """2^20 + 2 rows of 16385 with residual and codes: every pointer moves on."""
+    import torch
+    rows, cols = (1 << 20) + 2, 16385
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < rows * cols * 5 + (24 << 30):
+        pytest.skip("needs half of the card's memory")
+    announce(f"norm {rows}x{cols} residual, codes")
+    x, r, w = _data(2, cols, True)
+    want_y, want_scale, want_sum = (dev(z) for z in _run(x, r, w, "s8"))
+    bx, br = (torch.empty((rows, cols), dtype=torch.float16, device="cuda") for _ in range(2))
+    bx[:], br[:] = dev(x[0]), dev(r[0])
+    odd = torch.tensor([1, (1 << 20) - 1, 1 << 20], device="cuda")
+    bx[odd], br[odd] = dev(x[1]), dev(r[1])
+    y, scale = torch.empty((rows, cols), dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+    op = na.RmsNorm(output_dtype=na.DT_S8)
+    assert op.compute([na.tensor(y), na.tensor(scale), na.tensor(bx)],
+                      [na.tensor(bx), na.tensor(dev(w)), na.tensor(br)]) == na.OK
+    torch.cuda.synchronize()
+    for got, want in ((y, want_y), (scale, want_scale), (bx, want_sum)):
+        shape = (len(odd),) + got.shape[1:]
+        assert torch.equal(got[odd], want[1:].expand(shape))
+        got[odd] = want[0]
+        for r0 in range(0, rows, 1 << 18):
+            part = got[r0:r0 + (1 << 18)]
+            assert torch.equal(part, want[:1].expand(part.shape)), r0
+    del bx, br, y, got, part
+    torch.cuda.empty_cache()
