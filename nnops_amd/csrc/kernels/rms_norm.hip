@@ -322,7 +322,6 @@ __global__ __launch_bounds__(1024) void rms_norm_wide(const NormKern p)
     const T* x = static_cast<const T*>(p.x) + row * p.ld_x;
     const T* r = RES ? static_cast<const T*>(p.r) + row * p.ld_r : nullptr;
     const T* w = static_cast<const T*>(p.w);
-    float factor = 1.0f;                           // of h in u and in the squares (row_rescale)
     auto chunk = [&](int64_t at, int n, float (&h)[8], float (&u)[8]) {
         float f[8];
         if (n >= 8) {
@@ -343,34 +342,40 @@ __global__ __launch_bounds__(1024) void rms_norm_wide(const NormKern p)
             if constexpr (RES) {
                 h[e] = __fadd_rn(h[e], f[e]);
             }
-            u[e] = __fmul_rn(__fmul_rn(h[e], factor), u[e]);
+            u[e] = __fmul_rn(h[e], u[e]);
         }
     };
-    float ss = 0.0f, eps = p.eps;
+    float ss = 0.0f;
     uint32_t a = 0;
-    const auto sums = [&] {
-        for (int64_t at = (int64_t)threadIdx.x * 8; at < p.cols; at += 8192) {
-            float h[8], u[8];
-            chunk(at, (int)min((int64_t)8, p.cols - at), h, u);
-            float part = 0.0f;                     // a sum of sums: no long chain of one rounding each
+    for (int64_t at = (int64_t)threadIdx.x * 8; at < p.cols; at += 8192) {
+        float h[8], u[8];
+        chunk(at, (int)min((int64_t)8, p.cols - at), h, u);
+        float part = 0.0f;                         // a sum of sums: no long chain of one rounding each
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float x = __fmul_rn(h[e], factor);
-                part = __builtin_fmaf(x, x, part);
-                a = max(a, magnitude(u[e]));
-            }
-            ss += part;
+        for (int e = 0; e < 8; ++e) {
+            part = __builtin_fmaf(h[e], h[e], part);
+            a = max(a, magnitude(u[e]));
         }
-        row_reduce<16>(ss, a);
-    };
-    sums();
+        ss += part;
+    }
+    row_reduce<16>(ss, a);
+    float eps = p.eps, factor = 1.0f;              // of h (row_rescale)
     if constexpr (kRescales<T>) {
         factor = row_rescale(ss, (float)p.cols, eps);
         if (factor != 1.0f) {                      // (the same in the whole workgroup)
             __syncthreads();                       // row_reduce's words are read
             ss = 0.0f;
             a = 0;
-            sums();
+            for (int64_t at = (int64_t)threadIdx.x * 8; at < p.cols; at += 8192) {
+                float part = 0.0f;
+                for (int64_t i = at; i < min(at + 8, p.cols); ++i) {
+                    const float h = __fmul_rn(RES ? __fadd_rn((float)x[i], (float)r[i]) : (float)x[i], factor);
+                    part = __builtin_fmaf(h, h, part);
+                    a = max(a, magnitude(__fmul_rn(h, (float)w[i])));
+                }
+                ss += part;
+            }
+            row_reduce<16>(ss, a);
             eps = scaled_eps(p, factor);
         }
     }
@@ -383,6 +388,14 @@ __global__ __launch_bounds__(1024) void rms_norm_wide(const NormKern p)
         const int n = (int)min((int64_t)8, p.cols - at);
         float h[8], u[8];
         chunk(at, n, h, u);
+        if constexpr (kRescales<T>) {
+            if (factor != 1.0f) {                  // (past f32's range u may be infinite before)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    u[e] = e < n ? __fmul_rn(__fmul_rn(h[e], factor), (float)w[at + e]) : 0.0f;
+                }
+            }
+        }
         if constexpr (RES) {
             store_upto(static_cast<T*>(p.sum) + row * p.ld_sum + at, n, h);
         }
