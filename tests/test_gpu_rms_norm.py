@@ -267,3 +267,35 @@ def test_wide_rows_of_the_second_launch():
             assert torch.equal(part, want[:1].expand(part.shape)), r0
     del bx, br, y, got, part
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("cols,rows", [(500, 9000), (1000, 8200), (1100, 2500), (4096, 2100), (5001, 2100), (8192, 1100),
+                                       (16384, 600)])
+def test_rows_past_the_workgroups(cols, rows):
+    """More rows than the launch has units (of 1, 4, 8 and 16 waves): each takes
+    several, the next one's loads in flight; then the same in place."""
+    import torch
+    for f16 in (True, False) if cols < 8192 else (True,):
+        announce(f"norm rows in turn {rows}x{cols} f16={f16}")
+        x, r, w = _data(rows, cols, f16)
+        want = {}
+        for out in ("s8", "fp"):
+            want[out] = _run(x, r, w, out)
+            _check(x, r, w, out, *want[out])
+        _check(x, None, w, "s8", *_run(x, None, w, "s8"))
+        # sum over x and over the residual, y over the other
+        op = na.RmsNorm(output_dtype=na.DT_F16 if f16 else na.DT_F32)
+        dw = dev(w)
+        for over in ("x", "r"):
+            dx, dr = dev(x), dev(r)
+            total, y = (dx, dr) if over == "x" else (dr, dx)
+            assert op.compute([na.tensor(y), na.tensor(total)], [na.tensor(dx), na.tensor(dw), na.tensor(dr)]) == na.OK
+            torch.cuda.synchronize()
+            assert np.array_equal(host(y), want["fp"][0]) and np.array_equal(host(total), want["fp"][2])
+        op8 = na.RmsNorm(output_dtype=na.DT_S8)
+        dx, codes, scale = dev(x), torch.zeros((rows, cols), dtype=torch.int8, device="cuda"), torch.zeros(rows, device="cuda")
+        assert op8.compute([na.tensor(codes), na.tensor(scale), na.tensor(dx)],
+                           [na.tensor(dx), na.tensor(dw), na.tensor(dev(r))]) == na.OK
+        torch.cuda.synchronize()
+        for got, want8 in zip((codes, scale, dx), want["s8"]):
+            assert np.array_equal(host(got), want8)
