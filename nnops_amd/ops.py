@@ -33,10 +33,39 @@ def _ptr(x):
     return x.ctypes.data  # host (numpy) table: the caller keeps it alive
 
 
+def _row_step(sizes, strides):
+    """Elements from row to row of a view, the same between any two: what a
+    descriptor can say. A view whose rows lie otherwise (a slice of a middle dim,
+    a 1-D view with gaps, a broadcast) has no descriptor: taken for one it would
+    be read at the wrong places."""
+    cols = sizes[-1]
+    assert len(sizes) == 1 or strides[-1] == 1, "innermost dim must be contiguous"
+    step, rows = 0, 1
+    for i in range(len(sizes) - 2, -1, -1):
+        size, stride = sizes[i], strides[i]
+        if size == 1:
+            continue                        # (one row's stride may be anything)
+        if rows == 1:
+            step = stride
+        elif stride != step * rows:
+            raise ValueError(f"rows must be evenly spaced: shape {sizes}, strides {strides}")
+        rows *= size
+    if rows > 1:
+        if step < cols:
+            raise ValueError(f"rows must not overlap: shape {sizes}, strides {strides}")
+        return step
+    if len(sizes) == 1:
+        if cols > 1 and strides[0] != 1:
+            raise ValueError(f"a 1-D tensor must be contiguous: stride {strides[0]}")
+        return 0
+    return max(strides[-2], cols)
+
+
 def tensor(t, *, dtype=None, shape=None, scale=1.0, zero_point=0, scale_data=None,
            zero_point_data=None, granularity=None, pitch=None):
     """An NnopsTensor over a torch tensor (device memory). The innermost dim
-    must be contiguous; the row pitch is taken from stride(-2) unless given.
+    must be contiguous and the rows evenly spaced; the row pitch is their step
+    unless given (stride(-2) of a tensor given with another ``shape``).
     ``dtype``/``shape`` override the torch view (q4_1: pass DT_Q4_1 and the
     logical shape in values, the tensor being the uint8 block bytes).
     ``scale_data``/``zero_point_data`` may be host (numpy) or device (torch)."""
@@ -49,9 +78,13 @@ def tensor(t, *, dtype=None, shape=None, scale=1.0, zero_point=0, scale_data=Non
     x.data = t.data_ptr() if t is not None else None
     if pitch is not None:
         x.pitch = int(pitch)
-    elif t is not None and t.dim() >= 2 and t.numel() > 0:   # (an empty one's strides mean nothing)
-        assert t.stride(-1) == 1, "innermost dim must be contiguous"
-        x.pitch = t.stride(-2) * t.element_size()
+    elif t is not None and t.numel() > 0:   # (an empty one's strides mean nothing)
+        strides = t.stride()
+        if shape is None and strides and strides != (1,):
+            x.pitch = _row_step(shp, strides) * t.element_size()
+        elif len(strides) >= 2:
+            assert strides[-1] == 1, "innermost dim must be contiguous"
+            x.pitch = strides[-2] * t.element_size()
     x.scale = float(scale)
     x.zero_point = int(zero_point)
     keep = []

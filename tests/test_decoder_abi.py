@@ -372,3 +372,31 @@ def test_abi_workspace_size_of_refused_calls():
             assert f(C.byref(g)) == 0, (field, value)
         setattr(obj, field, old)
     assert f(C.byref(g)) == need
+
+
+# --- tensor(): views as descriptors ----------------------------------------------
+
+def test_tensor_of_views():
+    """A view whose rows are evenly spaced has their step as its pitch, whatever
+    its rank; any other is refused, not read as a dense one."""
+    import torch
+    x = torch.zeros((4, 10, 64), dtype=torch.float16)
+    for view, pitch in ((x, 128), (x[:, :, :32], 128), (x[1:, :, 8:24], 128), (x[:, 3], 1280), (x[:, 3, :16], 1280),
+                        (x[:, :1], 1280), (x[2:3, :4], 128), (x[1, 2:3, 5:9], 128), (x[:, ::2], 256), (x[1], 128),
+                        (x[1, 2], 0), (x[1, 2, :7], 0), (x[1:2, 4, :], 1280), (x[:, :, :1][:, :, 0:1], 128)):
+        t = na.tensor(view)
+        assert t.pitch == pitch and [t.dims[i] for i in range(t.rank)] == list(view.shape), view.stride()
+        assert t.data == view.data_ptr()
+    one = torch.zeros((5, 1)).t()                                        # strides (1, 1): a dense row
+    assert na.tensor(one).pitch == 20
+    assert na.tensor(torch.zeros((1, 4, 8)).transpose(0, 1)).pitch == 32  # [4, 1, 8], strides (8, 32, 1)
+    assert na.tensor(torch.zeros((0, 8))).pitch == 0
+    lengths = torch.zeros((6, 2), dtype=torch.int32)
+    cache = torch.zeros((9, 4, 16, 32), dtype=torch.int8)
+    for view in (x[:, :5], x[::2, :5], x[:, 2:4, :8], x[1, 2, ::2], lengths[:, 0], lengths.t()[1], cache[:, :2],
+                 cache[:, :, :8], torch.zeros(8).expand(3, 8), torch.zeros((1, 8)).expand(4, 8),
+                 torch.zeros(20).as_strided((3, 8), (6, 1))):
+        with pytest.raises((ValueError, AssertionError)):
+            na.tensor(view)
+    with pytest.raises(AssertionError):
+        na.tensor(x.transpose(1, 2))
