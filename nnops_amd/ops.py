@@ -393,8 +393,12 @@ def rotary_table(max_pos, rotary_dim, *, base=10000.0, factor=1.0, original_cont
     import torch
     if out is None:
         out = torch.empty((max_pos, rotary_dim), dtype=torch.float32, device=device)
+    elif out.dtype != torch.float32 or tuple(out.shape) != (max_pos, rotary_dim):
+        raise ValueError(f"out must be f32 [{max_pos}, {rotary_dim}], not {out.dtype} {list(out.shape)}")
+    elif out.numel() > 0 and (out.stride(1) != 1 or (max_pos > 1 and out.stride(0) < rotary_dim)):
+        raise ValueError(f"out's rows must be contiguous and not overlap: strides {out.stride()}")
     a = L.RotaryTableArgs()
-    a.table, a.max_pos, a.rotary_dim, a.ld_table = out.data_ptr(), max_pos, rotary_dim, out.stride(0)
+    a.table, a.max_pos, a.rotary_dim, a.ld_table = out.data_ptr(), max_pos, rotary_dim, max(out.stride(0), rotary_dim)
     a.base, a.factor, a.original_context = base, factor, original_context
     a.low_turns, a.high_turns, a.attention_factor = low_turns, high_turns, attention_factor
     rc = L.lib().nnops_hip_rotary_table(C.byref(a), _stream_ptr(stream))

@@ -400,3 +400,13 @@ def test_tensor_of_views():
             na.tensor(view)
     with pytest.raises(AssertionError):
         na.tensor(x.transpose(1, 2))
+
+
+def test_rotary_table_out():
+    """What the table is written to has to hold it: type, shape, rows."""
+    import torch
+    for out in (torch.zeros((4, 8), dtype=torch.float16), torch.zeros((3, 8)), torch.zeros((4, 6)), torch.zeros(32),
+                torch.zeros((8, 4)).t(), torch.zeros((1, 8)).expand(4, 8), torch.zeros((4, 16))[:, ::2]):
+        with pytest.raises(ValueError):
+            na.rotary_table(4, 8, out=out, stream=0)
+    assert na.rotary_table(0, 8, out=torch.zeros((0, 8)), stream=0).shape == (0, 8)
