@@ -129,18 +129,36 @@ def _stream_ptr(stream):
     return raw(device())
 
 
+class _StreamMemory:
+    """Memory of torch's allocator that belongs to a stream: once this is gone
+    it goes to later work of that stream only."""
+
+    def __init__(self, nbytes, device, stream):
+        import torch
+        self._free = torch.cuda.caching_allocator_delete
+        self._at = torch.cuda.caching_allocator_alloc(nbytes, device, stream)
+
+    def data_ptr(self):
+        return self._at
+
+    def __del__(self):
+        if getattr(self, "_at", 0):
+            self._free(self._at)
+            self._at = 0
+
+
 def _workspace(nbytes, device, stream=None):
-    """A buffer of the stream that uses it: once the call has returned, its
-    memory goes to later work of that stream only."""
+    """A buffer of the stream that uses it. (For a stream that is named: asked of
+    the allocator, 1.5 us; entering the stream for a torch tensor takes 7, as
+    long as a whole small call.)"""
     import torch
     if nbytes == 0:
         return None
     if stream is None:
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     if isinstance(stream, int):
-        stream = torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream()
-    with torch.cuda.stream(stream):
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+        return _StreamMemory(nbytes, torch.device(device).index, stream)
+    return _StreamMemory(nbytes, getattr(stream, "device_index", None), stream.cuda_stream)
 
 
 def _epilogue(ep, act=None, min_clip=-math.inf, max_clip=math.inf, quant=L.EQ_NONE,
