@@ -540,6 +540,19 @@ int nnops_hip_gemm_fp_plan(const NnopsGemmFpArgs* args, size_t workspace_bytes, 
 int nnops_hip_gemm_q4_1_plan(const NnopsGemmQ41Args* args, int32_t pass, size_t workspace_bytes,
                              NnopsGemmPlan* plan);
 
+typedef struct NnopsCacheAttentionPlan {
+    int32_t tile_rows;          /* rows (tokens x heads of a group) of a workgroup: 128 or 256 that share their
+                                   tiles of tokens, 16 otherwise */
+    int32_t one_page;           /* of those: a tile of 64 tokens lies in one page */
+    int32_t splits;             /* of the longest sequence that the page table has room for */
+    int32_t split_tokens;       /* tokens of a split */
+    int32_t join;               /* of the splits: 0 none, 1 four channels a lane, 2 a workgroup a row */
+    size_t workspace_bytes;
+} NnopsCacheAttentionPlan;
+
+/* OK, or what the call itself would say of the sizes. */
+int nnops_hip_cache_attention_plan(const NnopsCacheAttentionArgs* args, NnopsCacheAttentionPlan* plan);
+
 /* Library version and build target, for the caller's diagnostics. */
 const char* nnops_hip_build_info(void);
 

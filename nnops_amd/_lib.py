@@ -193,6 +193,11 @@ class GemmPlan(C.Structure):
                 ("short_stage", C.c_int32), ("in_place", C.c_int32), ("workspace_bytes", C.c_size_t)]
 
 
+class CacheAttentionPlan(C.Structure):
+    _fields_ = [("tile_rows", C.c_int32), ("one_page", C.c_int32), ("splits", C.c_int32), ("split_tokens", C.c_int32),
+                ("join", C.c_int32), ("workspace_bytes", C.c_size_t)]
+
+
 PLAN_NO_PASS, PLAN_PASS, PLAN_GATED_PASS = range(3)
 
 
@@ -230,6 +235,7 @@ SIGNATURES = {
     "nnops_hip_kv_cache_write": (C.c_int, [C.POINTER(KvRowsArgs), C.c_void_p]),
     "nnops_hip_kv_cache_read": (C.c_int, [C.POINTER(KvRowsArgs), C.c_void_p]),
     "nnops_hip_cache_attention_workspace_size": (C.c_size_t, [C.POINTER(CacheAttentionArgs)]),
+    "nnops_hip_cache_attention_plan": (C.c_int, [C.POINTER(CacheAttentionArgs), C.POINTER(CacheAttentionPlan)]),
     "nnops_hip_cache_attention": (C.c_int, [C.POINTER(CacheAttentionArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
     "nnops_matmul_attrs_init": (None, [C.POINTER(MatMulAttrs)]),
     "nnops_linear_attrs_init": (None, [C.POINTER(LinearAttrs)]),

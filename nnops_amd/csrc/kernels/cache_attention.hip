@@ -473,6 +473,7 @@ struct AttnPlan {
     int64_t items;        // row tiles, all KV heads
     int32_t tile_rows, per_seq, chunk, splits;
     bool tiled;           // attention_rows_tiled, else attention_rows16
+    bool join_few;        // attention_join_few joins the splits, else attention_join
     size_t workspace;
 };
 
@@ -542,6 +543,9 @@ AttnPlan attn_plan(const NnopsCacheAttentionArgs* g)
     const int64_t chunk = ((tiles + splits - 1) / splits + 3) / 4 * 4;
     a.chunk = (int32_t)(chunk > 4 ? chunk : 4);
     a.splits = (int32_t)(tiles > 0 ? (tiles + a.chunk - 1) / a.chunk : 1);
+    // (a wave per row where few rows and 4 splits leave it waiting: 8 x 1 of 1500
+    // 13.8 us, 12.6 with a workgroup; 1 x 64 of 2000 16.9 and 19.5)
+    a.join_few = a.splits <= kFewSplits && (a.splits <= 3 || g->rows * g->q_heads >= 1024);
     a.workspace = a.splits > 1 ? (size_t)a.splits * g->rows * g->q_heads * (g->cache.head_dim + 2) * 4 : 0;
     return a;
 }
@@ -578,9 +582,7 @@ void launch_attention(const AttnKern& k, const AttnPlan& a, hipStream_t s)
     } else {
         NNOPS_LAUNCH((attention_rows16<T, 256>), grid, dim3(256), 0, s, k);
     }
-    // (a wave per row where few rows and 4 splits leave it waiting: 8 x 1 of 1500
-    // 13.8 us, 12.6 with a workgroup; 1 x 64 of 2000 16.9 and 19.5)
-    if (a.splits > 1 && a.splits <= kFewSplits && (a.splits <= 3 || k.c.rows * k.q_heads >= 1024)) {
+    if (a.splits > 1 && a.join_few) {
         const int rows = 256 / join_lanes(k.c.d);   // of a workgroup
         NNOPS_LAUNCH(attention_join_few<T>, dim3((unsigned)((k.c.rows * k.q_heads + rows - 1) / rows)), dim3(256), 0, s, k);
     } else if (a.splits > 1) {
@@ -598,6 +600,25 @@ extern "C" size_t nnops_hip_cache_attention_workspace_size(const NnopsCacheAtten
     // (the tables' contents and the pointers play no part; a call that is refused,
     // or that has nothing to do, needs none)
     return check_shapes(g) >= 0 ? 0 : attn_plan(g).workspace;
+}
+
+extern "C" int nnops_hip_cache_attention_plan(const NnopsCacheAttentionArgs* g, NnopsCacheAttentionPlan* out)
+{
+    if (out == nullptr) {
+        return NNOPS_INVALID_ARGUMENT;
+    }
+    *out = NnopsCacheAttentionPlan{};
+    if (const int rc = check_shapes(g); rc >= 0) {
+        return rc;
+    }
+    const AttnPlan a = attn_plan(g);
+    out->tile_rows = a.tile_rows;
+    out->one_page = a.tiled && tiled_one_page(g->cache.head_dim, g->cache.page_tokens);
+    out->splits = a.splits;
+    out->split_tokens = a.chunk * kTile;
+    out->join = a.splits <= 1 ? 0 : a.join_few ? 1 : 2;
+    out->workspace_bytes = a.workspace;
+    return NNOPS_OK;
 }
 
 extern "C" int nnops_hip_cache_attention(const NnopsCacheAttentionArgs* g, void* workspace, size_t workspace_bytes,

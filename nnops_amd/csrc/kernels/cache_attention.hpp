@@ -269,6 +269,8 @@ __device__ __forceinline__ Acc product(typename Operand<T>::Vec a, const typenam
 // attention_rows_tiled's launch (cache_attention_tiled.hip): d, type and rows
 // of a workgroup that it has a kernel for.
 int tiled_rows(int64_t d, bool f16, int64_t page, int64_t rows);
+// Its form for tiles that lie in one page (wider heads come with such pages only).
+inline bool tiled_one_page(int64_t d, int64_t page) { return d > 128 || page >= kTile; }
 void launch_tiled(const AttnKern& k, const dim3& grid, bool f16, hipStream_t s);
 
 }  // namespace nnops_amd

@@ -576,7 +576,7 @@ namespace {
 template <typename T, int DP, int NW>
 void launch_one(const AttnKern& k, const dim3& grid, hipStream_t s)
 {
-    if (DP > 128 || k.c.page >= kTile) {           // (wider heads come with such pages only)
+    if (DP > 128 || tiled_one_page(k.c.d, k.c.page)) {
         NNOPS_LAUNCH((attention_rows_tiled<T, DP, NW, true>), grid, dim3(64 * NW), 0, s, k);
     } else if constexpr (DP <= 128) {
         NNOPS_LAUNCH((attention_rows_tiled<T, DP, NW, false>), grid, dim3(64 * NW), 0, s, k);

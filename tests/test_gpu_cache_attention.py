@@ -223,6 +223,26 @@ def test_hidden_values_do_not_show_in_tiles(page, f16):
         assert np.array_equal(want, _run(q, (kc, vc, k2, v2, t2), lens, [n] * seqs, **kw))
 
 
+# d, page, heads, group, sequences, rows of each, tokens of the longest, window, type, splits
+FEW_SPLITS = [(64, 16, 1, 2, 3, 1, 640, 0, True, 3), (128, 64, 2, 4, 2, 2, 700, 0, True, 3), (256, 32, 1, 3, 2, 1, 300, 0, True, 2),
+              (128, 128, 1, 16, 8, 8, 1000, 0, True, 4), (80, 16, 2, 8, 32, 2, 1900, 0, True, 8),
+              (64, 32, 2, 16, 16, 2, 1500, 1000, True, 5), (64, 64, 1, 4, 2, 1, 300, 0, False, 2),
+              (128, 16, 2, 8, 16, 4, 1100, 0, False, 5), (256, 256, 1, 4, 3, 1, 600, 0, False, 3)]
+
+
+@pytest.mark.parametrize("d,page,heads,group,seqs,n,tokens,window,f16,splits", FEW_SPLITS)
+def test_few_splits(d, page, heads, group, seqs, n, tokens, window, f16, splits):
+    """Few splits, joined by lanes of a wave; sequences of one split, of none and
+    of all beside one another."""
+    announce(f"attention few splits d={d} page={page} seqs={seqs} n={n} tokens={tokens} f16={f16}")
+    lens = [(tokens, n, 130, 300, tokens - 1, 0, 257, 700)[i % 8] for i in range(seqs)]
+    lens = [min(x, tokens) for x in lens]
+    cache = _cache(seqs, tokens, heads, page, d)
+    q = _q(40, seqs * n, heads * group * d, f16)
+    for ragged in (False, True):
+        _check(q, cache, lens, [n] * seqs, ragged=ragged, window=window, pad=4 if ragged else 0)
+
+
 def test_scales_far_apart():
     """Pages whose value scales differ by powers of ten, pages of zeros, the
     smallest scale; a scale of 0 reads as zeros."""
