@@ -498,8 +498,9 @@ int nnops_hip_kv_cache_read(const NnopsKvRowsArgs* args, void* stream);
  *   j <= p  and  (window == 0  or  p - j < window  or  j < sinks),
  * 0 where there are none. (The call's own rows are in the cache already.)
  * Scores, softmax statistics and sums are f32. f16: q and the codes enter the
- * matrix products exactly, the probabilities as f16 (of 14 bits more range);
- * f32: both exactly, as three bf16 parts.
+ * matrix products exactly, the probabilities as the sum of two f16 (22 bits),
+ * in calls whose rows share their tiles (nnops_hip_cache_attention_plan) as one
+ * f16 (11 bits, of 14 bits more range); f32: both exactly, as three bf16 parts.
  * nnops_hip_cache_attention_workspace_size bytes of workspace (16-byte
  * aligned) hold the partial results of long sequences that are split over the
  * chip; the size goes by the sizes in args alone (no pointer is followed), and

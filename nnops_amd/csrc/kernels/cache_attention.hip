@@ -29,8 +29,8 @@
 // channel 0's, the last tile is peeled off): the waits after one are for
 // everything (74 us for the batch below, and 42 against 35 at d 64).
 // One token of each of 64 sequences of up to 4096, 32 query and 8 KV heads, d 128:
-// 66.3 us, 4.68 TB/s; of one sequence of 126976: 55.0 us, 4.73 TB/s; of one of
-// 777: 9.0 us, two launches and the host's 5.
+// 68.2 us, 4.55 TB/s; of one sequence of 126976: 55.9 us, 4.65 TB/s; of one of
+// 777: 9.2 us, two launches and the host's 5.
 #include <type_traits>
 
 #include "cache_attention.hpp"
@@ -41,11 +41,12 @@ namespace {
 constexpr int kRows = 16;           // rows of a wave
 
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const AttnKern p)
+__global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void attention_rows16(const AttnKern p)
 {
     constexpr int kC = DP / 64;                    // 64-channel pieces of a key
     constexpr int kT = DP / 16;                    // 16-channel tiles of O
     typedef Operand<T> Op;
+    constexpr int kWeights = Op::kParts == 1 ? 2 : Op::kParts;   // parts of a probability
     constexpr int kPitch = DP + 4;
     __shared__ float s_o[4][kRows][kPitch];
     __shared__ float s_m[4][kRows], s_l[4][kRows];
@@ -220,7 +221,6 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
         }
         const float shift = m_run > kNone ? kLift - m_run : 0.0f;
         float sum = 0.0f, w[2][8];
-        typename Op::Vec pf[2][Op::kParts];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
@@ -229,10 +229,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_rows16(const
                 sum += w[t / 2][4 * (t % 2) + i];
             }
         }
-        Op::split(w[0], pf[0]);
-        Op::split(w[1], pf[1]);
         // a page of which the row sees nothing adds nothing, whatever its scale
         l_run += sum != 0.0f ? sum * sc.inv : 0.0f;
+        typename Op::Vec pf[2][kWeights];
+        Op::split(w[0], pf[0]);
+        Op::split(w[1], pf[1]);
 #pragma unroll
         for (int t = 0; t < kT; ++t) {
             o[t] = product<T>(Op::codes((uint32_t)vr[t].x, (uint32_t)vr[t].y), pf[0], o[t]);

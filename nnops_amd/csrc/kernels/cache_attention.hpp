@@ -140,7 +140,14 @@ __device__ __forceinline__ Scales softmax_scales(const AttnKern& p, PageScales s
 }
 
 // The operands of the two products, by the rows' type.
-//   f16: the rows as they are, the probabilities rounded to f16, codes as f16.
+//   f16: the rows as they are, codes as f16, the probabilities rounded to f16
+//        where many rows share their tiles, as the sum of two f16 (22 bits) where
+//        few rows have a workgroup. HBM bounds few rows: the second part costs 1
+//        to 5 % (us: one token over 777 9.1 -> 9.25, over 126976 55.4 -> 56.1, of 64
+//        sequences of up to 4096 66.4 -> 68.3, heads of 64 36.9 -> 38.6, of 256 49.5
+//        -> 50.5). The matrix cores bound many: a prompt of 4096 would take 196
+//        instead of 152, for an error that the output's own rounding to f16 exceeds
+//        (against 64 bits 2.6e-4 of the result, 2.1e-4 with that rounding alone).
 //   f32: each value as three bf16 parts that hold it exactly (8 bits each, by
 //        truncation, the last difference having no more), codes as bf16 (7 bits
 //        and a sign: exact), three products into one f32 accumulator. Two f16
@@ -170,6 +177,14 @@ struct Operand {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             v[0][e] = (_Float16)x[e];   // (in pairs: v_cvt_pk_f16_f32, to nearest)
+        }
+    }
+    static __device__ __forceinline__ void split(const float (&x)[8], Vec (&v)[2])
+    {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            v[0][e] = (_Float16)x[e];
+            v[1][e] = (_Float16)__fsub_rn(x[e], (float)v[0][e]);
         }
     }
     static __device__ __forceinline__ v4f mfma(Vec a, Vec b, v4f c)
@@ -255,12 +270,11 @@ struct Operand<float> {
 };
 
 // c + a (b's parts)
-template <typename T, typename Acc>
-__device__ __forceinline__ Acc product(typename Operand<T>::Vec a, const typename Operand<T>::Vec (&b)[Operand<T>::kParts],
-                                       Acc c)
+template <typename T, int N, typename Acc>
+__device__ __forceinline__ Acc product(typename Operand<T>::Vec a, const typename Operand<T>::Vec (&b)[N], Acc c)
 {
 #pragma unroll
-    for (int i = 0; i < Operand<T>::kParts; ++i) {
+    for (int i = 0; i < N; ++i) {
         c = Operand<T>::mfma(a, b[i], c);
     }
     return c;

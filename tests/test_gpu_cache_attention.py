@@ -243,6 +243,27 @@ def test_few_splits(d, page, heads, group, seqs, n, tokens, window, f16, splits)
         _check(q, cache, lens, [n] * seqs, ragged=ragged, window=window, pad=4 if ragged else 0)
 
 
+@pytest.mark.parametrize("d,page,heads,group", [(128, 64, 2, 4), (64, 16, 2, 3), (96, 32, 1, 16), (256, 64, 1, 2)])
+def test_weights_of_few_rows_hold_22_bits(d, page, heads, group):
+    """f16 rows, a few tokens of nearly equal weight: rounding the weights to
+    f16 would show (2^-12 of each, of results that cancel), the sum of two f16
+    leaves the output's rounding and the scores'."""
+    announce(f"attention weights d={d} page={page}")
+    lens, rows = [2, 3, 5, 9, 17, 33, 70, 300], [1] * 8
+    cache = _cache(8, 300, heads, page, d)
+    for size in (0.01, 1.0):
+        q = (size * dg.normal(41, (8, heads * group * d))).astype(np.float16)
+        got = _run(q, cache, lens, rows, ragged=False).astype(np.float64)
+        want, weight, spread = ref.attention(q, *cache, lens, rows)
+        # scores: as the other tests have it; weights: two f16, whose smallest step
+        # is 2^-30 of a weight that the running maximum stands for (64 there)
+        exact = ref.attention_tolerance(False, want, weight, spread, cache[3])
+        most = 127.0 * cache[3].max() * max(lens) * 2.0 ** -30
+        tol = exact + most + 1.01 * 2.0 ** -11 * abs(want) + 2.0 ** -24
+        worst = np.max(abs(got - want) / tol)
+        assert worst <= 1.0, (size, worst)
+
+
 def test_scales_far_apart():
     """Pages whose value scales differ by powers of ten, pages of zeros, the
     smallest scale; a scale of 0 reads as zeros."""
