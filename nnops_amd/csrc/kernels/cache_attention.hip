@@ -482,18 +482,26 @@ struct AttnPlan {
 // where a sequence has rows to fill one and the tiles, or the tiles by the
 // tokens they look at, fill the chip; 16 rows a workgroup, its waves sharing the
 // tokens, otherwise. Measured both ways (us, tiled / 16 rows; 32 query heads, 8
-// KV heads, d 128, f16, but where said):
-//   64 x 33 of 300    29.5 / 46.9     64 x 64 of 64     32.2 / 63.0
-//   1 x 64 of 2500    25.1 / 18.1     1 x 64 of 8000    28.7 / 31.7
-//   1 x 256 of 1000   25.9 / 17.0     1 x 256 of 8000   53.1 / 92.0
-//   16 x 128 of 128   16.6 / 33.2     8 x 200 of 1200   40.9 / 69.0
-//   f32 1 x 64 of 2500 29.8 / 26.4, of 8000 41.6 / 49.4; 16 x 128 of 300 44.2 / 64.9
-//   16 / 4 heads, d 64: 16 x 128 of 128 8.9 / 12.1, of 300 17.3 / 14.6; 1 x 256 of
-//   8000 37.6 / 34.0, f32 47.3 / 54.1
-//   ragged, of 2500: 24 of 1 to 100 rows 82.2 / 69.0, f32 135 / 111; 24 of 1 to 300
-//   122 / 192, d 64 60.8 / 56.5, f32 94.7 / 98.0; 7 of 1 to 300 67.7 / 78.5
-// (ragged calls: by their mean; f32 before its codes took one instruction each
-// instead of two and more, from which 16 rows gain the more). Splits of the longest sequence that the page
+// KV heads, d 128, but where said), where the rule takes the slower marked *:
+//   f16  64 x 33 of 300   32.4 / 57.8     64 x 64 of 64    32.3 / 58.7
+//        1 x 64 of 2500   26.3 / 20.9     1 x 64 of 8000   31.1 / 34.9
+//        1 x 256 of 1000  29.3 / 18.1     1 x 256 of 8000  52.9 / 96.6
+//        16 x 128 of 128  16.4 / 33.6     8 x 200 of 1200  44.0 / 93.8
+//        4 x 32 of 2000  *26.8 / 23.5     16 x 32 of 1000  32.1 / 32.1
+//   16 / 4 heads, d 64: 16 x 128 of 128 8.9 / 12.8, of 300 *20.6 / 17.9; 1 x 256 of
+//        8000 38.3 / 38.0; 8 x 200 of 1200 *34.7 / 32.6
+//   ragged, of 2500: 24 of 1 to 100 rows 85.2 / *125, of 1 to 300 141 / 275; d 64
+//        64.4 / *73.1 and 112 / 157; 7 of 1 to 300 78.5 / 103, d 64 62.2 / 60.1
+//   f32  64 x 33 of 300   87.8 / 86.7     64 x 64 of 64    54.9 / 110
+//        1 x 64 of 8000   45.6 / 40.2     1 x 256 of 1000  33.7 / 21.5
+//        1 x 200 of 4000  64.4 / 68.1     1 x 96 of 12000  77.0 / 93.3
+//        4 x 32 of 2000   32.3 / 27.0     2 x 128 of 8000  112 / 117
+//        2 x 256 of 1000 *45.9 / 38.6     8 x 200 of 1200  119 / 126
+//        d 64: 2 x 256 of 1000 30.6 / 22.5; 1 x 200 of 4000 35.8 / 41.7; 1 x 96 of
+//        12000 47.4 / 57.2; 16 / 4 heads 16 x 128 of 128 12.3 / 18.0, of 300 *24.9 / 23.0
+//   ragged, of 2500: 24 of 1 to 100 205 / 164, of 1 to 200 *290 / 270, of 1 to 300 365 /
+//        367; d 64 95.3 / 91.0, 151 / 150 and 170 / 202
+// (ragged calls: by their mean.) Splits of the longest sequence that the page
 // table has room for: as many workgroups as the chip holds at once (more of
 // them were slower: one token over 126976, 58 us with 512, 67 with 768, 72 with
 // 1024), no fewer than 4 tiles each, and none where a wave has no more than two
@@ -526,9 +534,10 @@ AttnPlan attn_plan(const NnopsCacheAttentionArgs* g)
     a.tile_rows = kRows;
     const bool ragged = g->cache.row_starts != nullptr;
     if (const int rows = mean > (ragged ? 256 : 96) ? tiled_rows(d, g->f16, g->cache.page_tokens, mean) : 0; rows > 0) {
-        // (tiles that are sure to be full; heads of 64 channels and fewer gain less)
+        // (tiles that are sure to be full; heads of 64 channels and fewer gain less,
+        // and so do wider f32 ones, whose four waves are in one phase)
         const int64_t items = ragged ? g->rows * group / rows * heads : items_of(rows);
-        const int64_t least = d <= 64 && (g->f16 || ragged) ? 7 << 15 : 7 << 14;
+        const int64_t least = d > 64 ? (g->f16 ? 7 << 14 : 9 << 15) : g->f16 || ragged ? 7 << 15 : 7 << 14;
         if (items >= 128 || items * tiles_of(rows) * d >= least) {
             a.tiled = true;
             a.tile_rows = rows;

@@ -108,7 +108,9 @@ def test_rules_of_the_rows():
         tiles = -(-least // (8 * d))
         assert plan(64, 1, 64 * tiles, d=d).tile_rows == 256
         assert plan(64, 1, 64 * (tiles - 1), d=d).tile_rows == 16
-    # f32 heads of 64: the same threshold as wider ones, unless ragged
+    # f32: 9 2^15 for wider heads (128 rows a tile); heads of 64 7 2^14 unless ragged
+    for tokens, want in ((64 * (9 << 15) // 1024, 128), (64 * (9 << 15) // 1024 - 64, 16)):
+        assert plan(32, 1, tokens, f16=False).tile_rows == want
     assert plan(64, 1, 64 * (7 << 14) // 512, d=64, f16=False).tile_rows == 256
     assert plan(33, 1, 64000, heads=8, group=4).tile_rows == 256 and plan(32, 1, 64000, heads=8, group=4).tile_rows == 128
 
