@@ -546,7 +546,7 @@ typedef struct NnopsCacheAttentionPlan {
                                    tiles of tokens, 16 otherwise */
     int32_t one_page;           /* of those: a tile of 64 tokens lies in one page */
     int32_t splits;             /* of the longest sequence that the page table has room for */
-    int32_t split_tokens;       /* tokens of a split */
+    int32_t split_tokens;       /* tokens of a split where it fills the table (fewer otherwise) */
     int32_t join;               /* of the splits: 0 none, 1 four channels a lane, 2 a workgroup a row */
     size_t workspace_bytes;
 } NnopsCacheAttentionPlan;

@@ -56,9 +56,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void at
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int n = lane % 16, g = lane / 16;
     const int kb = n / 4;                          // the token group of a lane's keys
-    // Without a window a wave's first tile is known before the sequence's length
-    // is: its page numbers are asked for beside it. (Past the sequence's end they
-    // may be anything; what is read through them is masked.)
+    // Without a window a wave's first tile is known before the lengths are, if
+    // sequences are not split or the longest fills the page table: its page numbers
+    // are asked for beside them. (Past the sequence's end they may be anything; what
+    // is read through them is masked.)
     const bool early = p.window == 0 && p.per_seq > 0 && c.table_pages > 0;
     int kid = 0, vid = 0;
     if (early) {
@@ -73,14 +74,15 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void at
     }
     const SeqRows& seq = rt.seq;
     const Span& span = rt.span;
-    const int b = rt.b, pmin = rt.pmin, pmax = rt.pmax, active = rt.active;
+    const int b = rt.b, pmin = rt.pmin, pmax = rt.pmax;
     const int row0 = rt.row0, rows = rt.rows;
     const int tok_last = pmax - (seq.len - seq.n);
     const int split = blockIdx.y;
-    if (split > 0 && split >= active) {
+    const int v0 = split * rt.chunk;
+    if (split > 0 && v0 >= span.tiles) {
         return;
     }
-    const int v0 = split * p.chunk, v1 = min(span.tiles, v0 + p.chunk);
+    const int v1 = min(span.tiles, v0 + rt.chunk);
 
     const int row = row0 + n;
     const bool is_row = row < rows;
@@ -245,7 +247,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void at
     };
     if (v0 + wave < v1) {
         int v = v0 + wave;
-        if (!early) {
+        if (!early || v0 != split * p.chunk) {
             ids(v);
         }
         const int first_k = kid, first_v = vid;
@@ -287,7 +289,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void at
     const int64_t token = seq.start + rtok;
     const int qh = kvh * p.group + (row0 + r - rtok * p.group);
     const int64_t at_part = ((int64_t)split * c.rows + token) * p.q_heads + qh;
-    const float scale = active > 1 ? 1.0f : l == 0.0f ? 0.0f : kDrop / l;
+    const float scale = rt.split ? 1.0f : l == 0.0f ? 0.0f : kDrop / l;
 #pragma unroll
     for (int i = 0; i < DP / 64; ++i) {
         const int ch = ch0 + 64 * i;
@@ -299,7 +301,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void at
         for (int w = 0; w < 4; ++w) {
             sum += f[w] * *reinterpret_cast<const v4f*>(&s_o[w][r][ch]);
         }
-        if (active > 1) {
+        if (rt.split) {
             *reinterpret_cast<v4f*>(&p.part[at_part * d + ch]) = sum;
         } else {
             T y[4];
@@ -310,14 +312,14 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void at
             __builtin_memcpy(static_cast<T*>(p.out) + token * p.ld_out + (int64_t)qh * d + ch, y, sizeof y);
         }
     }
-    if (active > 1 && ch0 == 0) {
+    if (rt.split && ch0 == 0) {
         p.part_ml[2 * at_part] = m;
         p.part_ml[2 * at_part + 1] = l;
     }
 }
 
 // The splits of a row that have something: 0 or 1 where there is nothing to
-// join (or the row is no sequence's).
+// join (or the row is no sequence's). Whole waves call it.
 __device__ __forceinline__ int splits_of(const AttnKern& p, int token, int qh)
 {
     const Paged& c = p.c;
@@ -334,13 +336,14 @@ __device__ __forceinline__ int splits_of(const AttnKern& p, int token, int qh)
     }
     RowTile rt;
     rt.seq = seq_rows(c, b);
+    const int chunk = chunk_of(p, rt.seq);
     const int tok = token - rt.seq.start;
     if (tok < 0 || tok >= rt.seq.n) {
         return 0;
     }
     const uint32_t row = (uint32_t)(tok * p.group) + (uint32_t)qh % (uint32_t)p.group;
-    place_tile(p, (int)(row / (uint32_t)p.tile_rows), rt);
-    return rt.active;
+    place_tile(p, (int)(row / (uint32_t)p.tile_rows), chunk, rt);
+    return rt.split ? (int)((uint32_t)(rt.span.tiles + chunk - 1) / (uint32_t)chunk) : 1;
 }
 
 // Joins the splits of the rows that have more than one. Few splits: 4 channels
@@ -355,12 +358,9 @@ __global__ __launch_bounds__(256) void attention_join_few(const AttnKern p)
     const int lanes = join_lanes(p.c.d);
     const uint32_t i = (blockIdx.x * 256 + threadIdx.x) / (uint32_t)lanes;
     const int token = (int)(i / (uint32_t)p.q_heads), qh = (int)(i - (uint32_t)token * p.q_heads);
-    if (token >= p.c.rows) {
-        return;
-    }
-    const int active = splits_of(p, token, qh);
+    const int active = splits_of(p, min(token, p.c.rows - 1), qh);
     const int d = p.c.d, ch = threadIdx.x % (uint32_t)lanes * 4;
-    if (active <= 1 || ch >= d) {
+    if (token >= p.c.rows || active <= 1 || ch >= d) {
         return;
     }
     const int64_t rows = (int64_t)p.c.rows * p.q_heads, at = (int64_t)token * p.q_heads + qh;
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(256) void attention_join(const AttnKern p)
 
 struct AttnPlan {
     int64_t items;        // row tiles, all KV heads
-    int32_t tile_rows, per_seq, chunk, splits;
+    int32_t tile_rows, per_seq, chunk, splits, tiles, whole;
     bool tiled;           // attention_rows_tiled, else attention_rows16
     bool join_few;        // attention_join_few joins the splits, else attention_join
     size_t workspace;
@@ -547,12 +547,14 @@ AttnPlan attn_plan(const NnopsCacheAttentionArgs* g)
     a.per_seq = g->cache.row_starts == nullptr ? (int32_t)(a.items / (b * heads)) : 0;
     const int64_t tiles = tiles_of(a.tile_rows);
     int64_t splits = ((a.tiled ? 256 : 512) + a.items - 1) / a.items;
-    const int64_t most = tiles <= 8 && g->f16 && d <= 128 && !a.tiled ? 1 : (tiles + 3) / 4;
+    a.whole = g->f16 && d <= 128 && !a.tiled ? 8 : 4;
+    const int64_t most = tiles <= a.whole ? 1 : (tiles + 3) / 4;
     splits = splits < most ? splits : most;
     splits = splits > 1 ? splits : 1;
     const int64_t chunk = ((tiles + splits - 1) / splits + 3) / 4 * 4;
     a.chunk = (int32_t)(chunk > 4 ? chunk : 4);
     a.splits = (int32_t)(tiles > 0 ? (tiles + a.chunk - 1) / a.chunk : 1);
+    a.tiles = (int32_t)tiles;
     // (a wave per row where few rows and 4 splits leave it waiting: 8 x 1 of 1500
     // 13.8 us, 12.6 with a workgroup; 1 x 64 of 2000 16.9 and 19.5)
     a.join_few = a.splits <= kFewSplits && (a.splits <= 3 || g->rows * g->q_heads >= 1024);
@@ -668,6 +670,10 @@ extern "C" int nnops_hip_cache_attention(const NnopsCacheAttentionArgs* g, void*
     k.sinks = g->sinks > INT32_MAX ? INT32_MAX : (int32_t)g->sinks;
     k.tile_rows = a.tile_rows;
     k.per_seq = a.per_seq;
+    k.splits = a.splits;
+    k.by_splits = a.splits > 1 ? (uint32_t)(((1ull << 32) + a.splits - 1) / a.splits) : 0;
+    k.tiles = a.tiles;
+    k.whole = a.whole;
     k.chunk = a.chunk;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (g->f16) {

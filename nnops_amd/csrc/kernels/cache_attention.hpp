@@ -30,7 +30,11 @@ struct AttnKern {
     int32_t q_heads, group, window, sinks;
     int32_t tile_rows;    // rows (tokens x heads of a group) of a workgroup
     int32_t per_seq;      // row tiles of a sequence, equal rows each (0: found by search)
-    int32_t chunk;        // tiles of 64 tokens that a split takes
+    int32_t splits;       // at most, of a tile of rows
+    uint32_t by_splits;   // ceil(2^32 / splits): to divide by it
+    int32_t tiles;        // of 64 tokens that the page table, or the window, has room for
+    int32_t whole;        // tiles of the longest sequence up to which none is split
+    int32_t chunk;        // tiles of a split where that sequence fills the table
 };
 
 // The tiles of 64 tokens that rows at positions pmin .. pmax look at: the
@@ -68,10 +72,63 @@ struct RowTile {
     int row0, rows;           // first row; rows of the sequence (entry: rows x heads fit 31 bits)
     int pmin, pmax;           // positions of the first and the last row
     Span span;
-    int active;               // splits that have tiles
+    int chunk;                // tiles of tokens that a split takes
+    bool split;               // it has more than one
 };
 
-__device__ __forceinline__ void place_tile(const AttnKern& p, int rt, RowTile& t)
+// The largest of a wave's values, all 0 or more, in all of its lanes: along rows
+// of 16 lanes, then from row to row, the last lane has it (a step of these takes
+// a few cycles, one through LDS 0.05 us).
+__device__ __forceinline__ int wave_max(int v)
+{
+#if __HIP_DEVICE_COMPILE__
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true));   // row_shr:1, 2, 4, 8
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, true));   // row_bcast:15, to rows 1 and 3
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, true));   // row_bcast:31, to rows 2 and 3
+    return __builtin_amdgcn_readlane(v, 63);
+#else
+    return v;
+#endif
+}
+
+// Tiles of tokens that a split takes: the longest sequence that has rows is
+// divided among the splits, whatever the page table has room for (one as wide as
+// a model's context, as a captured graph needs: one token over 2048, 64 splits of
+// 32 tiles each 19.1 us, by the sequence 10.6). Whole waves call it; the same in
+// all of them. (The product rounds up past the quotient at most: no more splits
+// than there are.)
+//   own: any sequence (in flight, beside the others). `longest`, of a lane: among
+// the sequences before the from-th, which were looked at already.
+__device__ __forceinline__ int chunk_of(const AttnKern& p, const SeqRows& own, int longest = 0, int from = 0)
+{
+    if (p.splits == 1) {
+        return std::numeric_limits<int>::max();
+    }
+    const Paged& c = p.c;
+    if (c.seqs == 1) {
+        longest = __builtin_amdgcn_readfirstlane(own.len);   // (scalar: loops over the tiles hang on it)
+    } else {
+        const int lane = threadIdx.x % 64;
+        if (from == 0) {                           // (no branch per lane: beside the loads of its own sequence)
+            const SeqRows s = seq_rows(c, min(lane, c.seqs - 1));
+            longest = s.n > 0 ? s.len : 0;
+            from = 64;
+        }
+        for (int b = from + lane; b < c.seqs; b += 64) {
+            const SeqRows s = seq_rows(c, b);
+            longest = s.n > 0 ? max(longest, s.len) : longest;
+        }
+        longest = wave_max(longest);
+    }
+    const int tiles = min((int)(((uint32_t)longest + kTile - 1) / kTile), p.tiles);
+    const uint32_t share = __umulhi((uint32_t)(tiles + p.splits - 1), p.by_splits);
+    return tiles <= p.whole ? p.whole : max((int)((share + 3u) & ~3u), 4);
+}
+
+__device__ __forceinline__ void place_tile(const AttnKern& p, int rt, int chunk, RowTile& t)
 {
     const uint32_t group = p.group;
     t.row0 = rt * p.tile_rows;
@@ -80,14 +137,15 @@ __device__ __forceinline__ void place_tile(const AttnKern& p, int rt, RowTile& t
     t.pmin = t.seq.len - t.seq.n + (int)((uint32_t)t.row0 / group);
     t.pmax = t.seq.len - t.seq.n + (int)(last / group);
     t.span = span_of(t.pmin, t.pmax, p.window, p.sinks);
-    t.active = (int)((uint32_t)(t.span.tiles + p.chunk - 1) / (uint32_t)p.chunk);
+    t.chunk = chunk;
+    t.split = t.span.tiles > chunk;
 }
 
 // The item-th tile. Later tiles of a sequence look at more tokens: `from_last`
 // numbers them from the last, so that the longest work begins first.
 __device__ __forceinline__ bool find_tile(const AttnKern& p, uint32_t item, bool from_last, RowTile& t)
 {
-    int rt;
+    int rt, chunk;
     if (p.per_seq > 0) {
         if (from_last) {
             const uint32_t back = item / (uint32_t)p.c.seqs;
@@ -98,16 +156,20 @@ __device__ __forceinline__ bool find_tile(const AttnKern& p, uint32_t item, bool
             rt = (int)(item - (uint32_t)t.b * p.per_seq);
         }
         t.seq = seq_rows(p.c, t.b);
+        chunk = chunk_of(p, t.seq);
     } else {
+        int longest = 0;
         const auto count = [&](const SeqRows& s) {
+            longest = s.n > 0 ? max(longest, s.len) : longest;
             return (int)((uint32_t)(s.n * p.group + p.tile_rows - 1) / (uint32_t)p.tile_rows);
         };
         if (!find_item(p.c, item, count, t.b, rt, t.seq)) {
             return false;
         }
+        chunk = chunk_of(p, t.seq, longest, (t.b / 64 + 1) * 64);
         rt = from_last ? count(t.seq) - 1 - rt : rt;
     }
-    place_tile(p, rt, t);
+    place_tile(p, rt, chunk, t);
     return true;
 }
 

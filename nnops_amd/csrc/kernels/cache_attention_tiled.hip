@@ -82,10 +82,11 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
     }
     const SeqRows& seq = rt.seq;
     const int split = blockIdx.y;
-    if (split > 0 && split >= rt.active) {
+    const int v0 = split * rt.chunk;
+    if (split > 0 && v0 >= rt.span.tiles) {
         return;
     }
-    const int v0 = split * p.chunk, v1 = min(rt.span.tiles, v0 + p.chunk);
+    const int v1 = min(rt.span.tiles, v0 + rt.chunk);
     const int tid = threadIdx.x, lane = tid % 64;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64);       // uniform: what hangs on it are scalar branches
     const int n = lane % 32, hh = lane / 32;
@@ -516,7 +517,7 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
     }
     l_run += across(l_run);
     const int64_t token = seq.start + tok;
-    if (rt.active > 1) {
+    if (rt.split) {
         const int64_t at_part = ((int64_t)split * c.rows + token) * p.q_heads + head;
         float* dst = p.part + at_part * d;
 #pragma unroll

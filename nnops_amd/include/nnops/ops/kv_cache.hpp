@@ -15,8 +15,9 @@
 ///   [sequences + 1], optional: sequence b has rows row_starts[b] up to
 ///   row_starts[b + 1] - 1 of the call (without it, as many each). A sequence's
 ///   rows are its last tokens.
-/// A page table with fewer columns costs less: attention sizes its launch by
-/// the longest sequence that the table has room for.
+/// A page table may be wider than any sequence: attention's launch, workspace and
+/// choice of kernel go by the longest sequence that the table has room for, the
+/// division of the work by the longest that there is.
 
 #include "nnops/core/op_base.hpp"
 

@@ -264,6 +264,26 @@ def test_weights_of_few_rows_hold_22_bits(d, page, heads, group):
         assert worst <= 1.0, (size, worst)
 
 
+@pytest.mark.parametrize("d,page,heads,group,n,f16", [(128, 64, 2, 4, 1, True), (64, 16, 2, 2, 1, False), (256, 32, 1, 2, 3, True),
+                                                      (128, 128, 4, 4, 40, True), (64, 16, 4, 8, 40, True), (64, 64, 4, 8, 40, False),
+                                                      (128, 32, 4, 4, 40, False)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (700, 30)])
+def test_wide_page_tables(d, page, heads, group, n, f16, window, sinks):
+    """A page table with room for far more tokens than any sequence holds, its
+    unused entries garbage: the split goes by what the rows look at (each
+    sequence its own), the results as ever."""
+    announce(f"attention wide table d={d} page={page} group={group} n={n} f16={f16} window={window}")
+    lens = [777, 2048, n, 513, 3000]
+    kc, vc, ks, vs, table = _cache(len(lens), 3000, heads, page, d)
+    wide = np.full((len(lens), 131072 // page), -5, np.int32)
+    wide[:, 1::2] = 1 << 30
+    for b, length in enumerate(lens):
+        wide[b, :-(-length // page)] = table[b, :-(-length // page)]
+    q = _q(42, len(lens) * n, heads * group * d, f16)
+    for ragged in (False, True):
+        _check(q, (kc, vc, ks, vs, wide), lens, [n] * len(lens), ragged=ragged, window=window, sinks=sinks)
+
+
 def test_scales_far_apart():
     """Pages whose value scales differ by powers of ten, pages of zeros, the
     smallest scale; a scale of 0 reads as zeros."""
