@@ -21,8 +21,8 @@
 // of a piece are issued a tile before it is written, its page number one before
 // that. Rows in LDS are 16 bytes longer than their data: 16 lanes' reads
 // of one column meet 16 bank groups, at constant offsets.
-// Measured: a prompt of 4096, 32 query and 8 KV heads of 128, f16, 137 GFLOP: 144 to
-// 152 us, 900 to 950 TFLOP/s, where a large f16 product reaches 1156 on this card;
+// Measured: a prompt of 4096, 32 query and 8 KV heads of 128, f16, 137 GFLOP: 143 to
+// 153 us, 900 to 960 TFLOP/s, where a large f16 product reaches 1156 on this card;
 // with four waves (128 rows), none a phase behind, 249 us.
 #include <type_traits>
 

@@ -18,10 +18,12 @@
 // reading, two channels by 16 tokens, so that its lanes write whole rows.
 // Measured, 8 heads of 128, f16: a prompt of 4096 tokens, pages of 16, 25 MB each
 // way: written in 10.6 us, read in 8.8; 32 sequences of 1000, pages of 64: read in
-// 20.6 us (98 MB, 4.8 TB/s), a token appended to each in 5.0. All waves of such a
-// write are resident at once: it is one chain (lengths, table, rows, the page's
-// maximum, codes) long, in which 8 vector instructions a value counted (now 4:
-// 11.6 -> 10.6 us); asking for the rows before the page number is looked at did not.
+// 20.6 us (98 MB, 4.8 TB/s), a token appended to each in 5.1, in 6.6 where every
+// page's scale grows (pages of 16: 4.9 and 5.9, of 128: 5.1 and 8.3). All waves of
+// the prompt's write are resident at once: it is one chain (lengths, table, rows,
+// the page's maximum, codes) long, in which 8 vector instructions a value counted
+// (now 4: 11.6 -> 10.6 us); asking for the rows before the page number is looked at
+// did not.
 #include "paged.hpp"
 
 namespace nnops_amd {

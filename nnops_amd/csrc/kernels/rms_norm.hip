@@ -13,7 +13,9 @@
 // Rows wider than 16 waves x 2 chunks (16384) are read twice.
 // Measured: 4096 rows of 4096 with residual and codes, 117 MB: 27 us, 4.3 TB/s; 777
 // rows of 5001, f16 to f16, 15.6 MB: 6.9 us a call (7.8 alone under the profiler),
-// most of it one load and store latency behind a launch; 8 rows of 4096: 4.4 us.
+// most of it one load and store latency behind a launch; 8 rows of 4096: 4.4 us;
+// rows read twice, 512 of 20000, f16 to f16, 41 MB: 12.1 us a call, with residual
+// and codes, 72 MB: 17.7.
 // Without a branch per element of a ragged last chunk (clamped loads, selected
 // after) the compiler flattened whole chunks too: 777 x 5001 took 9.2 us.
 #include "common.hpp"
