@@ -93,6 +93,14 @@ def test_long_sequences_are_split_and_joined():
             assert (p.tile_rows, p.join) == (16, 1) and (2 <= p.splits <= 8 if ragged else p.splits == splits)
 
 
+def test_many_sequences_are_split():
+    """test_splits_of_many_sequences."""
+    for seqs in (63, 64, 65, 130, 200):
+        for f16 in (True, False):
+            for rows, ragged in ((2 * seqs, False), (2 * seqs, True)):
+                assert plan(rows, seqs, 6000, heads=1, group=3, d=64, page=32, f16=f16, ragged=ragged).splits > 1
+
+
 # --- the rules ------------------------------------------------------------------------
 
 def test_rules_of_the_rows():

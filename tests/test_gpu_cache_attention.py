@@ -284,6 +284,26 @@ def test_wide_page_tables(d, page, heads, group, n, f16, window, sinks):
         _check(q, (kc, vc, ks, vs, wide), lens, [n] * len(lens), ragged=ragged, window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("seqs,longest", [(63, 62), (64, 0), (65, 64), (65, 63), (130, 129), (130, 70), (200, 100)])
+@pytest.mark.parametrize("f16", [True, False])
+def test_splits_of_many_sequences(seqs, longest, f16):
+    """More sequences than the 64 that a wave looks at in one step, the longest
+    anywhere among them (or one without rows, which does not count)."""
+    announce(f"attention splits of {seqs} sequences, longest {longest} f16={f16}")
+    heads, group, d, page, tokens = 1, 3, 64, 32, 1500
+    lens = 1 + dg.ints(43, (seqs,), 0, 119).astype(np.int64)
+    lens[longest], lens[seqs // 3] = tokens, 1300
+    kc, vc, ks, vs, table = _cache(seqs, tokens, heads, page, d)
+    wide = np.full((seqs, 4 * table.shape[1]), -1, np.int32)
+    wide[:, :table.shape[1]] = table
+    cache = (kc, vc, ks, vs, wide)
+    q = _q(44, 2 * seqs, group * d, f16)
+    for ragged in (False, True):
+        _check(q, cache, lens, [2] * seqs, ragged=ragged)
+    rows = [0 if i == longest else 1 + i % 3 for i in range(seqs)]
+    _check(_q(45, sum(rows), group * d, f16), cache, lens, rows, ragged=True)
+
+
 def test_scales_far_apart():
     """Pages whose value scales differ by powers of ten, pages of zeros, the
     smallest scale; a scale of 0 reads as zeros."""
