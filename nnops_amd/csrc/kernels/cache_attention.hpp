@@ -76,9 +76,8 @@ struct RowTile {
     bool split;               // it has more than one
 };
 
-// The largest of a wave's values, all 0 or more, in all of its lanes: along rows
-// of 16 lanes, then from row to row, the last lane has it (a step of these takes
-// a few cycles, one through LDS 0.05 us).
+// The largest of a wave's values, all 0 or more, as a scalar: along rows of 16
+// lanes, then from row to row, the last lane has it.
 __device__ __forceinline__ int wave_max(int v)
 {
 #if __HIP_DEVICE_COMPILE__
@@ -97,7 +96,9 @@ __device__ __forceinline__ int wave_max(int v)
 // Tiles of tokens that a split takes: the longest sequence that has rows is
 // divided among the splits, whatever the page table has room for (one as wide as
 // a model's context, as a captured graph needs: one token over 2048, 64 splits of
-// 32 tiles each 19.1 us, by the sequence 10.6). Whole waves call it; the same in
+// 32 tiles each 19.0 us, by the sequence 10.1; equal shares of each tile of rows
+// instead fill a second round where few are longer: f32 1 x 384 of 4000 94 -> 119).
+// Whole waves call it; the same in
 // all of them. (The product rounds up past the quotient at most: no more splits
 // than there are.)
 //   own: any sequence (in flight, beside the others). `longest`, of a lane: among
