@@ -519,6 +519,154 @@ size_t nnops_hip_cache_attention_workspace_size(const NnopsCacheAttentionArgs* a
 int nnops_hip_cache_attention(const NnopsCacheAttentionArgs* args, void* workspace, size_t workspace_bytes,
                               void* stream);
 
+/* Attention for sequences that share their first tokens (no counterpart in
+ * nnops): the same results as nnops_hip_cache_attention without a window, up to
+ * the order of the sums, with the tokens that a group of sequences shares read
+ * once for the group. Group g is the sequences group_starts[g] ..
+ * group_starts[g + 1] - 1, whose page tables hold the same pages for the first
+ * shared[g] tokens, as far as these fill whole pages (which the caller sees to;
+ * a sequence may be shorter, and may bring no rows). Read as shared: the whole
+ * pages and whole tiles of 64 tokens that every row of the group sees. Sequences
+ * in no group share nothing.
+ * group_starts and shared are device memory that the host does not see; starts
+ * are taken into [0, sequences], no group begins before the last one's end, and
+ * what is shared beyond the first sequence's tokens is not.
+ * Probabilities of f16 rows enter the second product as one f16 where a group's
+ * or sequence's rows share their tiles, as two where not. The workspace holds
+ * the parts of all rows: nnops_hip_prefix_attention_workspace_size bytes, 16-byte
+ * aligned, which need no initialization. */
+typedef struct NnopsPrefixAttentionArgs {
+    NnopsKvPages cache;
+    const void* q;              /* [rows][ld_q] f16 (f16) or f32 */
+    void* out;                  /* [rows][ld_out], q's type */
+    int64_t rows, q_heads, ld_q, ld_out; /* ld: elements */
+    int32_t f16;
+    float scale;                /* 0: 1 / sqrt(head_dim) */
+    int64_t groups;
+    const int32_t* group_starts; /* [groups + 1] */
+    const int32_t* shared;      /* [groups] */
+} NnopsPrefixAttentionArgs;
+
+size_t nnops_hip_prefix_attention_workspace_size(const NnopsPrefixAttentionArgs* args);
+int nnops_hip_prefix_attention(const NnopsPrefixAttentionArgs* args, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
+/* Page tables of a batch's continuations (no counterpart in nnops). A sequence
+ * of `lengths` tokens holds the pages in the first ceil(length / page_tokens)
+ * cells of its row of the table; refs[p] counts who holds page p (sequences of
+ * the table, and whoever else the caller counts), 0: free.
+ * Fork: all `sequences` are given up, and `children` take their place. Child i
+ * goes on from sequence parents[i] (outside [0, sequences): from nothing), L
+ * tokens, and has room for new_tokens[i] more (fewer, where negative):
+ *   new_lengths[i] = L' = L + new_tokens[i], taken into [0, new_table_pages *
+ *   page_tokens]; kept tokens K = min(L, L')
+ * Its first ceil(K / page_tokens) pages are the parent's. Where it grows past a
+ * page that K tokens fill in part, it will write into that page: if the page's
+ * only holders are children of this call that will, the first of them keeps it;
+ * the others take a fresh page each, and copies[i] = {old page, fresh page} says
+ * what nnops_hip_kv_cache_copy has to copy, for each layer's cache, before that
+ * (rows without: {-1, -1}). Pages up to ceil(L' / page_tokens) are fresh. Fresh
+ * pages are those whose count is 0 after the above, in ascending order, given out
+ * child by child, cell by cell; where there is none left, the cell is -1 (nothing
+ * is written there, and it reads as NaN). Cells past a child's pages are -1.
+ * new_refs: the counts after the call; may be refs. counts: {pages that are free
+ * now, cells that got none}. No other two arrays may overlap.
+ * The contents of the arrays are not seen by the host; a page number outside
+ * [0, pages) is no page, lengths are taken into what the table has room for.
+ * page_tokens: a power of two from 16 to 256. children, sequences <= 16384. */
+typedef struct NnopsKvForkArgs {
+    const int32_t* page_table;  /* [sequences][ld_table], table_pages columns */
+    int64_t sequences, table_pages, ld_table; /* ld: elements */
+    const int32_t* lengths;     /* [sequences] */
+    const int32_t* refs;        /* [pages] */
+    int64_t pages, page_tokens;
+    const int32_t* parents;     /* [children] */
+    const int32_t* new_tokens;  /* [children] */
+    int64_t children;
+    int32_t* new_table;         /* [children][ld_new_table], new_table_pages columns */
+    int64_t new_table_pages, ld_new_table;
+    int32_t* new_lengths;       /* [children] */
+    int32_t* new_refs;          /* [pages] */
+    int32_t* copies;            /* [children][2] */
+    int32_t* counts;            /* [2] */
+} NnopsKvForkArgs;
+
+size_t nnops_hip_kv_cache_fork_workspace_size(const NnopsKvForkArgs* args);
+int nnops_hip_kv_cache_fork(const NnopsKvForkArgs* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Compact: the pages that are held (refs != 0), U of them, moved to the numbers
+ * below U: the i-th that lies at U or above goes to the i-th free number below U,
+ * both ascending; copies[i] = {old, new} for nnops_hip_kv_cache_copy, {-1, -1}
+ * behind them. moved[p]: page p's new number, -1 for a free page (for tables that
+ * others keep). new_table: the table with the new numbers, -1 past a sequence's
+ * pages; new_refs: the counts, by new numbers. counts: {U, pages that move}.
+ * new_table may be page_table (with the same ld) and new_refs refs; no other two
+ * arrays may overlap. */
+typedef struct NnopsKvCompactArgs {
+    const int32_t* page_table;  /* [sequences][ld_table], table_pages columns */
+    int64_t sequences, table_pages, ld_table; /* ld: elements */
+    const int32_t* lengths;     /* [sequences] */
+    const int32_t* refs;        /* [pages] */
+    int64_t pages, page_tokens;
+    int32_t* new_table;         /* [sequences][ld_new_table] */
+    int64_t ld_new_table;
+    int32_t* new_refs;          /* [pages] */
+    int32_t* copies;            /* [pages / 2][2] */
+    int32_t* moved;             /* [pages] */
+    int32_t* counts;            /* [2] */
+} NnopsKvCompactArgs;
+
+size_t nnops_hip_kv_cache_compact_workspace_size(const NnopsKvCompactArgs* args);
+int nnops_hip_kv_cache_compact(const NnopsKvCompactArgs* args, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
+/* Copy: pages of a cache (codes and scales, all heads) copied to others of it,
+ * copies[i] = {from, to}; a row with a number outside [0, pages) is skipped. No
+ * page may be copied to twice, or both from and to. Sizes as of NnopsKvPages. */
+typedef struct NnopsKvCopyArgs {
+    int8_t* k;
+    int8_t* v;
+    float* k_scale;
+    float* v_scale;
+    int64_t pages, heads, page_tokens, head_dim;
+    const int32_t* copies;      /* [count][2] */
+    int64_t count;
+} NnopsKvCopyArgs;
+
+int nnops_hip_kv_cache_copy(const NnopsKvCopyArgs* args, void* stream);
+
+/* Log probabilities of given tokens, the entropy of the distribution and its
+ * most probable tokens (no counterpart in nnops). Of row r of the logits x:
+ *   log p_j = x_j - m - log s,  m = max x,  s = sum_j exp(x_j - m)
+ *   log_probs[r][i] = log p of tokens[r][i]; 0 where that is negative (no token),
+ *                     NaN where it is vocab or more
+ *   entropy[r] = - sum_j p_j log p_j
+ *   top_tokens[r], top_log_probs[r]: the `top` largest, in descending order, of
+ *                     equal logits the lower token first
+ * A logit of -inf has probability 0. A row of nothing else: every log probability
+ * -inf, the entropy 0. A row that holds a NaN or +inf: NaN, top_tokens -1.
+ * Sums are f32. top: 0 to 32, at most vocab (0: top_tokens and top_log_probs are
+ * not looked at). Rows are split over the chip where there are few of them: their
+ * parts are in the workspace, nnops_hip_token_log_probs_workspace_size bytes,
+ * 16-byte aligned, which need no initialization. */
+typedef struct NnopsTokenLogProbsArgs {
+    const void* logits;         /* [rows][ld_logits] f16 (f16) or f32, vocab columns */
+    int64_t rows, vocab, ld_logits; /* ld: elements */
+    int32_t f16, top;
+    const int32_t* tokens;      /* [rows][ld_tokens], per_row columns */
+    int64_t per_row, ld_tokens;
+    float* log_probs;           /* [rows][ld_log_probs] */
+    int64_t ld_log_probs;
+    float* entropy;             /* [rows] */
+    int32_t* top_tokens;        /* [rows][ld_top_tokens] */
+    float* top_log_probs;       /* [rows][ld_top_log_probs] */
+    int64_t ld_top_tokens, ld_top_log_probs;
+} NnopsTokenLogProbsArgs;
+
+size_t nnops_hip_token_log_probs_workspace_size(const NnopsTokenLogProbsArgs* args);
+int nnops_hip_token_log_probs(const NnopsTokenLogProbsArgs* args, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
 /* What the kernel selection of a call comes to (no counterpart in nnops; for
  * tests and for callers that tune shapes). Host code: the arguments' pointers
  * are looked at for their alignment only, and nothing is launched. */

@@ -91,8 +91,9 @@ typedef struct NnopsQuantLinearAttrs {
 } NnopsQuantLinearAttrs;
 
 /* The operators between the products of a decoder layer (no counterparts in
- * nnops; nnops/ops/rms_norm.hpp, rotary.hpp and kv_cache.hpp of the C++ headers
- * state inputs and outputs, nnops_amd.h the arithmetic). */
+ * nnops; nnops/ops/rms_norm.hpp, rotary.hpp, kv_cache.hpp, kv_pages.hpp and
+ * token_log_probs.hpp of the C++ headers state inputs and outputs, nnops_amd.h the
+ * arithmetic). */
 typedef struct NnopsRmsNormAttrs {
     float epsilon;
     int32_t output_dtype;   /* x's type, or NNOPS_S8 (then outputs y, scale) */
@@ -107,6 +108,18 @@ typedef struct NnopsCacheAttentionAttrs {
     float scale;            /* 0: 1 / sqrt(head_dim) */
     int64_t window, sinks;  /* window 0: none */
 } NnopsCacheAttentionAttrs;
+
+typedef struct NnopsPrefixAttentionAttrs {
+    float scale;            /* 0: 1 / sqrt(head_dim) */
+} NnopsPrefixAttentionAttrs;
+
+typedef struct NnopsKvCachePagesAttrs {
+    int64_t page_tokens;    /* 16, 32, 64 (default), 128 or 256 */
+} NnopsKvCachePagesAttrs;
+
+typedef struct NnopsTokenLogProbsAttrs {
+    int64_t top;            /* alternatives, 0 (default) to 32 */
+} NnopsTokenLogProbsAttrs;
 
 typedef struct NnopsOp NnopsOp;
 
@@ -128,7 +141,17 @@ NnopsOp* nnops_dequantize_linear_create(const NnopsQuantLinearAttrs* attrs, int3
  * KvCacheRead: inputs k_cache, v_cache, k_scale, v_scale, page_table, lengths
  * [, row_starts]; outputs k, v (output_dtype NNOPS_F32 / NNOPS_F16).
  * CacheAttention: inputs q, k_cache, v_cache, k_scale, v_scale, page_table,
- * lengths [, row_starts]; output q's shape and type. */
+ * lengths [, row_starts]; output q's shape and type.
+ * PrefixAttention: inputs q, k_cache, v_cache, k_scale, v_scale, page_table,
+ * lengths, group_starts, shared [, row_starts]; output q's shape and type.
+ * KvCacheFork: inputs page_table, lengths, refs, parents, new_tokens; outputs
+ * page_table, lengths, refs, copies, counts of the children.
+ * KvCacheCompact: inputs page_table, lengths, refs; outputs page_table, refs,
+ * copies, moved, counts.
+ * KvCacheCopy: input copies; outputs k_cache, v_cache, k_scale, v_scale (updated
+ * in place).
+ * TokenLogProbs: inputs logits, tokens; outputs log_probs, entropy [, top_tokens,
+ * top_log_probs]. */
 void nnops_rms_norm_attrs_init(NnopsRmsNormAttrs* attrs);
 NnopsOp* nnops_rms_norm_create(const NnopsRmsNormAttrs* attrs, int32_t backend);
 void nnops_rotary_attrs_init(NnopsRotaryAttrs* attrs);
@@ -137,6 +160,14 @@ NnopsOp* nnops_kv_cache_write_create(int32_t backend);
 NnopsOp* nnops_kv_cache_read_create(int32_t output_dtype, int32_t backend);
 void nnops_cache_attention_attrs_init(NnopsCacheAttentionAttrs* attrs);
 NnopsOp* nnops_cache_attention_create(const NnopsCacheAttentionAttrs* attrs, int32_t backend);
+void nnops_prefix_attention_attrs_init(NnopsPrefixAttentionAttrs* attrs);
+NnopsOp* nnops_prefix_attention_create(const NnopsPrefixAttentionAttrs* attrs, int32_t backend);
+void nnops_kv_cache_pages_attrs_init(NnopsKvCachePagesAttrs* attrs);
+NnopsOp* nnops_kv_cache_fork_create(const NnopsKvCachePagesAttrs* attrs, int32_t backend);
+NnopsOp* nnops_kv_cache_compact_create(const NnopsKvCachePagesAttrs* attrs, int32_t backend);
+NnopsOp* nnops_kv_cache_copy_create(int32_t backend);
+void nnops_token_log_probs_attrs_init(NnopsTokenLogProbsAttrs* attrs);
+NnopsOp* nnops_token_log_probs_create(const NnopsTokenLogProbsAttrs* attrs, int32_t backend);
 void nnops_op_destroy(NnopsOp* op);
 
 /* OpBase::prepackWeights (include/nnops/core/op_base.hpp:72-78) for MatMul /

@@ -118,6 +118,53 @@ class CacheAttentionArgs(C.Structure):
     ]
 
 
+class PrefixAttentionArgs(C.Structure):
+    _fields_ = [
+        ("cache", KvPages), ("q", C.c_void_p), ("out", C.c_void_p),
+        ("rows", C.c_int64), ("q_heads", C.c_int64), ("ld_q", C.c_int64), ("ld_out", C.c_int64),
+        ("f16", C.c_int32), ("scale", C.c_float),
+        ("groups", C.c_int64), ("group_starts", C.c_void_p), ("shared", C.c_void_p),
+    ]
+
+
+class KvForkArgs(C.Structure):
+    _fields_ = [
+        ("page_table", C.c_void_p), ("sequences", C.c_int64), ("table_pages", C.c_int64), ("ld_table", C.c_int64),
+        ("lengths", C.c_void_p), ("refs", C.c_void_p), ("pages", C.c_int64), ("page_tokens", C.c_int64),
+        ("parents", C.c_void_p), ("new_tokens", C.c_void_p), ("children", C.c_int64),
+        ("new_table", C.c_void_p), ("new_table_pages", C.c_int64), ("ld_new_table", C.c_int64),
+        ("new_lengths", C.c_void_p), ("new_refs", C.c_void_p), ("copies", C.c_void_p), ("counts", C.c_void_p),
+    ]
+
+
+class KvCompactArgs(C.Structure):
+    _fields_ = [
+        ("page_table", C.c_void_p), ("sequences", C.c_int64), ("table_pages", C.c_int64), ("ld_table", C.c_int64),
+        ("lengths", C.c_void_p), ("refs", C.c_void_p), ("pages", C.c_int64), ("page_tokens", C.c_int64),
+        ("new_table", C.c_void_p), ("ld_new_table", C.c_int64), ("new_refs", C.c_void_p), ("copies", C.c_void_p),
+        ("moved", C.c_void_p), ("counts", C.c_void_p),
+    ]
+
+
+class KvCopyArgs(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("pages", C.c_int64), ("heads", C.c_int64), ("page_tokens", C.c_int64), ("head_dim", C.c_int64),
+        ("copies", C.c_void_p), ("count", C.c_int64),
+    ]
+
+
+class TokenLogProbsArgs(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("rows", C.c_int64), ("vocab", C.c_int64), ("ld_logits", C.c_int64),
+        ("f16", C.c_int32), ("top", C.c_int32),
+        ("tokens", C.c_void_p), ("per_row", C.c_int64), ("ld_tokens", C.c_int64),
+        ("log_probs", C.c_void_p), ("ld_log_probs", C.c_int64), ("entropy", C.c_void_p),
+        ("top_tokens", C.c_void_p), ("top_log_probs", C.c_void_p),
+        ("ld_top_tokens", C.c_int64), ("ld_top_log_probs", C.c_int64),
+    ]
+
+
 class Tensor(C.Structure):
     _fields_ = [
         ("rank", C.c_int64), ("dims", C.c_int64 * 8), ("dtype", C.c_int32),
@@ -174,6 +221,18 @@ class RotaryAttrs(C.Structure):
 
 class CacheAttentionAttrs(C.Structure):
     _fields_ = [("scale", C.c_float), ("window", C.c_int64), ("sinks", C.c_int64)]
+
+
+class PrefixAttentionAttrs(C.Structure):
+    _fields_ = [("scale", C.c_float)]
+
+
+class KvCachePagesAttrs(C.Structure):
+    _fields_ = [("page_tokens", C.c_int64)]
+
+
+class TokenLogProbsAttrs(C.Structure):
+    _fields_ = [("top", C.c_int64)]
 
 
 class FpOutArgs(C.Structure):
@@ -237,6 +296,15 @@ SIGNATURES = {
     "nnops_hip_cache_attention_workspace_size": (C.c_size_t, [C.POINTER(CacheAttentionArgs)]),
     "nnops_hip_cache_attention_plan": (C.c_int, [C.POINTER(CacheAttentionArgs), C.POINTER(CacheAttentionPlan)]),
     "nnops_hip_cache_attention": (C.c_int, [C.POINTER(CacheAttentionArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "nnops_hip_prefix_attention_workspace_size": (C.c_size_t, [C.POINTER(PrefixAttentionArgs)]),
+    "nnops_hip_prefix_attention": (C.c_int, [C.POINTER(PrefixAttentionArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "nnops_hip_kv_cache_fork_workspace_size": (C.c_size_t, [C.POINTER(KvForkArgs)]),
+    "nnops_hip_kv_cache_fork": (C.c_int, [C.POINTER(KvForkArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "nnops_hip_kv_cache_compact_workspace_size": (C.c_size_t, [C.POINTER(KvCompactArgs)]),
+    "nnops_hip_kv_cache_compact": (C.c_int, [C.POINTER(KvCompactArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "nnops_hip_kv_cache_copy": (C.c_int, [C.POINTER(KvCopyArgs), C.c_void_p]),
+    "nnops_hip_token_log_probs_workspace_size": (C.c_size_t, [C.POINTER(TokenLogProbsArgs)]),
+    "nnops_hip_token_log_probs": (C.c_int, [C.POINTER(TokenLogProbsArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
     "nnops_matmul_attrs_init": (None, [C.POINTER(MatMulAttrs)]),
     "nnops_linear_attrs_init": (None, [C.POINTER(LinearAttrs)]),
     "nnops_matmul_create": (C.c_void_p, [C.POINTER(MatMulAttrs), C.c_int32]),
@@ -252,6 +320,14 @@ SIGNATURES = {
     "nnops_kv_cache_read_create": (C.c_void_p, [C.c_int32, C.c_int32]),
     "nnops_cache_attention_attrs_init": (None, [C.POINTER(CacheAttentionAttrs)]),
     "nnops_cache_attention_create": (C.c_void_p, [C.POINTER(CacheAttentionAttrs), C.c_int32]),
+    "nnops_prefix_attention_attrs_init": (None, [C.POINTER(PrefixAttentionAttrs)]),
+    "nnops_prefix_attention_create": (C.c_void_p, [C.POINTER(PrefixAttentionAttrs), C.c_int32]),
+    "nnops_kv_cache_pages_attrs_init": (None, [C.POINTER(KvCachePagesAttrs)]),
+    "nnops_kv_cache_fork_create": (C.c_void_p, [C.POINTER(KvCachePagesAttrs), C.c_int32]),
+    "nnops_kv_cache_compact_create": (C.c_void_p, [C.POINTER(KvCachePagesAttrs), C.c_int32]),
+    "nnops_kv_cache_copy_create": (C.c_void_p, [C.c_int32]),
+    "nnops_token_log_probs_attrs_init": (None, [C.POINTER(TokenLogProbsAttrs)]),
+    "nnops_token_log_probs_create": (C.c_void_p, [C.POINTER(TokenLogProbsAttrs), C.c_int32]),
     "nnops_op_destroy": (None, [C.c_void_p]),
     "nnops_op_prepack_weights": (C.c_int, [C.c_void_p, C.POINTER(Tensor), C.c_int32, C.POINTER(Tensor), C.c_int32,
                                            C.c_void_p]),

@@ -42,10 +42,15 @@ SOURCES = [
     "csrc/kernels/kv_cache.hip",
     "csrc/kernels/cache_attention.hip",
     "csrc/kernels/cache_attention_tiled.hip",
+    "csrc/kernels/prefix_attention.hip",
+    "csrc/kernels/kv_pages.hip",
+    "csrc/kernels/token_log_probs.hip",
     "csrc/host/ops.cpp",
     "csrc/host/quant_linear.cpp",
     "csrc/host/rms_norm.cpp",
     "csrc/host/kv_cache.cpp",
+    "csrc/host/kv_pages.cpp",
+    "csrc/host/token_log_probs.cpp",
     "csrc/host/capi_ops.cpp",
 ]
 

@@ -1,11 +1,13 @@
 // C facade over the operator classes (include/nnops_amd_ops.h): turns
 // NnopsTensor records into TensorDesc / TensorView and forwards each call.
 #include "nnops/ops/kv_cache.hpp"
+#include "nnops/ops/kv_pages.hpp"
 #include "nnops/ops/linear.hpp"
 #include "nnops/ops/matmul.hpp"
 #include "nnops/ops/quant_linear.hpp"
 #include "nnops/ops/rms_norm.hpp"
 #include "nnops/ops/rotary.hpp"
+#include "nnops/ops/token_log_probs.hpp"
 #include "nnops_amd_ops.h"
 
 #include <limits>
@@ -275,6 +277,78 @@ NnopsOp* nnops_cache_attention_create(const NnopsCacheAttentionAttrs* a, int32_t
     return h;
 }
 
+void nnops_prefix_attention_attrs_init(NnopsPrefixAttentionAttrs* a)
+{
+    if (a != nullptr) {
+        *a = NnopsPrefixAttentionAttrs{};
+    }
+}
+
+NnopsOp* nnops_prefix_attention_create(const NnopsPrefixAttentionAttrs* a, int32_t backend)
+{
+    PrefixAttentionAttributes attrs;
+    if (a != nullptr) {
+        attrs.scale = a->scale;
+    }
+    auto* h = new NnopsOp;
+    h->op = PrefixAttention::create(attrs, static_cast<Backend>(backend));
+    return h;
+}
+
+void nnops_kv_cache_pages_attrs_init(NnopsKvCachePagesAttrs* a)
+{
+    if (a != nullptr) {
+        a->page_tokens = KvCacheForkAttributes{}.page_tokens;
+    }
+}
+
+NnopsOp* nnops_kv_cache_fork_create(const NnopsKvCachePagesAttrs* a, int32_t backend)
+{
+    KvCacheForkAttributes attrs;
+    if (a != nullptr) {
+        attrs.page_tokens = a->page_tokens;
+    }
+    auto* h = new NnopsOp;
+    h->op = KvCacheFork::create(attrs, static_cast<Backend>(backend));
+    return h;
+}
+
+NnopsOp* nnops_kv_cache_compact_create(const NnopsKvCachePagesAttrs* a, int32_t backend)
+{
+    KvCacheCompactAttributes attrs;
+    if (a != nullptr) {
+        attrs.page_tokens = a->page_tokens;
+    }
+    auto* h = new NnopsOp;
+    h->op = KvCacheCompact::create(attrs, static_cast<Backend>(backend));
+    return h;
+}
+
+NnopsOp* nnops_kv_cache_copy_create(int32_t backend)
+{
+    auto* h = new NnopsOp;
+    h->op = KvCacheCopy::create(static_cast<Backend>(backend));
+    return h;
+}
+
+void nnops_token_log_probs_attrs_init(NnopsTokenLogProbsAttrs* a)
+{
+    if (a != nullptr) {
+        *a = NnopsTokenLogProbsAttrs{};
+    }
+}
+
+NnopsOp* nnops_token_log_probs_create(const NnopsTokenLogProbsAttrs* a, int32_t backend)
+{
+    TokenLogProbsAttributes attrs;
+    if (a != nullptr) {
+        attrs.top = a->top;
+    }
+    auto* h = new NnopsOp;
+    h->op = TokenLogProbs::create(attrs, static_cast<Backend>(backend));
+    return h;
+}
+
 void nnops_op_destroy(NnopsOp* op)
 {
     delete op;
@@ -372,10 +446,10 @@ size_t nnops_op_workspace_size(const NnopsOp* op, const NnopsTensor* inputs, int
 int nnops_op_compute(NnopsOp* op, const NnopsTensor* outputs, int32_t n_outputs,
                      const NnopsTensor* inputs, int32_t n_inputs, void* hip_stream, void* workspace)
 {
-    if (op == nullptr || n_inputs < 0 || n_outputs < 0 || n_inputs > 8 || n_outputs > 4) {
+    if (op == nullptr || n_inputs < 0 || n_outputs < 0 || n_inputs > 10 || n_outputs > 5) {
         return static_cast<int>(Status::invalid_argument);
     }
-    TensorView in[8], out[4];
+    TensorView in[10], out[5];
     for (int32_t i = 0; i < n_inputs; ++i) {
         in[i] = to_view(inputs[i]);
     }

@@ -1,40 +1,12 @@
-// KvCacheWrite, KvCacheRead and CacheAttention for Backend::HIP: descriptor
-// rules, lowered onto nnops_hip_kv_cache_write / _read and
-// nnops_hip_cache_attention.
+// KvCacheWrite, KvCacheRead, CacheAttention and PrefixAttention for Backend::HIP:
+// descriptor rules, lowered onto nnops_hip_kv_cache_write / _read,
+// nnops_hip_cache_attention and nnops_hip_prefix_attention.
 #include "nnops/ops/kv_cache.hpp"
 #include "nnops_amd.h"
 #include "views.hpp"
 
 namespace nnops {
 namespace {
-
-bool all_plain(std::span<const TensorDesc> d)
-{
-    for (const TensorDesc& t : d) {
-        if (!plain_dims(t)) {
-            return false;
-        }
-    }
-    return true;
-}
-
-/// The cache's four tensors.
-Status check_cache(std::span<const TensorDesc> c)
-{
-    const TensorDesc &k = c[0], &v = c[1], &ks = c[2], &vs = c[3];
-    if (k.rank != 4 || v.rank != 4 || ks.rank != 2 || vs.rank != 2) {
-        return Status::invalid_argument;
-    }
-    if (k.dtype != DataType::s8 || v.dtype != DataType::s8 || ks.dtype != DataType::f32 ||
-        vs.dtype != DataType::f32) {
-        return Status::invalid_argument;
-    }
-    if (v.dims[0] != k.dims[0] || v.dims[1] != k.dims[1] || v.dims[2] != k.dims[3] || v.dims[3] != k.dims[2] ||
-        ks.dims[0] != k.dims[0] || ks.dims[1] != k.dims[1] || !same_shape(ks, vs)) {
-        return Status::invalid_argument;
-    }
-    return dense(k) && dense(v) && dense(ks) && dense(vs) ? Status::ok : Status::unsupported;
-}
 
 /// page_table, lengths [, row_starts], for a call of `rows` rows.
 Status check_tables(std::span<const TensorDesc> t, int64_t rows)
@@ -202,6 +174,26 @@ Status KvCacheRead::compute(std::span<TensorView> outputs, std::span<const Tenso
 
 namespace {
 
+/// q, the cache and its tables, and the output of an attention.
+Status check_attention(std::span<const TensorDesc> inputs, std::span<const TensorDesc> tables, const TensorDesc& out)
+{
+    if (Status s = check_cache(inputs.subspan(1, 4)); !is_ok(s)) {
+        return s;
+    }
+    const TensorDesc& q = inputs[0];
+    if (q.rank != 2) {
+        return Status::invalid_argument;
+    }
+    if (Status s = check_tables(tables, q.dims[0]); !is_ok(s)) {
+        return s;
+    }
+    const int64_t width = inputs[1].dims[1] * inputs[1].dims[3];
+    if (width <= 0 || q.dims[1] <= 0 || q.dims[1] % width != 0 || !same_shape(q, out) || q.dtype != out.dtype) {
+        return Status::invalid_argument;
+    }
+    return is_float(q.dtype) ? Status::ok : Status::unsupported;
+}
+
 NnopsCacheAttentionArgs attention_args(const CacheAttentionAttributes& attrs, std::span<const TensorDesc> in,
                                        const TensorDesc& out)
 {
@@ -241,22 +233,7 @@ Status CacheAttention::validate(std::span<const TensorDesc> inputs, std::span<co
         !(attrs_.scale >= 0.0f) || attrs_.window < 0 || attrs_.sinks < 0) {
         return Status::invalid_argument;
     }
-    if (Status s = check_cache(inputs.subspan(1, 4)); !is_ok(s)) {
-        return s;
-    }
-    const TensorDesc& q = inputs[0];
-    if (q.rank != 2) {
-        return Status::invalid_argument;
-    }
-    if (Status s = check_tables(inputs.subspan(5), q.dims[0]); !is_ok(s)) {
-        return s;
-    }
-    const int64_t width = inputs[1].dims[1] * inputs[1].dims[3];
-    if (width <= 0 || q.dims[1] <= 0 || q.dims[1] % width != 0 || !same_shape(q, outputs[0]) ||
-        q.dtype != outputs[0].dtype) {
-        return Status::invalid_argument;
-    }
-    return is_float(q.dtype) ? Status::ok : Status::unsupported;
+    return check_attention(inputs, inputs.subspan(5), outputs[0]);
 }
 
 size_t CacheAttention::getWorkspaceSize(std::span<const TensorDesc> inputs, std::span<const TensorDesc> outputs) const
@@ -293,6 +270,107 @@ Status CacheAttention::compute(std::span<TensorView> outputs, std::span<const Te
     // the workspace is the one that getWorkspaceSize asks for
     const size_t bytes = nnops_hip_cache_attention_workspace_size(&a);
     return from_abi(nnops_hip_cache_attention(&a, workspace, workspace != nullptr ? bytes : 0, ctx.hip_stream));
+}
+
+namespace {
+
+/// page_table, lengths [, row_starts] of a PrefixAttention's inputs.
+template <typename V>
+struct Tables {
+    std::array<V, 3> at;
+    size_t n;
+    explicit Tables(std::span<const V> inputs) : n(inputs.size() > 9 ? 3 : 2)
+    {
+        at[0] = inputs[5];
+        at[1] = inputs[6];
+        if (n > 2) {
+            at[2] = inputs[9];
+        }
+    }
+    std::span<const V> span() const { return {at.data(), n}; }
+};
+
+NnopsPrefixAttentionArgs prefix_args(const PrefixAttentionAttributes& attrs, std::span<const TensorDesc> in,
+                                     const TensorDesc& out)
+{
+    NnopsPrefixAttentionArgs a{};
+    a.cache = pages_of(in.subspan(1, 4), in.subspan(5, 2));
+    a.rows = in[0].dims[0];
+    a.q_heads = a.cache.head_dim > 0 ? in[0].dims[1] / a.cache.head_dim : 0;
+    a.ld_q = row_step(in[0]);
+    a.ld_out = row_step(out);
+    a.f16 = in[0].dtype == DataType::f16;
+    a.scale = attrs.scale;
+    a.groups = in[8].dims[0];
+    return a;
+}
+
+}  // namespace
+
+std::unique_ptr<PrefixAttention> PrefixAttention::create(const PrefixAttentionAttributes& attrs, Backend backend)
+{
+    return std::unique_ptr<PrefixAttention>(new PrefixAttention(attrs, backend));
+}
+
+std::vector<TensorDesc> PrefixAttention::getOutputTensorDesc(std::span<const TensorDesc> inputs) const
+{
+    if (inputs.empty()) {
+        return {};
+    }
+    TensorDesc y = inputs[0];
+    y.row_stride_elems = 0;
+    return {y};
+}
+
+Status PrefixAttention::validate(std::span<const TensorDesc> inputs, std::span<const TensorDesc> outputs) const
+{
+    if (inputs.size() < 9 || inputs.size() > 10 || outputs.size() != 1 || !all_plain(inputs) || !all_plain(outputs) ||
+        !(attrs_.scale >= 0.0f)) {
+        return Status::invalid_argument;
+    }
+    const TensorDesc &starts = inputs[7], &shared = inputs[8];
+    if (starts.rank != 1 || shared.rank != 1 || starts.dtype != DataType::s32 || shared.dtype != DataType::s32 ||
+        starts.dims[0] != shared.dims[0] + 1) {
+        return Status::invalid_argument;
+    }
+    return check_attention(inputs, Tables<TensorDesc>(inputs).span(), outputs[0]);
+}
+
+size_t PrefixAttention::getWorkspaceSize(std::span<const TensorDesc> inputs, std::span<const TensorDesc> outputs) const
+{
+    if (!is_ok(validate(inputs, outputs))) {
+        return 0;
+    }
+    NnopsPrefixAttentionArgs a = prefix_args(attrs_, inputs, outputs[0]);
+    // (whether there are row starts plays a part, not where they are)
+    static const int32_t some = 0;
+    a.cache.row_starts = inputs.size() > 9 ? &some : nullptr;
+    return nnops_hip_prefix_attention_workspace_size(&a);
+}
+
+Status PrefixAttention::compute(std::span<TensorView> outputs, std::span<const TensorView> inputs,
+                                const ComputeContext& ctx, void* workspace)
+{
+    std::array<TensorDesc, 10> in;
+    std::array<TensorDesc, 1> out;
+    if (!descs_of(inputs, in) || !descs_of(std::span<const TensorView>(outputs), out)) {
+        return Status::invalid_argument;
+    }
+    if (backend_ != Backend::HIP) {
+        return Status::unsupported;
+    }
+    const std::span<const TensorDesc> id(in.data(), inputs.size());
+    if (Status s = validate(id, std::span<const TensorDesc>(out.data(), outputs.size())); !is_ok(s)) {
+        return s;
+    }
+    NnopsPrefixAttentionArgs a = prefix_args(attrs_, id, out[0]);
+    set_data(a.cache, inputs.subspan(1, 4), Tables<TensorView>(inputs).span());
+    a.q = inputs[0].ptr<const void>();
+    a.out = outputs[0].ptr<void>();
+    a.group_starts = inputs[7].ptr<const int32_t>();
+    a.shared = inputs[8].ptr<const int32_t>();
+    const size_t bytes = nnops_hip_prefix_attention_workspace_size(&a);
+    return from_abi(nnops_hip_prefix_attention(&a, workspace, workspace != nullptr ? bytes : 0, ctx.hip_stream));
 }
 
 }  // namespace nnops

@@ -80,4 +80,32 @@ bool descs_of(std::span<const TensorView> views, std::array<TensorDesc, N>& d)
     return true;
 }
 
+inline bool all_plain(std::span<const TensorDesc> d)
+{
+    for (const TensorDesc& t : d) {
+        if (!plain_dims(t)) {
+            return false;
+        }
+    }
+    return true;
+}
+
+/// The four tensors of a paged cache.
+inline Status check_cache(std::span<const TensorDesc> c)
+{
+    const TensorDesc &k = c[0], &v = c[1], &ks = c[2], &vs = c[3];
+    if (k.rank != 4 || v.rank != 4 || ks.rank != 2 || vs.rank != 2) {
+        return Status::invalid_argument;
+    }
+    if (k.dtype != DataType::s8 || v.dtype != DataType::s8 || ks.dtype != DataType::f32 ||
+        vs.dtype != DataType::f32) {
+        return Status::invalid_argument;
+    }
+    if (v.dims[0] != k.dims[0] || v.dims[1] != k.dims[1] || v.dims[2] != k.dims[3] || v.dims[3] != k.dims[2] ||
+        ks.dims[0] != k.dims[0] || ks.dims[1] != k.dims[1] || !same_shape(ks, vs)) {
+        return Status::invalid_argument;
+    }
+    return dense(k) && dense(v) && dense(ks) && dense(vs) ? Status::ok : Status::unsupported;
+}
+
 }  // namespace nnops

@@ -19,6 +19,22 @@ constexpr float kDrop = 0x1p-6f;    // 2^-kLift
 
 constexpr float kNone = -std::numeric_limits<float>::infinity();
 
+// What a launch looks at: sequences as they are; the tokens that groups of
+// sequences share, as one sequence each of all their rows, which see them all; or
+// what the sequences have behind those. (The last two leave all rows in parts.)
+enum AttnMode { kWhole, kShared, kOwn };
+
+// How a call with shared tokens is laid out (found on the device).
+struct PrefixPlan {
+    int32_t shared_chunk, own_chunk;   // tiles of a split
+};
+struct GroupPlan {
+    int32_t start, rows, tokens, table;   // rows of the call, tokens that all share, whose page table
+};
+struct MemberPlan {
+    int32_t group, skip;  // of a sequence: its group or -1, tiles that are the group's
+};
+
 struct AttnKern {
     Paged c;
     const void* q;
@@ -35,6 +51,11 @@ struct AttnKern {
     int32_t tiles;        // of 64 tokens that the page table, or the window, has room for
     int32_t whole;        // tiles of the longest sequence up to which none is split
     int32_t chunk;        // tiles of a split where that sequence fills the table
+    // kShared and kOwn
+    const PrefixPlan* plan;
+    const GroupPlan* group_plan;
+    const MemberPlan* members;
+    int32_t groups, first_part;
 };
 
 // The tiles of 64 tokens that rows at positions pmin .. pmax look at: the
@@ -74,6 +95,7 @@ struct RowTile {
     Span span;
     int chunk;                // tiles of tokens that a split takes
     bool split;               // it has more than one
+    int table;                // kShared: the sequence whose pages they are
 };
 
 // The largest of a wave's values, all 0 or more, as a scalar: along rows of 16
@@ -103,8 +125,12 @@ __device__ __forceinline__ int wave_max(int v)
 // than there are.)
 //   own: any sequence (in flight, beside the others). `longest`, of a lane: among
 // the sequences before the from-th, which were looked at already.
+template <AttnMode M>
 __device__ __forceinline__ int chunk_of(const AttnKern& p, const SeqRows& own, int longest = 0, int from = 0)
 {
+    if constexpr (M != kWhole) {
+        return M == kShared ? p.plan->shared_chunk : p.plan->own_chunk;
+    }
     if (p.splits == 1) {
         return std::numeric_limits<int>::max();
     }
@@ -129,6 +155,7 @@ __device__ __forceinline__ int chunk_of(const AttnKern& p, const SeqRows& own, i
     return tiles <= p.whole ? p.whole : max((int)((share + 3u) & ~3u), 4);
 }
 
+template <AttnMode M>
 __device__ __forceinline__ void place_tile(const AttnKern& p, int rt, int chunk, RowTile& t)
 {
     const uint32_t group = p.group;
@@ -138,39 +165,68 @@ __device__ __forceinline__ void place_tile(const AttnKern& p, int rt, int chunk,
     t.pmin = t.seq.len - t.seq.n + (int)((uint32_t)t.row0 / group);
     t.pmax = t.seq.len - t.seq.n + (int)(last / group);
     t.span = span_of(t.pmin, t.pmax, p.window, p.sinks);
+    if constexpr (M == kShared) {
+        const int tokens = t.seq.len;              // a multiple of the tile's
+        t.pmin = t.pmax = tokens - 1;
+        t.span = Span{0, 0, tokens / kTile};
+    } else if constexpr (M == kOwn) {
+        const int skip = p.members[t.b].skip;      // (no row's position lies before)
+        t.span = Span{0, skip, max(t.span.tiles - skip, 0)};
+    }
     t.chunk = chunk;
     t.split = t.span.tiles > chunk;
 }
 
+// A sequence of the launch.
+template <AttnMode M>
+__device__ __forceinline__ SeqRows seq_at(const AttnKern& p, int b)
+{
+    if constexpr (M == kShared) {
+        const GroupPlan g = p.group_plan[b];
+        return SeqRows{g.start, g.tokens > 0 ? g.rows : 0, g.tokens};
+    } else {
+        return seq_rows(p.c, b);
+    }
+}
+
 // The item-th tile. Later tiles of a sequence look at more tokens: `from_last`
 // numbers them from the last, so that the longest work begins first.
+template <AttnMode M>
 __device__ __forceinline__ bool find_tile(const AttnKern& p, uint32_t item, bool from_last, RowTile& t)
 {
     int rt, chunk;
+    const int seqs = M == kShared ? p.groups : p.c.seqs;
     if (p.per_seq > 0) {
         if (from_last) {
-            const uint32_t back = item / (uint32_t)p.c.seqs;
-            t.b = (int)(item - back * p.c.seqs);
+            const uint32_t back = item / (uint32_t)seqs;
+            t.b = (int)(item - back * seqs);
             rt = p.per_seq - 1 - (int)back;
         } else {
             t.b = (int)(item / (uint32_t)p.per_seq);
             rt = (int)(item - (uint32_t)t.b * p.per_seq);
         }
-        t.seq = seq_rows(p.c, t.b);
-        chunk = chunk_of(p, t.seq);
+        t.seq = seq_at<M>(p, t.b);
+        if (M == kShared && rt * p.tile_rows >= t.seq.n * p.group) {
+            return false;                          // (one group: it may have fewer rows than the call)
+        }
+        chunk = chunk_of<M>(p, t.seq);
     } else {
         int longest = 0;
         const auto count = [&](const SeqRows& s) {
             longest = s.n > 0 ? max(longest, s.len) : longest;
             return (int)((uint32_t)(s.n * p.group + p.tile_rows - 1) / (uint32_t)p.tile_rows);
         };
-        if (!find_item(p.c, item, count, t.b, rt, t.seq)) {
+        const auto at = [&](int b) { return seq_at<M>(p, b); };
+        if (!find_item(seqs, item, at, count, t.b, rt, t.seq)) {
             return false;
         }
-        chunk = chunk_of(p, t.seq, longest, (t.b / 64 + 1) * 64);
+        chunk = chunk_of<M>(p, t.seq, longest, (t.b / 64 + 1) * 64);
         rt = from_last ? count(t.seq) - 1 - rt : rt;
     }
-    place_tile(p, rt, chunk, t);
+    place_tile<M>(p, rt, chunk, t);
+    if constexpr (M == kShared) {
+        t.table = p.group_plan[t.b].table;
+    }
     return true;
 }
 
@@ -342,6 +398,21 @@ __device__ __forceinline__ Acc product(typename Operand<T>::Vec a, const typenam
     }
     return c;
 }
+
+// Lanes that join a row's parts, 4 channels each.
+__host__ __device__ __forceinline__ int join_lanes(int d) { return d <= 64 ? 16 : d <= 128 ? 32 : 64; }
+
+struct AttnPlan {
+    int64_t items;        // row tiles, all KV heads
+    int32_t tile_rows, per_seq, chunk, splits, tiles, whole;
+    bool tiled;           // attention_rows_tiled, else attention_rows16
+    bool join_few;        // attention_join_few joins the splits, else attention_join
+    size_t workspace;
+};
+
+// The choice for a call whose sizes check_attention_shapes lets pass (-1).
+int check_attention_shapes(const NnopsCacheAttentionArgs* g);
+AttnPlan attn_plan(const NnopsCacheAttentionArgs* g);
 
 // attention_rows_tiled's launch (cache_attention_tiled.hip): d, type and rows
 // of a workgroup that it has a kernel for.

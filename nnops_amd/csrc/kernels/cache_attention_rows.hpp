@@ -1,0 +1,327 @@
+// Causal attention over the paged 8-bit cache, with an optional sliding window
+// and first tokens that stay visible.
+//
+// Rows: the query heads that share a KV head attend to the same codes, so a
+// tile's rows are (token, head of the group), row = token * group + head. A
+// wave has 16 rows and walks tiles of 64 tokens:
+//   S^T[64 x 16] = K Q^T      v_mfma_f32_16x16x32_f16, K's codes as f16 (exact)
+//   online softmax over S^T   a lane holds 16 tokens of one row
+//   O^T[d x 16] += V^T P^T    P straight from the registers of S^T
+// Nothing crosses LDS until the end: which token a matrix row stands for is
+// free, so row m of score tile t is token 16 (m / 4) + 4 t + m % 4, and a lane
+// of group g = lane / 16 then holds tokens 16 g .. 16 g + 15: the very 16 bytes
+// that it loads of a channel's tokens (values lie with a channel's tokens side
+// by side). Likewise a lane's 16-byte piece of a key is 8 channels of each of
+// two k steps. Pages hold whole groups of 16 tokens, so a lane has one page and
+// one scale on each side per tile.
+//
+// Scales: with ks, vs the scales of a token's page,
+//   x = scale log2(e) (q . code) ks + log2(vs),  M = running max of x,
+//   P = 2^(x - M + 6),  O += P code,  l += P 2^-6 / vs,  out = 2^-6 O / l:
+// the value scale rides in the exponent (one fma), and P's largest weight is
+// the same whatever the scales are.
+//
+// Bound: HBM for few rows, the codes read once per KV head. Long sequences are
+// split over workgroups (partial O, M, l in the workspace, joined by a second
+// kernel); a workgroup's 4 waves take every fourth tile and join in LDS. A wave
+// has a tile's 16 KB (d 128) of codes in flight and 168 registers, three waves a
+// SIMD. No branch stands around a tile's loads (channels past d are loaded as
+// channel 0's, the last tile is peeled off): the waits after one are for
+// everything (74 us for the batch below, and 42 against 35 at d 64).
+// One token of each of 64 sequences of up to 4096, 32 query and 8 KV heads, d 128:
+// 68.2 us, 4.55 TB/s; of one sequence of 126976: 55.9 us, 4.65 TB/s; of one of
+// 777: 9.2 us, two launches and the host's 5.
+#pragma once
+
+#include <type_traits>
+
+#include "cache_attention.hpp"
+
+namespace nnops_amd {
+namespace {
+
+constexpr int kRows = 16;           // rows of a wave
+
+template <typename T, int DP, AttnMode M>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void attention_rows16(const AttnKern p)
+{
+    constexpr int kC = DP / 64;                    // 64-channel pieces of a key
+    constexpr int kT = DP / 16;                    // 16-channel tiles of O
+    typedef Operand<T> Op;
+    constexpr int kWeights = Op::kParts == 1 ? 2 : Op::kParts;   // parts of a probability
+    constexpr int kPitch = DP + 4;
+    __shared__ float s_o[4][kRows][kPitch];
+    __shared__ float s_m[4][kRows], s_l[4][kRows];
+    const Paged& c = p.c;
+    const uint32_t item = blockIdx.x / (uint32_t)c.heads;
+    const int kvh = (int)(blockIdx.x - item * c.heads);
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int n = lane % 16, g = lane / 16;
+    const int kb = n / 4;                          // the token group of a lane's keys
+    // Without a window a wave's first tile is known before the lengths are, if
+    // sequences are not split or the longest fills the page table: its page numbers
+    // are asked for beside them. (Past the sequence's end they may be anything; what
+    // is read through them is masked.)
+    const bool early = M == kWhole && p.window == 0 && p.per_seq > 0 && c.table_pages > 0;
+    int kid = 0, vid = 0;
+    if (early) {
+        const int32_t* row = c.table + (int64_t)(item / (uint32_t)p.per_seq) * c.ld_table;
+        const int base = kTile * ((int)blockIdx.y * p.chunk + wave), last = c.table_pages - 1;
+        kid = row[min((base + 16 * kb) >> c.page_log2, last)];
+        vid = row[min((base + 16 * g) >> c.page_log2, last)];
+    }
+    RowTile rt;
+    if (!find_tile<M>(p, item, false, rt)) {
+        return;
+    }
+    const SeqRows& seq = rt.seq;
+    const Span& span = rt.span;
+    const int b = rt.b, pmin = rt.pmin, pmax = rt.pmax;
+    const int row0 = rt.row0, rows = rt.rows;
+    const int tok_last = M == kShared ? (int)((uint32_t)(min(row0 + kRows, rows) - 1) / (uint32_t)p.group)
+                                      : pmax - (seq.len - seq.n);
+    const int split = blockIdx.y;
+    const int v0 = split * rt.chunk;
+    if (split > 0 && v0 >= span.tiles) {
+        return;
+    }
+    const int v1 = min(span.tiles, v0 + rt.chunk);
+
+    const int row = row0 + n;
+    const bool is_row = row < rows;
+    const int tok = is_row ? (int)((uint32_t)row / (uint32_t)p.group) : tok_last;
+    const int head = kvh * p.group + (is_row ? row - tok * p.group : 0);
+    const int pos = M == kShared ? pmax : seq.len - seq.n + tok;
+    const int d = c.d;
+
+    // Q's fragments: channels 64 i + 16 g + 8 h .. + 7 of a row are k step 2 i + h
+    typename Op::Vec qf[DP / 32][Op::kParts];
+    const T* qrow = static_cast<const T*>(p.q) + (int64_t)(seq.start + tok) * p.ld_q + (int64_t)head * d;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) {
+        const int at = 64 * (i / 2) + 16 * g + 8 * (i % 2);
+        T x[8] = {};
+        if (is_row && at < d) {
+            __builtin_memcpy(x, qrow + at, sizeof x);
+        }
+        Op::split(x, qf[i]);
+    }
+
+    v4f o[kT];
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+        o[t] = v4f{0, 0, 0, 0};
+    }
+    float m_run = kNone, l_run = 0.0f;
+    const int64_t page_bytes = (int64_t)c.page * d;
+    const int ktok = 16 * kb + n % 4;              // + 4 t: its token in the tile
+
+    // The codes of a wave's next tile are in flight while it works on this one:
+    // its keys from the scores on, its values from the second product on, its
+    // page numbers a tile earlier still. (Loads come back in order: page numbers
+    // asked for beside the keys they lead to would wait for this tile's values.)
+    const int32_t* table = c.table + (int64_t)(M == kShared ? rt.table : b) * c.ld_table;
+    const int64_t page_step = page_bytes * c.heads;
+    const int8_t* k_at = c.k + kvh * page_bytes + 16 * g;
+    const int8_t* v_at = c.v + kvh * page_bytes + n * c.page;
+    v4i kr[4][kC], vr[kT];
+    PageScales scale_next{0.0f, 0.0f, 0.0f};
+    // (a group past the last position has the last page's codes: they are masked)
+    // (page numbers as they lie in the table: looked at when they are used)
+    const auto ids = [&](int v) {
+        const int base = tile_base(span, v);
+        kid = table[min(base + 16 * kb, pmax) >> c.page_log2];
+        vid = table[min(base + 16 * g, pmax) >> c.page_log2];
+    };
+    int koff[kC];                                  // channels past d: channel 0's codes (q is 0 there)
+#pragma unroll
+    for (int i = 0; i < kC; ++i) {
+        koff[i] = 64 * i + 16 * g < d ? 64 * i : -16 * g;
+    }
+    const auto load_k = [&](int v, int page_k, int page_v) {
+        const int base = tile_base(span, v);
+        const int8_t* at = k_at + readable(c, page_k) * page_step + ((base + ktok) & (c.page - 1)) * d;
+        int kstep = 4 * d;
+        if constexpr (DP <= 128) {
+            // (its multiples are computed here, not kept over the loop: 168 registers
+            // instead of 256 and spills)
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("" : "+s"(kstep));
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int i = 0; i < kC; ++i) {
+                kr[t][i] = *reinterpret_cast<const v4i*>(at + koff[i] + (int64_t)(t * kstep));
+            }
+        }
+        scale_next = page_scales(c, page_v, kvh);
+    };
+    const auto load_v = [&](int v, int page_v) {
+        const int base = tile_base(span, v);
+        const int8_t* at = v_at + readable(c, page_v) * page_step + ((base + 16 * g) & (c.page - 1));
+        int vstep = 16 * c.page;
+        if constexpr (DP <= 128) {
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("" : "+s"(vstep));
+        }
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+            vr[t] = *reinterpret_cast<const v4i*>(at + (int64_t)((16 * t < d ? t : 0) * vstep));
+        }
+    };
+    // (no branch around the loads of a tile: it would wait for all of them)
+    const auto tile = [&](auto go_on, int v) {
+        constexpr bool more = decltype(go_on)::value;
+        const int next_v = vid;                    // the next tile's page
+        const int base = tile_base(span, v), vt0 = base + 16 * g;
+        const PageScales scale = scale_next;
+
+        v4f s[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            s[t] = v4f{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < kC; ++i) {
+                s[t] = product<T>(Op::codes((uint32_t)kr[t][i].x, (uint32_t)kr[t][i].y), qf[2 * i], s[t]);
+                s[t] = product<T>(Op::codes((uint32_t)kr[t][i].z, (uint32_t)kr[t][i].w), qf[2 * i + 1], s[t]);
+            }
+        }
+
+        const Scales sc = softmax_scales(p, scale);
+        if constexpr (more) {
+            const int next_k = kid;
+            ids(min(v + 8, v1 - 1));
+            load_k(v + 4, next_k, next_v);
+        }
+
+        float x[4][4];
+        float top = kNone;
+        const bool open =
+            M == kShared || (base + kTile - 1 <= pmin && (p.window == 0 || pmax - base < p.window));
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float y = __builtin_fmaf(s[t][i], sc.mul, sc.add);
+                if (!open) {
+                    const int at = vt0 + 4 * t + i;
+                    const bool seen = at <= pos && (p.window == 0 || pos - at < p.window || at < p.sinks);
+                    y = seen ? y : kNone;
+                }
+                x[t][i] = y;
+                top = fmaxf(top, y);
+            }
+        }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        if (__any(top > m_run + kLazy)) {
+            // (0 where nothing was seen before)
+            const float f = top > m_run ? __builtin_amdgcn_exp2f(m_run - top) : 1.0f;
+            l_run *= f;
+#pragma unroll
+            for (int t = 0; t < kT; ++t) {
+                o[t] *= f;
+            }
+            m_run = fmaxf(m_run, top);
+        }
+        const float shift = m_run > kNone ? kLift - m_run : 0.0f;
+        float sum = 0.0f, w[2][8];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[t / 2][4 * (t % 2) + i] = __builtin_amdgcn_exp2f(x[t][i] + shift);
+                sum += w[t / 2][4 * (t % 2) + i];
+            }
+        }
+        // a page of which the row sees nothing adds nothing, whatever its scale
+        l_run += sum != 0.0f ? sum * sc.inv : 0.0f;
+        typename Op::Vec pf[2][kWeights];
+        Op::split(w[0], pf[0]);
+        Op::split(w[1], pf[1]);
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+            o[t] = product<T>(Op::codes((uint32_t)vr[t].x, (uint32_t)vr[t].y), pf[0], o[t]);
+            o[t] = product<T>(Op::codes((uint32_t)vr[t].z, (uint32_t)vr[t].w), pf[1], o[t]);
+        }
+        if constexpr (more) {
+            load_v(v + 4, next_v);
+        }
+    };
+    if (v0 + wave < v1) {
+        int v = v0 + wave;
+        if (!early || v0 != split * p.chunk) {
+            ids(v);
+        }
+        const int first_k = kid, first_v = vid;
+        ids(min(v + 4, v1 - 1));
+        load_k(v, first_k, first_v);
+        load_v(v, first_v);
+        for (; v + 4 < v1; v += 4) {
+            tile(std::true_type{}, v);
+        }
+        tile(std::false_type{}, v);
+    }
+
+    // the waves' parts, brought to one maximum and summed
+    l_run += __shfl_xor(l_run, 16);
+    l_run += __shfl_xor(l_run, 32);
+    if (g == 0) {
+        s_m[wave][n] = m_run;
+        s_l[wave][n] = l_run;
+    }
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+        *reinterpret_cast<v4f*>(&s_o[wave][n][16 * t + 4 * g]) = o[t];
+    }
+    __syncthreads();
+    // 16 threads a row, 4 channels each at a time
+    const int r = threadIdx.x / 16, ch0 = threadIdx.x % 16 * 4;
+    if (row0 + r >= rows) {
+        return;
+    }
+    const float m = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+    float f[4], l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        // a wave that saw nothing has m = -inf and nothing to add
+        f[w] = s_m[w][r] < m ? __builtin_amdgcn_exp2f(s_m[w][r] - m) : 1.0f;
+        l += f[w] * s_l[w][r];
+    }
+    const int rtok = (int)((uint32_t)(row0 + r) / (uint32_t)p.group);
+    const int64_t token = seq.start + rtok;
+    const int qh = kvh * p.group + (row0 + r - rtok * p.group);
+    const bool parts = M != kWhole || rt.split;
+    const int64_t at_part = ((int64_t)(split + (M == kWhole ? 0 : p.first_part)) * c.rows + token) * p.q_heads + qh;
+    const float scale = parts ? 1.0f : l == 0.0f ? 0.0f : kDrop / l;
+#pragma unroll
+    for (int i = 0; i < DP / 64; ++i) {
+        const int ch = ch0 + 64 * i;
+        if (ch >= d) {
+            break;
+        }
+        v4f sum = v4f{0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            sum += f[w] * *reinterpret_cast<const v4f*>(&s_o[w][r][ch]);
+        }
+        if (parts) {
+            *reinterpret_cast<v4f*>(&p.part[at_part * d + ch]) = sum;
+        } else {
+            T y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                y[e] = (T)(sum[e] * scale);
+            }
+            __builtin_memcpy(static_cast<T*>(p.out) + token * p.ld_out + (int64_t)qh * d + ch, y, sizeof y);
+        }
+    }
+    if (parts && ch0 == 0) {
+        p.part_ml[2 * at_part] = m;
+        p.part_ml[2 * at_part + 1] = l;
+    }
+}
+
+}  // namespace
+}  // namespace nnops_amd

@@ -53,16 +53,16 @@ __device__ __forceinline__ int page_of(const Paged& p, int b, int page)
 // after another (fewer than 2^31 in all): its sequence and its number there;
 // false past the last. Whole waves call it (each wave searches for itself, 64
 // sequences a step); w is the same in all lanes.
-template <typename Count>
-__device__ __forceinline__ bool find_item(const Paged& p, uint32_t w, Count count, int& b, int& j, SeqRows& seq)
+template <typename At, typename Count>
+__device__ __forceinline__ bool find_item(int seqs, uint32_t w, At at, Count count, int& b, int& j, SeqRows& seq)
 {
     const int lane = threadIdx.x % 64;
     uint32_t before = 0;
-    for (int base = 0; base < p.seqs; base += 64) {
+    for (int base = 0; base < seqs; base += 64) {
         SeqRows s{0, 0, 0};
         uint32_t c = 0;
-        if (base + lane < p.seqs) {
-            s = seq_rows(p, base + lane);
+        if (base + lane < seqs) {
+            s = at(base + lane);
             c = (uint32_t)count(s);
         }
         uint32_t upto = c;
@@ -84,6 +84,12 @@ __device__ __forceinline__ bool find_item(const Paged& p, uint32_t w, Count coun
         before += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
     }
     return false;
+}
+
+template <typename Count>
+__device__ __forceinline__ bool find_item(const Paged& p, uint32_t w, Count count, int& b, int& j, SeqRows& seq)
+{
+    return find_item(p.seqs, w, [&](int i) { return seq_rows(p, i); }, count, b, j, seq);
 }
 
 // What every entry point checks of a cache: its sizes, then what it points to.

@@ -1,0 +1,451 @@
+// Attention for groups of sequences that share their first tokens: the kernels of
+// cache_attention over those tokens, with all rows of a group as one sequence's
+// (without a mask: every row sees them all), then over what each sequence has
+// behind them, and the parts of every row joined:
+//   out = sum_i 2^(M_i - M) O_i / sum_i 2^(M_i - M) l_i,  M = max M_i
+//
+// Bound: the codes are read once per group and tile of rows. A batch's single
+// tokens that would read a prompt once per sequence become a tile of up to 256
+// rows that the matrix cores bound.
+//
+// Which tokens are shared is found on the device first, by one workgroup: whole
+// tiles and whole pages that every row of the group sees. Rows then need no mask,
+// and a sequence's own tokens begin at a tile.
+#include "cache_attention_rows.hpp"
+#include "cache_attention_tiled.hpp"
+
+namespace nnops_amd {
+namespace {
+
+constexpr int kPlanThreads = 1024;
+
+struct PrefixKern {
+    AttnKern own;         // (its plan, group_plan and members are written)
+    const int32_t* group_starts;
+    const int32_t* shared;
+    int32_t* starts;      // workspace: group_starts, in order and in range
+    int32_t shared_splits;
+    uint32_t by_shared_splits;
+    int32_t ways;         // of the join: parts of a row that are summed side by side
+};
+
+// The largest of a workgroup's values, all 0 or more.
+__device__ __forceinline__ int group_max(int v, int* s_waves)
+{
+    v = wave_max(v);
+    __syncthreads();
+    if (threadIdx.x % 64 == 0) {
+        s_waves[threadIdx.x / 64] = v;
+    }
+    __syncthreads();
+    for (int w = 0; w < kPlanThreads / 64; ++w) {
+        v = max(v, s_waves[w]);
+    }
+    return v;
+}
+
+__device__ __forceinline__ int chunk_for(int tiles, int splits, uint32_t by_splits, int whole)
+{
+    if (splits == 1) {
+        return std::numeric_limits<int>::max();
+    }
+    const uint32_t share = __umulhi((uint32_t)(tiles + splits - 1), by_splits);
+    return tiles <= whole ? whole : max((int)((share + 3u) & ~3u), 4);
+}
+
+__global__ __launch_bounds__(kPlanThreads) void prefix_plan(const PrefixKern p)
+{
+    __shared__ int s_waves[kPlanThreads / 64];
+    const AttnKern& k = p.own;
+    const Paged& c = k.c;
+    GroupPlan* const groups = const_cast<GroupPlan*>(k.group_plan);
+    MemberPlan* const members = const_cast<MemberPlan*>(k.members);
+    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+    // starts that do not go back
+    int so_far = 0;
+    for (int base = 0; base <= k.groups; base += kPlanThreads) {
+        const int g = base + tid;
+        int v = g <= k.groups && k.groups > 0 ? min(max(p.group_starts[g], 0), c.seqs) : 0;
+#pragma unroll
+        for (int m = 1; m < 64; m *= 2) {
+            v = max(v, lane >= m ? __shfl_up(v, m) : 0);
+        }
+        __syncthreads();
+        if (lane == 63) {
+            s_waves[wave] = v;
+        }
+        __syncthreads();
+        int before = so_far;
+        for (int w = 0; w < kPlanThreads / 64; ++w) {
+            before = max(before, w < wave ? s_waves[w] : 0);
+            so_far = max(so_far, s_waves[w]);
+        }
+        if (g <= k.groups) {
+            p.starts[g] = max(v, before);
+        }
+    }
+    for (int b = tid; b < c.seqs; b += kPlanThreads) {
+        members[b] = MemberPlan{-1, 0};
+    }
+    __syncthreads();
+    int longest = 0;
+    const int whole_pages = max(c.page, kTile) - 1;
+    for (int g = wave; g < k.groups; g += kPlanThreads / 64) {
+        const int b0 = p.starts[g], b1 = p.starts[g + 1];
+        GroupPlan plan{0, 0, 0, b0};
+        int least = std::numeric_limits<int>::max(), first = c.rows, last = 0, len = 0;
+        for (int b = b0 + lane; b < b1; b += 64) {
+            const SeqRows s = seq_rows(c, b);
+            if (s.n > 0) {
+                least = min(least, s.len - s.n + 1);
+                first = min(first, s.start);
+                last = max(last, s.start + s.n);
+            }
+            len = b == b0 ? s.len : len;
+        }
+#pragma unroll
+        for (int m = 1; m < 64; m *= 2) {
+            least = min(least, __shfl_xor(least, m));
+            first = min(first, __shfl_xor(first, m));
+            last = max(last, __shfl_xor(last, m));
+            len = max(len, __shfl_xor(len, m));
+        }
+        if (first < last) {
+            plan.start = first;
+            plan.rows = last - first;
+            plan.tokens = max(min(min(p.shared[g], len), least), 0) & ~whole_pages;
+        }
+        longest = max(longest, plan.tokens);
+        if (lane == 0) {
+            groups[g] = plan;
+        }
+        for (int b = b0 + lane; b < b1; b += 64) {
+            members[b] = MemberPlan{g, plan.tokens / kTile};
+        }
+    }
+    __syncthreads();
+    int own = 0;
+    for (int b = tid; b < c.seqs; b += kPlanThreads) {
+        const SeqRows s = seq_rows(c, b);
+        own = s.n > 0 ? max(own, s.len - kTile * members[b].skip) : own;
+    }
+    longest = group_max(longest, s_waves);
+    own = group_max(own, s_waves);
+    if (tid == 0) {
+        PrefixPlan* const plan = const_cast<PrefixPlan*>(k.plan);
+        plan->shared_chunk = chunk_for(longest / kTile, p.shared_splits, p.by_shared_splits, 4);
+        plan->own_chunk = chunk_for(min((own + kTile - 1) / kTile, k.tiles), k.splits, k.by_splits, k.whole);
+    }
+}
+
+// Joins the parts of every row: lanes of 4 channels, `ways` of them a row, each
+// with every ways-th part.
+template <typename T>
+__global__ __launch_bounds__(256) void prefix_join(const PrefixKern p)
+{
+    __shared__ __attribute__((aligned(16))) v4f s_o[256];
+    __shared__ float s_m[16], s_l[16];
+    const AttnKern& k = p.own;
+    const Paged& c = k.c;
+    const int lanes = join_lanes(c.d), slot = threadIdx.x / (uint32_t)lanes, ways = p.ways;
+    const int way = slot % ways, per_block = 256 / lanes / ways;
+    const int64_t i = (int64_t)blockIdx.x * per_block + slot / ways;
+    const int token = (int)min(i / k.q_heads, (int64_t)c.rows - 1), qh = (int)(i % k.q_heads);
+    bool live = i < (int64_t)c.rows * k.q_heads;
+    RowTile rt;
+    if (c.row_starts == nullptr) {
+        rt.b = (int)((uint32_t)token / (uint32_t)c.uniform);
+    } else {
+        int lo = 0, hi = c.seqs;                   // the last sequence that starts at or before the row
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            (c.row_starts[mid] <= token ? lo : hi) = mid;
+        }
+        rt.b = lo;
+    }
+    rt.seq = seq_rows(c, rt.b);
+    const int tok = token - rt.seq.start;
+    live = live && tok >= 0 && tok < rt.seq.n;
+    int shared = 0, own = 0;
+    if (live) {
+        const uint32_t row = (uint32_t)(tok * k.group) + (uint32_t)qh % (uint32_t)k.group;
+        const int own_chunk = k.plan->own_chunk, shared_chunk = k.plan->shared_chunk;
+        place_tile<kOwn>(k, (int)(row / (uint32_t)k.tile_rows), own_chunk, rt);
+        shared = (int)(((uint32_t)k.members[rt.b].skip + (uint32_t)shared_chunk - 1) / (uint32_t)shared_chunk);
+        own = (int)(((uint32_t)rt.span.tiles + (uint32_t)own_chunk - 1) / (uint32_t)own_chunk);
+    }
+    const int parts = shared + own, d = c.d, ch = threadIdx.x % (uint32_t)lanes * 4;
+    const int64_t rows = (int64_t)c.rows * k.q_heads, at = (int64_t)token * k.q_heads + qh;
+    float m = kNone, l = 0.0f;
+    v4f o = v4f{0, 0, 0, 0};
+    constexpr int kBatch = 4;
+    for (int s = way; s < parts; s += kBatch * ways) {
+        float ms[kBatch], ls[kBatch];
+        v4f os[kBatch];
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+            const int n = s + e * ways, part = n < shared ? n : k.first_part + n - shared;
+            ms[e] = kNone;
+            ls[e] = 0.0f;
+            os[e] = v4f{0, 0, 0, 0};
+            if (n < parts) {
+                ms[e] = k.part_ml[2 * (part * rows + at)];
+                ls[e] = k.part_ml[2 * (part * rows + at) + 1];
+                if (ch < d) {
+                    os[e] = *reinterpret_cast<const v4f*>(k.part + (part * rows + at) * d + ch);
+                }
+            }
+        }
+        float top = m;
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+            top = fmaxf(top, ms[e]);
+        }
+        const float f = m < top ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
+        l *= f;
+        o *= f;
+        m = top;
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+            // (a part that saw nothing has -inf and nothing to add)
+            const float w = ms[e] < m ? __builtin_amdgcn_exp2f(ms[e] - m) : 1.0f;
+            l += w * ls[e];
+            o += w * os[e];
+        }
+    }
+    if (ways > 1) {
+        s_o[threadIdx.x] = o;
+        if (threadIdx.x % (uint32_t)lanes == 0) {
+            s_m[slot] = m;
+            s_l[slot] = l;
+        }
+        __syncthreads();
+        if (way != 0) {
+            return;
+        }
+        float top = kNone;
+        for (int w = 0; w < ways; ++w) {
+            top = fmaxf(top, s_m[slot + w]);
+        }
+        l = 0.0f;
+        o = v4f{0, 0, 0, 0};
+        for (int w = 0; w < ways; ++w) {
+            const float f = s_m[slot + w] < top ? __builtin_amdgcn_exp2f(s_m[slot + w] - top) : 1.0f;
+            l += f * s_l[slot + w];
+            o += f * s_o[threadIdx.x + w * lanes];
+        }
+    }
+    if (!live || ch >= d) {
+        return;
+    }
+    const float f = l == 0.0f ? 0.0f : kDrop / l;
+    T y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        y[e] = (T)(o[e] * f);
+    }
+    __builtin_memcpy(static_cast<T*>(k.out) + token * k.ld_out + (int64_t)qh * d + ch, y, sizeof y);
+}
+
+struct SharedPlan {
+    AttnPlan own;
+    int64_t items;        // tiles of the groups' rows, all KV heads
+    int32_t tile_rows, per_seq, splits, ways;
+    size_t groups_at, members_at, starts_at, parts_at, workspace;
+};
+
+NnopsCacheAttentionArgs whole_args(const NnopsPrefixAttentionArgs& g)
+{
+    NnopsCacheAttentionArgs a{};
+    a.cache = g.cache;
+    a.q = g.q;
+    a.out = g.out;
+    a.rows = g.rows;
+    a.q_heads = g.q_heads;
+    a.ld_q = g.ld_q;
+    a.ld_out = g.ld_out;
+    a.f16 = g.f16;
+    a.scale = g.scale;
+    return a;
+}
+
+int check_prefix(const NnopsPrefixAttentionArgs* g)
+{
+    if (g == nullptr || g->groups < 0) {
+        return NNOPS_INVALID_ARGUMENT;
+    }
+    const NnopsCacheAttentionArgs a = whole_args(*g);
+    if (const int rc = check_attention_shapes(&a); rc >= 0) {
+        return rc;
+    }
+    return g->groups > (1 << 24) || g->cache.sequences > (1 << 24) ? NNOPS_UNSUPPORTED : -1;
+}
+
+size_t up16(size_t n) { return (n + 15) / 16 * 16; }
+
+SharedPlan shared_plan(const NnopsPrefixAttentionArgs* g)
+{
+    SharedPlan a{};
+    const NnopsCacheAttentionArgs whole = whole_args(*g);
+    a.own = attn_plan(&whole);
+    const int64_t heads = g->cache.heads, group = g->q_heads / heads, d = g->cache.head_dim;
+    const int64_t groups = g->groups > 0 ? g->groups : 1;
+    const int64_t mean = (g->rows * group + groups - 1) / groups;
+    const int rows = mean > 32 ? tiled_rows(d, g->f16, g->cache.page_tokens, mean) : 0;
+    a.tile_rows = rows > 0 ? rows : kRows;
+    if (g->groups <= 1) {
+        a.per_seq = (int32_t)((g->rows * group + a.tile_rows - 1) / a.tile_rows);
+        a.items = a.per_seq * heads;
+    } else {
+        a.items = (g->rows * group / a.tile_rows + (groups < g->rows ? groups : g->rows)) * heads;
+    }
+    const int64_t tiles = g->cache.table_pages * g->cache.page_tokens / kTile;
+    int64_t splits = ((rows > 0 ? 256 : 512) + a.items - 1) / a.items;
+    const int64_t most = (tiles + 3) / 4;
+    splits = splits < most ? splits : most;
+    a.splits = (int32_t)(splits > 1 ? splits : 1);
+    const int64_t parts = a.splits + a.own.splits;
+    // workgroups to fill the chip, as long as each lane has a batch of parts
+    const int lanes = join_lanes((int)d);
+    a.ways = 1;
+    while (a.ways < 256 / lanes && 4 * a.ways < parts && g->rows * g->q_heads * a.ways * lanes < 512 * 256) {
+        a.ways *= 2;
+    }
+    a.groups_at = 16;
+    a.members_at = a.groups_at + up16(sizeof(GroupPlan) * (size_t)groups);
+    a.starts_at = a.members_at + up16(sizeof(MemberPlan) * (size_t)g->cache.sequences);
+    a.parts_at = a.starts_at + up16(4 * (size_t)(groups + 1));
+    a.workspace = a.parts_at + (size_t)parts * g->rows * g->q_heads * (d + 2) * 4;
+    return a;
+}
+
+template <typename T, int DP, int NW, AttnMode M>
+void launch_tiled_one(const AttnKern& k, const dim3& grid, hipStream_t s)
+{
+    if (DP > 128 || tiled_one_page(k.c.d, k.c.page)) {
+        NNOPS_LAUNCH((attention_rows_tiled<T, DP, NW, true, M>), grid, dim3(64 * NW), 0, s, k);
+    } else if constexpr (DP <= 128) {
+        NNOPS_LAUNCH((attention_rows_tiled<T, DP, NW, false, M>), grid, dim3(64 * NW), 0, s, k);
+    }
+}
+
+// (the kernels that tiled_rows names, and 16 rows a workgroup)
+template <typename T, AttnMode M>
+void launch_part(const AttnKern& k, const dim3& grid, hipStream_t s)
+{
+    const int d = k.c.d;
+    if (k.tile_rows == kRows) {
+        if (d <= 64) {
+            NNOPS_LAUNCH((attention_rows16<T, 64, M>), grid, dim3(256), 0, s, k);
+        } else if (d <= 128) {
+            NNOPS_LAUNCH((attention_rows16<T, 128, M>), grid, dim3(256), 0, s, k);
+        } else {
+            NNOPS_LAUNCH((attention_rows16<T, 256, M>), grid, dim3(256), 0, s, k);
+        }
+    } else if constexpr (sizeof(T) == 2) {
+        if (k.tile_rows == 256) {
+            d <= 64 ? launch_tiled_one<T, 64, 8, M>(k, grid, s) : launch_tiled_one<T, 128, 8, M>(k, grid, s);
+        } else {
+            d <= 64    ? launch_tiled_one<T, 64, 4, M>(k, grid, s)
+            : d <= 128 ? launch_tiled_one<T, 128, 4, M>(k, grid, s)
+                       : launch_tiled_one<T, 256, 4, M>(k, grid, s);
+        }
+    } else if (k.tile_rows == 256) {
+        launch_tiled_one<T, 64, 8, M>(k, grid, s);
+    } else {
+        d <= 64 ? launch_tiled_one<T, 64, 4, M>(k, grid, s) : launch_tiled_one<T, 128, 4, M>(k, grid, s);
+    }
+}
+
+uint32_t reciprocal(int n) { return n > 1 ? (uint32_t)(((1ull << 32) + n - 1) / n) : 0; }
+
+template <typename T>
+void launch_prefix(const PrefixKern& p, const SharedPlan& a, hipStream_t s)
+{
+    NNOPS_LAUNCH(prefix_plan, dim3(1), dim3(kPlanThreads), 0, s, p);
+    AttnKern k = p.own;
+    if (k.groups > 0) {
+        k.tile_rows = a.tile_rows;
+        k.per_seq = a.per_seq;
+        k.first_part = 0;
+        launch_part<T, kShared>(k, dim3((unsigned)a.items, (unsigned)a.splits), s);
+    }
+    launch_part<T, kOwn>(p.own, dim3((unsigned)a.own.items, (unsigned)a.own.splits), s);
+    const int64_t per_block = 256 / join_lanes(k.c.d) / a.ways;
+    const int64_t blocks = ((int64_t)k.c.rows * k.q_heads + per_block - 1) / per_block;
+    NNOPS_LAUNCH(prefix_join<T>, dim3((unsigned)blocks), dim3(256), 0, s, p);
+}
+
+}  // namespace
+}  // namespace nnops_amd
+
+using namespace nnops_amd;
+
+extern "C" size_t nnops_hip_prefix_attention_workspace_size(const NnopsPrefixAttentionArgs* g)
+{
+    return check_prefix(g) >= 0 ? 0 : shared_plan(g).workspace;
+}
+
+extern "C" int nnops_hip_prefix_attention(const NnopsPrefixAttentionArgs* g, void* workspace, size_t workspace_bytes,
+                                          void* stream)
+{
+    const TimingDisarm disarm;
+    if (const int rc = check_prefix(g); rc >= 0) {
+        return rc;
+    }
+    if (const int rc = check_page_memory(g->cache); rc >= 0) {
+        return rc;
+    }
+    const int64_t width = g->q_heads * g->cache.head_dim;
+    if (g->q == nullptr || g->out == nullptr || g->ld_q < width || g->ld_out < width ||
+        (g->groups > 0 && (g->group_starts == nullptr || g->shared == nullptr))) {
+        return NNOPS_INVALID_ARGUMENT;
+    }
+    const SharedPlan a = shared_plan(g);
+    if (a.own.items > INT32_MAX / 512 || a.items > INT32_MAX / 512 || a.own.splits > 65535 || a.splits > 65535 ||
+        g->rows * g->q_heads > INT32_MAX / 256) {
+        return NNOPS_UNSUPPORTED;
+    }
+    if (workspace == nullptr || workspace_bytes < a.workspace || (uintptr_t)workspace % 16 != 0) {
+        return NNOPS_NOT_INITIALIZED;
+    }
+    char* at = static_cast<char*>(workspace);
+    PrefixKern p{};
+    p.group_starts = g->group_starts;
+    p.shared = g->shared;
+    p.starts = reinterpret_cast<int32_t*>(at + a.starts_at);
+    p.shared_splits = a.splits;
+    p.by_shared_splits = reciprocal(a.splits);
+    p.ways = a.ways;
+    AttnKern& k = p.own;
+    k.c = paged(g->cache, g->rows);
+    k.q = g->q;
+    k.out = g->out;
+    k.ld_q = g->ld_q;
+    k.ld_out = g->ld_out;
+    k.part = reinterpret_cast<float*>(at + a.parts_at);
+    k.part_ml = k.part + (size_t)(a.splits + a.own.splits) * g->rows * g->q_heads * g->cache.head_dim;
+    const float scale = g->scale > 0.0f ? g->scale : 1.0f / __builtin_sqrtf((float)g->cache.head_dim);
+    k.scale_log2 = scale * 1.4426950408889634f;
+    k.q_heads = (int32_t)g->q_heads;
+    k.group = (int32_t)(g->q_heads / g->cache.heads);
+    k.tile_rows = a.own.tile_rows;
+    k.per_seq = a.own.per_seq;
+    k.splits = a.own.splits;
+    k.by_splits = reciprocal(a.own.splits);
+    k.tiles = a.own.tiles;
+    k.whole = a.own.whole;
+    k.chunk = a.own.chunk;
+    k.plan = reinterpret_cast<const PrefixPlan*>(at);
+    k.group_plan = reinterpret_cast<const GroupPlan*>(at + a.groups_at);
+    k.members = reinterpret_cast<const MemberPlan*>(at + a.members_at);
+    k.groups = (int32_t)g->groups;
+    k.first_part = a.splits;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (g->f16) {
+        launch_prefix<_Float16>(p, a, s);
+    } else {
+        launch_prefix<float>(p, a, s);
+    }
+    return hipGetLastError() == hipSuccess ? NNOPS_OK : NNOPS_INTERNAL;
+}

@@ -1,8 +1,8 @@
 #pragma once
 /// @file kv_cache.hpp
-/// @brief KvCacheWrite, KvCacheRead, CacheAttention — a key / value cache held
-/// in 8 bits, and attention over it, on the HIP backend (no counterpart in
-/// nnops).
+/// @brief KvCacheWrite, KvCacheRead, CacheAttention, PrefixAttention — a key / value
+/// cache held in 8 bits, and attention over it, on the HIP backend (no counterpart
+/// in nnops).
 ///
 /// The cache's tensors (dense, 16-byte aligned codes):
 ///   k_cache s8 [pages, heads, page_tokens, head_dim]
@@ -104,6 +104,39 @@ public:
 private:
     CacheAttention(const CacheAttentionAttributes& attrs, Backend backend) : attrs_(attrs), backend_(backend) {}
     CacheAttentionAttributes attrs_;
+    Backend backend_;
+};
+
+struct PrefixAttentionAttributes {
+    float scale = 0.0f;   ///< of the scores; 0: 1 / sqrt(head_dim)
+};
+
+/// inputs:  q [rows, q_heads * head_dim] (f16 / f32; q_heads a multiple of the
+///          cache's heads), k_cache, v_cache, k_scale, v_scale, page_table,
+///          lengths, group_starts s32 [groups + 1], shared s32 [groups]
+///          [, row_starts]
+/// output:  q's shape and type: CacheAttention's (without a window) for groups of
+///          sequences, group g those from group_starts[g] up to group_starts[g + 1]
+///          - 1, whose first shared[g] tokens lie in the same pages (as far as they
+///          fill whole pages): read once for the group.
+class PrefixAttention : public OpBase {
+public:
+    static std::unique_ptr<PrefixAttention> create(const PrefixAttentionAttributes& attrs = {},
+                                                   Backend backend = Backend::HIP);
+
+    std::vector<TensorDesc> getOutputTensorDesc(std::span<const TensorDesc> inputs) const override;
+    Status validate(std::span<const TensorDesc> inputs, std::span<const TensorDesc> outputs) const override;
+    size_t getWorkspaceSize(std::span<const TensorDesc> inputs,
+                            std::span<const TensorDesc> outputs) const override;
+    using OpBase::compute;
+    Status compute(std::span<TensorView> outputs, std::span<const TensorView> inputs,
+                   const ComputeContext& ctx = {}, void* workspace = nullptr) override;
+    Backend getBackend() const override { return backend_; }
+    const PrefixAttentionAttributes& attributes() const noexcept { return attrs_; }
+
+private:
+    PrefixAttention(const PrefixAttentionAttributes& attrs, Backend backend) : attrs_(attrs), backend_(backend) {}
+    PrefixAttentionAttributes attrs_;
     Backend backend_;
 };
 

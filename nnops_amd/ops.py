@@ -186,7 +186,7 @@ def _host_tables(scales, zps):
 
 
 # array types for a call's tensors (an empty list still has an address)
-_ARRAYS = [L.Tensor * max(1, n) for n in range(9)]
+_ARRAYS = [L.Tensor * max(1, n) for n in range(11)]
 
 
 class _Op:
@@ -400,6 +400,80 @@ class CacheAttention(_Op):
         L.lib().nnops_cache_attention_attrs_init(C.byref(a))
         a.scale, a.window, a.sinks = scale, window, sinks
         super().__init__(L.lib().nnops_cache_attention_create(C.byref(a), backend))
+
+
+class PrefixAttention(_Op):
+    """:class:`CacheAttention` for groups of sequences that share their first
+    tokens, which are read once for a group. inputs: q [rows, q_heads *
+    head_dim] (f16/f32), k_cache, v_cache, k_scale, v_scale, page_table, lengths,
+    group_starts s32 [groups + 1], shared s32 [groups] (, row_starts); output:
+    q's shape and type. Group g is the sequences group_starts[g] up to
+    group_starts[g + 1] - 1; the page tables of its sequences hold the same pages
+    for the first shared[g] tokens, as far as these fill whole pages (what
+    :class:`KvCacheFork` leaves of a common parent). ``scale`` 0: 1 /
+    sqrt(head_dim)."""
+
+    def __init__(self, *, scale=0.0, backend=L.BACKEND_HIP):
+        a = L.PrefixAttentionAttrs()
+        L.lib().nnops_prefix_attention_attrs_init(C.byref(a))
+        a.scale = scale
+        super().__init__(L.lib().nnops_prefix_attention_create(C.byref(a), backend))
+
+
+class KvCacheFork(_Op):
+    """The page tables of a batch's continuations. inputs: page_table s32 [B, P],
+    lengths s32 [B], refs s32 [pages] (holders of each page, 0: free), parents
+    s32 [N] (-1: none), new_tokens s32 [N] (negative: cut back); outputs:
+    page_table s32 [N, any], lengths s32 [N], refs s32 [pages] (the input's if
+    wanted), copies s32 [N, 2], counts s32 [2] (free pages left, cells that got
+    none). The B sequences are given up; child i goes on from parents[i] in the
+    same pages, with fresh ones for new_tokens[i] more. A page in part full that
+    several would write into is replaced for all but one of them:
+    :class:`KvCacheCopy` makes the copies in each layer's cache."""
+
+    def __init__(self, *, page_tokens, backend=L.BACKEND_HIP):
+        a = L.KvCachePagesAttrs()
+        L.lib().nnops_kv_cache_pages_attrs_init(C.byref(a))
+        a.page_tokens = page_tokens
+        super().__init__(L.lib().nnops_kv_cache_fork_create(C.byref(a), backend))
+
+
+class KvCacheCompact(_Op):
+    """The pages in use moved to the lowest numbers. inputs: page_table s32 [B,
+    P], lengths s32 [B], refs s32 [pages]; outputs: page_table and refs (the
+    inputs' if wanted), copies s32 [pages // 2, 2] for :class:`KvCacheCopy`, moved
+    s32 [pages] (a page's new number, -1 where it is free), counts s32 [2] (pages
+    in use, pages that move)."""
+
+    def __init__(self, *, page_tokens, backend=L.BACKEND_HIP):
+        a = L.KvCachePagesAttrs()
+        L.lib().nnops_kv_cache_pages_attrs_init(C.byref(a))
+        a.page_tokens = page_tokens
+        super().__init__(L.lib().nnops_kv_cache_compact_create(C.byref(a), backend))
+
+
+class KvCacheCopy(_Op):
+    """Pages of a cache copied to others of it. inputs: copies s32 [n, 2], from
+    and to (a pair with a number that is no page is skipped); outputs, updated in
+    place: k_cache, v_cache, k_scale, v_scale."""
+    _takes_workspace = False       # (asking costs a tenth of a small call)
+
+    def __init__(self, *, backend=L.BACKEND_HIP):
+        super().__init__(L.lib().nnops_kv_cache_copy_create(backend))
+
+
+class TokenLogProbs(_Op):
+    """inputs: logits [T, V] (f16/f32), tokens s32 [T, n] or [T]; outputs:
+    log_probs f32 of tokens' shape (0 where a token is negative, NaN where it is V
+    or more), entropy f32 [T] and, with ``top``, top_tokens s32 [T, top] and
+    top_log_probs f32 [T, top], the most probable first, of equal logits the lower
+    token. ``top``: 0 to 32."""
+
+    def __init__(self, *, top=0, backend=L.BACKEND_HIP):
+        a = L.TokenLogProbsAttrs()
+        L.lib().nnops_token_log_probs_attrs_init(C.byref(a))
+        a.top = top
+        super().__init__(L.lib().nnops_token_log_probs_create(C.byref(a), backend))
 
 
 def rotary_table(max_pos, rotary_dim, *, base=10000.0, factor=1.0, original_context=0, low_turns=1.0,

@@ -1,0 +1,271 @@
+"""PrefixAttention against attention in 64 bits over each sequence's own tokens:
+groups of different sizes and prefixes, single tokens and ragged rows, rows inside
+what is shared, sequences in no group, prefixes that end inside pages and tiles,
+pages that do not exist, NaN, group starts out of order, strides, graphs."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import datagen as dg
+import decoder_ref as ref
+import nnops_amd as na
+from gpu_util import announce, dev, host, pitched
+
+pytestmark = pytest.mark.gpu
+
+
+def _cache(lens, groups, shared, heads, page, d, seed=1, spare=2, wide=0):
+    """codes and scales (numpy), and a table whose groups' sequences hold the same
+    pages as far as `shared` fills them."""
+    per = [-(-n // page) for n in lens]
+    n = sum(per) + spare
+    kc, vc = dg.ints(seed, (n, heads, page, d), -127, 127), dg.ints(seed + 1, (n, heads, d, page), -127, 127)
+    ks = (0.01 * np.exp(0.5 * dg.normal(seed + 2, (n, heads)))).astype(np.float32)
+    vs = (0.02 * np.exp(0.7 * dg.normal(seed + 3, (n, heads)))).astype(np.float32)
+    order = iter(np.argsort(dg.unit(seed + 4, n)))
+    table = np.full((len(lens), max(max(per), 1) + wide), -1, np.int32)
+    for i, p in enumerate(per):
+        table[i, :p] = [next(order) for _ in range(p)]
+    for g, s in enumerate(shared):
+        a = groups[g]
+        for b in range(a + 1, groups[g + 1]):
+            k = max(0, min(s, lens[a], lens[b])) // page
+            table[b, :k] = table[a, :k]
+    return kc, vc, ks, vs, table
+
+
+def _run(q, cache, lens, rows, groups, shared, *, ragged, pad=0, scale=0.0, stream=None):
+    import torch
+    kc, vc, ks, vs, table = cache
+    starts = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+    dq = pitched(q, q.shape[1] + pad)
+    out = pitched(np.full(q.shape, 7, q.dtype), q.shape[1] + 2 * pad)
+    ints = [np.array(x, np.int32) for x in (lens, groups, shared)]
+    ins = [na.tensor(dq)] + [na.tensor(dev(x)) for x in [kc, vc, ks, vs, table] + ints]
+    ins += [na.tensor(dev(starts))] if ragged else []
+    op = na.PrefixAttention(scale=scale)
+    outs = [na.tensor(out)]
+    assert op.validate(ins, outs) == na.OK
+    assert op.compute(outs, ins, stream=stream) == na.OK
+    torch.cuda.synchronize()
+    return host(out)
+
+
+def _check(q, cache, lens, rows, groups, shared, *, scale=0.0, **kw):
+    got = _run(q, cache, lens, rows, groups, shared, scale=scale, **kw).astype(np.float64)
+    want, weight, spread = ref.attention(q, *cache, lens, rows, scale=scale or None)
+    tol = ref.attention_tolerance(q.dtype == np.float16, want, weight, spread, cache[3])
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    ok = ~np.isnan(want)
+    worst = np.max((abs(got - want) / tol)[ok]) if ok.any() else 0.0
+    assert worst <= 1.0, worst
+    return got
+
+
+def _q(seed, t, width, f16):
+    return dg.normal(seed, (t, width)).astype(np.float16 if f16 else np.float32)
+
+
+SIZES = [(128, 64, 2, 4), (128, 16, 1, 1), (64, 32, 2, 8), (80, 16, 2, 5), (96, 128, 1, 16), (256, 64, 1, 2), (16, 256, 3, 1),
+         (112, 64, 2, 7), (64, 16, 1, 71), (192, 32, 1, 3)]
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("d,page,heads,group", SIZES)
+def test_single_tokens(d, page, heads, group, f16):
+    """Two groups and a sequence in none; prefixes around tiles and pages."""
+    announce(f"prefix d={d} page={page} heads={heads} group={group} f16={f16}")
+    groups, shared = [1, 5, 8], [300, 130]
+    lens = [70, 301, 364, 500, 333, 131, 257, 140]
+    cache = _cache(lens, groups, shared, heads, page, d)
+    q = _q(3, len(lens), heads * group * d, f16)
+    a = _check(q, cache, lens, [1] * 8, groups, shared, ragged=False)
+    b = _check(q, cache, lens, [1] * 8, groups, shared, ragged=True, pad=3)
+    assert np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("d,page,heads,group", [(128, 64, 2, 4), (64, 16, 2, 3), (80, 128, 1, 5), (256, 64, 1, 2), (32, 32, 1, 8)])
+def test_ragged_rows(d, page, heads, group, f16):
+    """Rows of several tokens, of none, rows that lie inside what is shared (which
+    is then not shared so far), a sequence that is a whole prompt."""
+    announce(f"prefix ragged d={d} page={page} group={group} f16={f16}")
+    groups, shared = [0, 4, 7], [512, 200]
+    lens, rows = [600, 520, 513, 700, 200, 290, 256], [3, 1, 0, 80, 0, 33, 1]
+    cache = _cache(lens, groups, shared, heads, page, d)
+    _check(_q(4, sum(rows), heads * group * d, f16), cache, lens, rows, groups, shared, ragged=True, pad=2)
+    # (the prompt's first row sees only itself: nothing is shared)
+    rows = [3, 513, 0, 1, 200, 2, 1]
+    lens[1] = 513
+    _check(_q(5, sum(rows), heads * group * d, f16), cache, lens, rows, groups, shared, ragged=True)
+    # the last rows: at the border of what is shared and one before
+    lens = [513, 512, 575, 576, 64, 65, 128]
+    cache = _cache(lens, groups, shared, heads, page, d)
+    _check(_q(6, 7, heads * group * d, f16), cache, lens, [1] * 7, groups, shared, ragged=False)
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("d,page,heads,group", [(128, 64, 2, 8), (128, 16, 2, 8), (64, 64, 2, 8), (64, 16, 4, 8), (256, 64, 1, 8),
+                                                (96, 128, 1, 8), (192, 32, 1, 8)])
+def test_tiles_of_many_rows(d, page, heads, group, f16):
+    """Groups with rows enough for tiles of 128 and of 256 rows, several tiles."""
+    announce(f"prefix tiles d={d} page={page} heads={heads} f16={f16}")
+    groups, shared = [0, 10], [640]
+    lens = [640 + 7 * i + 9 for i in range(10)]
+    cache = _cache(lens, groups, shared, heads, page, d)
+    _check(_q(7, 10, heads * group * d, f16), cache, lens, [1] * 10, groups, shared, ragged=False)
+    rows = [9, 1, 7, 0, 9, 5, 9, 9, 30, 2]
+    _check(_q(8, sum(rows), heads * group * d, f16), cache, lens, rows, groups, shared, ragged=True, pad=4)
+    # the same rows in two groups
+    _check(_q(8, sum(rows), heads * group * d, f16), cache, lens, rows, [0, 4, 10], [640, 500], ragged=True)
+
+
+@pytest.mark.parametrize("prefix,page,group,members,n", [(6000, 64, 4, 3, 1), (6000, 16, 1, 2, 1), (5100, 128, 8, 5, 2),
+                                                         (3000, 32, 4, 40, 1)])
+def test_long_prefixes(prefix, page, group, members, n):
+    """Prefixes that are split, own tokens that are split too, one table with room
+    for far more."""
+    announce(f"prefix long {prefix} page={page} group={group} members={members} n={n}")
+    heads, d = 2, 64
+    lens = [prefix + n + 13 * i for i in range(members)]
+    lens[-1] += 3000
+    for f16 in (True, False):
+        for wide in (0, 2000):
+            cache = _cache(lens, [0, members], [prefix], heads, page, d, wide=wide)
+            q = _q(7, members * n, heads * group * d, f16)
+            a = _check(q, cache, lens, [n] * members, [0, members], [prefix], ragged=False)
+            b = _check(q, cache, lens, [n] * members, [0, members], [prefix], ragged=True)
+            assert np.max(abs(a - b)) <= 2.0 ** -9 * np.max(abs(a))
+
+
+@pytest.mark.parametrize("f16", [True, False])
+def test_nothing_shared(f16):
+    """No groups, groups of one, of none, prefixes of 0, negative, beyond all
+    tokens, shorter than a page; empty sequences; more rows than tokens."""
+    announce(f"prefix nothing f16={f16}")
+    heads, group, d, page = 2, 4, 64, 32
+    lens, rows = [100, 0, 3, 250, 64], [1, 1, 5, 2, 64]
+    q = _q(9, sum(rows), heads * group * d, f16)
+    for groups, shared in (([0], []), ([0, 1, 2, 3, 4, 5], [64, 0, 2, 10 ** 9, -4]), ([2, 2, 2, 4], [9, 64, 31]),
+                           ([0, 0], [50]), ([0, 5], [0])):
+        cache = _cache(lens, groups, shared, heads, page, d)
+        got = _check(q, cache, lens, rows, groups, shared, ragged=True)
+        assert (got[1] == 0).all() and (got[2:4] == 0).all()       # no tokens; rows before the first
+
+
+def test_group_starts_out_of_order():
+    """Nothing out of range is read, and every row is still its own sequence's
+    attention: the tables of all agree here."""
+    announce("prefix starts")
+    heads, group, d, page = 1, 4, 64, 16
+    lens = [200, 220, 190, 205, 300, 192]
+    cache = _cache(lens, [0, 6], [180], heads, page, d)
+    q = _q(11, 6, heads * group * d, True)
+    want = _check(q, cache, lens, [1] * 6, [0, 6], [180], ragged=False)
+    for groups in ([5, 2, 6], [0, 4, 2, 6], [-9, 3, 99], [0, 2 ** 31 - 1, -2 ** 31], [6, 6, 0], [3, 0, 3]):
+        shared = [150] * (len(groups) - 1)
+        got = _check(q, cache, lens, [1] * 6, groups, shared, ragged=False)
+        assert np.max(abs(got - want)) <= 2.0 ** -9 * np.max(abs(want))
+
+
+def test_rows_of_no_sequence_are_left_alone():
+    announce("prefix rows left")
+    heads, group, d, page = 1, 2, 64, 16
+    lens, rows = [200, 210], [2, 1]
+    cache = _cache(lens, [0, 2], [190], heads, page, d)
+    q = _q(12, 8, heads * group * d, True)
+    import torch
+    out = torch.full(q.shape, 7.0, dtype=torch.float16, device="cuda")
+    starts = dev(np.array([1, 3, 4], np.int32))
+    ins = [na.tensor(dev(x)) for x in [q, *cache] + [np.array(x, np.int32) for x in (lens, [0, 2], [190])]]
+    assert na.PrefixAttention().compute([na.tensor(out)], ins + [na.tensor(starts)]) == na.OK
+    torch.cuda.synchronize()
+    got = host(out)
+    assert (got[[0, 4, 5, 6, 7]] == 7).all()
+    want, weight, spread = ref.attention(q[1:4], *cache, lens, rows)
+    tol = ref.attention_tolerance(True, want, weight, spread, cache[3])
+    assert (abs(got[1:4] - want) <= tol).all()
+
+
+@pytest.mark.parametrize("f16", [True, False])
+def test_pages_that_do_not_exist_and_nan(f16):
+    """A missing page of the prefix shows in the whole group, one of a sequence's
+    own only there; NaN scales the same; tokens past a sequence's last do not."""
+    announce(f"prefix bad pages f16={f16}")
+    heads, group, d, page = 2, 2, 64, 64
+    groups, shared = [0, 3, 6], [256, 256]
+    lens = [300, 320, 260, 257, 300, 310]
+    cache = _cache(lens, groups, shared, heads, page, d, spare=9)
+    kc, vc, ks, vs, table = cache
+    table[0:3, 2] = 10 ** 6                      # of the first group's prefix
+    table[4, 4] = -3                             # of one sequence's own
+    ks[table[5, 4], 1] = np.nan                  # one head of one page
+    q = _q(13, 6, heads * group * d, f16)
+    got = _check(q, cache, lens, [1] * 6, groups, shared, ragged=False)
+    assert np.isnan(got[:3]).all() and np.isnan(got[4]).all() and np.isfinite(got[3]).all()
+    assert np.isfinite(got[5, :group * d]).all() and np.isnan(got[5, group * d:]).all()
+    # behind the last token: whatever it is
+    vs[table[3, 4]] = np.float32(0.01)
+    vc[table[3, 4], :, :, 1:] = 127
+    _check(q, cache, lens, [1] * 6, groups, shared, ragged=False)
+
+
+def test_scale_and_equal_to_cache_attention():
+    """The same numbers as CacheAttention's up to the order of sums."""
+    import torch
+    announce("prefix against cache attention")
+    heads, group, d, page, members = 8, 4, 128, 64, 33
+    groups, shared = [0, 20, members], [4096, 1000]
+    lens = [4096 + 5 * i + 1 for i in range(20)] + [1001 + 100 * i for i in range(13)]
+    cache = _cache(lens, groups, shared, heads, page, d)
+    q = _q(14, members, heads * group * d, True)
+    got = _run(q, cache, lens, [1] * members, groups, shared, ragged=False, scale=0.05).astype(np.float64)
+    out = torch.empty(q.shape, dtype=torch.float16, device="cuda")
+    ins = [na.tensor(dev(x)) for x in [q, *cache, np.array(lens, np.int32)]]
+    assert na.CacheAttention(scale=0.05).compute([na.tensor(out)], ins) == na.OK
+    torch.cuda.synchronize()
+    want = host(out).astype(np.float64)
+    assert np.linalg.norm(got - want) <= 2.0 ** -10 * np.linalg.norm(want)
+
+
+def test_graph_streams_and_repeats():
+    """A captured call follows lengths and prefixes that change before a replay;
+    two streams at once; the same bits every time."""
+    import torch
+    announce("prefix graph")
+    heads, group, d, page, members = 2, 4, 64, 16, 12
+    groups, shared = [0, 5, members], [700, 300]
+    lens = [701 + 3 * i for i in range(5)] + [301 + 50 * i for i in range(7)]
+    cache = _cache([n + 100 for n in lens], groups, shared, heads, page, d, wide=40)
+    q = _q(15, members, heads * group * d, True)
+    T = na.tensor
+    runs = []
+    for _ in range(2):
+        out = torch.empty(q.shape, dtype=torch.float16, device="cuda")
+        held = [dev(x) for x in [q, *cache] + [np.array(x, np.int32) for x in (lens, groups, shared)]]
+        op = na.PrefixAttention()
+        ins = [T(x) for x in held]
+        ws = torch.empty(op.workspace_size(ins, [T(out)]), dtype=torch.uint8, device="cuda")
+        runs.append((torch.cuda.Stream(), op, ins, out, ws, held))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for s, op, ins, out, ws, _ in runs:
+            assert op.compute([T(out)], ins, stream=s, workspace=ws) == na.OK
+    torch.cuda.synchronize()
+    assert torch.equal(runs[0][3], runs[1][3])
+    s, op, ins, out, ws, held = runs[0]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        assert op.compute([T(out)], ins, stream=s, workspace=ws) == na.OK
+    for step in range(3):
+        held[6].copy_(dev(np.array(lens, np.int32) + 33 * step))
+        held[8].copy_(dev(np.array(shared, np.int32) - 100 * step))
+        ws.fill_(0xff)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        now = [n + 33 * step for n in lens]
+        want, weight, spread = ref.attention(q, *cache, now, [1] * members)
+        tol = ref.attention_tolerance(True, want, weight, spread, cache[3])
+        assert (abs(host(out) - want) <= tol).all(), step
