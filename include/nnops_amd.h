@@ -645,8 +645,8 @@ int nnops_hip_kv_cache_copy(const NnopsKvCopyArgs* args, void* stream);
  *                     equal logits the lower token first
  * A logit of -inf has probability 0. A row of nothing else: every log probability
  * -inf, the entropy 0. A row that holds a NaN or +inf: NaN, top_tokens -1.
- * Sums are f32. top: 0 to 32, at most vocab (0: top_tokens and top_log_probs are
- * not looked at). Rows are split over the chip where there are few of them: their
+ * Sums are f32. vocab: up to 2^21. top: 0 to 32, at most vocab (0: top_tokens and
+ * top_log_probs are not looked at). Rows are split over the chip where there are few of them: their
  * parts are in the workspace, nnops_hip_token_log_probs_workspace_size bytes,
  * 16-byte aligned, which need no initialization. */
 typedef struct NnopsTokenLogProbsArgs {

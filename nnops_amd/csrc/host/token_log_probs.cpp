@@ -72,7 +72,8 @@ Status TokenLogProbs::validate(std::span<const TensorDesc> inputs, std::span<con
             return Status::invalid_argument;
         }
     }
-    return is_float(inputs[0].dtype) && attrs_.top <= 32 ? Status::ok : Status::unsupported;
+    const bool sizes = attrs_.top <= 32 && inputs[0].dims[1] <= (1 << 21);
+    return is_float(inputs[0].dtype) && sizes ? Status::ok : Status::unsupported;
 }
 
 size_t TokenLogProbs::getWorkspaceSize(std::span<const TensorDesc> inputs, std::span<const TensorDesc> outputs) const

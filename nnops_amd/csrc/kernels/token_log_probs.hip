@@ -1,21 +1,21 @@
 // Log probabilities of given tokens, the entropy and the most probable tokens of
 // rows of logits, in one pass over them.
 //
-// With a reference r for a row (its largest logit so far) and y_j = (x_j - r)
-// log2(e):
+// A workgroup holds a row, or a part of a long one, in its registers (up to 64
+// logits a thread, all of its loads in flight at once): the maximum first, then
+// with a reference r and y_j = (x_j - r) log2(e)
 //   s = sum 2^y_j,  t = sum y_j 2^y_j
 //   log p_j = ln 2 (y_j - log2 s),  entropy = ln 2 (log2 s - t / s)
-// and s, t are brought to a new reference when the maximum grows (by d = y of the
-// old one: s' = 2^d s, t' = 2^d (t + d s)), which a row's first tiles do and later
-// ones hardly. f16 rows: y = fma(x, log2(e), -r log2(e)): the rounding of the
-// second product is the same for all, and drops out. f32 rows: (x - r) log2(e),
-// which masks of the type's lowest value do not take out of f32's range.
+// A part's s and t are brought to another's reference by d, the y of its own: s' =
+// 2^d s, t' = 2^d (t + d s). f16 rows: y = fma(x, log2(e), -r log2(e)): the rounding
+// of the second product is the same for all, and drops out. f32 rows: (x - r)
+// log2(e), which masks of the type's lowest value do not take out of f32's range.
 //
-// The most probable: keys of 64 bits, the logit's bits in an order that whole
-// numbers have, then the token's complement, so that no two are equal. A wave
-// keeps those above a threshold (the top-th of what it has seen, as far as it
-// knows) in LDS and drops all but the top when there is no room: after the first
-// tile about top ln(n / 512) of n logits come that far.
+// The most probable: the top-th largest of the maxima of 32 groups of 16 lanes is
+// a logit that at least `top` reach, and few more do (of 32768 random ones 31 for
+// 20, 111 for 32): those go into LDS as keys of 64 bits, the logit's bits in an
+// order that whole numbers have, then the token's complement, so that no two are
+// equal, and each counts the keys above it.
 //
 // Bound: HBM, the logits read once.
 #include <limits>
@@ -25,10 +25,14 @@
 namespace nnops_amd {
 namespace {
 
-constexpr int kTile = 512;          // logits of a wave's step, 8 a lane
-constexpr int kCap = 1024;          // keys that a wave has room for
+constexpr int kThreads = 512;
+constexpr int kSpan = 8 * kThreads; // logits that the threads have side by side, 8 each
+constexpr int kMostChunks = 8;      // of those a part
+constexpr int kGroups = kThreads / 16;
 constexpr int kMostTop = 32;
 constexpr int kMostSplits = 64;
+constexpr int kRoom = 2048;         // keys above a threshold ...
+constexpr int kKeys = kRoom + kSpan;   // ... and those of a span that are equal to it
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNone = -std::numeric_limits<float>::infinity();
 
@@ -42,7 +46,7 @@ struct LogProbsKern {
     int64_t ld_x, ld_tokens, ld_log_probs, ld_top_tokens, ld_top_log_probs;
     int32_t vocab, per_row, top, splits, part;   // part: logits of a split
     float* stats;         // workspace: reference, s, t of [rows][splits]
-    uint64_t* keys;       //   keys of [rows][splits][top]
+    uint64_t* keys;       //   keys of [rows][splits][top], 0 where a split has fewer
 };
 
 // The reference that goes with a maximum, y against it, and y of an old one.
@@ -54,10 +58,7 @@ struct Reference<_Float16> {
     static __device__ __forceinline__ float of(float m) { return m * kLog2e; }
     static __device__ __forceinline__ float y(float x, float r) { return __builtin_fmaf(x, kLog2e, -r); }
     static __device__ __forceinline__ float step(float old, float r) { return old - r; }
-    static __device__ __forceinline__ float log_p(float x, float r, float s)
-    {
-        return (y(x, r) - log2f(s)) * kLn2;
-    }
+    static __device__ __forceinline__ float log_p(float x, float r, float s) { return (y(x, r) - log2f(s)) * kLn2; }
 };
 template <>
 struct Reference<float> {
@@ -81,353 +82,466 @@ __device__ __forceinline__ float logit_of(uint64_t key)
 }
 __device__ __forceinline__ int token_of(uint64_t key) { return (int)~(uint32_t)key; }
 
-// What a wave's lanes put into LDS is there for the others.
-__device__ __forceinline__ void wave_sync()
+// A lane's value from elsewhere in its 16: step 0 to 3 of a reduction over them.
+template <int kStep>
+__device__ __forceinline__ uint32_t from_row(uint32_t v)
 {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#if __HIP_DEVICE_COMPILE__
+    constexpr int kCtrl = kStep == 0 ? 0xb1 : kStep == 1 ? 0x4e : kStep == 2 ? 0x141 : 0x140;   // pairs, quads, mirrors
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, 0xf, 0xf, true);
+#else
+    return v;
+#endif
+}
+template <int kStep = 0>
+__device__ __forceinline__ float row_max(float v)
+{
+    if constexpr (kStep < 4) {
+        return row_max<kStep + 1>(fmaxf(v, __uint_as_float(from_row<kStep>(__float_as_uint(v)))));
+    }
+    return v;
+}
+template <int kStep = 0>
+__device__ __forceinline__ float row_sum(float v)
+{
+    if constexpr (kStep < 4) {
+        return row_sum<kStep + 1>(v + __uint_as_float(from_row<kStep>(__float_as_uint(v))));
+    }
+    return v;
+}
+template <int kStep = 0>
+__device__ __forceinline__ uint64_t row_max(uint64_t v)
+{
+    if constexpr (kStep < 4) {
+        const uint64_t o = (uint64_t)from_row<kStep>((uint32_t)(v >> 32)) << 32 | from_row<kStep>((uint32_t)v);
+        return row_max<kStep + 1>(o > v ? o : v);
+    }
+    return v;
 }
 
-__device__ __forceinline__ uint64_t lane_key(uint64_t key, int lane)
+// The largest of 8 logits; NaNs count for nothing.
+__device__ __forceinline__ float max_of(const float (&v)[8])
 {
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), lane) << 32 |
-           (uint32_t)__builtin_amdgcn_readlane((int)key, lane);
-}
-
-__device__ __forceinline__ int lanes_below(uint64_t mask)
-{
-    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
-}
-
-// The `top` largest of buf[0 .. n), in descending order at its begin; returns how
-// many. Whole waves. As long as there are many: those that are at least the top-th
-// of the lanes' largest stay (the lanes below it lose all of theirs, half and more).
-__device__ __forceinline__ int keep_top(uint64_t* buf, int n, int top)
-{
-    const int lane = threadIdx.x % 64;
-    wave_sync();
-    while (n > 128) {
-        uint64_t mine[kCap / 64], best = 0;
+    float m = fmaxf(v[0], v[1]);
 #pragma unroll
-        for (int j = 0; j < kCap / 64; ++j) {
-            mine[j] = 64 * j + lane < n ? buf[64 * j + lane] : 0;
-            best = mine[j] > best ? mine[j] : best;
-        }
-        int rank = 0;
-        for (int l = 0; l < 64; ++l) {
-            rank += lane_key(best, l) > best;
-        }
-        const uint64_t least = lane_key(best, __builtin_ctzll(__ballot(rank == top - 1)));
-        wave_sync();
-        n = 0;
+    for (int e = 2; e < 8; ++e) {
+        m = fmaxf(m, v[e]);
+    }
+    return m;
+}
+__device__ __forceinline__ float max_of(const _Float16 (&v)[8])
+{
+#if __HIP_DEVICE_COMPILE__
+    uint32_t w[4], a, b;
+    __builtin_memcpy(w, v, sizeof w);
+    asm("v_pk_max_f16 %0, %1, %2" : "=v"(a) : "v"(w[0]), "v"(w[1]));   // (the builtin makes quiet NaNs first)
+    asm("v_pk_max_f16 %0, %1, %2" : "=v"(b) : "v"(w[2]), "v"(w[3]));
+    asm("v_pk_max_f16 %0, %0, %1" : "+v"(a) : "v"(b));
+    _Float16 h[2];
+    __builtin_memcpy(h, &a, sizeof h);
+    return fmaxf((float)h[0], (float)h[1]);
+#else
+    return (float)v[0];
+#endif
+}
+
+// A value of all lanes' largest, or sum, of those that are the same in 16 lanes.
+__device__ __forceinline__ float lane_of(float v, int lane)
+{
+#if __HIP_DEVICE_COMPILE__
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
+#else
+    return v;
+#endif
+}
+
+// The top-th largest of the groups' values (equal ones count each).
+template <typename V>
+__device__ __forceinline__ V top_of(const V (&group)[kGroups], int top)
+{
+    const int mine = threadIdx.x % kGroups;
+    const V v = group[mine];
+    int rank = 0;
 #pragma unroll
-        for (int j = 0; j < kCap / 64; ++j) {
-            const bool stays = mine[j] >= least;
-            const uint64_t mask = __ballot(stays);
-            if (stays) {
-                buf[n + lanes_below(mask)] = mine[j];
+    for (int i = 0; i < kGroups; ++i) {
+        rank += group[i] > v || (group[i] == v && i < mine);
+    }
+    const int lane = __builtin_ctzll(__ballot(rank == top - 1));
+    if constexpr (sizeof(V) == 4) {
+        return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
+    } else {
+        return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+               (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+    }
+}
+
+struct Shared {
+    uint64_t key[kKeys];
+    uint64_t key_group[kGroups];
+    float group[kGroups], s[kGroups], t[kGroups];
+    int keys, left;
+};
+
+// Of sh.key[0 .. n): one of this thread's and how many are above it; a thread without
+// any has 0 and its own number. More than 64 keys are thinned first: those that reach
+// the top-th of the groups' largest stay. (Where none goes, that group had a single
+// key, or none: there is at most a key a thread.) Every thread calls it.
+__device__ __forceinline__ uint64_t rank_keys(Shared& sh, int n, int top, int& rank)
+{
+    const int tid = threadIdx.x;
+    while (n > 64) {
+        uint64_t best = 0;
+        for (int i = tid; i < n; i += kThreads) {
+            best = sh.key[i] > best ? sh.key[i] : best;
+        }
+        best = row_max(best);
+        if (tid % 16 == 0) {
+            sh.key_group[tid / 16] = best;
+        }
+        if (tid == 0) {
+            sh.left = 0;
+        }
+        __syncthreads();
+        uint64_t least = top_of(sh.key_group, top);
+        least = least > 0 ? least : 1;             // (fewer groups than that have any)
+        for (int i = 0; i < n; i += kThreads) {
+            const uint64_t mine = i + tid < n ? sh.key[i + tid] : 0;
+            __syncthreads();                       // (what stays goes over keys that were looked at)
+            if (mine >= least) {
+                sh.key[atomicAdd(&sh.left, 1)] = mine;
             }
-            n += __popcll(mask);
         }
-        wave_sync();
+        __syncthreads();
+        const int left = sh.left;
+        __syncthreads();
+        if (left == n) {                           // (see above)
+            break;
+        }
+        n = left;
     }
-    const uint64_t a = lane < n ? buf[lane] : 0, b = 64 + lane < n ? buf[64 + lane] : 0;
-    int rank_a = 0, rank_b = 0;
-    for (int i = 0; i < n; ++i) {
-        const uint64_t other = buf[i];
-        rank_a += other > a;
-        rank_b += other > b;
+    const uint64_t key = tid < n ? sh.key[tid] : 0;
+    rank = 0;
+    if (tid < n) {
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+            rank += sh.key[i] > key;
+        }
+    } else {
+        rank = tid;                                // (behind the last key: nothing)
     }
-    wave_sync();
-    if (lane < n && rank_a < top) {
-        buf[rank_a] = a;
-    }
-    if (64 + lane < n && rank_b < top) {
-        buf[rank_b] = b;
-    }
-    wave_sync();
-    return min(n, top);
+    return key;
 }
 
 struct Stats {
     float r, s, t;
 };
 
+// Another reference's s and t, added.
 template <typename T>
-__device__ __forceinline__ Stats join(const Stats& a, const Stats& b)
+__device__ __forceinline__ void join(Stats& a, const Stats& x)
 {
-    typedef Reference<T> Ref;
-    const float r = fmaxf(a.r, b.r);
-    Stats j{r, 0.0f, 0.0f};
-    for (const Stats& x : {a, b}) {
-        if (x.s != 0.0f) {                         // (NaN: joins)
-            const float d = Ref::step(x.r, r), f = exp2f(d);
-            j.s += x.s * f;
-            j.t += f != 0.0f ? f * __builtin_fmaf(d, x.s, x.t) : 0.0f;
-        }
+    if (x.s != 0.0f) {                             // (NaN: joins)
+        const float d = Reference<T>::step(x.r, a.r), f = exp2f(d);
+        a.s += x.s * f;
+        a.t += f != 0.0f ? f * __builtin_fmaf(d, x.s, x.t) : 0.0f;
     }
-    return j;
 }
 
-// What a workgroup writes of a whole row.
+// A given token of a row, and its logit: asked for before the row is looked at.
 template <typename T>
-__device__ __forceinline__ void write_row(const LogProbsKern& p, int64_t row, const Stats& w, const uint64_t* best)
+struct Given {
+    int token;
+    T logit;
+};
+template <typename T>
+__device__ __forceinline__ Given<T> given(const LogProbsKern& p, int64_t row, int i)
+{
+    Given<T> g{-1, (T)0.0f};
+    if (i < p.per_row) {
+        g.token = p.tokens[row * p.ld_tokens + i];
+        if ((uint32_t)g.token < (uint32_t)p.vocab) {
+            g.logit = static_cast<const T*>(p.x)[row * p.ld_x + g.token];
+        }
+    }
+    return g;
+}
+__device__ __forceinline__ int given_of(int tid) { return kThreads - 1 - tid; }   // (the first threads have keys)
+
+// What a workgroup writes of a whole row; a thread its key, where it is among the top,
+// and its given tokens.
+template <typename T>
+__device__ __forceinline__ void write_row(const LogProbsKern& p, int64_t row, const Stats& w, uint64_t key, int rank,
+                                          Given<T> g)
 {
     typedef Reference<T> Ref;
     const int tid = threadIdx.x;
     const float nan = __uint_as_float(0x7fc00000u);
     const bool bad = !(w.s < std::numeric_limits<float>::infinity()), none = w.s == 0.0f;
     const auto log_p = [&](float x) { return bad ? nan : none ? kNone : Ref::log_p(x, w.r, w.s); };
-    if (tid < p.top) {
-        const uint64_t key = best[tid];
-        p.top_tokens[row * p.ld_top_tokens + tid] = bad ? -1 : token_of(key);
-        p.top_log_probs[row * p.ld_top_log_probs + tid] = log_p(logit_of(key));
+    const int to = bad ? tid : rank;
+    if (to < p.top) {
+        p.top_tokens[row * p.ld_top_tokens + to] = bad ? -1 : token_of(key);
+        p.top_log_probs[row * p.ld_top_log_probs + to] = log_p(logit_of(key));
     }
-    if (tid == 0) {
+    if (tid == kThreads - 1) {
         p.entropy[row] = bad ? nan : none ? 0.0f : fmaxf((log2f(w.s) - w.t / w.s) * kLn2, 0.0f);
     }
-    const T* x = static_cast<const T*>(p.x) + row * p.ld_x;
-    for (int i = tid; i < p.per_row; i += 256) {
-        const int token = p.tokens[row * p.ld_tokens + i];
-        const float lp = token < 0 ? 0.0f : token < p.vocab ? log_p((float)x[token]) : nan;
-        p.log_probs[row * p.ld_log_probs + i] = lp;
+    for (int i = given_of(tid); i < p.per_row;) {
+        p.log_probs[row * p.ld_log_probs + i] = g.token < 0 ? 0.0f : g.token < p.vocab ? log_p((float)g.logit) : nan;
+        i += kThreads;
+        g = given<T>(p, row, i);
     }
 }
 
-// The waves' stats and keys (each wave's at buf + kCap wave, `n` of them) as a
-// workgroup's: in every thread, and in s_best.
+// The keys of a part x[0 .. n) whose logits reach `least` in more places than there is
+// room for (equal ones: masks; a few groups that have nearly all that is large), read
+// again: how many there are. At least the `top` largest are among them. Every thread
+// calls it.
 template <typename T>
-__device__ __forceinline__ Stats join_waves(const Stats& mine, int n, int top, uint64_t* bufs, uint64_t* s_best,
-                                            Stats* s_stats, int* s_n)
+__device__ __forceinline__ int many_keys(Shared& sh, const T* x, int begin, int n, float least, int top)
 {
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-    if (lane == 0) {
-        s_stats[wave] = mine;
-        s_n[wave] = n;
+    const int tid = threadIdx.x;
+    __syncthreads();
+    if (tid == 0) {
+        sh.keys = 0;
     }
     __syncthreads();
-    if (top > 0 && wave == 0) {
-        // key i of wave w is slot 32 w + i
-        uint64_t key[2];
-        int rank[2] = {0, 0};
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int w = 2 * h + lane / 32, i = lane % 32;
-            key[h] = i < s_n[w] ? bufs[w * kCap + i] : 0;
-        }
-        for (int l = 0; l < 64; ++l) {
-            const uint64_t a = lane_key(key[0], l), b = lane_key(key[1], l);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                rank[h] += (a > key[h]) + (b > key[h]);
-            }
-        }
-        // (absent ones come last: there are `top` others, but in rows that are not finite)
-        if (lane < top) {
-            s_best[lane] = 0;
-        }
-        wave_sync();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (key[h] != 0 && rank[h] < top) {
-                s_best[rank[h]] = key[h];
+    for (int at = tid; at < n; at += kThreads) {
+        const float v = (float)x[at];
+        if (v > least) {
+            const int to = atomicAdd(&sh.keys, 1);
+            if (to < kRoom) {
+                sh.key[to] = key_of(v, begin + at);
             }
         }
     }
-    Stats w = join<T>(join<T>(s_stats[0], s_stats[1]), join<T>(s_stats[2], s_stats[3]));
     __syncthreads();
-    return w;
+    int keys = sh.keys;
+    __syncthreads();
+    if (keys <= kRoom) {
+        // the equal ones in order, until there are enough
+        for (int j = 0; j < n && keys < top; j += kSpan) {
+            for (int at = j + tid; at < min(j + kSpan, n); at += kThreads) {
+                const float v = (float)x[at];
+                if (v == least) {
+                    sh.key[atomicAdd(&sh.keys, 1)] = key_of(v, begin + at);
+                }
+            }
+            __syncthreads();
+            keys = sh.keys;
+            __syncthreads();
+        }
+        return keys;
+    }
+    // one after another
+    uint64_t above = ~0ull;
+    for (int i = 0; i < top; ++i) {
+        uint64_t next = 0;
+        for (int at = tid; at < n; at += kThreads) {
+            const uint64_t k = key_of((float)x[at], begin + at);
+            next = k < above && k > next ? k : next;
+        }
+        next = row_max(next);
+        if (tid % 16 == 0) {
+            sh.key_group[tid / 16] = next;
+        }
+        __syncthreads();
+        above = top_of(sh.key_group, 1);
+        if (tid == 0) {
+            sh.key[i] = above;
+        }
+        __syncthreads();
+    }
+    return top;
 }
 
-template <typename T, bool kTop>
-__global__ __launch_bounds__(256) void log_probs(const LogProbsKern p)
+template <typename T, int kChunks, bool kTop>
+__global__ __launch_bounds__(kThreads, 4) void log_probs(const LogProbsKern p)
 {
     typedef Reference<T> Ref;
-    __shared__ uint64_t s_buf[kTop ? 4 * kCap : 1];
-    __shared__ uint64_t s_best[kMostTop];
-    __shared__ Stats s_stats[4];
-    __shared__ int s_n[4];
-    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    __shared__ Shared sh;
+    const int tid = threadIdx.x;
     const int64_t row = blockIdx.x / (uint32_t)p.splits;
     const int split = (int)(blockIdx.x - (uint32_t)row * p.splits);
-    const T* x = static_cast<const T*>(p.x) + row * p.ld_x;
-    const int begin = split * p.part, end = (int)min((int64_t)begin + p.part, (int64_t)p.vocab);
-    uint64_t* buf = s_buf + (kTop ? wave * kCap : 0);
-    int n = 0;
-    bool full = false;                             // at least top keys above the threshold, or at it
-    float least = kNone;
-    float m = Ref::kLeast, r = Ref::of(m), s = 0.0f, t = 0.0f;
-
-    const auto load = [&](int at, T (&v)[8]) {
-        const int i = at + 8 * lane;
-        if (at + kTile <= end) {
-            __builtin_memcpy(v, x + i, sizeof v);
+    const int begin = split * p.part, n = min(p.part, p.vocab - begin);
+    const T* x = static_cast<const T*>(p.x) + row * p.ld_x + begin;
+    const Given<T> g = p.splits == 1 ? given<T>(p, row, given_of(tid)) : Given<T>{};
+    T v[kChunks][8];
+    float high[kChunks], best = kNone;
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) {
+        const int at = j * kSpan + 8 * tid;
+        if (j * kSpan + kSpan <= n) {
+            __builtin_memcpy(v[j], x + at, sizeof v[j]);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                v[e] = i + e < end ? x[i + e] : (T)kNone;
+                v[j][e] = (T)kNone;
+            }
+            if (at + 8 <= n) {
+                __builtin_memcpy(v[j], x + at, sizeof v[j]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (at + e < n) {
+                        v[j][e] = x[at + e];
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) {
+        high[j] = max_of(v[j]);
+        best = fmaxf(best, high[j]);
+    }
+    best = row_max(best);
+    if (tid % 16 == 0) {
+        sh.group[tid / 16] = best;
+    }
+    if (tid == 0) {
+        sh.keys = 0;
+    }
+    __syncthreads();
+    float m = row_max(sh.group[tid % kGroups]);
+    m = fmaxf(lane_of(m, 0), lane_of(m, 16));
+    const float r = Ref::of(fmaxf(m, Ref::kLeast));
+    // (each phase converts f16 logits anew: kept as f32 they would take the registers of
+    // another workgroup)
+    const auto forget = [&] {
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) {
+                v4i w;
+                __builtin_memcpy(&w, v[j], sizeof w);
+                asm volatile("" : "+v"(w));
+                __builtin_memcpy(v[j], &w, sizeof w);
             }
         }
     };
-    const auto take = [&](int at, const T (&raw)[8]) {
-        float v[8], high = kNone;
+    forget();
+    float least = kNone;
+    if constexpr (kTop) {
+        least = top_of(sh.group, p.top);
+        const T reach = (T)least;                  // (one of the logits: exact)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            v[e] = (float)raw[e];
-            high = fmaxf(high, v[e]);
-        }
-        if (__any(high > m)) {
-            float top = high;
+        for (int j = 0; j < kChunks; ++j) {
+            if (j * kSpan < n && __any(high[j] >= least)) {
 #pragma unroll
-            for (int i = 1; i < 64; i *= 2) {
-                top = fmaxf(top, __shfl_xor(top, i));
-            }
-            m = top;
-            const float old = r;
-            r = Ref::of(m);
-            const float d = fmaxf(Ref::step(old, r), -1e30f), f = exp2f(d);   // (s and t are 0 at first)
-            t = f * __builtin_fmaf(d, s, t);
-            s *= f;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float y = Ref::y(v[e], r), w = __builtin_amdgcn_exp2f(y);
-            s += w;
-            t = __builtin_fmaf(w, fmaxf(y, -256.0f), t);   // (0 times -inf)
-        }
-        if constexpr (kTop) {
-            if (full && !__any(high > least)) {
-                return;
-            }
-            if (n + kTile > kCap) {
-                n = keep_top(buf, n, p.top);
-                least = logit_of(buf[p.top - 1]);
-            }
-            bool equal = false;
-            if (!full && at + kTile <= end) {
-                // the top-th of the lanes' largest: as many are at least that
-                int rank = 0;
-                for (int l = 0; l < 64; ++l) {
-                    const float other = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(high), l));
-                    rank += other > high || (other == high && l < lane);
+                for (int e = 0; e < 8; ++e) {
+                    const int at = j * kSpan + 8 * tid + e;
+                    if (v[j][e] >= reach && at < n) {
+                        const int to = atomicAdd(&sh.keys, 1);
+                        if (to < kRoom) {
+                            sh.key[to] = key_of((float)v[j][e], begin + at);
+                        }
+                    }
                 }
-                const int at_lane = __builtin_ctzll(__ballot(rank == p.top - 1));
-                least = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(high), at_lane));
-                equal = true;
-                full = true;
             }
-            const bool all = !full;                // (less than a tile: it is the wave's last)
+        }
+    }
+    forget();
+    float s = 0.0f, t = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) {
+        if (j * kSpan < n) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int token = at + 8 * lane + e;
-                const bool in = token < end && (all || v[e] > least || (equal && v[e] == least));
-                const uint64_t mask = __ballot(in);
-                if (in) {
-                    buf[n + lanes_below(mask)] = key_of(v[e], token);
-                }
-                n += __popcll(mask);
-            }
-        }
-    };
-    int at = begin + kTile * wave;
-    if (at < end) {
-        T v[3][8];
-        load(at, v[0]);
-        if (at + 4 * kTile < end) {
-            load(at + 4 * kTile, v[1]);
-        }
-        for (; at < end; at += 12 * kTile) {
-#pragma unroll
-            for (int i = 0; i < 3; ++i) {
-                if (at + 4 * kTile * i < end) {
-                    if (at + 4 * kTile * (i + 2) < end) {
-                        load(at + 4 * kTile * (i + 2), v[(i + 2) % 3]);
-                    }
-                    take(at + 4 * kTile * i, v[i]);
-                }
+                const float y = Ref::y((float)v[j][e], r), w = __builtin_amdgcn_exp2f(y);
+                s += w;
+                t = __builtin_fmaf(w, fmaxf(y, -256.0f), t);   // (0 times -inf)
             }
         }
     }
+    s = row_sum(s);
+    t = row_sum(t);
+    if (tid % 16 == 0) {
+        sh.s[tid / 16] = s;
+        sh.t[tid / 16] = t;
+    }
+    __syncthreads();
+    s = row_sum(sh.s[tid % kGroups]);
+    t = row_sum(sh.t[tid % kGroups]);
+    const Stats w{r, lane_of(s, 0) + lane_of(s, 16), lane_of(t, 0) + lane_of(t, 16)};
+    uint64_t key = 0;
+    int rank = tid;
     if constexpr (kTop) {
-        n = keep_top(buf, n, p.top);
+        int keys = sh.keys;
+        if (keys > kRoom) {
+            keys = many_keys(sh, x, begin, n, least, p.top);
+        }
+        key = rank_keys(sh, keys, p.top, rank);
     }
-#pragma unroll
-    for (int i = 1; i < 64; i *= 2) {
-        s += __shfl_xor(s, i);
-        t += __shfl_xor(t, i);
-    }
-    const Stats w = join_waves<T>(Stats{r, s, t}, n, kTop ? p.top : 0, s_buf, s_best, s_stats, s_n);
     if (p.splits == 1) {
-        write_row<T>(p, row, w, s_best);
+        write_row<T>(p, row, w, key, rank, g);
         return;
     }
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
         float* to = p.stats + 3 * (int64_t)blockIdx.x;
         to[0] = w.r;
         to[1] = w.s;
         to[2] = w.t;
     }
-    if (kTop && (int)threadIdx.x < p.top) {
-        p.keys[(int64_t)blockIdx.x * p.top + threadIdx.x] = s_best[threadIdx.x];
+    if (kTop && rank < p.top) {
+        p.keys[(int64_t)blockIdx.x * p.top + rank] = key;
     }
 }
 
-// The splits of a row: at most 64, whose keys fit the waves' room.
+// The splits of a row, at most 64: a lane each.
 template <typename T>
-__global__ __launch_bounds__(256) void log_probs_join(const LogProbsKern p)
+__device__ __forceinline__ Stats join_splits(const LogProbsKern& p, int64_t row)
 {
-    __shared__ uint64_t s_buf[4 * kCap];
-    __shared__ uint64_t s_best[kMostTop];
-    __shared__ Stats s_stats[4];
-    __shared__ int s_n[4];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const int64_t row = blockIdx.x;
-    Stats mine{Reference<T>::kLeast, 0.0f, 0.0f};
-    mine.r = Reference<T>::of(mine.r);
-    if (wave == 0 && lane < p.splits) {
+    const int lane = threadIdx.x % 64;
+    Stats w{Reference<T>::of(Reference<T>::kLeast), 0.0f, 0.0f};
+    if (lane < p.splits) {
         const float* from = p.stats + 3 * (row * p.splits + lane);
-        mine = Stats{from[0], from[1], from[2]};
+        w = Stats{from[0], from[1], from[2]};
     }
-#pragma unroll
-    for (int i = 1; i < 64; i *= 2) {
-        mine = join<T>(mine, Stats{__shfl_xor(mine.r, i), __shfl_xor(mine.s, i), __shfl_xor(mine.t, i)});
+    const float r = row_max(w.r);
+    Stats sum{fmaxf(fmaxf(lane_of(r, 0), lane_of(r, 16)), fmaxf(lane_of(r, 32), lane_of(r, 48))), 0.0f, 0.0f};
+    join<T>(sum, w);
+    const float s = row_sum(sum.s), t = row_sum(sum.t);
+    sum.s = (lane_of(s, 0) + lane_of(s, 16)) + (lane_of(s, 32) + lane_of(s, 48));
+    sum.t = (lane_of(t, 0) + lane_of(t, 16)) + (lane_of(t, 32) + lane_of(t, 48));
+    return sum;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void log_probs_join(const LogProbsKern p)
+{
+    __shared__ Shared sh;
+    const int tid = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    const Given<T> g = given<T>(p, row, given_of(tid));
+    const int all = p.splits * p.top;              // at most 2048
+    for (int i = tid; i < all; i += kThreads) {
+        sh.key[i] = p.keys[row * all + i];
     }
-    uint64_t* buf = s_buf + wave * kCap;
-    int n = 0;
-    if (p.top > 0) {
-        const int all = p.splits * p.top, share = (all + 3) / 4;   // at most 512
-        const uint64_t* keys = p.keys + row * all;
-        const int first = wave * share, mine_n = max(min(share, all - first), 0);
-        for (int i = 0; i < mine_n; i += 64) {     // (a split of fewer than top logits has 0 behind them)
-            const uint64_t key = i + lane < mine_n ? keys[first + i + lane] : 0;
-            const uint64_t mask = __ballot(key != 0);
-            if (key != 0) {
-                buf[n + lanes_below(mask)] = key;
-            }
-            n += __popcll(mask);
-        }
-        n = keep_top(buf, n, p.top);
-    }
-    write_row<T>(p, row, join_waves<T>(mine, n, p.top, s_buf, s_best, s_stats, s_n), s_best);
+    const Stats sum = join_splits<T>(p, row);
+    __syncthreads();
+    int rank;
+    const uint64_t key = rank_keys(sh, all, p.top, rank);
+    // (a row that is not bad has `top` keys that are not 0)
+    write_row<T>(p, row, sum, key, key != 0 ? rank : kMostTop, g);
 }
 
 struct LogProbsPlan {
-    int32_t splits, part;
+    int32_t splits, part, chunks;
     size_t stats, workspace;
 };
 
-// Splits of a row: as many workgroups as the chip holds, each with 2048 logits (a
-// tile for each wave) or more.
+// A workgroup's spans: as many as leave 512 workgroups.
 LogProbsPlan log_probs_plan(const NnopsTokenLogProbsArgs* g)
 {
     LogProbsPlan a{};
-    const int64_t most = (g->vocab + 4 * kTile - 1) / (4 * kTile);
-    int64_t splits = (1024 + g->rows - 1) / g->rows;
-    splits = splits < most ? splits : most;
-    splits = splits < kMostSplits ? splits : kMostSplits;
-    const int64_t part = ((g->vocab + splits - 1) / splits + 4 * kTile - 1) / (4 * kTile) * (4 * kTile);
-    a.part = (int32_t)(part < INT32_MAX ? part : INT32_MAX);
+    const auto parts = [&](int64_t chunks) { return (g->vocab + chunks * kSpan - 1) / (chunks * kSpan); };
+    a.chunks = kMostChunks;
+    while (a.chunks > 1 && parts(a.chunks / 2) <= kMostSplits &&
+           (parts(a.chunks / 2) == parts(a.chunks) || g->rows * parts(a.chunks) < 512)) {
+        a.chunks /= 2;
+    }
+    const int64_t splits = parts(a.chunks), part = ((g->vocab + splits - 1) / splits + 7) / 8 * 8;
+    a.part = (int32_t)part;
     a.splits = (int32_t)((g->vocab + part - 1) / part);
     if (a.splits > 1) {
         a.stats = ((size_t)12 * g->rows * a.splits + 15) / 16 * 16;
@@ -450,23 +564,32 @@ int check_log_probs(const NnopsTokenLogProbsArgs* g)
     if (g->vocab == 0) {
         return NNOPS_INVALID_ARGUMENT;
     }
-    if (g->rows > (1 << 22) || g->vocab > INT32_MAX / 2 || g->per_row > INT32_MAX / 2) {
+    if (g->rows > (1 << 22) || g->vocab > (int64_t)kMostSplits * kMostChunks * kSpan || g->per_row > INT32_MAX / 2) {
         return NNOPS_UNSUPPORTED;
     }
     return -1;
 }
 
-template <typename T>
-void launch_log_probs(const LogProbsKern& k, int64_t rows, hipStream_t s)
+template <typename T, int kChunks>
+void launch_chunks(const LogProbsKern& k, int64_t rows, hipStream_t s)
 {
     const dim3 grid((unsigned)(rows * k.splits));
     if (k.top > 0) {
-        NNOPS_LAUNCH((log_probs<T, true>), grid, dim3(256), 0, s, k);
+        NNOPS_LAUNCH((log_probs<T, kChunks, true>), grid, dim3(kThreads), 0, s, k);
     } else {
-        NNOPS_LAUNCH((log_probs<T, false>), grid, dim3(256), 0, s, k);
+        NNOPS_LAUNCH((log_probs<T, kChunks, false>), grid, dim3(kThreads), 0, s, k);
     }
+}
+
+template <typename T>
+void launch_log_probs(const LogProbsKern& k, int chunks, int64_t rows, hipStream_t s)
+{
+    chunks == 1   ? launch_chunks<T, 1>(k, rows, s)
+    : chunks == 2 ? launch_chunks<T, 2>(k, rows, s)
+    : chunks == 4 ? launch_chunks<T, 4>(k, rows, s)
+                  : launch_chunks<T, 8>(k, rows, s);
     if (k.splits > 1) {
-        NNOPS_LAUNCH(log_probs_join<T>, dim3((unsigned)rows), dim3(256), 0, s, k);
+        NNOPS_LAUNCH(log_probs_join<T>, dim3((unsigned)rows), dim3(kThreads), 0, s, k);
     }
 }
 
@@ -519,9 +642,9 @@ extern "C" int nnops_hip_token_log_probs(const NnopsTokenLogProbsArgs* g, void* 
     k.keys = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + a.stats);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (g->f16) {
-        launch_log_probs<_Float16>(k, g->rows, s);
+        launch_log_probs<_Float16>(k, a.chunks, g->rows, s);
     } else {
-        launch_log_probs<float>(k, g->rows, s);
+        launch_log_probs<float>(k, a.chunks, g->rows, s);
     }
     return hipGetLastError() == hipSuccess ? NNOPS_OK : NNOPS_INTERNAL;
 }

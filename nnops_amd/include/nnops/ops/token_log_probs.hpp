@@ -14,7 +14,7 @@ struct TokenLogProbsAttributes {
     int64_t top = 0;            ///< alternatives, 0 to 32
 };
 
-/// inputs:  logits [T, V] (f16 / f32), tokens s32 [T, n] (or [T])
+/// inputs:  logits [T, V] (f16 / f32, V up to 2^21), tokens s32 [T, n] (or [T])
 /// outputs: log_probs f32 of tokens' shape, entropy f32 [T] and, with top > 0,
 ///          top_tokens s32 [T, top], top_log_probs f32 [T, top]
 class TokenLogProbs : public OpBase {

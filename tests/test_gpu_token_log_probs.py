@@ -65,7 +65,8 @@ def _x(seed, rows, vocab, f16, size=3.0):
 
 @pytest.mark.parametrize("f16", [True, False])
 @pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 2), (5, 7), (2, 63), (2, 65), (3, 511), (3, 512), (3, 513), (2, 2047),
-                                        (2, 2048), (2, 2049), (5, 4100), (1, 100003), (3, 50257), (1030, 77), (1500, 2600)])
+                                        (2, 2048), (2, 2049), (5, 4100), (1, 100003), (3, 50257), (1030, 77), (1500, 2600),
+                                        (1, 1 << 21), (513, 32768), (520, 32769)])
 def test_sizes(rows, vocab, f16):
     announce(f"log probs rows={rows} vocab={vocab} f16={f16}")
     x = _x(rows + vocab, rows, vocab, f16)
@@ -91,6 +92,23 @@ def test_orders(order, f16):
         x[1:] += (np.arange(1, rows) % 3)[:, None].astype(x.dtype)
         _check(x, np.array([[0, vocab - 1]] * rows, np.int32), 20)
         _check(x, np.array([[vocab // 2]] * rows, np.int32), 32)
+
+
+@pytest.mark.parametrize("f16", [True, False])
+def test_crowded_groups(f16):
+    """Rows whose large logits lie in the columns of few threads, so that nearly all
+    of these reach any threshold; runs of allowed tokens in a masked vocabulary."""
+    announce(f"log probs crowded f16={f16}")
+    for vocab in (32768, 30000, 131072):
+        x = _x(vocab, 4, vocab, f16, 0.5)
+        i = np.arange(vocab)
+        x[0, i % 4096 < 8 * 160] += 8                    # 10 of 32 groups
+        x[1, i % 4096 >= 4096 - 8 * 400] += 8
+        x[2, :] = -np.inf
+        x[2, 5000:5300] = _x(2, 1, 300, f16)[0]
+        x[3, i % 4096 >= 128] = -np.inf                  # one group
+        for top in (1, 12, 32):
+            _check(x, np.array([[5001]] * 4, np.int32), top)
 
 
 @pytest.mark.parametrize("f16", [True, False])

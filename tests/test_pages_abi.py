@@ -124,6 +124,8 @@ def test_token_log_probs_rules():
         assert op.validate([x, tok], with_(outs, at, new)) == INVALID
     assert op.validate([x, tok], outs[:2]) == INVALID and na.TokenLogProbs().validate([x, tok], outs) == INVALID
     assert op.validate([desc([5, 100], S8), tok], outs) == UNSUPPORTED
+    for vocab, status in ((1 << 21, na.OK), ((1 << 21) + 1, UNSUPPORTED)):
+        assert op.validate([desc([5, vocab], F16), tok], outs) == status
     many = na.TokenLogProbs(top=33)
     assert many.validate([x, tok], [desc(s, d) for s, d in many.output_descs([x, tok])]) == UNSUPPORTED
     assert na.TokenLogProbs(top=-1).validate([x, tok], outs[:2]) == INVALID
@@ -268,7 +270,7 @@ def probs_args(**kw):
 @pytest.mark.parametrize("kw,status", [
     (dict(rows=-1), INVALID), (dict(vocab=-1), INVALID), (dict(per_row=-1), INVALID), (dict(top=-1), INVALID),
     (dict(top=101), INVALID), (dict(top=33), UNSUPPORTED), (dict(vocab=0, top=0), INVALID), (dict(rows=1 << 23), UNSUPPORTED),
-    (dict(ld_logits=99), INVALID), (dict(logits=None), INVALID), (dict(entropy=None), INVALID), (dict(tokens=None), INVALID),
+    (dict(vocab=(1 << 21) + 1, ld_logits=1 << 22), UNSUPPORTED), (dict(ld_logits=99), INVALID), (dict(logits=None), INVALID), (dict(entropy=None), INVALID), (dict(tokens=None), INVALID),
     (dict(log_probs=None), INVALID), (dict(ld_tokens=2), INVALID), (dict(top_tokens=None), INVALID),
     (dict(ld_top_log_probs=3), INVALID), (dict(rows=0), na.OK),
 ])
