@@ -11,11 +11,11 @@
 // of the second product is the same for all, and drops out. f32 rows: (x - r)
 // log2(e), which masks of the type's lowest value do not take out of f32's range.
 //
-// The most probable: the top-th largest of the maxima of 32 groups of 16 lanes is
-// a logit that at least `top` reach, and few more do (of 32768 random ones 31 for
-// 20, 111 for 32): those go into LDS as keys of 64 bits, the logit's bits in an
-// order that whole numbers have, then the token's complement, so that no two are
-// equal, and each counts the keys above it.
+// The most probable: the top-th largest of the maxima of 64 groups of 8 lanes is a
+// logit that at least `top` reach, and few more do (of random ones 64 ln(64 / (64 -
+// top)): 24 for 20, 44 for 32): those go into LDS as keys of 64 bits, the logit's bits
+// in an order that whole numbers have, then the token's complement, so that no two
+// are equal, and each counts the keys above it.
 //
 // Bound: HBM, the logits read once.
 #include <limits>
@@ -28,11 +28,12 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kSpan = 8 * kThreads; // logits that the threads have side by side, 8 each
 constexpr int kMostChunks = 8;      // of those a part
+constexpr int kWaves = kThreads / 64;
 constexpr int kGroups = kThreads / 16;
 constexpr int kMostTop = 32;
 constexpr int kMostSplits = 64;
-constexpr int kRoom = 2048;         // keys above a threshold ...
-constexpr int kKeys = kRoom + kSpan;   // ... and those of a span that are equal to it
+constexpr int kRoom = 2048;         // keys above a threshold, as many of each wave ...
+constexpr int kAllKeys = kRoom + kSpan;   // ... and those of a span that are equal to it
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNone = -std::numeric_limits<float>::infinity();
 
@@ -69,19 +70,6 @@ struct Reference<float> {
     static __device__ __forceinline__ float log_p(float x, float r, float s) { return (x - r) - logf(s); }
 };
 
-__device__ __forceinline__ uint64_t key_of(float x, int token)
-{
-    const uint32_t b = __float_as_uint(x + 0.0f);  // (-0 and 0 are equal)
-    const uint32_t order = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
-    return (uint64_t)order << 32 | ~(uint32_t)token;
-}
-__device__ __forceinline__ float logit_of(uint64_t key)
-{
-    const uint32_t order = (uint32_t)(key >> 32);
-    return __uint_as_float(order ^ (order & 0x80000000u ? 0x80000000u : ~0u));
-}
-__device__ __forceinline__ int token_of(uint64_t key) { return (int)~(uint32_t)key; }
-
 // A lane's value from elsewhere in its 16: step 0 to 3 of a reduction over them.
 template <int kStep>
 __device__ __forceinline__ uint32_t from_row(uint32_t v)
@@ -93,11 +81,11 @@ __device__ __forceinline__ uint32_t from_row(uint32_t v)
     return v;
 #endif
 }
-template <int kStep = 0>
+template <int kStep = 0, int kSteps = 4>
 __device__ __forceinline__ float row_max(float v)
 {
-    if constexpr (kStep < 4) {
-        return row_max<kStep + 1>(fmaxf(v, __uint_as_float(from_row<kStep>(__float_as_uint(v)))));
+    if constexpr (kStep < kSteps) {
+        return row_max<kStep + 1, kSteps>(fmaxf(v, __uint_as_float(from_row<kStep>(__float_as_uint(v)))));
     }
     return v;
 }
@@ -106,6 +94,14 @@ __device__ __forceinline__ float row_sum(float v)
 {
     if constexpr (kStep < 4) {
         return row_sum<kStep + 1>(v + __uint_as_float(from_row<kStep>(__float_as_uint(v))));
+    }
+    return v;
+}
+template <int kStep, int kSteps>
+__device__ __forceinline__ uint32_t row_max(uint32_t v)
+{
+    if constexpr (kStep < kSteps) {
+        return row_max<kStep + 1, kSteps>(max(v, from_row<kStep>(v)));
     }
     return v;
 }
@@ -155,41 +151,86 @@ __device__ __forceinline__ float lane_of(float v, int lane)
 #endif
 }
 
-// The top-th largest of the groups' values (equal ones count each).
-template <typename V>
-__device__ __forceinline__ V top_of(const V (&group)[kGroups], int top)
+// Whole numbers in the order of the values.
+__device__ __forceinline__ uint32_t order_of(float x)
+{
+    const uint32_t b = __float_as_uint(x + 0.0f);  // (-0 and 0 are equal)
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t order)
+{
+    return __uint_as_float(order ^ (order & 0x80000000u ? 0x80000000u : ~0u));
+}
+
+__device__ __forceinline__ uint64_t key_of(float x, int token)
+{
+    return (uint64_t)order_of(x) << 32 | ~(uint32_t)token;
+}
+__device__ __forceinline__ float logit_of(uint64_t key) { return value_of((uint32_t)(key >> 32)); }
+__device__ __forceinline__ int token_of(uint64_t key) { return (int)~(uint32_t)key; }
+
+// The top-th largest of the lanes' numbers, bit by bit down to `last`: the largest
+// that as many reach.
+template <int kLast>
+__device__ __forceinline__ uint32_t top_of_lanes(uint32_t mine, int top)
+{
+    uint32_t least = 0;
+#pragma unroll
+    for (int bit = 31; bit >= kLast; --bit) {
+        const uint32_t more = least | 1u << bit;
+        least = __popcll(__ballot(mine >= more)) >= top ? more : least;
+    }
+    return least;
+}
+
+// Of their values. (f16 values as f32 end in 13 zeros, which order_of turns into ones
+// below 0.)
+template <typename T>
+__device__ __forceinline__ float top_value(float v, int top)
+{
+    constexpr int kLast = sizeof(T) == 2 ? 13 : 0;
+    uint32_t least = top_of_lanes<kLast>(order_of(v), top);
+    if (kLast > 0 && (least & 0x80000000u) == 0) {
+        least |= (1u << kLast) - 1;
+    }
+    return value_of(least);
+}
+
+// The top-th largest of the groups' keys.
+__device__ __forceinline__ uint64_t top_of(const uint64_t (&group)[kGroups], int top)
 {
     const int mine = threadIdx.x % kGroups;
-    const V v = group[mine];
+    const uint64_t v = group[mine];
     int rank = 0;
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
         rank += group[i] > v || (group[i] == v && i < mine);
     }
     const int lane = __builtin_ctzll(__ballot(rank == top - 1));
-    if constexpr (sizeof(V) == 4) {
-        return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
-    } else {
-        return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
-               (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
-    }
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }
 
+template <int kKeys>
 struct Shared {
     uint64_t key[kKeys];
     uint64_t key_group[kGroups];
-    float group[kGroups], s[kGroups], t[kGroups];
+    float group[2 * kGroups], s[kGroups], t[kGroups];
+    uint32_t order_group[2 * kGroups];
+    int count[kWaves];
     int keys, left;
 };
 
 // Of sh.key[0 .. n): one of this thread's and how many are above it; a thread without
-// any has 0 and its own number. More than 64 keys are thinned first: those that reach
-// the top-th of the groups' largest stay. (Where none goes, that group had a single
-// key, or none: there is at most a key a thread.) Every thread calls it.
-__device__ __forceinline__ uint64_t rank_keys(Shared& sh, int n, int top, int& rank)
+// any has 0 and its own number. More keys than threads are thinned first: those that
+// reach the top-th of the groups' largest stay, which is a single one of its group (of
+// 16 and more; keys of 0 all go). Then once by their logits alone. Every thread calls
+// it.
+template <int kKeys>
+__device__ __forceinline__ uint64_t rank_keys(Shared<kKeys>& sh, int n, int top, int& rank)
 {
     const int tid = threadIdx.x;
-    while (n > 64) {
+    while (n > kThreads) {
         uint64_t best = 0;
         for (int i = tid; i < n; i += kThreads) {
             best = sh.key[i] > best ? sh.key[i] : best;
@@ -203,7 +244,7 @@ __device__ __forceinline__ uint64_t rank_keys(Shared& sh, int n, int top, int& r
         }
         __syncthreads();
         uint64_t least = top_of(sh.key_group, top);
-        least = least > 0 ? least : 1;             // (fewer groups than that have any)
+        least = least > 0 ? least : 1;             // (what is 0 is no key)
         for (int i = 0; i < n; i += kThreads) {
             const uint64_t mine = i + tid < n ? sh.key[i + tid] : 0;
             __syncthreads();                       // (what stays goes over keys that were looked at)
@@ -212,12 +253,25 @@ __device__ __forceinline__ uint64_t rank_keys(Shared& sh, int n, int top, int& r
             }
         }
         __syncthreads();
-        const int left = sh.left;
+        n = sh.left;
         __syncthreads();
-        if (left == n) {                           // (see above)
-            break;
+    }
+    if (n > 64) {
+        const uint64_t mine = tid < n ? sh.key[tid] : 0;
+        const uint32_t order = (uint32_t)(mine >> 32), best = row_max<0, 3>(order);
+        if (tid % 8 == 0) {
+            sh.order_group[tid / 8] = best;
         }
-        n = left;
+        if (tid == 0) {
+            sh.left = 0;
+        }
+        __syncthreads();
+        const uint32_t least = top_of_lanes<0>(sh.order_group[tid % 64], top);
+        if (tid < n && order >= least) {
+            sh.key[atomicAdd(&sh.left, 1)] = mine;
+        }
+        __syncthreads();
+        n = sh.left;
     }
     const uint64_t key = tid < n ? sh.key[tid] : 0;
     rank = 0;
@@ -265,16 +319,15 @@ __device__ __forceinline__ Given<T> given(const LogProbsKern& p, int64_t row, in
     }
     return g;
 }
-__device__ __forceinline__ int given_of(int tid) { return kThreads - 1 - tid; }   // (the first threads have keys)
 
-// What a workgroup writes of a whole row; a thread its key, where it is among the top,
-// and its given tokens.
+// What `threads` threads write of a whole row: each its key, where it is among the top,
+// and given tokens (from the last thread on: the first have keys).
 template <typename T>
 __device__ __forceinline__ void write_row(const LogProbsKern& p, int64_t row, const Stats& w, uint64_t key, int rank,
-                                          Given<T> g)
+                                          Given<T> g, int threads)
 {
     typedef Reference<T> Ref;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x % (uint32_t)threads;
     const float nan = __uint_as_float(0x7fc00000u);
     const bool bad = !(w.s < std::numeric_limits<float>::infinity()), none = w.s == 0.0f;
     const auto log_p = [&](float x) { return bad ? nan : none ? kNone : Ref::log_p(x, w.r, w.s); };
@@ -283,12 +336,12 @@ __device__ __forceinline__ void write_row(const LogProbsKern& p, int64_t row, co
         p.top_tokens[row * p.ld_top_tokens + to] = bad ? -1 : token_of(key);
         p.top_log_probs[row * p.ld_top_log_probs + to] = log_p(logit_of(key));
     }
-    if (tid == kThreads - 1) {
+    if (tid == threads - 1) {
         p.entropy[row] = bad ? nan : none ? 0.0f : fmaxf((log2f(w.s) - w.t / w.s) * kLn2, 0.0f);
     }
-    for (int i = given_of(tid); i < p.per_row;) {
+    for (int i = threads - 1 - tid; i < p.per_row;) {
         p.log_probs[row * p.ld_log_probs + i] = g.token < 0 ? 0.0f : g.token < p.vocab ? log_p((float)g.logit) : nan;
-        i += kThreads;
+        i += threads;
         g = given<T>(p, row, i);
     }
 }
@@ -298,7 +351,7 @@ __device__ __forceinline__ void write_row(const LogProbsKern& p, int64_t row, co
 // again: how many there are. At least the `top` largest are among them. Every thread
 // calls it.
 template <typename T>
-__device__ __forceinline__ int many_keys(Shared& sh, const T* x, int begin, int n, float least, int top)
+__device__ __forceinline__ int many_keys(Shared<kAllKeys>& sh, const T* x, int begin, int n, float least, int top)
 {
     const int tid = threadIdx.x;
     __syncthreads();
@@ -359,13 +412,13 @@ template <typename T, int kChunks, bool kTop>
 __global__ __launch_bounds__(kThreads, 4) void log_probs(const LogProbsKern p)
 {
     typedef Reference<T> Ref;
-    __shared__ Shared sh;
+    __shared__ Shared<kTop ? kAllKeys : 1> sh;
     const int tid = threadIdx.x;
     const int64_t row = blockIdx.x / (uint32_t)p.splits;
     const int split = (int)(blockIdx.x - (uint32_t)row * p.splits);
     const int begin = split * p.part, n = min(p.part, p.vocab - begin);
     const T* x = static_cast<const T*>(p.x) + row * p.ld_x + begin;
-    const Given<T> g = p.splits == 1 ? given<T>(p, row, given_of(tid)) : Given<T>{};
+    const Given<T> g = p.splits == 1 ? given<T>(p, row, kThreads - 1 - tid) : Given<T>{};
     T v[kChunks][8];
     float high[kChunks], best = kNone;
 #pragma unroll
@@ -395,16 +448,14 @@ __global__ __launch_bounds__(kThreads, 4) void log_probs(const LogProbsKern p)
         high[j] = max_of(v[j]);
         best = fmaxf(best, high[j]);
     }
-    best = row_max(best);
-    if (tid % 16 == 0) {
-        sh.group[tid / 16] = best;
-    }
-    if (tid == 0) {
-        sh.keys = 0;
+    best = row_max<0, 3>(best);
+    if (tid % 8 == 0) {
+        sh.group[tid / 8] = best;
     }
     __syncthreads();
-    float m = row_max(sh.group[tid % kGroups]);
-    m = fmaxf(lane_of(m, 0), lane_of(m, 16));
+    const float group = sh.group[tid % 64], high_row = row_max(group);
+    const float m = fmaxf(fmaxf(lane_of(high_row, 0), lane_of(high_row, 16)),
+                          fmaxf(lane_of(high_row, 32), lane_of(high_row, 48)));
     const float r = Ref::of(fmaxf(m, Ref::kLeast));
     // (each phase converts f16 logits anew: kept as f32 they would take the registers of
     // another workgroup)
@@ -422,22 +473,31 @@ __global__ __launch_bounds__(kThreads, 4) void log_probs(const LogProbsKern p)
     forget();
     float least = kNone;
     if constexpr (kTop) {
-        least = top_of(sh.group, p.top);
+        // (the top-th of the maxima of 64 groups of 8 lanes)
+        least = top_value<T>(group, p.top);
         const T reach = (T)least;                  // (one of the logits: exact)
+        uint64_t* const room = sh.key + kRoom + tid / 64 * (kRoom / kWaves);
+        int count = least > kNone ? 0 : kRoom;     // (-inf: what is behind the row reaches it too)
 #pragma unroll
         for (int j = 0; j < kChunks; ++j) {
-            if (j * kSpan < n && __any(high[j] >= least)) {
+            if (j * kSpan < n && least > kNone && __any(high[j] >= least)) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const int at = j * kSpan + 8 * tid + e;
-                    if (v[j][e] >= reach && at < n) {
-                        const int to = atomicAdd(&sh.keys, 1);
-                        if (to < kRoom) {
-                            sh.key[to] = key_of((float)v[j][e], begin + at);
+                    const bool in = v[j][e] >= reach;
+                    const uint64_t mask = __ballot(in);
+                    if (mask != 0) {
+                        const int to = count + (int)__builtin_amdgcn_mbcnt_hi(
+                                                   (uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+                        if (in && to < kRoom / kWaves) {
+                            room[to] = key_of((float)v[j][e], begin + j * kSpan + 8 * tid + e);
                         }
+                        count += __popcll(mask);
                     }
                 }
             }
+        }
+        if (tid % 64 == 0) {
+            sh.count[tid / 64] = count;
         }
     }
     forget();
@@ -466,14 +526,23 @@ __global__ __launch_bounds__(kThreads, 4) void log_probs(const LogProbsKern p)
     uint64_t key = 0;
     int rank = tid;
     if constexpr (kTop) {
-        int keys = sh.keys;
-        if (keys > kRoom) {
+        int keys = 0, most = 0;
+        for (int i = 0; i < kWaves; ++i) {
+            const int count = sh.count[i];
+            for (int at = tid; at < min(count, kRoom / kWaves); at += kThreads) {
+                sh.key[keys + at] = sh.key[kRoom + i * (kRoom / kWaves) + at];
+            }
+            keys += count;
+            most = max(most, count);
+        }
+        __syncthreads();
+        if (most > kRoom / kWaves) {
             keys = many_keys(sh, x, begin, n, least, p.top);
         }
         key = rank_keys(sh, keys, p.top, rank);
     }
     if (p.splits == 1) {
-        write_row<T>(p, row, w, key, rank, g);
+        write_row<T>(p, row, w, key, rank, g, kThreads);
         return;
     }
     if (tid == 0) {
@@ -506,23 +575,32 @@ __device__ __forceinline__ Stats join_splits(const LogProbsKern& p, int64_t row)
     return sum;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void log_probs_join(const LogProbsKern p)
+// (Without alternatives a wave has a row, and a workgroup eight.)
+template <typename T, bool kTop>
+__global__ __launch_bounds__(kThreads) void log_probs_join(const LogProbsKern p, int64_t rows)
 {
-    __shared__ Shared sh;
     const int tid = threadIdx.x;
-    const int64_t row = blockIdx.x;
-    const Given<T> g = given<T>(p, row, given_of(tid));
-    const int all = p.splits * p.top;              // at most 2048
-    for (int i = tid; i < all; i += kThreads) {
-        sh.key[i] = p.keys[row * all + i];
+    if constexpr (kTop) {
+        __shared__ Shared<kMostSplits * kMostTop> sh;
+        const int64_t row = blockIdx.x;
+        const Given<T> g = given<T>(p, row, kThreads - 1 - tid);
+        const int all = p.splits * p.top;
+        for (int i = tid; i < all; i += kThreads) {
+            sh.key[i] = p.keys[row * all + i];
+        }
+        const Stats sum = join_splits<T>(p, row);
+        __syncthreads();
+        int rank;
+        const uint64_t key = rank_keys(sh, all, p.top, rank);
+        // (a row that is not bad has `top` keys that are not 0)
+        write_row<T>(p, row, sum, key, key != 0 ? rank : kMostTop, g, kThreads);
+    } else {
+        const int64_t row = (int64_t)blockIdx.x * kWaves + tid / 64;
+        if (row < rows) {
+            const Given<T> g = given<T>(p, row, 63 - tid % 64);
+            write_row<T>(p, row, join_splits<T>(p, row), 0, kMostTop, g, 64);
+        }
     }
-    const Stats sum = join_splits<T>(p, row);
-    __syncthreads();
-    int rank;
-    const uint64_t key = rank_keys(sh, all, p.top, rank);
-    // (a row that is not bad has `top` keys that are not 0)
-    write_row<T>(p, row, sum, key, key != 0 ? rank : kMostTop, g);
 }
 
 struct LogProbsPlan {
@@ -530,14 +608,18 @@ struct LogProbsPlan {
     size_t stats, workspace;
 };
 
-// A workgroup's spans: as many as leave 512 workgroups.
+// A row that a workgroup can hold is not split (one launch; us, split / not, 10
+// alternatives: 1 x 32000 8.1 / 6.5, 64 x 32000 8.1 / 6.7, 200 x 32000 10.8 / 7.6). Longer
+// ones: the largest parts that leave 256 workgroups (that / 512 / 1024: 1 x 131072 8.4
+// / 8.2 / 8.2, 64 x 151000 13.3 / 14.0 / 15.0, 128 x 131072 14.8 / 14.9 / 16.8, 300 x
+// 131072 22.1 / 22.1 / 22.0).
 LogProbsPlan log_probs_plan(const NnopsTokenLogProbsArgs* g)
 {
     LogProbsPlan a{};
     const auto parts = [&](int64_t chunks) { return (g->vocab + chunks * kSpan - 1) / (chunks * kSpan); };
     a.chunks = kMostChunks;
-    while (a.chunks > 1 && parts(a.chunks / 2) <= kMostSplits &&
-           (parts(a.chunks / 2) == parts(a.chunks) || g->rows * parts(a.chunks) < 512)) {
+    while (a.chunks > 1 && (parts(a.chunks) == 1 ? parts(a.chunks / 2) == 1
+                                                 : parts(a.chunks / 2) <= kMostSplits && g->rows * parts(a.chunks) < 256)) {
         a.chunks /= 2;
     }
     const int64_t splits = parts(a.chunks), part = ((g->vocab + splits - 1) / splits + 7) / 8 * 8;
@@ -589,7 +671,12 @@ void launch_log_probs(const LogProbsKern& k, int chunks, int64_t rows, hipStream
     : chunks == 4 ? launch_chunks<T, 4>(k, rows, s)
                   : launch_chunks<T, 8>(k, rows, s);
     if (k.splits > 1) {
-        NNOPS_LAUNCH(log_probs_join<T>, dim3((unsigned)rows), dim3(kThreads), 0, s, k);
+        if (k.top > 0) {
+            NNOPS_LAUNCH((log_probs_join<T, true>), dim3((unsigned)rows), dim3(kThreads), 0, s, k, rows);
+        } else {
+            const unsigned blocks = (unsigned)((rows + kWaves - 1) / kWaves);
+            NNOPS_LAUNCH((log_probs_join<T, false>), dim3(blocks), dim3(kThreads), 0, s, k, rows);
+        }
     }
 }
 

@@ -151,6 +151,9 @@ def test_nan_and_infinity(f16):
         got = _check(x, np.array([[0, 3]] * 7, np.int32), 4)
         assert (got[2][[1, 2, 3, 4, 5]] == -1).all() and np.isfinite(got[3][[0, 6]]).all()
         _check(x, np.array([[0, 3]] * 7, np.int32), 0)
+        _check(x, np.array([[0, 3]] * 7, np.int32), 32)
+    x = np.full((1, 200000), np.nan, np.float16 if f16 else np.float32)
+    assert (_check(x, np.array([[0]], np.int32), 32)[2] == -1).all()
 
 
 def test_large_values():
