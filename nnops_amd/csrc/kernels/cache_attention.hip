@@ -24,7 +24,7 @@ __device__ __forceinline__ int splits_of(const AttnKern& p, int token, int qh)
     }
     RowTile rt;
     rt.seq = seq_rows(c, b);
-    const int chunk = chunk_of<kWhole>(p, rt.seq);
+    const int chunk = chunk_of(p, rt.seq);
     const int tok = token - rt.seq.start;
     if (tok < 0 || tok >= rt.seq.n) {
         return 0;

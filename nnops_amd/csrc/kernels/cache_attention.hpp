@@ -52,10 +52,14 @@ struct AttnKern {
     int32_t whole;        // tiles of the longest sequence up to which none is split
     int32_t chunk;        // tiles of a split where that sequence fills the table
     // kShared and kOwn
-    const PrefixPlan* plan;
-    const GroupPlan* group_plan;
-    const MemberPlan* members;
-    int32_t groups, first_part;
+    PrefixPlan* plan;     // workspace, as are the next two: written before these launches, or
+    GroupPlan* group_plan;   // (`few`) found by each wave, and written by one for the join
+    MemberPlan* members;
+    const int32_t* group_starts;
+    const int32_t* shared;
+    int32_t groups, first_part, few;
+    int32_t shared_splits;       // as splits and by_splits, of the tokens that groups share
+    uint32_t by_shared_splits;
 };
 
 // The tiles of 64 tokens that rows at positions pmin .. pmax look at: the
@@ -115,6 +119,17 @@ __device__ __forceinline__ int wave_max(int v)
 #endif
 }
 
+// Tiles of a split where the longest sequence (of shared tokens, or of what is behind
+// them) has so many: see chunk_of.
+__device__ __forceinline__ int chunk_for(int tiles, int splits, uint32_t by_splits, int whole)
+{
+    if (splits == 1) {
+        return std::numeric_limits<int>::max();
+    }
+    const uint32_t share = __umulhi((uint32_t)(tiles + splits - 1), by_splits);
+    return tiles <= whole ? whole : max((int)((share + 3u) & ~3u), 4);
+}
+
 // Tiles of tokens that a split takes: the longest sequence that has rows is
 // divided among the splits, whatever the page table has room for (one as wide as
 // a model's context, as a captured graph needs: one token over 2048, 64 splits of
@@ -125,12 +140,8 @@ __device__ __forceinline__ int wave_max(int v)
 // than there are.)
 //   own: any sequence (in flight, beside the others). `longest`, of a lane: among
 // the sequences before the from-th, which were looked at already.
-template <AttnMode M>
 __device__ __forceinline__ int chunk_of(const AttnKern& p, const SeqRows& own, int longest = 0, int from = 0)
 {
-    if constexpr (M != kWhole) {
-        return M == kShared ? p.plan->shared_chunk : p.plan->own_chunk;
-    }
     if (p.splits == 1) {
         return std::numeric_limits<int>::max();
     }
@@ -156,7 +167,7 @@ __device__ __forceinline__ int chunk_of(const AttnKern& p, const SeqRows& own, i
 }
 
 template <AttnMode M>
-__device__ __forceinline__ void place_tile(const AttnKern& p, int rt, int chunk, RowTile& t)
+__device__ __forceinline__ void place_tile(const AttnKern& p, int rt, int chunk, RowTile& t, int skip = 0)
 {
     const uint32_t group = p.group;
     t.row0 = rt * p.tile_rows;
@@ -170,23 +181,73 @@ __device__ __forceinline__ void place_tile(const AttnKern& p, int rt, int chunk,
         t.pmin = t.pmax = tokens - 1;
         t.span = Span{0, 0, tokens / kTile};
     } else if constexpr (M == kOwn) {
-        const int skip = p.members[t.b].skip;      // (no row's position lies before)
-        t.span = Span{0, skip, max(t.span.tiles - skip, 0)};
+        t.span = Span{0, skip, max(t.span.tiles - skip, 0)};   // (no row's position lies before)
     }
     t.chunk = chunk;
     t.split = t.span.tiles > chunk;
 }
 
-// A sequence of the launch.
-template <AttnMode M>
-__device__ __forceinline__ SeqRows seq_at(const AttnKern& p, int b)
+// The plan of a call of up to 64 sequences and 8 groups, as every wave finds it: lane
+// g has group g, lane b sequence b.
+constexpr int kFewGroups = 8;
+struct FewPlan {
+    SeqRows seq;
+    GroupPlan of_group;
+    MemberPlan member;
+    int shared_chunk, own_chunk;
+};
+
+// What a group shares: whole tiles and whole pages that its first sequence has and
+// every row sees.
+__device__ __forceinline__ int shared_tokens(const Paged& c, int shared, int len, int least)
 {
-    if constexpr (M == kShared) {
-        const GroupPlan g = p.group_plan[b];
-        return SeqRows{g.start, g.tokens > 0 ? g.rows : 0, g.tokens};
-    } else {
-        return seq_rows(p.c, b);
+    return max(min(min(shared, len), least), 0) & ~(max(c.page, kTile) - 1);
+}
+
+__device__ __forceinline__ FewPlan few_plan(const AttnKern& p)
+{
+    const Paged& c = p.c;
+    const int lane = threadIdx.x % 64;
+    constexpr int kBig = std::numeric_limits<int>::max();
+    FewPlan f{};
+    if (lane < c.seqs) {
+        f.seq = seq_rows(c, lane);
     }
+    int starts = p.groups > 0 ? min(max(p.group_starts[min(lane, p.groups)], 0), c.seqs) : 0;
+    const int shared = lane < p.groups ? p.shared[lane] : 0;
+#pragma unroll
+    for (int m = 1; m <= kFewGroups; m *= 2) {     // (starts do not go back)
+        const int before = __shfl_up(starts, m);
+        starts = lane >= m ? max(starts, before) : starts;
+    }
+    f.member = MemberPlan{-1, 0};
+    int longest = 0;
+    for (int g = 0; g < p.groups; ++g) {
+        const int b0 = __builtin_amdgcn_readlane(starts, g), b1 = __builtin_amdgcn_readlane(starts, g + 1);
+        const bool in = lane >= b0 && lane < b1;
+        const uint64_t rows = __ballot(in && f.seq.n > 0);
+        GroupPlan plan{0, 0, 0, b0};
+        if (rows != 0) {
+            const int first = __builtin_ctzll(rows), last = 63 - __builtin_clzll(rows);
+            const int sees = max(f.seq.len - f.seq.n + 1, 0);
+            const int least = kBig - wave_max(in && f.seq.n > 0 ? kBig - sees : 0);
+            plan.start = __builtin_amdgcn_readlane(f.seq.start, first);
+            plan.rows = max(__builtin_amdgcn_readlane(f.seq.start + f.seq.n, last) - plan.start, 0);
+            plan.tokens = shared_tokens(c, __builtin_amdgcn_readlane(shared, g),
+                                        __builtin_amdgcn_readlane(f.seq.len, b0), least);
+        }
+        longest = max(longest, plan.tokens);
+        if (lane == g) {
+            f.of_group = plan;
+        }
+        if (in) {
+            f.member = MemberPlan{g, plan.tokens / kTile};
+        }
+    }
+    const int own = wave_max(f.seq.n > 0 ? f.seq.len - kTile * f.member.skip : 0);
+    f.shared_chunk = chunk_for(longest / kTile, p.shared_splits, p.by_shared_splits, 4);
+    f.own_chunk = chunk_for(min((own + kTile - 1) / kTile, p.tiles), p.splits, p.by_splits, p.whole);
+    return f;
 }
 
 // The item-th tile. Later tiles of a sequence look at more tokens: `from_last`
@@ -196,6 +257,26 @@ __device__ __forceinline__ bool find_tile(const AttnKern& p, uint32_t item, bool
 {
     int rt, chunk;
     const int seqs = M == kShared ? p.groups : p.c.seqs;
+    FewPlan few{};
+    if (M != kWhole && p.few) {
+        few = few_plan(p);
+        if (M == kOwn && item == 0 && blockIdx.y == 0 && threadIdx.x < 64 && (int)threadIdx.x < p.c.seqs) {
+            // (what the join needs; by the first workgroup of each KV head, all the same)
+            p.members[threadIdx.x] = few.member;
+            *p.plan = PrefixPlan{few.shared_chunk, few.own_chunk};
+        }
+    }
+    const auto at = [&](int b) {
+        if constexpr (M == kShared) {
+            GroupPlan g = few.of_group;            // (few: asked by lane b)
+            if (!p.few) {
+                g = p.group_plan[b];
+            }
+            return SeqRows{g.start, g.tokens > 0 ? g.rows : 0, g.tokens};
+        } else {
+            return seq_rows(p.c, b);
+        }
+    };
     if (p.per_seq > 0) {
         if (from_last) {
             const uint32_t back = item / (uint32_t)seqs;
@@ -205,28 +286,45 @@ __device__ __forceinline__ bool find_tile(const AttnKern& p, uint32_t item, bool
             t.b = (int)(item / (uint32_t)p.per_seq);
             rt = (int)(item - (uint32_t)t.b * p.per_seq);
         }
-        t.seq = seq_at<M>(p, t.b);
-        if (M == kShared && rt * p.tile_rows >= t.seq.n * p.group) {
-            return false;                          // (one group: it may have fewer rows than the call)
+        t.seq = at(t.b);
+        if constexpr (M == kShared) {              // one group, which may have fewer rows than the call
+            t.seq.start = __builtin_amdgcn_readfirstlane(t.seq.start);
+            t.seq.n = __builtin_amdgcn_readfirstlane(t.seq.n);
+            t.seq.len = __builtin_amdgcn_readfirstlane(t.seq.len);
+            if (rt * p.tile_rows >= t.seq.n * p.group) {
+                return false;
+            }
         }
-        chunk = chunk_of<M>(p, t.seq);
+        chunk = M == kWhole ? chunk_of(p, t.seq) : 0;
     } else {
         int longest = 0;
         const auto count = [&](const SeqRows& s) {
             longest = s.n > 0 ? max(longest, s.len) : longest;
             return (int)((uint32_t)(s.n * p.group + p.tile_rows - 1) / (uint32_t)p.tile_rows);
         };
-        const auto at = [&](int b) { return seq_at<M>(p, b); };
         if (!find_item(seqs, item, at, count, t.b, rt, t.seq)) {
             return false;
         }
-        chunk = chunk_of<M>(p, t.seq, longest, (t.b / 64 + 1) * 64);
+        chunk = M == kWhole ? chunk_of(p, t.seq, longest, (t.b / 64 + 1) * 64) : 0;
         rt = from_last ? count(t.seq) - 1 - rt : rt;
     }
-    place_tile<M>(p, rt, chunk, t);
+    int skip = 0;
     if constexpr (M == kShared) {
-        t.table = p.group_plan[t.b].table;
+        chunk = few.shared_chunk;
+        t.table = __builtin_amdgcn_readlane(few.of_group.table, t.b);
+        if (!p.few) {
+            chunk = p.plan->shared_chunk;
+            t.table = p.group_plan[t.b].table;
+        }
+    } else if constexpr (M == kOwn) {
+        chunk = few.own_chunk;
+        skip = __builtin_amdgcn_readlane(few.member.skip, t.b);
+        if (!p.few) {
+            chunk = p.plan->own_chunk;
+            skip = p.members[t.b].skip;
+        }
     }
+    place_tile<M>(p, rt, chunk, t, skip);
     return true;
 }
 

@@ -42,19 +42,23 @@ namespace {
 
 constexpr int kRows = 16;           // rows of a wave
 
+// What the waves of a workgroup join.
+template <int DP>
+struct WaveParts {
+    float o[4][kRows][DP + 4];
+    float m[4][kRows], l[4][kRows];
+};
+
 template <typename T, int DP, AttnMode M>
-__global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void attention_rows16(const AttnKern p)
+__device__ __forceinline__ void attend_rows16(const AttnKern& p, WaveParts<DP>& sh, uint32_t block, int split)
 {
     constexpr int kC = DP / 64;                    // 64-channel pieces of a key
     constexpr int kT = DP / 16;                    // 16-channel tiles of O
     typedef Operand<T> Op;
     constexpr int kWeights = Op::kParts == 1 ? 2 : Op::kParts;   // parts of a probability
-    constexpr int kPitch = DP + 4;
-    __shared__ float s_o[4][kRows][kPitch];
-    __shared__ float s_m[4][kRows], s_l[4][kRows];
     const Paged& c = p.c;
-    const uint32_t item = blockIdx.x / (uint32_t)c.heads;
-    const int kvh = (int)(blockIdx.x - item * c.heads);
+    const uint32_t item = block / (uint32_t)c.heads;
+    const int kvh = (int)(block - item * c.heads);
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int n = lane % 16, g = lane / 16;
     const int kb = n / 4;                          // the token group of a lane's keys
@@ -66,7 +70,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void at
     int kid = 0, vid = 0;
     if (early) {
         const int32_t* row = c.table + (int64_t)(item / (uint32_t)p.per_seq) * c.ld_table;
-        const int base = kTile * ((int)blockIdx.y * p.chunk + wave), last = c.table_pages - 1;
+        const int base = kTile * (split * p.chunk + wave), last = c.table_pages - 1;
         kid = row[min((base + 16 * kb) >> c.page_log2, last)];
         vid = row[min((base + 16 * g) >> c.page_log2, last)];
     }
@@ -80,7 +84,6 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void at
     const int row0 = rt.row0, rows = rt.rows;
     const int tok_last = M == kShared ? (int)((uint32_t)(min(row0 + kRows, rows) - 1) / (uint32_t)p.group)
                                       : pmax - (seq.len - seq.n);
-    const int split = blockIdx.y;
     const int v0 = split * rt.chunk;
     if (split > 0 && v0 >= span.tiles) {
         return;
@@ -268,12 +271,12 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void at
     l_run += __shfl_xor(l_run, 16);
     l_run += __shfl_xor(l_run, 32);
     if (g == 0) {
-        s_m[wave][n] = m_run;
-        s_l[wave][n] = l_run;
+        sh.m[wave][n] = m_run;
+        sh.l[wave][n] = l_run;
     }
 #pragma unroll
     for (int t = 0; t < kT; ++t) {
-        *reinterpret_cast<v4f*>(&s_o[wave][n][16 * t + 4 * g]) = o[t];
+        *reinterpret_cast<v4f*>(&sh.o[wave][n][16 * t + 4 * g]) = o[t];
     }
     __syncthreads();
     // 16 threads a row, 4 channels each at a time
@@ -281,13 +284,13 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void at
     if (row0 + r >= rows) {
         return;
     }
-    const float m = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+    const float m = fmaxf(fmaxf(sh.m[0][r], sh.m[1][r]), fmaxf(sh.m[2][r], sh.m[3][r]));
     float f[4], l = 0.0f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
         // a wave that saw nothing has m = -inf and nothing to add
-        f[w] = s_m[w][r] < m ? __builtin_amdgcn_exp2f(s_m[w][r] - m) : 1.0f;
-        l += f[w] * s_l[w][r];
+        f[w] = sh.m[w][r] < m ? __builtin_amdgcn_exp2f(sh.m[w][r] - m) : 1.0f;
+        l += f[w] * sh.l[w][r];
     }
     const int rtok = (int)((uint32_t)(row0 + r) / (uint32_t)p.group);
     const int64_t token = seq.start + rtok;
@@ -304,7 +307,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void at
         v4f sum = v4f{0, 0, 0, 0};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            sum += f[w] * *reinterpret_cast<const v4f*>(&s_o[w][r][ch]);
+            sum += f[w] * *reinterpret_cast<const v4f*>(&sh.o[w][r][ch]);
         }
         if (parts) {
             *reinterpret_cast<v4f*>(&p.part[at_part * d + ch]) = sum;
@@ -321,6 +324,13 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void at
         p.part_ml[2 * at_part] = m;
         p.part_ml[2 * at_part + 1] = l;
     }
+}
+
+template <typename T, int DP, AttnMode M>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void attention_rows16(const AttnKern p)
+{
+    __shared__ WaveParts<DP> sh;
+    attend_rows16<T, DP, M>(p, sh, blockIdx.x, blockIdx.y);
 }
 
 }  // namespace

@@ -20,12 +20,8 @@ namespace {
 constexpr int kPlanThreads = 1024;
 
 struct PrefixKern {
-    AttnKern own;         // (its plan, group_plan and members are written)
-    const int32_t* group_starts;
-    const int32_t* shared;
+    AttnKern own;
     int32_t* starts;      // workspace: group_starts, in order and in range
-    int32_t shared_splits;
-    uint32_t by_shared_splits;
     int32_t ways;         // of the join: parts of a row that are summed side by side
 };
 
@@ -44,28 +40,17 @@ __device__ __forceinline__ int group_max(int v, int* s_waves)
     return v;
 }
 
-__device__ __forceinline__ int chunk_for(int tiles, int splits, uint32_t by_splits, int whole)
-{
-    if (splits == 1) {
-        return std::numeric_limits<int>::max();
-    }
-    const uint32_t share = __umulhi((uint32_t)(tiles + splits - 1), by_splits);
-    return tiles <= whole ? whole : max((int)((share + 3u) & ~3u), 4);
-}
-
 __global__ __launch_bounds__(kPlanThreads) void prefix_plan(const PrefixKern p)
 {
     __shared__ int s_waves[kPlanThreads / 64];
     const AttnKern& k = p.own;
     const Paged& c = k.c;
-    GroupPlan* const groups = const_cast<GroupPlan*>(k.group_plan);
-    MemberPlan* const members = const_cast<MemberPlan*>(k.members);
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
     // starts that do not go back
     int so_far = 0;
     for (int base = 0; base <= k.groups; base += kPlanThreads) {
         const int g = base + tid;
-        int v = g <= k.groups && k.groups > 0 ? min(max(p.group_starts[g], 0), c.seqs) : 0;
+        int v = g <= k.groups && k.groups > 0 ? min(max(k.group_starts[g], 0), c.seqs) : 0;
 #pragma unroll
         for (int m = 1; m < 64; m *= 2) {
             v = max(v, lane >= m ? __shfl_up(v, m) : 0);
@@ -85,11 +70,10 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan(const PrefixKern p)
         }
     }
     for (int b = tid; b < c.seqs; b += kPlanThreads) {
-        members[b] = MemberPlan{-1, 0};
+        k.members[b] = MemberPlan{-1, 0};
     }
     __syncthreads();
     int longest = 0;
-    const int whole_pages = max(c.page, kTile) - 1;
     for (int g = wave; g < k.groups; g += kPlanThreads / 64) {
         const int b0 = p.starts[g], b1 = p.starts[g + 1];
         GroupPlan plan{0, 0, 0, b0};
@@ -113,28 +97,27 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan(const PrefixKern p)
         if (first < last) {
             plan.start = first;
             plan.rows = last - first;
-            plan.tokens = max(min(min(p.shared[g], len), least), 0) & ~whole_pages;
+            plan.tokens = shared_tokens(c, k.shared[g], len, least);
         }
         longest = max(longest, plan.tokens);
         if (lane == 0) {
-            groups[g] = plan;
+            k.group_plan[g] = plan;
         }
         for (int b = b0 + lane; b < b1; b += 64) {
-            members[b] = MemberPlan{g, plan.tokens / kTile};
+            k.members[b] = MemberPlan{g, plan.tokens / kTile};
         }
     }
     __syncthreads();
     int own = 0;
     for (int b = tid; b < c.seqs; b += kPlanThreads) {
         const SeqRows s = seq_rows(c, b);
-        own = s.n > 0 ? max(own, s.len - kTile * members[b].skip) : own;
+        own = s.n > 0 ? max(own, s.len - kTile * k.members[b].skip) : own;
     }
     longest = group_max(longest, s_waves);
     own = group_max(own, s_waves);
     if (tid == 0) {
-        PrefixPlan* const plan = const_cast<PrefixPlan*>(k.plan);
-        plan->shared_chunk = chunk_for(longest / kTile, p.shared_splits, p.by_shared_splits, 4);
-        plan->own_chunk = chunk_for(min((own + kTile - 1) / kTile, k.tiles), k.splits, k.by_splits, k.whole);
+        *k.plan = PrefixPlan{chunk_for(longest / kTile, k.shared_splits, k.by_shared_splits, 4),
+                             chunk_for(min((own + kTile - 1) / kTile, k.tiles), k.splits, k.by_splits, k.whole)};
     }
 }
 
@@ -170,8 +153,9 @@ __global__ __launch_bounds__(256) void prefix_join(const PrefixKern p)
     if (live) {
         const uint32_t row = (uint32_t)(tok * k.group) + (uint32_t)qh % (uint32_t)k.group;
         const int own_chunk = k.plan->own_chunk, shared_chunk = k.plan->shared_chunk;
-        place_tile<kOwn>(k, (int)(row / (uint32_t)k.tile_rows), own_chunk, rt);
-        shared = (int)(((uint32_t)k.members[rt.b].skip + (uint32_t)shared_chunk - 1) / (uint32_t)shared_chunk);
+        const int skip = k.members[rt.b].skip;
+        place_tile<kOwn>(k, (int)(row / (uint32_t)k.tile_rows), own_chunk, rt, skip);
+        shared = (int)(((uint32_t)skip + (uint32_t)shared_chunk - 1) / (uint32_t)shared_chunk);
         own = (int)(((uint32_t)rt.span.tiles + (uint32_t)own_chunk - 1) / (uint32_t)own_chunk);
     }
     const int parts = shared + own, d = c.d, ch = threadIdx.x % (uint32_t)lanes * 4;
@@ -300,15 +284,24 @@ SharedPlan shared_plan(const NnopsPrefixAttentionArgs* g)
         a.items = (g->rows * group / a.tile_rows + (groups < g->rows ? groups : g->rows)) * heads;
     }
     const int64_t tiles = g->cache.table_pages * g->cache.page_tokens / kTile;
-    int64_t splits = ((rows > 0 ? 256 : 512) + a.items - 1) / a.items;
-    const int64_t most = (tiles + 3) / 4;
-    splits = splits < most ? splits : most;
-    a.splits = (int32_t)(splits > 1 ? splits : 1);
+    // Splits by rounds of the chip's workgroups: a round takes its tiles of tokens and
+    // about `extra` tiles' time to begin, and to write its parts.
+    const int64_t chip = rows > 0 ? 256 : 512, extra = 5;
+    const int64_t most = (tiles + 3) / 4 < 4 * chip / a.items + 1 ? (tiles + 3) / 4 : 4 * chip / a.items + 1;
+    a.splits = 1;
+    int64_t best = INT64_MAX;
+    for (int64_t n = 1; n <= most; ++n) {
+        const int64_t cost = (a.items * n + chip - 1) / chip * ((tiles + n - 1) / n + extra);
+        if (cost < best) {
+            best = cost;
+            a.splits = (int32_t)n;
+        }
+    }
     const int64_t parts = a.splits + a.own.splits;
     // workgroups to fill the chip, as long as each lane has a batch of parts
     const int lanes = join_lanes((int)d);
     a.ways = 1;
-    while (a.ways < 256 / lanes && 4 * a.ways < parts && g->rows * g->q_heads * a.ways * lanes < 512 * 256) {
+    while (a.ways < 256 / lanes && 4 * a.ways < parts && g->rows * g->q_heads * a.ways * lanes < 2048 * 256) {
         a.ways *= 2;
     }
     a.groups_at = 16;
@@ -359,18 +352,49 @@ void launch_part(const AttnKern& k, const dim3& grid, hipStream_t s)
 
 uint32_t reciprocal(int n) { return n > 1 ? (uint32_t)(((1ull << 32) + n - 1) / n) : 0; }
 
+// Shared and own tokens in one launch, where both take 16 rows a workgroup: the first
+// `shared` workgroups, `items` a split, and those behind them.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void attention_both16(
+    const AttnKern s, const AttnKern o, uint32_t items, uint32_t shared, uint32_t own_items)
+{
+    __shared__ WaveParts<DP> sh;
+    if (blockIdx.x < shared) {
+        const uint32_t split = blockIdx.x / items;
+        attend_rows16<T, DP, kShared>(s, sh, blockIdx.x - split * items, (int)split);
+    } else {
+        const uint32_t block = blockIdx.x - shared, split = block / own_items;
+        attend_rows16<T, DP, kOwn>(o, sh, block - split * own_items, (int)split);
+    }
+}
+
 template <typename T>
 void launch_prefix(const PrefixKern& p, const SharedPlan& a, hipStream_t s)
 {
-    NNOPS_LAUNCH(prefix_plan, dim3(1), dim3(kPlanThreads), 0, s, p);
-    AttnKern k = p.own;
-    if (k.groups > 0) {
-        k.tile_rows = a.tile_rows;
-        k.per_seq = a.per_seq;
-        k.first_part = 0;
-        launch_part<T, kShared>(k, dim3((unsigned)a.items, (unsigned)a.splits), s);
+    if (!p.own.few) {
+        NNOPS_LAUNCH(prefix_plan, dim3(1), dim3(kPlanThreads), 0, s, p);
     }
-    launch_part<T, kOwn>(p.own, dim3((unsigned)a.own.items, (unsigned)a.own.splits), s);
+    AttnKern k = p.own;
+    k.tile_rows = a.tile_rows;
+    k.per_seq = a.per_seq;
+    k.first_part = 0;
+    const uint32_t shared = k.groups > 0 ? (uint32_t)(a.items * a.splits) : 0, own = (uint32_t)(a.own.items * a.own.splits);
+    if (a.tile_rows == kRows && p.own.tile_rows == kRows) {
+        const dim3 grid(shared + own);
+        const uint32_t items = (uint32_t)a.items, own_items = (uint32_t)a.own.items;
+        if (k.c.d <= 64) {
+            NNOPS_LAUNCH((attention_both16<T, 64>), grid, dim3(256), 0, s, k, p.own, items, shared, own_items);
+        } else if (k.c.d <= 128) {
+            NNOPS_LAUNCH((attention_both16<T, 128>), grid, dim3(256), 0, s, k, p.own, items, shared, own_items);
+        } else {
+            NNOPS_LAUNCH((attention_both16<T, 256>), grid, dim3(256), 0, s, k, p.own, items, shared, own_items);
+        }
+    } else {
+        if (shared > 0) {
+            launch_part<T, kShared>(k, dim3((unsigned)a.items, (unsigned)a.splits), s);
+        }
+        launch_part<T, kOwn>(p.own, dim3((unsigned)a.own.items, (unsigned)a.own.splits), s);
+    }
     const int64_t per_block = 256 / join_lanes(k.c.d) / a.ways;
     const int64_t blocks = ((int64_t)k.c.rows * k.q_heads + per_block - 1) / per_block;
     NNOPS_LAUNCH(prefix_join<T>, dim3((unsigned)blocks), dim3(256), 0, s, p);
@@ -402,7 +426,7 @@ extern "C" int nnops_hip_prefix_attention(const NnopsPrefixAttentionArgs* g, voi
         return NNOPS_INVALID_ARGUMENT;
     }
     const SharedPlan a = shared_plan(g);
-    if (a.own.items > INT32_MAX / 512 || a.items > INT32_MAX / 512 || a.own.splits > 65535 || a.splits > 65535 ||
+    if (a.own.items * a.own.splits > INT32_MAX / 512 || a.items * a.splits > INT32_MAX / 512 || a.own.splits > 65535 || a.splits > 65535 ||
         g->rows * g->q_heads > INT32_MAX / 256) {
         return NNOPS_UNSUPPORTED;
     }
@@ -411,11 +435,7 @@ extern "C" int nnops_hip_prefix_attention(const NnopsPrefixAttentionArgs* g, voi
     }
     char* at = static_cast<char*>(workspace);
     PrefixKern p{};
-    p.group_starts = g->group_starts;
-    p.shared = g->shared;
     p.starts = reinterpret_cast<int32_t*>(at + a.starts_at);
-    p.shared_splits = a.splits;
-    p.by_shared_splits = reciprocal(a.splits);
     p.ways = a.ways;
     AttnKern& k = p.own;
     k.c = paged(g->cache, g->rows);
@@ -436,9 +456,14 @@ extern "C" int nnops_hip_prefix_attention(const NnopsPrefixAttentionArgs* g, voi
     k.tiles = a.own.tiles;
     k.whole = a.own.whole;
     k.chunk = a.own.chunk;
-    k.plan = reinterpret_cast<const PrefixPlan*>(at);
-    k.group_plan = reinterpret_cast<const GroupPlan*>(at + a.groups_at);
-    k.members = reinterpret_cast<const MemberPlan*>(at + a.members_at);
+    k.plan = reinterpret_cast<PrefixPlan*>(at);
+    k.group_plan = reinterpret_cast<GroupPlan*>(at + a.groups_at);
+    k.members = reinterpret_cast<MemberPlan*>(at + a.members_at);
+    k.group_starts = g->group_starts;
+    k.shared = g->shared;
+    k.few = g->cache.sequences <= 64 && g->groups <= kFewGroups;
+    k.shared_splits = a.splits;
+    k.by_shared_splits = reciprocal(a.splits);
     k.groups = (int32_t)g->groups;
     k.first_part = a.splits;
     hipStream_t s = static_cast<hipStream_t>(stream);
