@@ -58,6 +58,7 @@ struct AttnKern {
     const int32_t* group_starts;
     const int32_t* shared;
     int32_t groups, first_part, few;
+    int32_t join_here;    // kOwn, unsplit: joins the shared tokens' parts itself
     int32_t shared_splits;       // as splits and by_splits, of the tokens that groups share
     uint32_t by_shared_splits;
 };
@@ -100,6 +101,7 @@ struct RowTile {
     int chunk;                // tiles of tokens that a split takes
     bool split;               // it has more than one
     int table;                // kShared: the sequence whose pages they are
+    int shared_parts;         // kOwn: parts of the tokens that its group shares
 };
 
 // The largest of a wave's values, all 0 or more, as a scalar: along rows of 16
@@ -319,10 +321,13 @@ __device__ __forceinline__ bool find_tile(const AttnKern& p, uint32_t item, bool
     } else if constexpr (M == kOwn) {
         chunk = few.own_chunk;
         skip = __builtin_amdgcn_readlane(few.member.skip, t.b);
+        uint32_t shared_chunk = (uint32_t)few.shared_chunk;
         if (!p.few) {
             chunk = p.plan->own_chunk;
             skip = p.members[t.b].skip;
+            shared_chunk = (uint32_t)p.plan->shared_chunk;
         }
+        t.shared_parts = (int)(((uint32_t)skip + shared_chunk - 1) / shared_chunk);
     }
     place_tile<M>(p, rt, chunk, t, skip);
     return true;

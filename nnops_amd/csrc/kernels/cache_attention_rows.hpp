@@ -49,8 +49,91 @@ struct WaveParts {
     float m[4][kRows], l[4][kRows];
 };
 
+// What the lanes that share a row's parts join.
+struct WayParts {
+    __attribute__((aligned(16))) v4f o[256];
+    float m[16], l[16];
+};
+
+// One part more: M and l of a row, 4 channels of its O.
+__device__ __forceinline__ void join_part(float& m, float& l, v4f& o, float pm, float pl, const v4f& po)
+{
+    const float top = fmaxf(m, pm);
+    // (a part that saw nothing has -inf and nothing to add)
+    const float f = m < top ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
+    const float w = pm < top ? __builtin_amdgcn_exp2f(pm - top) : 1.0f;
+    l = f * l + w * pl;
+    o = f * o + w * po;
+    m = top;
+}
+
+// Every step-th of the parts from first on, of n in all: number s is at part(s).
+template <int kBatch, typename Part>
+__device__ __forceinline__ void join_parts(const AttnKern& p, int64_t at, int ch, int first, int step, int n, Part part,
+                                           float& m, float& l, v4f& o)
+{
+    const int64_t rows = (int64_t)p.c.rows * p.q_heads;
+    for (int s = first; s < n; s += kBatch * step) {
+        float ms[kBatch], ls[kBatch];
+        v4f os[kBatch];
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+            const int i = s + e * step;
+            ms[e] = kNone;
+            ls[e] = 0.0f;
+            os[e] = v4f{0, 0, 0, 0};
+            if (i < n) {
+                const int64_t from = part(i) * rows + at;
+                ms[e] = p.part_ml[2 * from];
+                ls[e] = p.part_ml[2 * from + 1];
+                if (ch < p.c.d) {
+                    os[e] = *reinterpret_cast<const v4f*>(p.part + from * p.c.d + ch);
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+            join_part(m, l, o, ms[e], ls[e], os[e]);
+        }
+    }
+}
+
+// The `ways` neighbouring slots of lanes that have parts of one row: the first of them
+// gets the sum. Every thread of the workgroup calls it.
+__device__ __forceinline__ void join_ways(WayParts& sh, int lanes, int ways, float& m, float& l, v4f& o)
+{
+    const int slot = threadIdx.x / (uint32_t)lanes;
+    if (ways > 1) {
+        sh.o[threadIdx.x] = o;
+        if (threadIdx.x % (uint32_t)lanes == 0) {
+            sh.m[slot] = m;
+            sh.l[slot] = l;
+        }
+        __syncthreads();
+        if (slot % ways == 0) {
+            for (int w = 1; w < ways; ++w) {
+                join_part(m, l, o, sh.m[slot + w], sh.l[slot + w], sh.o[threadIdx.x + w * lanes]);
+            }
+        }
+    }
+}
+
+// 4 channels of a row's result.
+template <typename T>
+__device__ __forceinline__ void write_result(const AttnKern& p, int64_t token, int qh, int ch, float l, const v4f& o)
+{
+    const float f = l == 0.0f ? 0.0f : kDrop / l;
+    T y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        y[e] = (T)(o[e] * f);
+    }
+    __builtin_memcpy(static_cast<T*>(p.out) + token * p.ld_out + (int64_t)qh * p.c.d + ch, y, sizeof y);
+}
+
 template <typename T, int DP, AttnMode M>
-__device__ __forceinline__ void attend_rows16(const AttnKern& p, WaveParts<DP>& sh, uint32_t block, int split)
+__device__ __forceinline__ void attend_rows16(const AttnKern& p, WaveParts<DP>& sh, uint32_t block, int split,
+                                              WayParts* join = nullptr)
 {
     constexpr int kC = DP / 64;                    // 64-channel pieces of a key
     constexpr int kT = DP / 16;                    // 16-channel tiles of O
@@ -279,6 +362,37 @@ __device__ __forceinline__ void attend_rows16(const AttnKern& p, WaveParts<DP>& 
         *reinterpret_cast<v4f*>(&sh.o[wave][n][16 * t + 4 * g]) = o[t];
     }
     __syncthreads();
+    if constexpr (M == kOwn) {
+        if (p.join_here) {
+            // the waves' parts and those of the shared tokens, by as many lanes a row as
+            // there are
+            const int lanes = join_lanes(d), slots = 256 / lanes, slot = threadIdx.x / (uint32_t)lanes;
+            const int here = min(kRows, rows - row0), ch = threadIdx.x % (uint32_t)lanes * 4;
+            int ways = 1;
+            while (2 * ways * here <= slots) {
+                ways *= 2;
+            }
+            for (int r0 = 0; r0 < here; r0 += slots / ways) {   // (once, if there is more than one way)
+                const int r = r0 + slot / ways, way = slot % ways;
+                const int at_row = min(row0 + r, rows - 1), t = (int)((uint32_t)at_row / (uint32_t)p.group);
+                const int64_t token = seq.start + t;
+                const int qh = kvh * p.group + (at_row - t * p.group);
+                float m = kNone, l = 0.0f;
+                v4f o4 = v4f{0, 0, 0, 0};
+                if (r < here) {
+                    join_parts<8>(p, token * p.q_heads + qh, ch, way, ways, rt.shared_parts, [](int s) { return s; }, m, l, o4);
+                    for (int w = way; w < 4 && ch < d; w += ways) {
+                        join_part(m, l, o4, sh.m[w][r], sh.l[w][r], *reinterpret_cast<const v4f*>(&sh.o[w][r][ch]));
+                    }
+                }
+                join_ways(*join, lanes, ways, m, l, o4);
+                if (r < here && way == 0 && ch < d) {
+                    write_result<T>(p, token, qh, ch, l, o4);
+                }
+            }
+            return;
+        }
+    }
     // 16 threads a row, 4 channels each at a time
     const int r = threadIdx.x / 16, ch0 = threadIdx.x % 16 * 4;
     if (row0 + r >= rows) {
@@ -330,7 +444,12 @@ template <typename T, int DP, AttnMode M>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void attention_rows16(const AttnKern p)
 {
     __shared__ WaveParts<DP> sh;
-    attend_rows16<T, DP, M>(p, sh, blockIdx.x, blockIdx.y);
+    if constexpr (M == kOwn) {
+        __shared__ WayParts join;
+        attend_rows16<T, DP, M>(p, sh, blockIdx.x, blockIdx.y, &join);
+    } else {
+        attend_rows16<T, DP, M>(p, sh, blockIdx.x, blockIdx.y);
+    }
 }
 
 }  // namespace

@@ -74,6 +74,8 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
     __shared__ __attribute__((aligned(16))) uint16_t s_k[2][kTile * kPitchK];
     __shared__ __attribute__((aligned(16))) uint16_t s_v[2][DP * kPitchV];
     __shared__ __attribute__((aligned(16))) v4f s_scale[4][4];       // mul, add, inv of the groups of 16 tokens
+    constexpr int kPitchO = 36;
+    __shared__ __attribute__((aligned(16))) float s_o[M == kWhole ? 1 : NW][32 * kPitchO];   // 32 x 32 of a wave's O
 
     const Paged& c = p.c;
     const uint32_t item = blockIdx.x / (uint32_t)c.heads;
@@ -514,13 +516,57 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p
         }
     }
 
+    if constexpr (M != kWhole) {
+        // Parts of all rows: a tile of 32 channels at a time through LDS, whole lines of
+        // a row by 8 lanes. (From the registers a store has 32 bytes of each of 32 rows:
+        // 8 heads of 256 rows, 32 splits of 4 tiles 29.6 us, most of it 33 MB of parts.)
+        l_run += across(l_run);
+        const int64_t slot = split + p.first_part;
+        if (is_row && hh == 0) {
+            const int64_t at_part = (slot * c.rows + seq.start + tok) * p.q_heads + head;
+            p.part_ml[2 * at_part] = m_run;
+            p.part_ml[2 * at_part + 1] = l_run;
+        }
+        float* const mine = s_o[wave];
+        float* dst[4];
+        bool stored[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = wrow + 8 * i + lane / 8, t = (int)((uint32_t)r / group);
+            stored[i] = r < rt.rows;
+            dst[i] = p.part + ((slot * c.rows + seq.start + t) * p.q_heads + kvh * p.group + (r - t * p.group)) * d +
+                     lane % 8 * 4;
+        }
+#pragma unroll
+        for (int t = 0; t < kOut; ++t) {
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                *reinterpret_cast<v4f*>(mine + n * kPitchO + 2 * r + 4 * hh) =
+                    v4f{o[t][r], o[t][r + 1], o[t][r + 2], o[t][r + 3]};
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const v4f x = *reinterpret_cast<const v4f*>(mine + (8 * i + lane / 8) * kPitchO + lane % 8 * 4);
+                if (stored[i] && 32 * t + lane % 8 * 4 < d) {
+                    *reinterpret_cast<v4f*>(dst[i] + 32 * t) = x;
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        }
+        return;
+    }
     if (!is_row) {
         return;                                    // no barrier below
     }
     l_run += across(l_run);
     const int64_t token = seq.start + tok;
-    if (M != kWhole || rt.split) {
-        const int64_t at_part = ((int64_t)(split + (M == kWhole ? 0 : p.first_part)) * c.rows + token) * p.q_heads + head;
+    if (rt.split) {
+        const int64_t at_part = ((int64_t)split * c.rows + token) * p.q_heads + head;
         float* dst = p.part + at_part * d;
 #pragma unroll
         for (int t = 0; t < kOut; ++t) {

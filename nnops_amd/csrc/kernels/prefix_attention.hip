@@ -126,8 +126,7 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan(const PrefixKern p)
 template <typename T>
 __global__ __launch_bounds__(256) void prefix_join(const PrefixKern p)
 {
-    __shared__ __attribute__((aligned(16))) v4f s_o[256];
-    __shared__ float s_m[16], s_l[16];
+    __shared__ WayParts sh;
     const AttnKern& k = p.own;
     const Paged& c = k.c;
     const int lanes = join_lanes(c.d), slot = threadIdx.x / (uint32_t)lanes, ways = p.ways;
@@ -158,83 +157,22 @@ __global__ __launch_bounds__(256) void prefix_join(const PrefixKern p)
         shared = (int)(((uint32_t)skip + (uint32_t)shared_chunk - 1) / (uint32_t)shared_chunk);
         own = (int)(((uint32_t)rt.span.tiles + (uint32_t)own_chunk - 1) / (uint32_t)own_chunk);
     }
-    const int parts = shared + own, d = c.d, ch = threadIdx.x % (uint32_t)lanes * 4;
-    const int64_t rows = (int64_t)c.rows * k.q_heads, at = (int64_t)token * k.q_heads + qh;
+    const int ch = threadIdx.x % (uint32_t)lanes * 4;
     float m = kNone, l = 0.0f;
     v4f o = v4f{0, 0, 0, 0};
-    constexpr int kBatch = 4;
-    for (int s = way; s < parts; s += kBatch * ways) {
-        float ms[kBatch], ls[kBatch];
-        v4f os[kBatch];
-#pragma unroll
-        for (int e = 0; e < kBatch; ++e) {
-            const int n = s + e * ways, part = n < shared ? n : k.first_part + n - shared;
-            ms[e] = kNone;
-            ls[e] = 0.0f;
-            os[e] = v4f{0, 0, 0, 0};
-            if (n < parts) {
-                ms[e] = k.part_ml[2 * (part * rows + at)];
-                ls[e] = k.part_ml[2 * (part * rows + at) + 1];
-                if (ch < d) {
-                    os[e] = *reinterpret_cast<const v4f*>(k.part + (part * rows + at) * d + ch);
-                }
-            }
-        }
-        float top = m;
-#pragma unroll
-        for (int e = 0; e < kBatch; ++e) {
-            top = fmaxf(top, ms[e]);
-        }
-        const float f = m < top ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
-        l *= f;
-        o *= f;
-        m = top;
-#pragma unroll
-        for (int e = 0; e < kBatch; ++e) {
-            // (a part that saw nothing has -inf and nothing to add)
-            const float w = ms[e] < m ? __builtin_amdgcn_exp2f(ms[e] - m) : 1.0f;
-            l += w * ls[e];
-            o += w * os[e];
-        }
+    join_parts<4>(k, (int64_t)token * k.q_heads + qh, ch, way, ways, shared + own,
+                  [&](int s) { return s < shared ? s : k.first_part + s - shared; }, m, l, o);
+    join_ways(sh, lanes, ways, m, l, o);
+    if (live && way == 0 && ch < c.d) {
+        write_result<T>(k, token, qh, ch, l, o);
     }
-    if (ways > 1) {
-        s_o[threadIdx.x] = o;
-        if (threadIdx.x % (uint32_t)lanes == 0) {
-            s_m[slot] = m;
-            s_l[slot] = l;
-        }
-        __syncthreads();
-        if (way != 0) {
-            return;
-        }
-        float top = kNone;
-        for (int w = 0; w < ways; ++w) {
-            top = fmaxf(top, s_m[slot + w]);
-        }
-        l = 0.0f;
-        o = v4f{0, 0, 0, 0};
-        for (int w = 0; w < ways; ++w) {
-            const float f = s_m[slot + w] < top ? __builtin_amdgcn_exp2f(s_m[slot + w] - top) : 1.0f;
-            l += f * s_l[slot + w];
-            o += f * s_o[threadIdx.x + w * lanes];
-        }
-    }
-    if (!live || ch >= d) {
-        return;
-    }
-    const float f = l == 0.0f ? 0.0f : kDrop / l;
-    T y[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        y[e] = (T)(o[e] * f);
-    }
-    __builtin_memcpy(static_cast<T*>(k.out) + token * k.ld_out + (int64_t)qh * d + ch, y, sizeof y);
 }
 
 struct SharedPlan {
     AttnPlan own;
     int64_t items;        // tiles of the groups' rows, all KV heads
     int32_t tile_rows, per_seq, splits, ways;
+    bool join_here;       // own tokens, 16 rows a workgroup and unsplit: they join the parts themselves
     size_t groups_at, members_at, starts_at, parts_at, workspace;
 };
 
@@ -297,7 +235,8 @@ SharedPlan shared_plan(const NnopsPrefixAttentionArgs* g)
             a.splits = (int32_t)n;
         }
     }
-    const int64_t parts = a.splits + a.own.splits;
+    a.join_here = a.tile_rows != kRows && a.own.tile_rows == kRows && a.own.splits == 1;
+    const int64_t parts = a.splits + (a.join_here ? 0 : a.own.splits);
     // workgroups to fill the chip, as long as each lane has a batch of parts
     const int lanes = join_lanes((int)d);
     a.ways = 1;
@@ -394,6 +333,9 @@ void launch_prefix(const PrefixKern& p, const SharedPlan& a, hipStream_t s)
             launch_part<T, kShared>(k, dim3((unsigned)a.items, (unsigned)a.splits), s);
         }
         launch_part<T, kOwn>(p.own, dim3((unsigned)a.own.items, (unsigned)a.own.splits), s);
+        if (p.own.join_here) {
+            return;
+        }
     }
     const int64_t per_block = 256 / join_lanes(k.c.d) / a.ways;
     const int64_t blocks = ((int64_t)k.c.rows * k.q_heads + per_block - 1) / per_block;
@@ -444,7 +386,7 @@ extern "C" int nnops_hip_prefix_attention(const NnopsPrefixAttentionArgs* g, voi
     k.ld_q = g->ld_q;
     k.ld_out = g->ld_out;
     k.part = reinterpret_cast<float*>(at + a.parts_at);
-    k.part_ml = k.part + (size_t)(a.splits + a.own.splits) * g->rows * g->q_heads * g->cache.head_dim;
+    k.part_ml = k.part + (size_t)(a.splits + (a.join_here ? 0 : a.own.splits)) * g->rows * g->q_heads * g->cache.head_dim;
     const float scale = g->scale > 0.0f ? g->scale : 1.0f / __builtin_sqrtf((float)g->cache.head_dim);
     k.scale_log2 = scale * 1.4426950408889634f;
     k.q_heads = (int32_t)g->q_heads;
@@ -462,6 +404,7 @@ extern "C" int nnops_hip_prefix_attention(const NnopsPrefixAttentionArgs* g, voi
     k.group_starts = g->group_starts;
     k.shared = g->shared;
     k.few = g->cache.sequences <= 64 && g->groups <= kFewGroups;
+    k.join_here = a.join_here;
     k.shared_splits = a.splits;
     k.by_shared_splits = reciprocal(a.splits);
     k.groups = (int32_t)g->groups;
