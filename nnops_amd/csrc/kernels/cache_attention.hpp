@@ -60,6 +60,7 @@ struct AttnKern {
     int32_t groups, first_part, few;
     int32_t join_here;    // kOwn, unsplit: joins the shared tokens' parts itself
     int32_t shared_splits;       // as splits and by_splits, of the tokens that groups share
+    uint32_t shared_unit;        // tiles that a split of them is a multiple of: 4 where waves take every 4th
     uint32_t by_shared_splits;
 };
 
@@ -123,13 +124,13 @@ __device__ __forceinline__ int wave_max(int v)
 
 // Tiles of a split where the longest sequence (of shared tokens, or of what is behind
 // them) has so many: see chunk_of.
-__device__ __forceinline__ int chunk_for(int tiles, int splits, uint32_t by_splits, int whole)
+__device__ __forceinline__ int chunk_for(int tiles, int splits, uint32_t by_splits, int whole, uint32_t unit = 4)
 {
     if (splits == 1) {
         return std::numeric_limits<int>::max();
     }
     const uint32_t share = __umulhi((uint32_t)(tiles + splits - 1), by_splits);
-    return tiles <= whole ? whole : max((int)((share + 3u) & ~3u), 4);
+    return tiles <= whole ? whole : max((int)((share + unit - 1) & ~(unit - 1)), 4);
 }
 
 // Tiles of tokens that a split takes: the longest sequence that has rows is
@@ -247,7 +248,7 @@ __device__ __forceinline__ FewPlan few_plan(const AttnKern& p)
         }
     }
     const int own = wave_max(f.seq.n > 0 ? f.seq.len - kTile * f.member.skip : 0);
-    f.shared_chunk = chunk_for(longest / kTile, p.shared_splits, p.by_shared_splits, 4);
+    f.shared_chunk = chunk_for(longest / kTile, p.shared_splits, p.by_shared_splits, 4, p.shared_unit);
     f.own_chunk = chunk_for(min((own + kTile - 1) / kTile, p.tiles), p.splits, p.by_splits, p.whole);
     return f;
 }

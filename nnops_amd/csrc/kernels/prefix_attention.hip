@@ -116,7 +116,7 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan(const PrefixKern p)
     longest = group_max(longest, s_waves);
     own = group_max(own, s_waves);
     if (tid == 0) {
-        *k.plan = PrefixPlan{chunk_for(longest / kTile, k.shared_splits, k.by_shared_splits, 4),
+        *k.plan = PrefixPlan{chunk_for(longest / kTile, k.shared_splits, k.by_shared_splits, 4, k.shared_unit),
                              chunk_for(min((own + kTile - 1) / kTile, k.tiles), k.splits, k.by_splits, k.whole)};
     }
 }
@@ -224,12 +224,12 @@ SharedPlan shared_plan(const NnopsPrefixAttentionArgs* g)
     const int64_t tiles = g->cache.table_pages * g->cache.page_tokens / kTile;
     // Splits by rounds of the chip's workgroups: a round takes its tiles of tokens and
     // about `extra` tiles' time to begin, and to write its parts.
-    const int64_t chip = rows > 0 ? 256 : 512, extra = 5;
+    const int64_t chip = rows > 0 ? 256 : 512, extra = 5, fine = 64;
     const int64_t most = (tiles + 3) / 4 < 4 * chip / a.items + 1 ? (tiles + 3) / 4 : 4 * chip / a.items + 1;
     a.splits = 1;
     int64_t best = INT64_MAX;
     for (int64_t n = 1; n <= most; ++n) {
-        const int64_t cost = (a.items * n + chip - 1) / chip * ((tiles + n - 1) / n + extra);
+        const int64_t cost = (a.items * n + chip - 1) / chip * (fine * tiles / n + fine * extra);
         if (cost < best) {
             best = cost;
             a.splits = (int32_t)n;
@@ -406,6 +406,7 @@ extern "C" int nnops_hip_prefix_attention(const NnopsPrefixAttentionArgs* g, voi
     k.few = g->cache.sequences <= 64 && g->groups <= kFewGroups;
     k.join_here = a.join_here;
     k.shared_splits = a.splits;
+    k.shared_unit = a.tile_rows == kRows ? 4 : 1;
     k.by_shared_splits = reciprocal(a.splits);
     k.groups = (int32_t)g->groups;
     k.first_part = a.splits;
