@@ -67,33 +67,43 @@ __device__ __forceinline__ void join_part(float& m, float& l, v4f& o, float pm, 
     m = top;
 }
 
-// Every step-th of the parts from first on, of n in all: number s is at part(s).
-template <int kBatch, typename Part>
-__device__ __forceinline__ void join_parts(const AttnKern& p, int64_t at, int ch, int first, int step, int n, Part part,
-                                           float& m, float& l, v4f& o)
+// Every step-th of the parts from first on, of n in all: number s is at part(s). Of
+// kAtOnce rows side by side, their loads in flight together.
+template <int kBatch, int kAtOnce, typename Part>
+__device__ __forceinline__ void join_parts(const AttnKern& p, const int64_t (&at)[kAtOnce], int ch, int first, int step,
+                                           int n, Part part, float (&m)[kAtOnce], float (&l)[kAtOnce], v4f (&o)[kAtOnce])
 {
     const int64_t rows = (int64_t)p.c.rows * p.q_heads;
     for (int s = first; s < n; s += kBatch * step) {
-        float ms[kBatch], ls[kBatch];
-        v4f os[kBatch];
+        float ms[kAtOnce][kBatch], ls[kAtOnce][kBatch];
+        v4f os[kAtOnce][kBatch];
 #pragma unroll
         for (int e = 0; e < kBatch; ++e) {
             const int i = s + e * step;
-            ms[e] = kNone;
-            ls[e] = 0.0f;
-            os[e] = v4f{0, 0, 0, 0};
+#pragma unroll
+            for (int a = 0; a < kAtOnce; ++a) {
+                ms[a][e] = kNone;
+                ls[a][e] = 0.0f;
+                os[a][e] = v4f{0, 0, 0, 0};
+            }
             if (i < n) {
-                const int64_t from = part(i) * rows + at;
-                ms[e] = p.part_ml[2 * from];
-                ls[e] = p.part_ml[2 * from + 1];
-                if (ch < p.c.d) {
-                    os[e] = *reinterpret_cast<const v4f*>(p.part + from * p.c.d + ch);
+#pragma unroll
+                for (int a = 0; a < kAtOnce; ++a) {
+                    const int64_t from = part(i) * rows + at[a];
+                    ms[a][e] = p.part_ml[2 * from];
+                    ls[a][e] = p.part_ml[2 * from + 1];
+                    if (ch < p.c.d) {
+                        os[a][e] = *reinterpret_cast<const v4f*>(p.part + from * p.c.d + ch);
+                    }
                 }
             }
         }
 #pragma unroll
         for (int e = 0; e < kBatch; ++e) {
-            join_part(m, l, o, ms[e], ls[e], os[e]);
+#pragma unroll
+            for (int a = 0; a < kAtOnce; ++a) {
+                join_part(m[a], l[a], o[a], ms[a][e], ls[a][e], os[a][e]);
+            }
         }
     }
 }
@@ -372,22 +382,50 @@ __device__ __forceinline__ void attend_rows16(const AttnKern& p, WaveParts<DP>& 
             while (2 * ways * here <= slots) {
                 ways *= 2;
             }
-            for (int r0 = 0; r0 < here; r0 += slots / ways) {   // (once, if there is more than one way)
-                const int r = r0 + slot / ways, way = slot % ways;
-                const int at_row = min(row0 + r, rows - 1), t = (int)((uint32_t)at_row / (uint32_t)p.group);
-                const int64_t token = seq.start + t;
-                const int qh = kvh * p.group + (at_row - t * p.group);
-                float m = kNone, l = 0.0f;
-                v4f o4 = v4f{0, 0, 0, 0};
-                if (r < here) {
-                    join_parts<8>(p, token * p.q_heads + qh, ch, way, ways, rt.shared_parts, [](int s) { return s; }, m, l, o4);
-                    for (int w = way; w < 4 && ch < d; w += ways) {
-                        join_part(m, l, o4, sh.m[w][r], sh.l[w][r], *reinterpret_cast<const v4f*>(&sh.o[w][r][ch]));
+            const int way = slot % ways, step = slots / ways;
+            constexpr int kAtOnce = DP > 64 ? 2 : 1;            // (with one way)
+            for (int r0 = 0; r0 < here; r0 += kAtOnce * step) {   // (once, if there is more than one way)
+                int64_t at[kAtOnce];
+                float m[kAtOnce], l[kAtOnce];
+                v4f o4[kAtOnce];
+#pragma unroll
+                for (int a = 0; a < kAtOnce; ++a) {
+                    const int row = min(row0 + r0 + a * step + slot / ways, rows - 1);
+                    const int t = (int)((uint32_t)row / (uint32_t)p.group);
+                    at[a] = (int64_t)(seq.start + t) * p.q_heads + kvh * p.group + (row - t * p.group);
+                    m[a] = kNone;
+                    l[a] = 0.0f;
+                    o4[a] = v4f{0, 0, 0, 0};
+                }
+                const auto part = [](int s) { return s; };
+                if (kAtOnce > 1 && r0 + step < here) {
+                    join_parts<4>(p, at, ch, way, ways, rt.shared_parts, part, m, l, o4);
+                } else {
+                    const int64_t one[1] = {at[0]};
+                    float m1[1] = {m[0]}, l1[1] = {l[0]};
+                    v4f o1[1] = {o4[0]};
+                    join_parts<8>(p, one, ch, way, ways, rt.shared_parts, part, m1, l1, o1);
+                    m[0] = m1[0];
+                    l[0] = l1[0];
+                    o4[0] = o1[0];
+                }
+#pragma unroll
+                for (int a = 0; a < kAtOnce; ++a) {
+                    const int row = r0 + a * step + slot / ways;
+                    if (row < here) {
+                        for (int w = way; w < 4 && ch < d; w += ways) {
+                            join_part(m[a], l[a], o4[a], sh.m[w][row], sh.l[w][row],
+                                      *reinterpret_cast<const v4f*>(&sh.o[w][row][ch]));
+                        }
                     }
                 }
-                join_ways(*join, lanes, ways, m, l, o4);
-                if (r < here && way == 0 && ch < d) {
-                    write_result<T>(p, token, qh, ch, l, o4);
+                join_ways(*join, lanes, ways, m[0], l[0], o4[0]);
+#pragma unroll
+                for (int a = 0; a < kAtOnce; ++a) {
+                    if (r0 + a * step + slot / ways < here && way == 0 && ch < d) {
+                        const int64_t token = at[a] / p.q_heads;
+                        write_result<T>(p, token, (int)(at[a] - token * p.q_heads), ch, l[a], o4[a]);
+                    }
                 }
             }
             return;

@@ -158,13 +158,14 @@ __global__ __launch_bounds__(256) void prefix_join(const PrefixKern p)
         own = (int)(((uint32_t)rt.span.tiles + (uint32_t)own_chunk - 1) / (uint32_t)own_chunk);
     }
     const int ch = threadIdx.x % (uint32_t)lanes * 4;
-    float m = kNone, l = 0.0f;
-    v4f o = v4f{0, 0, 0, 0};
-    join_parts<4>(k, (int64_t)token * k.q_heads + qh, ch, way, ways, shared + own,
-                  [&](int s) { return s < shared ? s : k.first_part + s - shared; }, m, l, o);
-    join_ways(sh, lanes, ways, m, l, o);
+    const int64_t at[1] = {(int64_t)token * k.q_heads + qh};
+    float m[1] = {kNone}, l[1] = {0.0f};
+    v4f o[1] = {v4f{0, 0, 0, 0}};
+    join_parts<4>(k, at, ch, way, ways, shared + own, [&](int s) { return s < shared ? s : k.first_part + s - shared; }, m,
+                  l, o);
+    join_ways(sh, lanes, ways, m[0], l[0], o[0]);
     if (live && way == 0 && ch < c.d) {
-        write_result<T>(k, token, qh, ch, l, o);
+        write_result<T>(k, token, qh, ch, l[0], o[0]);
     }
 }
 
