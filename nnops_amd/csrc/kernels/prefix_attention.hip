@@ -214,7 +214,15 @@ SharedPlan shared_plan(const NnopsPrefixAttentionArgs* g)
     const int64_t heads = g->cache.heads, group = g->q_heads / heads, d = g->cache.head_dim;
     const int64_t groups = g->groups > 0 ? g->groups : 1;
     const int64_t mean = (g->rows * group + groups - 1) / groups;
-    const int rows = mean > 32 ? tiled_rows(d, g->f16, g->cache.page_tokens, mean) : 0;
+    // Tiles of many rows where they fill more than a quarter and there is work enough for
+    // their longer beginning and end; 16 rows a workgroup otherwise, in one launch with
+    // the sequences' own tokens (us, tiled / 16 rows; n sequences of one token, 32 query
+    // and 8 KV heads of 128, f16; shared tokens 4096 and 32768): 16 27.3 / 19.2 and 50.7 /
+    // 39.7, 24 28.6 / 23.5 and 53.2 / 54.1, 32 30.4 / 23.8 and 55.9 / 64.1, 48 36.5 / 27.4 and
+    // 68.7 / 94.4; over 8192, 32 of them, d 64 26.3 / 19.1, d 256 59.3 / 64.4, f32 41.0 / 34.7.
+    const int64_t room = g->cache.table_pages * g->cache.page_tokens;
+    const bool much = (double)g->rows * g->q_heads * d * room >= 0x1p31;
+    const int rows = mean > 64 && much ? tiled_rows(d, g->f16, g->cache.page_tokens, mean) : 0;
     a.tile_rows = rows > 0 ? rows : kRows;
     if (g->groups <= 1) {
         a.per_seq = (int32_t)((g->rows * group + a.tile_rows - 1) / a.tile_rows);
@@ -222,7 +230,7 @@ SharedPlan shared_plan(const NnopsPrefixAttentionArgs* g)
     } else {
         a.items = (g->rows * group / a.tile_rows + (groups < g->rows ? groups : g->rows)) * heads;
     }
-    const int64_t tiles = g->cache.table_pages * g->cache.page_tokens / kTile;
+    const int64_t tiles = room / kTile;
     // Splits by rounds of the chip's workgroups: a round takes its tiles of tokens and
     // about `extra` tiles' time to begin, and to write its parts.
     const int64_t chip = rows > 0 ? 256 : 512, extra = 5, fine = 64;
