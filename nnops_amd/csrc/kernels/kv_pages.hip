@@ -32,6 +32,15 @@ __device__ __forceinline__ int wave_before(int v, int& total)
     return upto - v;
 }
 
+__device__ __forceinline__ int wave_max(int v)
+{
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+        v = max(v, __shfl_xor(v, m));
+    }
+    return v;
+}
+
 // The same over a workgroup of kPlan threads; s_waves: one int a wave. Every
 // thread calls it, with a barrier before the next call's.
 __device__ __forceinline__ int group_before(int v, int* s_waves, int& total)
@@ -259,6 +268,153 @@ __global__ __launch_bounds__(kPlan) void fork_take(const ForkKern p)
     }
 }
 
+// The same by one workgroup, counts and lists in LDS: four cells a thread and step.
+constexpr int kSmallPages = 12288, kSmallRows = 1024, kSmallCells = 1 << 16;
+
+__global__ __launch_bounds__(kPlan) void fork_small(const ForkKern p)
+{
+    __shared__ int s_refs[kSmallPages];
+    __shared__ int s_list[kSmallPages];            // writers, then the first of them, then the free pages
+    __shared__ int s_held[kSmallRows], s_parent[kSmallRows], s_shared[kSmallRows], s_fresh[kSmallRows];
+    __shared__ int s_tail[kSmallRows], s_at[kSmallRows + 1];
+    __shared__ uint8_t s_kind[kSmallRows], s_writes[kSmallRows];
+    __shared__ int s_waves[kPlan / 64];
+    const int tid = threadIdx.x;
+    for (int i = tid; i < p.pages; i += kPlan) {
+        s_refs[i] = p.refs[i];
+        s_list[i] = 0;
+    }
+    int held = 0;
+    if (tid < p.seqs) {
+        held = pages_of(length_of(p, tid), p.page_log2);
+        s_held[tid] = held;
+    }
+    if (tid < p.children) {
+        int parent, kept, will;
+        tokens_of(p, tid, parent, kept, will);
+        const int shared = pages_of(kept, p.page_log2);
+        s_parent[tid] = parent;
+        s_shared[tid] = shared;
+        s_fresh[tid] = pages_of(will, p.page_log2) - shared;
+        s_writes[tid] = will > kept && (kept & ((1 << p.page_log2) - 1)) != 0;
+        s_tail[tid] = kNoTail;
+        p.new_lengths[tid] = will;
+    }
+    held = wave_max(held);
+    if (tid % 64 == 0) {
+        s_waves[tid / 64] = held;
+    }
+    __syncthreads();
+    int most = 0;                                  // pages of the longest
+    for (int w = 0; w < kPlan / 64; ++w) {
+        most = max(most, s_waves[w]);
+    }
+    const uint32_t old_cells = (uint32_t)p.seqs * most, new_cells = (uint32_t)p.children * p.new_pages;
+    for (uint32_t base = 0; base < old_cells + new_cells; base += 4 * kPlan) {
+        int row[4], col[4], id[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t i = base + e * kPlan + tid;
+            const bool old = i < old_cells;
+            const uint32_t j = old ? i : i - old_cells, wide = old ? (uint32_t)most : (uint32_t)p.new_pages;
+            row[e] = -1;
+            id[e] = -1;
+            if (i < old_cells + new_cells) {
+                const int r = (int)(j / wide);
+                col[e] = (int)(j - r * wide);
+                row[e] = old ? r : p.seqs + r;
+                const int from = old ? r : s_parent[r];
+                if (col[e] < (old ? s_held[r] : s_shared[r])) {
+                    id[e] = p.table[from * p.ld_table + col[e]];
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int page = (uint32_t)id[e] < (uint32_t)p.pages ? id[e] : -1;
+            const int i = row[e] - p.seqs;
+            if (row[e] >= 0 && i < 0) {
+                if (page >= 0) {
+                    atomicSub(&s_refs[page], 1);
+                }
+            } else if (i >= 0) {
+                if (page >= 0) {
+                    atomicAdd(&s_refs[page], 1);
+                }
+                if (s_writes[i] && col[e] == s_shared[i] - 1) {
+                    s_tail[i] = page >= 0 ? page : kNoPage;
+                    if (page >= 0) {
+                        atomicAdd(&s_list[page], 1);
+                    }
+                }
+                p.new_table[i * p.ld_new + col[e]] = page;
+            }
+        }
+    }
+    __syncthreads();
+    const int tail = tid < p.children ? s_tail[tid] : kNoTail;
+    const bool alone = tail >= 0 && s_refs[tail] <= s_list[tail];
+    __syncthreads();
+    if (tail >= 0) {
+        s_list[tail] = p.children;
+    }
+    __syncthreads();
+    if (tail >= 0) {
+        atomicMin(&s_list[tail], tid);
+    }
+    __syncthreads();
+    const int kind = tail == kNoPage ? 2 : tail >= 0 && !(alone && s_list[tail] == tid) ? 1 : 0;
+    int want;
+    const int at = group_before(tid < p.children ? s_fresh[tid] + (kind != 0) : 0, s_waves, want);
+    if (tid < p.children) {
+        s_at[tid] = at;
+        s_kind[tid] = (uint8_t)kind;
+        if (kind != 1) {                           // (else by the thread that has the fresh page)
+            p.copies[2 * tid] = -1;
+            p.copies[2 * tid + 1] = -1;
+        }
+    }
+    const int share = (p.pages + kPlan - 1) / kPlan, first = min(share * tid, p.pages), end = min(first + share, p.pages);
+    int free = 0;
+    for (int i = first; i < end; ++i) {
+        free += s_refs[i] == 0;
+    }
+    int found;
+    int rank = group_before(free, s_waves, found);
+    for (int i = first; i < end && rank < want; ++i) {
+        if (s_refs[i] == 0) {
+            s_list[rank++] = i;
+        }
+    }
+    __syncthreads();
+    const int got = min(want, found);
+    for (int r = tid; r < want; r += kPlan) {
+        int lo = 0, hi = p.children;               // the last child that begins at or before r
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            (s_at[mid] <= r ? lo : hi) = mid;
+        }
+        const int k = r - s_at[lo], page = r < got ? s_list[r] : -1;
+        p.new_table[lo * p.ld_new + s_shared[lo] + k - (s_kind[lo] != 0)] = page;
+        if (page >= 0) {
+            s_refs[page] = 1;
+        }
+        if (s_kind[lo] == 1 && k == 0) {
+            atomicSub(&s_refs[s_tail[lo]], 1);
+            p.copies[2 * lo] = page >= 0 ? s_tail[lo] : -1;
+            p.copies[2 * lo + 1] = page;
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < p.pages; i += kPlan) {
+        p.new_refs[i] = s_refs[i];
+    }
+    if (tid == 0) {
+        p.counts[0] = found - got;
+        p.counts[1] = want - got;
+    }
+}
+
 // --- compact ---------------------------------------------------------------------
 
 constexpr int kBlock = 4096;        // pages of a workgroup, 16 a thread
@@ -428,6 +584,110 @@ __global__ __launch_bounds__(256) void compact_apply(const CompactKern p)
     }
 }
 
+// The same by one workgroup: 16 pages a thread, their counts in its registers.
+constexpr int kCompactPages = 16 * kPlan, kCompactCells = 1 << 16;
+
+__global__ __launch_bounds__(kPlan) void compact_small(const CompactKern p)
+{
+    __shared__ int s_code[kCompactPages];          // new numbers, -1 for a free page
+    __shared__ int s_to[kCompactPages / 2];        // where the i-th page that moves goes
+    __shared__ int s_waves[kPlan / 64];
+    const int tid = threadIdx.x, at = 16 * tid;
+    int refs[16];
+    uint32_t bits = 0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        refs[e] = 0;
+    }
+    if (at + 16 <= p.pages) {
+        __builtin_memcpy(refs, p.refs + at, sizeof refs);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            if (at + e < p.pages) {
+                refs[e] = p.refs[at + e];
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        bits |= (uint32_t)(refs[e] != 0) << e;
+    }
+    int u, below;
+    const int before = group_before(__popc(bits), s_waves, u);
+    group_before(__popc(bits & ((1u << min(max(u - at, 0), 16)) - 1)), s_waves, below);
+    const int moves = u - below;
+    int rank = before;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const int j = at + e;
+        const bool is = (bits >> e & 1) != 0;
+        if (!is && j < u) {
+            s_to[j - rank] = j;
+        }
+        rank += is;
+    }
+    __syncthreads();
+    rank = before;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const int j = at + e;
+        const bool is = (bits >> e & 1) != 0;
+        if (j < p.pages) {
+            int to = is ? j : -1;
+            if (is && j >= u) {
+                to = s_to[rank - below];
+                p.copies[2 * (rank - below)] = j;
+                p.copies[2 * (rank - below) + 1] = to;
+            }
+            s_code[j] = to;
+            if (to >= 0) {
+                p.new_refs[to] = refs[e];
+            }
+            if (j >= u) {
+                p.new_refs[j] = 0;
+            }
+        }
+        rank += is;
+    }
+    for (int i = moves + tid; i < p.pages / 2; i += kPlan) {
+        p.copies[2 * i] = -1;
+        p.copies[2 * i + 1] = -1;
+    }
+    if (tid == 0) {
+        p.counts[0] = u;
+        p.counts[1] = moves;
+    }
+    __syncthreads();
+    for (int j = tid; j < p.pages; j += kPlan) {
+        p.moved[j] = s_code[j];
+    }
+    const uint32_t cells = (uint32_t)p.seqs * p.table_pages;
+    for (uint32_t base = 0; base < cells; base += 4 * kPlan) {
+        int row[4], col[4], id[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t i = base + e * kPlan + tid;
+            row[e] = -1;
+            id[e] = -1;
+            if (i < cells) {
+                row[e] = (int)(i / (uint32_t)p.table_pages);
+                col[e] = (int)(i - (uint32_t)row[e] * p.table_pages);
+                const int64_t len = min((int64_t)max(p.lengths[row[e]], 0), (int64_t)p.table_pages << p.page_log2);
+                if (col[e] < pages_of((int)len, p.page_log2)) {
+                    id[e] = p.table[row[e] * p.ld_table + col[e]];
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (row[e] >= 0) {
+                p.new_table[row[e] * p.ld_new + col[e]] = (uint32_t)id[e] < (uint32_t)p.pages ? s_code[id[e]] : -1;
+            }
+        }
+    }
+}
+
 // --- copy ------------------------------------------------------------------------
 
 constexpr int kPiece = 16384;       // bytes of a workgroup, four 16-byte loads a thread in flight
@@ -547,14 +807,27 @@ bool apart(const Range (&in)[kIn], const Range (&out)[kOut], const int (&same)[k
 
 size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 
+// One launch: as far as the counts fit in LDS, and a workgroup's cells take no longer
+// than two more launches.
+bool fork_is_small(const NnopsKvForkArgs* g)
+{
+    return g->pages <= kSmallPages && g->sequences <= kSmallRows && g->children <= kSmallRows &&
+           g->sequences * g->table_pages + g->children * g->new_table_pages <= kSmallCells;
+}
+
 size_t fork_workspace(const NnopsKvForkArgs* g)
 {
-    return 3 * align16(4 * (size_t)g->pages) + align16(sizeof(Child) * (size_t)g->children);
+    return fork_is_small(g) ? 0 : 3 * align16(4 * (size_t)g->pages) + align16(sizeof(Child) * (size_t)g->children);
+}
+
+bool compact_is_small(const NnopsKvCompactArgs* g)
+{
+    return g->pages <= kCompactPages && g->sequences * g->table_pages <= kCompactCells;
 }
 
 size_t compact_workspace(const NnopsKvCompactArgs* g)
 {
-    return align16(4 * (size_t)((g->pages + kBlock - 1) / kBlock)) + align16(4 * (size_t)g->pages);
+    return compact_is_small(g) ? 0 : align16(4 * (size_t)((g->pages + kBlock - 1) / kBlock)) + align16(4 * (size_t)g->pages);
 }
 
 }  // namespace
@@ -627,6 +900,10 @@ extern "C" int nnops_hip_kv_cache_fork(const NnopsKvForkArgs* g, void* workspace
         return NNOPS_UNSUPPORTED;
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
+    if (fork_is_small(g)) {
+        NNOPS_LAUNCH(fork_small, dim3(1), dim3(kPlan), 0, s, k);
+        return hipGetLastError() == hipSuccess ? NNOPS_OK : NNOPS_INTERNAL;
+    }
     if (g->pages > 0) {
         NNOPS_LAUNCH(fork_clear, dim3((unsigned)((g->pages + 255) / 256)), dim3(256), 0, s, k);
     }
@@ -697,6 +974,10 @@ extern "C" int nnops_hip_kv_cache_compact(const NnopsKvCompactArgs* g, void* wor
         return NNOPS_UNSUPPORTED;
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
+    if (compact_is_small(g)) {
+        NNOPS_LAUNCH(compact_small, dim3(1), dim3(kPlan), 0, s, k);
+        return hipGetLastError() == hipSuccess ? NNOPS_OK : NNOPS_INTERNAL;
+    }
     if (k.blocks > 0) {
         NNOPS_LAUNCH(compact_count, dim3((unsigned)k.blocks), dim3(256), 0, s, k);
     }

@@ -65,7 +65,8 @@ def _check_fork(table, lens, refs, parents, new, wide, page, **kw):
 
 
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
-@pytest.mark.parametrize("b,n,wide,pages", [(1, 1, 1, 2), (1, 9, 3, 40), (7, 5, 4, 60), (20, 33, 5, 300), (64, 64, 9, 900)])
+@pytest.mark.parametrize("b,n,wide,pages", [(1, 1, 1, 2), (1, 9, 3, 40), (7, 5, 4, 60), (20, 33, 5, 300), (64, 64, 9, 900),
+                                            (64, 70, 9, 13000)])
 def test_fork(page, b, n, wide, pages):
     """Children with parents of their own, twins, none; growth from nothing to
     whole pages, cuts, and refs in place."""
@@ -112,33 +113,35 @@ def test_fork_given_up_pages_are_free_at_once():
     assert t.tolist() == [[2, 3, -1, -1], [0, 1, -1, -1]] and rf.tolist() == [1] * 4 and counts.tolist() == [0, 0]
 
 
+@pytest.mark.parametrize("held", [0, 20000])      # (pages that somebody else holds: more than a workgroup counts)
 @pytest.mark.parametrize("seed", range(4))
-def test_fork_without_pages_enough(seed):
+def test_fork_without_pages_enough(seed, held):
     """Cells that get none are -1 and are counted; tables too narrow cut lengths."""
     announce(f"fork short {seed}")
     r = np.random.RandomState(seed)
     table, lens, refs = _tables(r, 12, 6, 16, 40)
     refs[r.rand(40) < 0.5] += 1
+    refs = np.concatenate([refs, np.ones(held, np.int64)])
     parents = r.randint(-1, 12, 30)
     got = _check_fork(table, lens, refs, parents, r.randint(-20, 150, 30), 7, 16)
     assert got[4][1] > 0
     _check_fork(table, lens, refs, parents, np.full(30, 2 ** 31 - 1), 3, 16)
     _check_fork(table, lens, refs, parents, np.full(30, -2 ** 31), 3, 16)
     # (what got none is asked for again by the next call)
-    more = np.zeros(200, np.int64)
-    more[:40] = got[2]
+    more = np.concatenate([got[2], np.zeros(160, np.int64)])
     _check_fork(got[0], got[1], more, np.arange(30), np.full(30, 1), 9, 16)
 
 
-def test_fork_of_tables_that_hold_no_pages():
+@pytest.mark.parametrize("pages", [200, 13000])
+def test_fork_of_tables_that_hold_no_pages(pages):
     """Page numbers out of range, lengths and parents too: no memory is touched by
     them, and the rest is as defined."""
-    announce("fork junk")
+    announce(f"fork junk {pages}")
     r = np.random.RandomState(5)
-    table, lens, refs = _tables(r, 30, 8, 16, 200, junk=0.3)
+    table, lens, refs = _tables(r, 30, 8, 16, pages, junk=0.3)
     lens = lens.astype(np.int64)
     lens[3], lens[4], lens[5] = -9, 2 ** 31 - 1, -2 ** 31
-    refs = ref.holders(table, lens, 16, 200)
+    refs = ref.holders(table, lens, 16, pages)
     parents = r.randint(-3, 33, 50)
     parents[:2] = 2 ** 31 - 1, -2 ** 31
     _check_fork(table, lens, refs, parents, r.randint(-30, 60, 50), 9, 16)
@@ -148,6 +151,7 @@ def test_fork_of_tables_that_hold_no_pages():
     (3, 4, 700, 1000, 40000),              # rows of several chunks
     (40, 1100, 3, 4, 2500),                # more children than the workgroup has threads
     (2, 3, 2, 2, 70000),                   # more pages than one step looks at
+    (20, 30, 3, 4, 12288), (20, 30, 3, 4, 12289), (1024, 1024, 3, 4, 9000), (3, 2, 9000, 9001, 3000),
     (1500, 7, 2, 3, 4000), (5, 0, 3, 2, 50), (0, 6, 0, 5, 60), (4, 4, 3, 0, 50), (3, 2, 4, 4, 0), (0, 0, 0, 0, 0)])
 def test_fork_sizes(b, n, wide, out_wide, pages):
     announce(f"fork sizes {b} {n} {wide} {out_wide} {pages}")
@@ -190,7 +194,8 @@ def _check_compact(table, lens, refs, page, *, in_place=False, pad=0):
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("b,wide,page,pages", [(1, 1, 16, 1), (3, 2, 16, 7), (9, 5, 64, 64), (20, 6, 16, 500),
                                                (50, 300, 16, 30000), (3, 3, 256, 9000), (0, 0, 16, 20), (4, 0, 16, 20),
-                                               (3, 2, 16, 0), (5, 4, 32, 4096), (5, 4, 32, 8192)])
+                                               (3, 2, 16, 0), (5, 4, 32, 4096), (5, 4, 32, 8192),
+                                               (5, 4, 32, 16384), (5, 4, 32, 16385), (3, 22000, 16, 2000)])
 def test_compact(b, wide, page, pages, in_place):
     announce(f"compact {b} {wide} page={page} pages={pages} in_place={in_place}")
     r = np.random.RandomState(pages + b)
@@ -201,7 +206,9 @@ def test_compact(b, wide, page, pages, in_place):
 
 
 @pytest.mark.parametrize("pages,pattern", [(100, "none"), (100, "all"), (101, "upper"), (4097, "upper"), (4096, "lower"),
-                                           (12288, "one block"), (9001, "last"), (8192, "odd"), (2, "upper"), (1, "all")])
+                                           (12288, "one block"), (9001, "last"), (8192, "odd"), (2, "upper"), (1, "all"),
+                                           (40960, "upper"), (40961, "lower"), (20480, "one block"), (24000, "last"),
+                                           (32768, "odd"), (16385, "all"), (30000, "none")])
 def test_compact_patterns(pages, pattern):
     """Nothing held, all, only the upper half, a block that ends at the border."""
     announce(f"compact pattern {pages} {pattern}")
@@ -215,13 +222,14 @@ def test_compact_patterns(pages, pattern):
     assert again[4][1] == 0
 
 
-def test_compact_of_tables_that_hold_no_pages():
-    announce("compact junk")
+@pytest.mark.parametrize("pages", [200, 20000])
+def test_compact_of_tables_that_hold_no_pages(pages):
+    announce(f"compact junk {pages}")
     r = np.random.RandomState(8)
-    table, lens, refs = _tables(r, 30, 8, 16, 200, junk=0.3)
+    table, lens, refs = _tables(r, 30, 8, 16, pages, junk=0.3)
     lens = lens.astype(np.int64)
     lens[3], lens[4] = -9, 2 ** 31 - 1
-    refs[r.rand(200) < 0.1] = 0                       # (tables that say more than the counts)
+    refs[r.rand(pages) < 0.1] = 0                       # (tables that say more than the counts)
     _check_compact(table, lens, refs, 16)
 
 
