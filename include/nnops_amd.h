@@ -699,6 +699,18 @@ typedef struct NnopsCacheAttentionPlan {
     size_t workspace_bytes;
 } NnopsCacheAttentionPlan;
 
+typedef struct NnopsPrefixAttentionPlan {
+    int32_t shared_rows;        /* rows of a workgroup over the shared tokens: 16, 128 or 256 */
+    int32_t shared_splits;      /* of these tokens, at most */
+    int32_t own_rows;           /* and over each sequence's own tokens */
+    int32_t own_splits;
+    int32_t launches;           /* of kernels */
+    int32_t join;               /* parts joined: 0 where own tokens are looked at, 1 by a kernel of their own */
+    size_t workspace_bytes;
+} NnopsPrefixAttentionPlan;
+
+int nnops_hip_prefix_attention_plan(const NnopsPrefixAttentionArgs* args, NnopsPrefixAttentionPlan* plan);
+
 /* OK, or what the call itself would say of the sizes. */
 int nnops_hip_cache_attention_plan(const NnopsCacheAttentionArgs* args, NnopsCacheAttentionPlan* plan);
 

@@ -257,6 +257,11 @@ class CacheAttentionPlan(C.Structure):
                 ("join", C.c_int32), ("workspace_bytes", C.c_size_t)]
 
 
+class PrefixAttentionPlan(C.Structure):
+    _fields_ = [("shared_rows", C.c_int32), ("shared_splits", C.c_int32), ("own_rows", C.c_int32),
+                ("own_splits", C.c_int32), ("launches", C.c_int32), ("join", C.c_int32), ("workspace_bytes", C.c_size_t)]
+
+
 PLAN_NO_PASS, PLAN_PASS, PLAN_GATED_PASS = range(3)
 
 
@@ -298,6 +303,7 @@ SIGNATURES = {
     "nnops_hip_cache_attention": (C.c_int, [C.POINTER(CacheAttentionArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
     "nnops_hip_prefix_attention_workspace_size": (C.c_size_t, [C.POINTER(PrefixAttentionArgs)]),
     "nnops_hip_prefix_attention": (C.c_int, [C.POINTER(PrefixAttentionArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "nnops_hip_prefix_attention_plan": (C.c_int, [C.POINTER(PrefixAttentionArgs), C.POINTER(PrefixAttentionPlan)]),
     "nnops_hip_kv_cache_fork_workspace_size": (C.c_size_t, [C.POINTER(KvForkArgs)]),
     "nnops_hip_kv_cache_fork": (C.c_int, [C.POINTER(KvForkArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
     "nnops_hip_kv_cache_compact_workspace_size": (C.c_size_t, [C.POINTER(KvCompactArgs)]),

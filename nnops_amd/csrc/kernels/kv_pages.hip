@@ -269,7 +269,7 @@ __global__ __launch_bounds__(kPlan) void fork_take(const ForkKern p)
 }
 
 // The same by one workgroup, counts and lists in LDS: four cells a thread and step.
-constexpr int kSmallPages = 12288, kSmallRows = 1024, kSmallCells = 1 << 16;
+constexpr int kSmallPages = 12288, kSmallRows = 1024, kSmallCells = 12288;
 
 __global__ __launch_bounds__(kPlan) void fork_small(const ForkKern p)
 {
@@ -585,7 +585,7 @@ __global__ __launch_bounds__(256) void compact_apply(const CompactKern p)
 }
 
 // The same by one workgroup: 16 pages a thread, their counts in its registers.
-constexpr int kCompactPages = 16 * kPlan, kCompactCells = 1 << 16;
+constexpr int kCompactPages = 16 * kPlan, kCompactCells = 6144;
 
 __global__ __launch_bounds__(kPlan) void compact_small(const CompactKern p)
 {
@@ -729,7 +729,7 @@ __global__ __launch_bounds__(256) void kv_copy(const CopyKern p)
     for (int e = 0; e < 4; ++e) {
         const int j = 256 * e + (int)threadIdx.x;
         if (j < n) {
-            dst[j] = x[e];
+            __builtin_nontemporal_store(x[e], dst + j);
         }
     }
     if (at == 0) {

@@ -173,6 +173,7 @@ struct SharedPlan {
     AttnPlan own;
     int64_t items;        // tiles of the groups' rows, all KV heads
     int32_t tile_rows, per_seq, splits, ways;
+    bool few;             // every wave finds the plan
     bool join_here;       // own tokens, 16 rows a workgroup and unsplit: they join the parts themselves
     size_t groups_at, members_at, starts_at, parts_at, workspace;
 };
@@ -244,6 +245,7 @@ SharedPlan shared_plan(const NnopsPrefixAttentionArgs* g)
             a.splits = (int32_t)n;
         }
     }
+    a.few = g->cache.sequences <= 64 && g->groups <= kFewGroups;
     a.join_here = a.tile_rows != kRows && a.own.tile_rows == kRows && a.own.splits == 1;
     const int64_t parts = a.splits + (a.join_here ? 0 : a.own.splits);
     // workgroups to fill the chip, as long as each lane has a batch of parts
@@ -361,6 +363,27 @@ extern "C" size_t nnops_hip_prefix_attention_workspace_size(const NnopsPrefixAtt
     return check_prefix(g) >= 0 ? 0 : shared_plan(g).workspace;
 }
 
+extern "C" int nnops_hip_prefix_attention_plan(const NnopsPrefixAttentionArgs* g, NnopsPrefixAttentionPlan* out)
+{
+    if (out == nullptr) {
+        return NNOPS_INVALID_ARGUMENT;
+    }
+    *out = NnopsPrefixAttentionPlan{};
+    if (const int rc = check_prefix(g); rc >= 0) {
+        return rc;
+    }
+    const SharedPlan a = shared_plan(g);
+    const bool both = a.tile_rows == kRows && a.own.tile_rows == kRows;
+    out->shared_rows = a.tile_rows;
+    out->shared_splits = a.splits;
+    out->own_rows = a.own.tile_rows;
+    out->own_splits = a.own.splits;
+    out->launches = !a.few + (both || g->groups == 0 ? 1 : 2) + !a.join_here;
+    out->join = !a.join_here;
+    out->workspace_bytes = a.workspace;
+    return NNOPS_OK;
+}
+
 extern "C" int nnops_hip_prefix_attention(const NnopsPrefixAttentionArgs* g, void* workspace, size_t workspace_bytes,
                                           void* stream)
 {
@@ -412,7 +435,7 @@ extern "C" int nnops_hip_prefix_attention(const NnopsPrefixAttentionArgs* g, voi
     k.members = reinterpret_cast<MemberPlan*>(at + a.members_at);
     k.group_starts = g->group_starts;
     k.shared = g->shared;
-    k.few = g->cache.sequences <= 64 && g->groups <= kFewGroups;
+    k.few = a.few;
     k.join_here = a.join_here;
     k.shared_splits = a.splits;
     k.shared_unit = a.tile_rows == kRows ? 4 : 1;

@@ -4,12 +4,15 @@ what is shared, sequences in no group, prefixes that end inside pages and tiles,
 pages that do not exist, NaN, group starts out of order, strides, graphs."""
 from __future__ import annotations
 
+import ctypes as C
+
 import numpy as np
 import pytest
 
 import datagen as dg
 import decoder_ref as ref
 import nnops_amd as na
+from nnops_amd import _lib as L
 from gpu_util import announce, dev, host, pitched
 
 pytestmark = pytest.mark.gpu
@@ -105,20 +108,69 @@ def test_ragged_rows(d, page, heads, group, f16):
     _check(_q(6, 7, heads * group * d, f16), cache, lens, [1] * 7, groups, shared, ragged=False)
 
 
+def _plan(heads, group, d, page, columns, rows, sequences, groups, f16, ragged):
+    a = L.PrefixAttentionArgs(rows=rows, q_heads=heads * group, f16=int(f16), groups=groups)
+    a.cache = L.KvPages(pages=1, heads=heads, page_tokens=page, head_dim=d, sequences=sequences, table_pages=columns,
+                        row_starts=16 if ragged else None)
+    p = L.PrefixAttentionPlan()
+    assert na.lib().nnops_hip_prefix_attention_plan(C.byref(a), C.byref(p)) == na.OK
+    return p
+
+
 @pytest.mark.parametrize("f16", [True, False])
 @pytest.mark.parametrize("d,page,heads,group", [(128, 64, 2, 8), (128, 16, 2, 8), (64, 64, 2, 8), (64, 16, 4, 8), (256, 64, 1, 8),
-                                                (96, 128, 1, 8), (192, 32, 1, 8)])
+                                                (96, 128, 1, 8), (192, 32, 1, 8), (256, 128, 2, 5)])
 def test_tiles_of_many_rows(d, page, heads, group, f16):
-    """Groups with rows enough for tiles of 128 and of 256 rows, several tiles."""
+    """Groups with rows enough for tiles of 128 and of 256 rows, several tiles. (The
+    choice goes by the table's room: wide ones, of which the sequences fill little.)"""
     announce(f"prefix tiles d={d} page={page} heads={heads} f16={f16}")
     groups, shared = [0, 10], [640]
     lens = [640 + 7 * i + 9 for i in range(10)]
-    cache = _cache(lens, groups, shared, heads, page, d)
-    _check(_q(7, 10, heads * group * d, f16), cache, lens, [1] * 10, groups, shared, ragged=False)
-    rows = [9, 1, 7, 0, 9, 5, 9, 9, 30, 2]
-    _check(_q(8, sum(rows), heads * group * d, f16), cache, lens, rows, groups, shared, ragged=True, pad=4)
-    # the same rows in two groups
-    _check(_q(8, sum(rows), heads * group * d, f16), cache, lens, rows, [0, 4, 10], [640, 500], ragged=True)
+    wide = 2 ** 31 // (10 * heads * group * d * page)
+    cache = _cache(lens, groups, shared, heads, page, d, wide=wide)
+    columns = cache[4].shape[1]
+    tiled = d <= 128 or (f16 and page >= 64)                   # (wider heads: f16, a tile in one page)
+    for rows in ([1] * 10, [9, 1, 7, 0, 9, 5, 9, 9, 30, 2], [40] * 10):
+        p = _plan(heads, group, d, page, columns, sum(rows), 10, 1, f16, True)
+        many = 256 if d <= (128 if f16 else 64) and sum(rows) * group > 128 else 128
+        assert p.shared_rows == (many if tiled and sum(rows) * group > 64 else 16)
+        _check(_q(7, sum(rows), heads * group * d, f16), cache, lens, rows, groups, shared, ragged=True, pad=4)
+        # the same rows in two groups and none, in eight and more
+        _check(_q(8, sum(rows), heads * group * d, f16), cache, lens, rows, [0, 4, 9], [640, 500], ragged=True)
+        many = list(range(11))
+        _check(_q(8, sum(rows), heads * group * d, f16), cache, lens, rows, many, [640] * 10, ragged=True)
+    _check(_q(9, 20, heads * group * d, f16), cache, lens, [2] * 10, groups, shared, ragged=False)
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("d,page,heads,group,members", [(128, 64, 8, 4, 70), (64, 16, 8, 1, 80), (80, 32, 8, 3, 66), (256, 64, 8, 4, 64)])
+def test_own_tokens_join_the_parts(d, page, heads, group, members, f16):
+    """Batches so large that own tokens are not split: where they are looked at, the
+    parts are joined. More than 64 sequences: a kernel finds the plan first."""
+    announce(f"prefix joined d={d} page={page} members={members} f16={f16}")
+    groups, shared = [1, 41, members - 1], [320, 200]
+    lens = [320 + 3 * (i % 20) + 9 for i in range(members)]
+    wide = 2 ** 31 // (members * heads * group * d * page)
+    cache = _cache(lens, groups, shared, heads, page, d, wide=wide)
+    for rows, ragged in (([1] * members, False), ([i % 4 for i in range(members)], True), ([5] * members, True)):
+        p = _plan(heads, group, d, page, cache[4].shape[1], sum(rows), members, 2, f16, ragged)
+        if p.shared_rows != 16 and p.own_splits == 1 and p.own_rows == 16:
+            assert p.join == 0 and p.launches == 2 + (members > 64)
+        q = _q(9, sum(rows), heads * group * d, f16)
+        a = _check(q, cache, lens, rows, groups, shared, ragged=ragged, pad=2)
+        assert np.array_equal(a, _run(q, cache, lens, rows, groups, shared, ragged=ragged).astype(np.float64))
+
+
+def test_every_way_is_reached():
+    """The plans that the tests above are meant for (f16, d 128)."""
+    few = _plan(2, 4, 128, 64, 10, 8, 8, 2, True, False)
+    assert (few.shared_rows, few.own_rows, few.launches, few.join) == (16, 16, 2, 1)
+    many = _plan(8, 4, 128, 64, 600, 64, 64, 1, True, False)
+    assert (many.shared_rows, many.own_rows, many.own_splits, many.launches, many.join) == (256, 16, 1, 2, 0)
+    assert _plan(8, 4, 128, 64, 600, 65, 65, 1, True, False).launches == 3
+    tiles = _plan(8, 4, 128, 64, 600, 6400, 64, 1, True, False)
+    assert (tiles.shared_rows, tiles.own_rows, tiles.launches, tiles.join) == (256, 256, 3, 1)
+    assert _plan(8, 4, 128, 64, 600, 64, 64, 0, True, False).launches == 1
 
 
 @pytest.mark.parametrize("prefix,page,group,members,n", [(6000, 64, 4, 3, 1), (6000, 16, 1, 2, 1), (5100, 128, 8, 5, 2),
