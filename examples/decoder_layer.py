@@ -55,11 +55,14 @@ class DecoderLayer:
         self.linear_add = na.Linear(output_dtype=na.DT_F16, add_to=True)
         self.rotary = na.Rotary(head_dim=head_dim)
         self.write, self.attention = na.KvCacheWrite(), na.CacheAttention(window=window, sinks=sinks)
+        self.prefix_attention = na.PrefixAttention()
 
-    def __call__(self, x, positions, starts, lengths, page_table):
+    def __call__(self, x, positions, starts, lengths, page_table, groups=None):
         """x f16 [T, width]; positions s32 [T]; starts s32 [B + 1], or None where
         every sequence has as many rows; lengths s32 [B] with these rows;
-        page_table s32 [B, pages of a sequence]. Returns the layer's output."""
+        page_table s32 [B, pages of a sequence]; groups: (s32 [G + 1], s32 [G])
+        where sequences share first tokens (without a window). Returns the layer's
+        output."""
         t, d, hq, hk = x.shape[0], self.head_dim, self.heads, self.kv_heads
         new = dict(device=x.device, dtype=torch.float16)
         codes, scale = torch.empty_like(x, dtype=torch.int8), torch.empty(t, device=x.device)
@@ -83,7 +86,10 @@ class DecoderLayer:
                                     T(self.qkv, scale_data=self.qkv_scale, granularity=1)])
         run(self.rotary, [T(qk)], [T(qk), T(positions), T(self.table)])
         run(self.write, pages, [T(k), T(v)] + where + ends)
-        run(self.attention, [T(o)], [T(q)] + pages + where + ends)
+        if groups is None:
+            run(self.attention, [T(o)], [T(q)] + pages + where + ends)
+        else:
+            run(self.prefix_attention, [T(o)], [T(q)] + pages + where + [T(g) for g in groups] + ends)
         run(self.linear, [T(y)], [T(o), self.o])
         run(self.to_f16, [T(normed), T(total)], [T(y), T(self.norm2), T(x)])
         run(self.gated, [T(hidden)], [T(normed), self.up])

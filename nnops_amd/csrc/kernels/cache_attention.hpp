@@ -3,6 +3,7 @@
 #pragma once
 
 #include <limits>
+#include <type_traits>
 
 #include "paged.hpp"
 
@@ -51,7 +52,10 @@ struct AttnKern {
     int32_t tiles;        // of 64 tokens that the page table, or the window, has room for
     int32_t whole;        // tiles of the longest sequence up to which none is split
     int32_t chunk;        // tiles of a split where that sequence fills the table
-    // kShared and kOwn
+};
+
+// Of kShared and kOwn.
+struct PartKern : AttnKern {
     PrefixPlan* plan;     // workspace, as are the next two: written before these launches, or
     GroupPlan* group_plan;   // (`few`) found by each wave, and written by one for the join
     MemberPlan* members;
@@ -63,6 +67,20 @@ struct AttnKern {
     uint32_t shared_unit;        // tiles that a split of them is a multiple of: 4 where waves take every 4th
     uint32_t by_shared_splits;
 };
+
+template <AttnMode M>
+using KernOf = std::conditional_t<M == kWhole, AttnKern, PartKern>;
+
+// Where a launch's parts begin among a row's.
+template <AttnMode M>
+__device__ __forceinline__ int first_part(const KernOf<M>& p)
+{
+    if constexpr (M == kWhole) {
+        return 0;
+    } else {
+        return p.first_part;
+    }
+}
 
 // The tiles of 64 tokens that rows at positions pmin .. pmax look at: the
 // first `sink_tiles`, then those from `first` on, `tiles` in all.
@@ -207,7 +225,7 @@ __device__ __forceinline__ int shared_tokens(const Paged& c, int shared, int len
     return max(min(min(shared, len), least), 0) & ~(max(c.page, kTile) - 1);
 }
 
-__device__ __forceinline__ FewPlan few_plan(const AttnKern& p)
+__device__ __forceinline__ FewPlan few_plan(const PartKern& p)
 {
     const Paged& c = p.c;
     const int lane = threadIdx.x % 64;
@@ -256,17 +274,19 @@ __device__ __forceinline__ FewPlan few_plan(const AttnKern& p)
 // The item-th tile. Later tiles of a sequence look at more tokens: `from_last`
 // numbers them from the last, so that the longest work begins first.
 template <AttnMode M>
-__device__ __forceinline__ bool find_tile(const AttnKern& p, uint32_t item, bool from_last, RowTile& t)
+__device__ __forceinline__ bool find_tile(const KernOf<M>& p, uint32_t item, bool from_last, RowTile& t)
 {
-    int rt, chunk;
-    const int seqs = M == kShared ? p.groups : p.c.seqs;
+    int rt, chunk = 0, seqs = p.c.seqs;
     FewPlan few{};
-    if (M != kWhole && p.few) {
-        few = few_plan(p);
-        if (M == kOwn && item == 0 && blockIdx.y == 0 && threadIdx.x < 64 && (int)threadIdx.x < p.c.seqs) {
-            // (what the join needs; by the first workgroup of each KV head, all the same)
-            p.members[threadIdx.x] = few.member;
-            *p.plan = PrefixPlan{few.shared_chunk, few.own_chunk};
+    if constexpr (M != kWhole) {
+        seqs = M == kShared ? p.groups : seqs;
+        if (p.few) {
+            few = few_plan(p);
+            if (M == kOwn && item == 0 && blockIdx.y == 0 && threadIdx.x < 64 && (int)threadIdx.x < p.c.seqs) {
+                // (what the join needs; by the first workgroup of each KV head, all the same)
+                p.members[threadIdx.x] = few.member;
+                *p.plan = PrefixPlan{few.shared_chunk, few.own_chunk};
+            }
         }
     }
     const auto at = [&](int b) {
@@ -298,7 +318,9 @@ __device__ __forceinline__ bool find_tile(const AttnKern& p, uint32_t item, bool
                 return false;
             }
         }
-        chunk = M == kWhole ? chunk_of(p, t.seq) : 0;
+        if constexpr (M == kWhole) {
+            chunk = chunk_of(p, t.seq);
+        }
     } else {
         int longest = 0;
         const auto count = [&](const SeqRows& s) {
@@ -308,7 +330,9 @@ __device__ __forceinline__ bool find_tile(const AttnKern& p, uint32_t item, bool
         if (!find_item(seqs, item, at, count, t.b, rt, t.seq)) {
             return false;
         }
-        chunk = M == kWhole ? chunk_of(p, t.seq, longest, (t.b / 64 + 1) * 64) : 0;
+        if constexpr (M == kWhole) {
+            chunk = chunk_of(p, t.seq, longest, (t.b / 64 + 1) * 64);
+        }
         rt = from_last ? count(t.seq) - 1 - rt : rt;
     }
     int skip = 0;

@@ -142,7 +142,7 @@ __device__ __forceinline__ void write_result(const AttnKern& p, int64_t token, i
 }
 
 template <typename T, int DP, AttnMode M>
-__device__ __forceinline__ void attend_rows16(const AttnKern& p, WaveParts<DP>& sh, uint32_t block, int split,
+__device__ __forceinline__ void attend_rows16(const KernOf<M>& p, WaveParts<DP>& sh, uint32_t block, int split,
                                               WayParts* join = nullptr)
 {
     constexpr int kC = DP / 64;                    // 64-channel pieces of a key
@@ -448,7 +448,7 @@ __device__ __forceinline__ void attend_rows16(const AttnKern& p, WaveParts<DP>& 
     const int64_t token = seq.start + rtok;
     const int qh = kvh * p.group + (row0 + r - rtok * p.group);
     const bool parts = M != kWhole || rt.split;
-    const int64_t at_part = ((int64_t)(split + (M == kWhole ? 0 : p.first_part)) * c.rows + token) * p.q_heads + qh;
+    const int64_t at_part = ((int64_t)(split + first_part<M>(p)) * c.rows + token) * p.q_heads + qh;
     const float scale = parts ? 1.0f : l == 0.0f ? 0.0f : kDrop / l;
 #pragma unroll
     for (int i = 0; i < DP / 64; ++i) {
@@ -479,7 +479,7 @@ __device__ __forceinline__ void attend_rows16(const AttnKern& p, WaveParts<DP>& 
 }
 
 template <typename T, int DP, AttnMode M>
-__global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void attention_rows16(const AttnKern p)
+__global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void attention_rows16(const KernOf<M> p)
 {
     __shared__ WaveParts<DP> sh;
     if constexpr (M == kOwn) {

@@ -58,7 +58,7 @@ __device__ __forceinline__ V uniform_load(const V* p)
 // kOne: pages of 64 tokens and more, so that a tile lies in one: its number and
 // scales are scalars, its codes at a scalar base and fixed offsets.
 template <typename T, int DP, int NW, bool kOne, AttnMode M>
-__global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const AttnKern p)
+__global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const KernOf<M> p)
 {
     typedef Operand<T> Op;
     typedef typename Op::Vec Vec;

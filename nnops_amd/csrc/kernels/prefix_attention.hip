@@ -20,7 +20,7 @@ namespace {
 constexpr int kPlanThreads = 1024;
 
 struct PrefixKern {
-    AttnKern own;
+    PartKern own;
     int32_t* starts;      // workspace: group_starts, in order and in range
     int32_t ways;         // of the join: parts of a row that are summed side by side
 };
@@ -43,7 +43,7 @@ __device__ __forceinline__ int group_max(int v, int* s_waves)
 __global__ __launch_bounds__(kPlanThreads) void prefix_plan(const PrefixKern p)
 {
     __shared__ int s_waves[kPlanThreads / 64];
-    const AttnKern& k = p.own;
+    const PartKern& k = p.own;
     const Paged& c = k.c;
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
     // starts that do not go back
@@ -127,7 +127,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void prefix_join(const PrefixKern p)
 {
     __shared__ WayParts sh;
-    const AttnKern& k = p.own;
+    const PartKern& k = p.own;
     const Paged& c = k.c;
     const int lanes = join_lanes(c.d), slot = threadIdx.x / (uint32_t)lanes, ways = p.ways;
     const int way = slot % ways, per_block = 256 / lanes / ways;
@@ -263,7 +263,7 @@ SharedPlan shared_plan(const NnopsPrefixAttentionArgs* g)
 }
 
 template <typename T, int DP, int NW, AttnMode M>
-void launch_tiled_one(const AttnKern& k, const dim3& grid, hipStream_t s)
+void launch_tiled_one(const PartKern& k, const dim3& grid, hipStream_t s)
 {
     if (DP > 128 || tiled_one_page(k.c.d, k.c.page)) {
         NNOPS_LAUNCH((attention_rows_tiled<T, DP, NW, true, M>), grid, dim3(64 * NW), 0, s, k);
@@ -274,7 +274,7 @@ void launch_tiled_one(const AttnKern& k, const dim3& grid, hipStream_t s)
 
 // (the kernels that tiled_rows names, and 16 rows a workgroup)
 template <typename T, AttnMode M>
-void launch_part(const AttnKern& k, const dim3& grid, hipStream_t s)
+void launch_part(const PartKern& k, const dim3& grid, hipStream_t s)
 {
     const int d = k.c.d;
     if (k.tile_rows == kRows) {
@@ -306,7 +306,7 @@ uint32_t reciprocal(int n) { return n > 1 ? (uint32_t)(((1ull << 32) + n - 1) / 
 // `shared` workgroups, `items` a split, and those behind them.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void attention_both16(
-    const AttnKern s, const AttnKern o, uint32_t items, uint32_t shared, uint32_t own_items)
+    const PartKern s, const PartKern o, uint32_t items, uint32_t shared, uint32_t own_items)
 {
     __shared__ WaveParts<DP> sh;
     if (blockIdx.x < shared) {
@@ -324,7 +324,7 @@ void launch_prefix(const PrefixKern& p, const SharedPlan& a, hipStream_t s)
     if (!p.own.few) {
         NNOPS_LAUNCH(prefix_plan, dim3(1), dim3(kPlanThreads), 0, s, p);
     }
-    AttnKern k = p.own;
+    PartKern k = p.own;
     k.tile_rows = a.tile_rows;
     k.per_seq = a.per_seq;
     k.first_part = 0;
@@ -411,7 +411,7 @@ extern "C" int nnops_hip_prefix_attention(const NnopsPrefixAttentionArgs* g, voi
     PrefixKern p{};
     p.starts = reinterpret_cast<int32_t*>(at + a.starts_at);
     p.ways = a.ways;
-    AttnKern& k = p.own;
+    PartKern& k = p.own;
     k.c = paged(g->cache, g->rows);
     k.q = g->q;
     k.out = g->out;
