@@ -53,7 +53,8 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan(const PrefixKern p)
         int v = g <= k.groups && k.groups > 0 ? min(max(k.group_starts[g], 0), c.seqs) : 0;
 #pragma unroll
         for (int m = 1; m < 64; m *= 2) {
-            v = max(v, lane >= m ? __shfl_up(v, m) : 0);
+            const int before = __shfl_up(v, m);    // (by all lanes: one that takes no part gives nothing)
+            v = lane >= m ? max(v, before) : v;
         }
         __syncthreads();
         if (lane == 63) {

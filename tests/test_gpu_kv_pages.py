@@ -152,6 +152,7 @@ def test_fork_of_tables_that_hold_no_pages(pages):
     (40, 1100, 3, 4, 2500),                # more children than the workgroup has threads
     (2, 3, 2, 2, 70000),                   # more pages than one step looks at
     (20, 30, 3, 4, 12288), (20, 30, 3, 4, 12289), (1024, 1024, 3, 4, 9000), (3, 2, 9000, 9001, 3000),
+    (300, 16384, 2, 2, 60000), (16384, 100, 1, 2, 14000), (1025, 3, 1, 1, 1100), (3, 1025, 1, 1, 1100),
     (1500, 7, 2, 3, 4000), (5, 0, 3, 2, 50), (0, 6, 0, 5, 60), (4, 4, 3, 0, 50), (3, 2, 4, 4, 0), (0, 0, 0, 0, 0)])
 def test_fork_sizes(b, n, wide, out_wide, pages):
     announce(f"fork sizes {b} {n} {wide} {out_wide} {pages}")

@@ -219,6 +219,59 @@ def test_group_starts_out_of_order():
         shared = [150] * (len(groups) - 1)
         got = _check(q, cache, lens, [1] * 6, groups, shared, ragged=False)
         assert np.max(abs(got - want)) <= 2.0 ** -9 * np.max(abs(want))
+    # more sequences and groups than a wave finds the plan of, past one step of 1024
+    lens = [150 + i % 70 for i in range(90)]
+    cache = _cache(lens, [0, 90], [140], heads, page, d)
+    q = _q(12, 90, heads * group * d, True)
+    r = np.random.RandomState(4)
+    starts = np.sort(r.randint(0, 91, 1500))
+    for groups in ([0, 40, 20, 90], [89, 3, 90], list(starts), list(r.permutation(starts)), [7] * 1200 + [90, 3, 90]):
+        _check(q, cache, lens, [1] * 90, groups, [140] * (len(groups) - 1), ragged=False)
+
+
+def test_a_bad_row_shows_in_itself_only():
+    """NaN and infinite queries, in 16-row workgroups and in tiles."""
+    announce("prefix bad rows")
+    heads, group, d, page, members = 2, 8, 64, 64, 12
+    lens = [400 + 7 * i for i in range(members)]
+    for wide in (0, 2 ** 31 // (members * heads * group * d * page)):
+        cache = _cache(lens, [0, members], [384], heads, page, d, wide=wide)
+        q = _q(16, members, heads * group * d, True)
+        want = _check(q, cache, lens, [1] * members, [0, members], [384], ragged=False)
+        q[3, 5], q[7, 70] = np.nan, np.inf
+        got = _run(q, cache, lens, [1] * members, [0, members], [384], ragged=False).astype(np.float64)
+        bad = np.zeros(got.shape, bool)
+        bad[3, :d], bad[7, d:2 * d] = True, True
+        assert np.isnan(got[bad]).all() and np.array_equal(got[~bad], want[~bad])
+
+
+def test_pitched_tables_and_caches_past_32_bits():
+    """A page table that is part of a wider one; pages that lie past 4 GiB."""
+    import torch
+    announce("prefix pitched tables, large cache")
+    heads, group, d, page, pages = 8, 2, 128, 256, 17000
+    k = torch.zeros((pages, heads, page, d), dtype=torch.int8, device="cuda")
+    v = torch.zeros((pages, heads, d, page), dtype=torch.int8, device="cuda")
+    assert k.numel() > 2 ** 32
+    lens, groups, shared = [600, 530, 513], [0, 3], [512]
+    used = [16999, 16500, 3, 16998, 9]
+    table = np.array([[16999, 16500, 3], [16999, 16500, 16998], [16999, 16500, 9]], np.int32)
+    small = _cache([1280], [0, 1], [0], heads, page, d, spare=0)
+    kc, vc, ks, vs, _ = small
+    scales = [torch.zeros((pages, heads), device="cuda") for _ in range(2)]
+    for i, p in enumerate(used):
+        k[p], v[p] = dev(kc[i]), dev(vc[i])
+        scales[0][p], scales[1][p] = dev(ks[i]), dev(vs[i])
+    near = np.vectorize(used.index)(table)
+    q = _q(17, 3, heads * group * d, True)
+    out = torch.empty(q.shape, dtype=torch.float16, device="cuda")
+    wide = pitched(table, 11)
+    ins = [dev(q), k, v, *scales, wide] + [dev(np.array(x, np.int32)) for x in (lens, groups, shared)]
+    assert na.PrefixAttention().compute([na.tensor(out)], [na.tensor(x) for x in ins]) == na.OK
+    torch.cuda.synchronize()
+    want, weight, spread = ref.attention(q, kc, vc, ks, vs, near, lens, [1] * 3)
+    assert (abs(host(out) - want) <= ref.attention_tolerance(True, want, weight, spread, vs)).all()
+    del k, v
 
 
 def test_rows_of_no_sequence_are_left_alone():

@@ -180,7 +180,14 @@ def test_given_tokens():
     bad = x.copy()
     bad[0, 0] = np.nan
     assert _run(bad, tokens, 0)[0][0, 0] == 0.0
-    op, T = na.TokenLogProbs(), na.tensor
+    wide = torch.full((3, 900), 5, dtype=torch.int32, device="cuda")
+    wide[:, 100:800] = dev(tokens)
+    lp, h = torch.empty((3, 700), device="cuda"), torch.empty(3, device="cuda")
+    T = na.tensor
+    assert na.TokenLogProbs().compute([T(lp), T(h)], [T(dev(x)), T(wide[:, 100:800])]) == na.OK
+    torch.cuda.synchronize()
+    assert np.array_equal(host(lp), got[0], equal_nan=True)
+    op = na.TokenLogProbs()
     none = torch.empty((3, 0), dtype=torch.int32, device="cuda")
     h = torch.empty(3, device="cuda")
     assert op.compute([T(none.float()), T(h)], [T(dev(x)), T(none)]) == na.OK
