@@ -8,9 +8,14 @@
 // tokens that would read a prompt once per sequence become a tile of up to 256
 // rows that the matrix cores bound.
 //
-// Which tokens are shared is found on the device first, by one workgroup: whole
-// tiles and whole pages that every row of the group sees. Rows then need no mask,
-// and a sequence's own tokens begin at a tile.
+// Which tokens are shared is found on the device: whole tiles and whole pages that
+// every row of the group sees. Rows then need no mask, and a sequence's own tokens
+// begin at a tile. Every wave finds it for few sequences (a launch less: 4 sequences of
+// 1990 16 -> 12.6 us), one workgroup before the others for more.
+// Measured, 32 query and 8 KV heads of 128, f16: 64 sequences of a token each, 32768
+// shared and up to 400 of their own: 70 us (without sharing 4.3 GB would be read: 900),
+// of which the shared tokens 54 (34.4 GFLOP) and the rest with the join 17 to 22; 4 of a
+// token each, 1900 and up to 90: 12.4; 530 rows over 8000: 118.
 #include "cache_attention_rows.hpp"
 #include "cache_attention_tiled.hpp"
 
