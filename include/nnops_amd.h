@@ -531,10 +531,12 @@ int nnops_hip_cache_attention(const NnopsCacheAttentionArgs* args, void* workspa
  * group_starts and shared are device memory that the host does not see; starts
  * are taken into [0, sequences], no group begins before the last one's end, and
  * what is shared beyond the first sequence's tokens is not.
+ * Where the page table has room for so few tokens that reading them once saves
+ * nothing, every sequence is looked at by itself.
  * Probabilities of f16 rows enter the second product as one f16 where a group's
  * or sequence's rows share their tiles, as two where not. The workspace holds
  * the parts of all rows: nnops_hip_prefix_attention_workspace_size bytes, 16-byte
- * aligned, which need no initialization. */
+ * aligned, which need no initialization (0: none is needed). */
 typedef struct NnopsPrefixAttentionArgs {
     NnopsKvPages cache;
     const void* q;              /* [rows][ld_q] f16 (f16) or f32 */
@@ -700,7 +702,8 @@ typedef struct NnopsCacheAttentionPlan {
 } NnopsCacheAttentionPlan;
 
 typedef struct NnopsPrefixAttentionPlan {
-    int32_t shared_rows;        /* rows of a workgroup over the shared tokens: 16, 128 or 256 */
+    int32_t shared_rows;        /* rows of a workgroup over the shared tokens: 16, 128 or 256; 0: the table has so
+                                   little room that every sequence is looked at by itself */
     int32_t shared_splits;      /* of these tokens, at most */
     int32_t own_rows;           /* and over each sequence's own tokens */
     int32_t own_splits;

@@ -234,7 +234,7 @@ __device__ __forceinline__ FewPlan few_plan(const PartKern& p)
     if (lane < c.seqs) {
         f.seq = seq_rows(c, lane);
     }
-    int starts = p.groups > 0 ? min(max(p.group_starts[min(lane, p.groups)], 0), c.seqs) : 0;
+    int starts = min(max(p.group_starts[min(lane, p.groups)], 0), c.seqs);
     const int shared = lane < p.groups ? p.shared[lane] : 0;
 #pragma unroll
     for (int m = 1; m <= kFewGroups; m *= 2) {     // (starts do not go back)

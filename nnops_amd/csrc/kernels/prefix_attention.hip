@@ -13,9 +13,9 @@
 // begin at a tile. Every wave finds it for few sequences (a launch less: 4 sequences of
 // 1990 16 -> 12.6 us), one workgroup before the others for more.
 // Measured, 32 query and 8 KV heads of 128, f16: 64 sequences of a token each, 32768
-// shared and up to 400 of their own: 70 us (without sharing 4.3 GB would be read: 900),
-// of which the shared tokens 54 (34.4 GFLOP) and the rest with the join 17 to 22; 4 of a
-// token each, 1900 and up to 90: 12.4; 530 rows over 8000: 118.
+// shared and up to 400 of their own: 70 us (each sequence by itself: 406), of which the
+// shared tokens 54 (34.4 GFLOP) and the rest with the join 17 to 22; 530 rows over 8000: 118
+// (289).
 #include "cache_attention_rows.hpp"
 #include "cache_attention_tiled.hpp"
 
@@ -55,7 +55,7 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan(const PrefixKern p)
     int so_far = 0;
     for (int base = 0; base <= k.groups; base += kPlanThreads) {
         const int g = base + tid;
-        int v = g <= k.groups && k.groups > 0 ? min(max(k.group_starts[g], 0), c.seqs) : 0;
+        int v = g <= k.groups ? min(max(k.group_starts[g], 0), c.seqs) : 0;
 #pragma unroll
         for (int m = 1; m < 64; m *= 2) {
             const int before = __shfl_up(v, m);    // (by all lanes: one that takes no part gives nothing)
@@ -179,6 +179,7 @@ struct SharedPlan {
     AttnPlan own;
     int64_t items;        // tiles of the groups' rows, all KV heads
     int32_t tile_rows, per_seq, splits, ways;
+    bool share;           // else: as CacheAttention, every sequence by itself
     bool few;             // every wave finds the plan
     bool join_here;       // own tokens, 16 rows a workgroup and unsplit: they join the parts themselves
     size_t groups_at, members_at, starts_at, parts_at, workspace;
@@ -213,13 +214,55 @@ int check_prefix(const NnopsPrefixAttentionArgs* g)
 
 size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 
+// Whether what is shared is read once, or each sequence looked at by itself, which the
+// tables allow. Both read as many tokens as the table has room for, a tile of rows at
+// a time, and full or not, a tile takes the same time: sharing pays where it fills tiles
+// that a sequence's rows fill in part, or makes them larger, and costs the parts of every
+// row. The rates are those of the kernels, of a row, token and channel (and 64 more for
+// the softmax). Measured, by itself / shared in us, what is taken marked *; n sequences of
+// r tokens, 32 query and 8 KV heads of 128, 500, 2000 and 8000 shared tokens:
+//   f16, 4 x 1     *10.6 / 12.3    *13.0 / 12.6    17.4 / *17.0
+//        16 x 1    *12.1 / 12.0    18.8 / *15.1    35.7 / *21.4
+//        48 x 1    15.9 / *15.6    31.1 / *20.6    77.5 / *35.4
+//        48 x 3    *17.6 / 20.4    *31.9 / 34.2    79.1 / *56.1
+//        48 x 8    *18.1 / 31.7    43.6 / *41.8    140 / *79.8
+//        48 x 33   *40.7 / 64.3    *114 / 115      403 / *308
+//        48 x 97   *71.4 / 160     *199 / 307      *703 / 791
+//        16 x up to 97 *32.7 / 55.6 88.4 / *70.5  310 / *156
+//   f32, 48 x 1    19.6 / *19.7    35.3 / *24.9    92.0 / *38.6
+//        48 x 33   *97.6 / 114     301 / *238      1099 / *651
+// Over 179 calls of such sizes and of 8 and 2 heads of 64, what is taken is 1 % slower than the
+// faster one in the mean, 14 % if it always were the one, 13 % the other.
+bool sharing_pays(const NnopsPrefixAttentionArgs& g, const SharedPlan& a)
+{
+    const double d = (double)g.cache.head_dim, seqs = (double)g.cache.sequences, groups = (double)g.groups;
+    const double rows = (double)g.rows * g.q_heads / g.cache.heads;
+    const double work = (double)g.cache.heads * (d + 64) * g.cache.table_pages * g.cache.page_tokens;
+    const auto rate = [&](int tile) { return tile == kRows ? g.f16 ? 1.0e8 : 1.1e8 : g.f16 ? 4.5e8 : 1.35e8; };   // a us
+    // rows that tiles hold, `of` in equal shares or of unknown ones
+    const auto held = [&](double of, double tile, bool equal) {
+        const double share = rows / of;
+        return of * (equal ? __builtin_ceil(share / tile) * tile : share + tile / 2 > tile ? share + tile / 2 : tile);
+    };
+    const double part = 0.85e-6 * 4 * g.rows * g.q_heads * d;             // us, written and read
+    const double alone = held(seqs, a.own.tile_rows, g.cache.row_starts == nullptr) * work / rate(a.own.tile_rows) +
+                         (a.own.splits > 1 ? a.own.splits * part : 0);
+    const double shared = held(groups, a.tile_rows, g.groups == 1) * work / rate(a.tile_rows) +
+                          (a.splits + (a.join_here ? 0 : a.own.splits)) * part + 1.2;
+    return shared < alone;
+}
+
 SharedPlan shared_plan(const NnopsPrefixAttentionArgs* g)
 {
     SharedPlan a{};
     const NnopsCacheAttentionArgs whole = whole_args(*g);
     a.own = attn_plan(&whole);
     const int64_t heads = g->cache.heads, group = g->q_heads / heads, d = g->cache.head_dim;
-    const int64_t groups = g->groups > 0 ? g->groups : 1;
+    if (g->groups == 0) {
+        a.workspace = a.own.workspace;
+        return a;
+    }
+    const int64_t groups = g->groups;
     const int64_t mean = (g->rows * group + groups - 1) / groups;
     // Tiles of many rows where they fill more than a quarter and there is work enough for
     // their longer beginning and end; 16 rows a workgroup otherwise, in one launch with
@@ -231,7 +274,7 @@ SharedPlan shared_plan(const NnopsPrefixAttentionArgs* g)
     const bool much = (double)g->rows * g->q_heads * d * room >= 0x1p31;
     const int rows = mean > 64 && much ? tiled_rows(d, g->f16, g->cache.page_tokens, mean) : 0;
     a.tile_rows = rows > 0 ? rows : kRows;
-    if (g->groups <= 1) {
+    if (groups == 1) {
         a.per_seq = (int32_t)((g->rows * group + a.tile_rows - 1) / a.tile_rows);
         a.items = a.per_seq * heads;
     } else {
@@ -254,6 +297,11 @@ SharedPlan shared_plan(const NnopsPrefixAttentionArgs* g)
     a.few = g->cache.sequences <= 64 && g->groups <= kFewGroups;
     a.join_here = a.tile_rows != kRows && a.own.tile_rows == kRows && a.own.splits == 1;
     const int64_t parts = a.splits + (a.join_here ? 0 : a.own.splits);
+    a.share = sharing_pays(*g, a);
+    if (!a.share) {
+        a.workspace = a.own.workspace;
+        return a;
+    }
     // workgroups to fill the chip, as long as each lane has a batch of parts
     const int lanes = join_lanes((int)d);
     a.ways = 1;
@@ -334,7 +382,7 @@ void launch_prefix(const PrefixKern& p, const SharedPlan& a, hipStream_t s)
     k.tile_rows = a.tile_rows;
     k.per_seq = a.per_seq;
     k.first_part = 0;
-    const uint32_t shared = k.groups > 0 ? (uint32_t)(a.items * a.splits) : 0, own = (uint32_t)(a.own.items * a.own.splits);
+    const uint32_t shared = (uint32_t)(a.items * a.splits), own = (uint32_t)(a.own.items * a.own.splits);
     if (a.tile_rows == kRows && p.own.tile_rows == kRows) {
         const dim3 grid(shared + own);
         const uint32_t items = (uint32_t)a.items, own_items = (uint32_t)a.own.items;
@@ -346,9 +394,7 @@ void launch_prefix(const PrefixKern& p, const SharedPlan& a, hipStream_t s)
             NNOPS_LAUNCH((attention_both16<T, 256>), grid, dim3(256), 0, s, k, p.own, items, shared, own_items);
         }
     } else {
-        if (shared > 0) {
-            launch_part<T, kShared>(k, dim3((unsigned)a.items, (unsigned)a.splits), s);
-        }
+        launch_part<T, kShared>(k, dim3((unsigned)a.items, (unsigned)a.splits), s);
         launch_part<T, kOwn>(p.own, dim3((unsigned)a.own.items, (unsigned)a.own.splits), s);
         if (p.own.join_here) {
             return;
@@ -379,14 +425,19 @@ extern "C" int nnops_hip_prefix_attention_plan(const NnopsPrefixAttentionArgs* g
         return rc;
     }
     const SharedPlan a = shared_plan(g);
+    out->own_rows = a.own.tile_rows;
+    out->own_splits = a.own.splits;
+    out->workspace_bytes = a.workspace;
+    if (!a.share) {
+        out->launches = 1 + (a.own.splits > 1);
+        out->join = a.own.splits > 1;
+        return NNOPS_OK;
+    }
     const bool both = a.tile_rows == kRows && a.own.tile_rows == kRows;
     out->shared_rows = a.tile_rows;
     out->shared_splits = a.splits;
-    out->own_rows = a.own.tile_rows;
-    out->own_splits = a.own.splits;
-    out->launches = !a.few + (both || g->groups == 0 ? 1 : 2) + !a.join_here;
+    out->launches = !a.few + (both ? 1 : 2) + !a.join_here;
     out->join = !a.join_here;
-    out->workspace_bytes = a.workspace;
     return NNOPS_OK;
 }
 
@@ -406,6 +457,10 @@ extern "C" int nnops_hip_prefix_attention(const NnopsPrefixAttentionArgs* g, voi
         return NNOPS_INVALID_ARGUMENT;
     }
     const SharedPlan a = shared_plan(g);
+    if (!a.share) {
+        const NnopsCacheAttentionArgs whole = whole_args(*g);
+        return nnops_hip_cache_attention(&whole, workspace, workspace_bytes, stream);
+    }
     if (a.own.items * a.own.splits > INT32_MAX / 512 || a.items * a.splits > INT32_MAX / 512 || a.own.splits > 65535 || a.splits > 65535 ||
         g->rows * g->q_heads > INT32_MAX / 256) {
         return NNOPS_UNSUPPORTED;

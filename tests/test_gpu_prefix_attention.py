@@ -1,7 +1,9 @@
 """PrefixAttention against attention in 64 bits over each sequence's own tokens:
 groups of different sizes and prefixes, single tokens and ragged rows, rows inside
 what is shared, sequences in no group, prefixes that end inside pages and tiles,
-pages that do not exist, NaN, group starts out of order, strides, graphs."""
+pages that do not exist, NaN, group starts out of order, strides, graphs. Where a
+table has little room every sequence is looked at by itself: the tests widen theirs
+so that what is shared is read once, and make the call with the narrow one too."""
 from __future__ import annotations
 
 import ctypes as C
@@ -38,9 +40,37 @@ def _cache(lens, groups, shared, heads, page, d, seed=1, spare=2, wide=0):
     return kc, vc, ks, vs, table
 
 
-def _run(q, cache, lens, rows, groups, shared, *, ragged, pad=0, scale=0.0, stream=None):
+def _plan(heads, group, d, page, columns, rows, sequences, groups, f16, ragged):
+    a = L.PrefixAttentionArgs(rows=rows, q_heads=heads * group, f16=int(f16), groups=groups)
+    a.cache = L.KvPages(pages=1, heads=heads, page_tokens=page, head_dim=d, sequences=sequences, table_pages=columns,
+                        row_starts=16 if ragged else None)
+    p = L.PrefixAttentionPlan()
+    assert na.lib().nnops_hip_prefix_attention_plan(C.byref(a), C.byref(p)) == na.OK
+    return p
+
+
+def _widened(q, cache, lens, groups, ragged):
+    """The table with columns enough that what is shared is read once, which no number
+    is where each sequence's rows (nearly) fill tiles, or groups are hardly more than one."""
+    kc, table = cache[0], cache[4]
+    _, heads, page, d = kc.shape
+    columns, seqs, n = table.shape[1], len(lens), len(groups) - 1
+    group = q.shape[1] // heads // d
+
+    def plan(columns):
+        return _plan(heads, group, d, page, columns, q.shape[0], seqs, n, q.dtype == np.float16, ragged)
+    while plan(columns).shared_rows == 0 and columns * seqs < 2 ** 25:
+        columns += columns // 4 + 1
+    full = q.shape[0] * group > 64 * seqs or not ragged and q.shape[0] // seqs * group % 16 == 0
+    assert plan(columns).shared_rows or full or 2 * n > seqs
+    return np.pad(table, ((0, 0), (0, columns - table.shape[1])), constant_values=-1)
+
+
+def _run(q, cache, lens, rows, groups, shared, *, ragged, pad=0, scale=0.0, stream=None, share=True):
     import torch
     kc, vc, ks, vs, table = cache
+    if share and len(groups) - 1 in range(1, len(lens)):
+        table = _widened(q, cache, lens, groups, ragged)
     starts = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
     dq = pitched(q, q.shape[1] + pad)
     out = pitched(np.full(q.shape, 7, q.dtype), q.shape[1] + 2 * pad)
@@ -56,13 +86,14 @@ def _run(q, cache, lens, rows, groups, shared, *, ragged, pad=0, scale=0.0, stre
 
 
 def _check(q, cache, lens, rows, groups, shared, *, scale=0.0, **kw):
-    got = _run(q, cache, lens, rows, groups, shared, scale=scale, **kw).astype(np.float64)
     want, weight, spread = ref.attention(q, *cache, lens, rows, scale=scale or None)
     tol = ref.attention_tolerance(q.dtype == np.float16, want, weight, spread, cache[3])
-    assert np.array_equal(np.isnan(got), np.isnan(want))
     ok = ~np.isnan(want)
-    worst = np.max((abs(got - want) / tol)[ok]) if ok.any() else 0.0
-    assert worst <= 1.0, worst
+    for share in (False, True):
+        got = _run(q, cache, lens, rows, groups, shared, scale=scale, share=share, **kw).astype(np.float64)
+        assert np.array_equal(np.isnan(got), np.isnan(want)), share
+        worst = np.max((abs(got - want) / tol)[ok]) if ok.any() else 0.0
+        assert worst <= 1.0, (share, worst)
     return got
 
 
@@ -85,7 +116,7 @@ def test_single_tokens(d, page, heads, group, f16):
     q = _q(3, len(lens), heads * group * d, f16)
     a = _check(q, cache, lens, [1] * 8, groups, shared, ragged=False)
     b = _check(q, cache, lens, [1] * 8, groups, shared, ragged=True, pad=3)
-    assert np.array_equal(a, b)
+    assert np.array_equal(a, b) or group >= 16             # (rows that nearly fill tiles: one of them by itself)
 
 
 @pytest.mark.parametrize("f16", [True, False])
@@ -108,15 +139,6 @@ def test_ragged_rows(d, page, heads, group, f16):
     _check(_q(6, 7, heads * group * d, f16), cache, lens, [1] * 7, groups, shared, ragged=False)
 
 
-def _plan(heads, group, d, page, columns, rows, sequences, groups, f16, ragged):
-    a = L.PrefixAttentionArgs(rows=rows, q_heads=heads * group, f16=int(f16), groups=groups)
-    a.cache = L.KvPages(pages=1, heads=heads, page_tokens=page, head_dim=d, sequences=sequences, table_pages=columns,
-                        row_starts=16 if ragged else None)
-    p = L.PrefixAttentionPlan()
-    assert na.lib().nnops_hip_prefix_attention_plan(C.byref(a), C.byref(p)) == na.OK
-    return p
-
-
 @pytest.mark.parametrize("f16", [True, False])
 @pytest.mark.parametrize("d,page,heads,group", [(128, 64, 2, 8), (128, 16, 2, 8), (64, 64, 2, 8), (64, 16, 4, 8), (256, 64, 1, 8),
                                                 (96, 128, 1, 8), (192, 32, 1, 8), (256, 128, 2, 5)])
@@ -135,10 +157,9 @@ def test_tiles_of_many_rows(d, page, heads, group, f16):
         many = 256 if d <= (128 if f16 else 64) and sum(rows) * group > 128 else 128
         assert p.shared_rows == (many if tiled and sum(rows) * group > 64 else 16)
         _check(_q(7, sum(rows), heads * group * d, f16), cache, lens, rows, groups, shared, ragged=True, pad=4)
-        # the same rows in two groups and none, in eight and more
-        _check(_q(8, sum(rows), heads * group * d, f16), cache, lens, rows, [0, 4, 9], [640, 500], ragged=True)
-        many = list(range(11))
-        _check(_q(8, sum(rows), heads * group * d, f16), cache, lens, rows, many, [640] * 10, ragged=True)
+        # the same rows in two groups and none, in nine, in as many as there are sequences
+        for starts, of in (([0, 4, 9], [640, 500]), ([0, 2, 3, 4, 5, 6, 7, 8, 9, 10], [640] * 9), (list(range(11)), [640] * 10)):
+            _check(_q(8, sum(rows), heads * group * d, f16), cache, lens, rows, starts, of, ragged=True)
     _check(_q(9, 20, heads * group * d, f16), cache, lens, [2] * 10, groups, shared, ragged=False)
 
 
@@ -163,14 +184,19 @@ def test_own_tokens_join_the_parts(d, page, heads, group, members, f16):
 
 def test_every_way_is_reached():
     """The plans that the tests above are meant for (f16, d 128)."""
-    few = _plan(2, 4, 128, 64, 10, 8, 8, 2, True, False)
+    few = _plan(2, 4, 128, 64, 100, 8, 8, 2, True, False)
     assert (few.shared_rows, few.own_rows, few.launches, few.join) == (16, 16, 2, 1)
+    alone = _plan(2, 4, 128, 64, 1, 8, 8, 2, True, False)
+    assert (alone.shared_rows, alone.own_splits, alone.launches, alone.join, alone.workspace_bytes) == (0, 1, 1, 0, 0)
+    alone = _plan(2, 4, 128, 64, 10, 8, 8, 2, True, False)
+    assert (alone.shared_rows, alone.launches, alone.join) == (0, 2, 1) and alone.workspace_bytes > 0
+    assert _plan(8, 4, 128, 64, 600, 64, 64, 64, True, False).shared_rows == 0         # nothing is read twice
     many = _plan(8, 4, 128, 64, 600, 64, 64, 1, True, False)
     assert (many.shared_rows, many.own_rows, many.own_splits, many.launches, many.join) == (256, 16, 1, 2, 0)
     assert _plan(8, 4, 128, 64, 600, 65, 65, 1, True, False).launches == 3
     tiles = _plan(8, 4, 128, 64, 600, 6400, 64, 1, True, False)
     assert (tiles.shared_rows, tiles.own_rows, tiles.launches, tiles.join) == (256, 256, 3, 1)
-    assert _plan(8, 4, 128, 64, 600, 64, 64, 0, True, False).launches == 1
+    assert _plan(8, 4, 128, 64, 600, 64, 64, 0, True, False).shared_rows == 0
 
 
 @pytest.mark.parametrize("prefix,page,group,members,n", [(6000, 64, 4, 3, 1), (6000, 16, 1, 2, 1), (5100, 128, 8, 5, 2),
@@ -224,9 +250,16 @@ def test_group_starts_out_of_order():
     cache = _cache(lens, [0, 90], [140], heads, page, d)
     q = _q(12, 90, heads * group * d, True)
     r = np.random.RandomState(4)
-    starts = np.sort(r.randint(0, 91, 1500))
-    for groups in ([0, 40, 20, 90], [89, 3, 90], list(starts), list(r.permutation(starts)), [7] * 1200 + [90, 3, 90]):
+    starts = np.sort(r.randint(0, 91, 80))
+    for groups in ([0, 40, 20, 90], [89, 3, 90], list(starts), list(r.permutation(starts)), [7] * 60 + [90, 3, 90],
+                   [7] * 1200 + [90, 3, 90]):
         _check(q, cache, lens, [1] * 90, groups, [140] * (len(groups) - 1), ragged=False)
+    lens = [50 + i % 70 for i in range(1300)]
+    cache = _cache(lens, [0, 1300], [48], heads, page, d)
+    q = _q(13, 1300, heads * group * d, True)
+    starts = np.sort(r.randint(0, 1301, 1200))
+    for groups in (list(starts), list(r.permutation(starts)), [700] * 1150 + [1300, 3, 1300]):
+        _check(q, cache, lens, [1] * 1300, groups, [48] * (len(groups) - 1), ragged=False)
 
 
 def test_a_bad_row_shows_in_itself_only():
@@ -265,7 +298,8 @@ def test_pitched_tables_and_caches_past_32_bits():
     near = np.vectorize(used.index)(table)
     q = _q(17, 3, heads * group * d, True)
     out = torch.empty(q.shape, dtype=torch.float16, device="cuda")
-    wide = pitched(table, 11)
+    wide = pitched(np.pad(table, ((0, 0), (0, 20)), constant_values=-1), 31)
+    assert _plan(heads, group, d, page, 23, 3, 3, 1, True, False).shared_rows == 16
     ins = [dev(q), k, v, *scales, wide] + [dev(np.array(x, np.int32)) for x in (lens, groups, shared)]
     assert na.PrefixAttention().compute([na.tensor(out)], [na.tensor(x) for x in ins]) == na.OK
     torch.cuda.synchronize()
@@ -278,7 +312,13 @@ def test_rows_of_no_sequence_are_left_alone():
     announce("prefix rows left")
     heads, group, d, page = 1, 2, 64, 16
     lens, rows = [200, 210], [2, 1]
-    cache = _cache(lens, [0, 2], [190], heads, page, d)
+    for wide in (0, 30000):
+        _rows_left(heads, group, d, page, lens, rows, _cache(lens, [0, 2], [190], heads, page, d, wide=wide))
+
+
+def _rows_left(heads, group, d, page, lens, rows, cache):
+    plan = _plan(heads, group, d, page, cache[4].shape[1], 8, 2, 1, True, True)
+    assert plan.shared_rows == (16 if cache[4].shape[1] > 30000 else 0)
     q = _q(12, 8, heads * group * d, True)
     import torch
     out = torch.full(q.shape, 7.0, dtype=torch.float16, device="cuda")
@@ -342,7 +382,8 @@ def test_graph_streams_and_repeats():
     heads, group, d, page, members = 2, 4, 64, 16, 12
     groups, shared = [0, 5, members], [700, 300]
     lens = [701 + 3 * i for i in range(5)] + [301 + 50 * i for i in range(7)]
-    cache = _cache([n + 100 for n in lens], groups, shared, heads, page, d, wide=40)
+    cache = _cache([n + 100 for n in lens], groups, shared, heads, page, d, wide=500)
+    assert _plan(heads, group, d, page, cache[4].shape[1], members, members, 2, True, False).shared_rows == 16
     q = _q(15, members, heads * group * d, True)
     T = na.tensor
     runs = []

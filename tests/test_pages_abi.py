@@ -91,7 +91,7 @@ def test_prefix_attention_rules():
     assert op.output_descs(ins) == [([6, 512], F16)]
     assert op.validate(ins, [q]) == na.OK
     assert op.validate(ins + [desc([4], S32)], [q]) == na.OK
-    assert op.workspace_size(ins, [q]) > 2 * 6 * 8 * 66 * 4 - 1
+    assert op.workspace_size(ins, [q]) == 0                                         # little room: nothing is read once
     assert op.validate([q] + c + tables() + [desc([1], S32), desc([0], S32)], [q]) == na.OK
     for g in ([desc([2], S32), desc([2], S32)], [desc([3], F32), desc([2], S32)], [desc([3], S32), desc([2], F32)],
               [desc([3, 1], S32), desc([2], S32)], [desc([3], S32), desc([2, 1], S32)], groups[:1]):
@@ -252,6 +252,8 @@ def test_prefix_call_refusals(kw, status):
 
 def test_prefix_workspace():
     lib, a = na.lib(), prefix_args()
+    assert lib.nnops_hip_prefix_attention_workspace_size(C.byref(a)) == 0      # a table of so little room
+    a = prefix_args(table_pages=16000, ld_table=16000)
     need = lib.nnops_hip_prefix_attention_workspace_size(C.byref(a))
     assert need >= 2 * 6 * 8 * 66 * 4                         # a part of the prefix's and one of its own for every row
     for at, size in ((None, need), (99 * BASE, need - 1), (99 * BASE + 8, need)):
