@@ -575,7 +575,8 @@ int nnops_hip_prefix_attention(const NnopsPrefixAttentionArgs* args, void* works
  * now, cells that got none}. No other two arrays may overlap.
  * The contents of the arrays are not seen by the host; a page number outside
  * [0, pages) is no page, lengths are taken into what the table has room for.
- * page_tokens: a power of two from 16 to 256. children, sequences <= 16384. */
+ * page_tokens: a power of two from 16 to 256. children, sequences <= 16384; cells
+ * of the new table < 2^31. */
 typedef struct NnopsKvForkArgs {
     const int32_t* page_table;  /* [sequences][ld_table], table_pages columns */
     int64_t sequences, table_pages, ld_table; /* ld: elements */
@@ -648,9 +649,10 @@ int nnops_hip_kv_cache_copy(const NnopsKvCopyArgs* args, void* stream);
  * A logit of -inf has probability 0. A row of nothing else: every log probability
  * -inf, the entropy 0. A row that holds a NaN or +inf: NaN, top_tokens -1.
  * Sums are f32. vocab: up to 2^21. top: 0 to 32, at most vocab (0: top_tokens and
- * top_log_probs are not looked at). Rows are split over the chip where there are few of them: their
- * parts are in the workspace, nnops_hip_token_log_probs_workspace_size bytes,
- * 16-byte aligned, which need no initialization. */
+ * top_log_probs are not looked at). rows: up to 2^22, and parts of 32768 logits fewer
+ * than 2^23. Rows are split over the chip where there are few of them: their parts
+ * are in the workspace, nnops_hip_token_log_probs_workspace_size bytes, 16-byte
+ * aligned, which need no initialization. */
 typedef struct NnopsTokenLogProbsArgs {
     const void* logits;         /* [rows][ld_logits] f16 (f16) or f32, vocab columns */
     int64_t rows, vocab, ld_logits; /* ld: elements */

@@ -761,8 +761,8 @@ int check_fork(const NnopsKvForkArgs* g)
     }
     if (!page_tokens_fit(g->page_tokens) || g->sequences > kMostRows || g->children > kMostRows ||
         g->pages > INT32_MAX / 4 || g->table_pages > INT32_MAX / g->page_tokens ||
-        g->new_table_pages > INT32_MAX / g->page_tokens) {
-        return NNOPS_UNSUPPORTED;
+        g->new_table_pages > INT32_MAX / g->page_tokens || g->children * g->new_table_pages > INT32_MAX) {
+        return NNOPS_UNSUPPORTED;                  // (what all ask for is an int)
     }
     return -1;
 }

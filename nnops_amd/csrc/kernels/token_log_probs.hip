@@ -653,7 +653,8 @@ int check_log_probs(const NnopsTokenLogProbsArgs* g)
     if (g->rows > (1 << 22) || g->vocab > (int64_t)kMostSplits * kMostChunks * kSpan || g->per_row > INT32_MAX / 2) {
         return NNOPS_UNSUPPORTED;
     }
-    return -1;
+    // (threads of a launch: fewer than 2^32)
+    return g->rows * log_probs_plan(g).splits < (int64_t)1 << 23 ? -1 : NNOPS_UNSUPPORTED;
 }
 
 template <typename T, int kChunks>

@@ -171,6 +171,7 @@ def compact_args(**kw):
     (dict(new_table=BASE + 44), INVALID),
     (dict(new_lengths=2 * BASE), INVALID), (dict(copies=10 * BASE - 4), INVALID), (dict(new_refs=3 * BASE + 4), INVALID),
     (dict(new_refs=4 * BASE), INVALID),
+    (dict(children=16384, new_table_pages=1 << 17, ld_new_table=1 << 17), UNSUPPORTED),    # cells past an int
 ])
 def test_fork_call_refusals(kw, status):
     lib, a = na.lib(), fork_args(**kw)
@@ -276,6 +277,7 @@ def probs_args(**kw):
     (dict(vocab=(1 << 21) + 1, ld_logits=1 << 22), UNSUPPORTED), (dict(ld_logits=99), INVALID), (dict(logits=None), INVALID), (dict(entropy=None), INVALID), (dict(tokens=None), INVALID),
     (dict(log_probs=None), INVALID), (dict(ld_tokens=2), INVALID), (dict(top_tokens=None), INVALID),
     (dict(ld_top_log_probs=3), INVALID), (dict(rows=0), na.OK),
+    (dict(rows=1 << 22, vocab=33000, ld_logits=33000), UNSUPPORTED),                       # threads past 2^32
 ])
 def test_probs_call_refusals(kw, status):
     a = probs_args(**kw)
