@@ -576,7 +576,7 @@ int nnops_hip_prefix_attention(const NnopsPrefixAttentionArgs* args, void* works
  * The contents of the arrays are not seen by the host; a page number outside
  * [0, pages) is no page, lengths are taken into what the table has room for.
  * page_tokens: a power of two from 16 to 256. children, sequences <= 16384; cells
- * of the new table < 2^31. */
+ * of the new table < 2^30. */
 typedef struct NnopsKvForkArgs {
     const int32_t* page_table;  /* [sequences][ld_table], table_pages columns */
     int64_t sequences, table_pages, ld_table; /* ld: elements */

@@ -171,7 +171,7 @@ def compact_args(**kw):
     (dict(new_table=BASE + 44), INVALID),
     (dict(new_lengths=2 * BASE), INVALID), (dict(copies=10 * BASE - 4), INVALID), (dict(new_refs=3 * BASE + 4), INVALID),
     (dict(new_refs=4 * BASE), INVALID),
-    (dict(children=16384, new_table_pages=1 << 17, ld_new_table=1 << 17), UNSUPPORTED),    # cells past an int
+    (dict(children=16384, new_table_pages=1 << 16, ld_new_table=1 << 16), UNSUPPORTED),    # 2^30 cells
 ])
 def test_fork_call_refusals(kw, status):
     lib, a = na.lib(), fork_args(**kw)
