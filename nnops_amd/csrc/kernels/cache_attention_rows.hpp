@@ -42,10 +42,11 @@ namespace {
 
 constexpr int kRows = 16;           // rows of a wave
 
-// What the waves of a workgroup join.
+// What the waves of a workgroup join. (aligned: 16 bytes at once, which a reference
+// alone does not let the compiler see; 16 x 4096 at d 256 53.9 -> 53.3 us)
 template <int DP>
 struct WaveParts {
-    float o[4][kRows][DP + 4];
+    __attribute__((aligned(16))) float o[4][kRows][DP + 4];
     float m[4][kRows], l[4][kRows];
 };
 
