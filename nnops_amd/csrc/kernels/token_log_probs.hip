@@ -25,6 +25,7 @@
 #include <limits>
 
 #include "common.hpp"
+#include "key_rooms.hpp"
 
 namespace nnops_amd {
 namespace {
@@ -38,6 +39,8 @@ constexpr int kMostTop = 32;
 constexpr int kMostSplits = 64;
 constexpr int kRoom = 2048;         // keys above a threshold, as many of each wave ...
 constexpr int kAllKeys = kRoom + kSpan;   // ... and those of a span that are equal to it
+constexpr int kWaveRoom = kRoom / kWaves;
+static_assert(2 * kRoom <= kAllKeys && kWaveRoom <= kThreads);   // (the waves' rooms, behind the keys of all; a thread each)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNone = -std::numeric_limits<float>::infinity();
 
@@ -480,7 +483,7 @@ __global__ __launch_bounds__(kThreads, 4) void log_probs(const LogProbsKern p)
         // (the top-th of the maxima of 64 groups of 8 lanes)
         least = top_value<T>(group, p.top);
         const T reach = (T)least;                  // (one of the logits: exact)
-        uint64_t* const room = sh.key + kRoom + tid / 64 * (kRoom / kWaves);
+        uint64_t* const room = sh.key + kRoom + tid / 64 * kWaveRoom;
         int count = least > kNone ? 0 : kRoom;     // (-inf: what is behind the row reaches it too)
 #pragma unroll
         for (int j = 0; j < kChunks; ++j) {
@@ -492,7 +495,7 @@ __global__ __launch_bounds__(kThreads, 4) void log_probs(const LogProbsKern p)
                     if (mask != 0) {
                         const int to = count + (int)__builtin_amdgcn_mbcnt_hi(
                                                    (uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
-                        if (in && to < kRoom / kWaves) {
+                        if (in && to < kWaveRoom) {
                             room[to] = key_of((float)v[j][e], begin + j * kSpan + 8 * tid + e);
                         }
                         count += __popcll(mask);
@@ -530,18 +533,22 @@ __global__ __launch_bounds__(kThreads, 4) void log_probs(const LogProbsKern p)
     uint64_t key = 0;
     int rank = tid;
     if constexpr (kTop) {
-        int keys = 0, most = 0;
+        int count[kWaves], to[kWaves];
+#pragma unroll
         for (int i = 0; i < kWaves; ++i) {
-            const int count = sh.count[i];
-            for (int at = tid; at < min(count, kRoom / kWaves); at += kThreads) {
-                sh.key[keys + at] = sh.key[kRoom + i * (kRoom / kWaves) + at];
-            }
-            keys += count;
-            most = max(most, count);
+            count[i] = sh.count[i];
         }
-        __syncthreads();
-        if (most > kRoom / kWaves) {
+        int keys = gather_rooms(count, kWaveRoom, to);
+        if (keys < 0) {                            // (the same in all threads)
             keys = many_keys(sh, x, begin, n, least, p.top);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWaves; ++i) {
+                if (tid < count[i]) {
+                    sh.key[to[i] + tid] = sh.key[kRoom + i * kWaveRoom + tid];
+                }
+            }
+            __syncthreads();
         }
         key = rank_keys(sh, keys, p.top, rank);
     }

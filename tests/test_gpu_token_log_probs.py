@@ -137,6 +137,38 @@ def test_masks(f16):
 
 
 @pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("vocab", [40, 1984, 8192, 16384, 32768, 70000])
+def test_more_keys_than_rooms(vocab, f16):
+    """Rows whose threshold more logits reach than a wave has room for, in many
+    workgroups at once: all equal, masked but for a few groups (which leave none),
+    one group, runs of equal ones among others. Every row has its own results, with
+    sums, counts and alternatives that are the same in all rows alike."""
+    announce(f"log probs rooms vocab={vocab} f16={f16}")
+    i = np.arange(vocab)
+    x = _x(vocab, 6, vocab, f16)
+    x[0, :] = 1.5
+    x[1, i % 4096 >= 64 * 7] = -np.inf               # 7 of 64 groups
+    x[2, 5:] = -np.inf
+    x[3, i % 3 != 0] = np.float16(x[3].astype(np.float32).max()) + 1
+    x[4, : vocab // 2] = -2.0
+    x[4, vocab // 2:] = -3.0
+    tokens = np.array([[0, vocab // 2, vocab - 1]] * 6, np.int32)
+    rows = np.arange(600 if vocab <= 16384 else 300) % 6
+    for top in (5, 8, 32):
+        one = _check(x, tokens, top)
+        many = _run(x[rows], tokens[rows], top)
+        lp, entropy, best, best_lp = ref.log_probs(x, tokens, top)
+        tol_lp, tol_h = ref.log_probs_tolerance(x, lp, entropy)
+        _near(many[0], lp[rows], np.broadcast_to(tol_lp, lp.shape)[rows])
+        _near(many[1], entropy[rows], np.broadcast_to(tol_h, entropy.shape)[rows])
+        assert np.array_equal(many[2], best[rows]) and np.array_equal(one[2], best)
+        _near(many[3], best_lp[rows], np.broadcast_to(ref.log_probs_tolerance(x, best_lp, entropy)[0], best_lp.shape)[rows])
+        for k in range(6):                            # the same row, the same bits
+            for got in many:
+                assert (got[rows == k] == got[k]).all() or np.isnan(got[k]).any()
+
+
+@pytest.mark.parametrize("f16", [True, False])
 def test_nan_and_infinity(f16):
     """They show in their row, and only there."""
     announce(f"log probs nan f16={f16}")
