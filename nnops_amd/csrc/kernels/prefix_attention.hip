@@ -252,6 +252,22 @@ bool sharing_pays(const NnopsPrefixAttentionArgs& g, const SharedPlan& a)
     return shared < alone;
 }
 
+// Workgroups of the join.
+int64_t join_blocks(const NnopsPrefixAttentionArgs& g, const SharedPlan& a)
+{
+    const int64_t per_block = 256 / join_lanes((int)g.cache.head_dim) / a.ways;
+    return (g.rows * g.q_heads + per_block - 1) / per_block;
+}
+
+// Whether its launches hold what is shared (fewer than 2^31 threads each): larger
+// calls are left to the other way, whose launches are fewer.
+bool shared_way_fits(const NnopsPrefixAttentionArgs& g, const SharedPlan& a)
+{
+    constexpr int64_t kMost = INT32_MAX / 512;
+    return a.own.items * a.own.splits <= kMost && a.items * a.splits <= kMost && a.own.splits <= 65535 &&
+           a.splits <= 65535 && (a.join_here || join_blocks(g, a) <= INT32_MAX / 256);
+}
+
 SharedPlan shared_plan(const NnopsPrefixAttentionArgs* g)
 {
     SharedPlan a{};
@@ -297,16 +313,16 @@ SharedPlan shared_plan(const NnopsPrefixAttentionArgs* g)
     a.few = g->cache.sequences <= 64 && g->groups <= kFewGroups;
     a.join_here = a.tile_rows != kRows && a.own.tile_rows == kRows && a.own.splits == 1;
     const int64_t parts = a.splits + (a.join_here ? 0 : a.own.splits);
-    a.share = sharing_pays(*g, a);
-    if (!a.share) {
-        a.workspace = a.own.workspace;
-        return a;
-    }
     // workgroups to fill the chip, as long as each lane has a batch of parts
     const int lanes = join_lanes((int)d);
     a.ways = 1;
     while (a.ways < 256 / lanes && 4 * a.ways < parts && g->rows * g->q_heads * a.ways * lanes < 2048 * 256) {
         a.ways *= 2;
+    }
+    a.share = shared_way_fits(*g, a) && sharing_pays(*g, a);
+    if (!a.share) {
+        a.workspace = a.own.workspace;
+        return a;
     }
     a.groups_at = 16;
     a.members_at = a.groups_at + up16(sizeof(GroupPlan) * (size_t)groups);
@@ -373,7 +389,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : sizeof(T) == 2 ? 3 : 2) void at
 }
 
 template <typename T>
-void launch_prefix(const PrefixKern& p, const SharedPlan& a, hipStream_t s)
+void launch_prefix(const PrefixKern& p, const SharedPlan& a, int64_t blocks, hipStream_t s)
 {
     if (!p.own.few) {
         NNOPS_LAUNCH(prefix_plan, dim3(1), dim3(kPlanThreads), 0, s, p);
@@ -400,8 +416,6 @@ void launch_prefix(const PrefixKern& p, const SharedPlan& a, hipStream_t s)
             return;
         }
     }
-    const int64_t per_block = 256 / join_lanes(k.c.d) / a.ways;
-    const int64_t blocks = ((int64_t)k.c.rows * k.q_heads + per_block - 1) / per_block;
     NNOPS_LAUNCH(prefix_join<T>, dim3((unsigned)blocks), dim3(256), 0, s, p);
 }
 
@@ -461,10 +475,6 @@ extern "C" int nnops_hip_prefix_attention(const NnopsPrefixAttentionArgs* g, voi
         const NnopsCacheAttentionArgs whole = whole_args(*g);
         return nnops_hip_cache_attention(&whole, workspace, workspace_bytes, stream);
     }
-    if (a.own.items * a.own.splits > INT32_MAX / 512 || a.items * a.splits > INT32_MAX / 512 || a.own.splits > 65535 || a.splits > 65535 ||
-        g->rows * g->q_heads > INT32_MAX / 256) {
-        return NNOPS_UNSUPPORTED;
-    }
     if (workspace == nullptr || workspace_bytes < a.workspace || (uintptr_t)workspace % 16 != 0) {
         return NNOPS_NOT_INITIALIZED;
     }
@@ -505,9 +515,9 @@ extern "C" int nnops_hip_prefix_attention(const NnopsPrefixAttentionArgs* g, voi
     k.first_part = a.splits;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (g->f16) {
-        launch_prefix<_Float16>(p, a, s);
+        launch_prefix<_Float16>(p, a, join_blocks(*g, a), s);
     } else {
-        launch_prefix<float>(p, a, s);
+        launch_prefix<float>(p, a, join_blocks(*g, a), s);
     }
     return hipGetLastError() == hipSuccess ? NNOPS_OK : NNOPS_INTERNAL;
 }

@@ -415,3 +415,27 @@ def test_graph_streams_and_repeats():
         want, weight, spread = ref.attention(q, *cache, now, [1] * members)
         tol = ref.attention_tolerance(True, want, weight, spread, cache[3])
         assert (abs(host(out) - want) <= tol).all(), step
+
+
+def test_more_rows_than_2_to_the_23():
+    """A call whose rows times heads pass what a launch of a workgroup each would hold:
+    sequences from all over it."""
+    import torch
+    announce("prefix many rows")
+    heads, group, d, page, members, n = 8, 16, 16, 64, 1024, 65
+    assert members * n * heads * group > 2 ** 23
+    groups, shared = [0, members], [640]
+    lens = [640 + n + i % 50 for i in range(members)]
+    cache = _cache(lens, groups, shared, heads, page, d, wide=188)
+    assert _plan(heads, group, d, page, cache[4].shape[1], members * n, members, 1, True, False).shared_rows == 256
+    q = _q(18, members * n, heads * group * d, True)
+    out = torch.full(q.shape, 7.0, dtype=torch.float16, device="cuda")
+    ins = [na.tensor(dev(x)) for x in [q, *cache] + [np.array(x, np.int32) for x in (lens, groups, shared)]]
+    assert na.PrefixAttention().compute([na.tensor(out)], ins) == na.OK
+    torch.cuda.synchronize()
+    some = [0, 1, 500, 1009, 1010, 1022, 1023]         # (2^23 / 128 / 65: sequence 1008)
+    at = np.concatenate([np.arange(b * n, (b + 1) * n) for b in some])
+    of = [*cache[:4], cache[4][some, :12]]
+    want, weight, spread = ref.attention(q[at], *of, [lens[b] for b in some], [n] * len(some))
+    got = host(out)[at]
+    assert (abs(got - want) <= ref.attention_tolerance(True, want, weight, spread, cache[3])).all()
