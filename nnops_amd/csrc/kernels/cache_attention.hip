@@ -293,7 +293,11 @@ extern "C" size_t nnops_hip_cache_attention_workspace_size(const NnopsCacheAtten
 {
     // (the tables' contents and the pointers play no part; a call that is refused,
     // or that has nothing to do, needs none)
-    return check_attention_shapes(g) >= 0 ? 0 : attn_plan(g).workspace;
+    if (check_attention_shapes(g) >= 0) {
+        return 0;
+    }
+    const AttnPlan a = attn_plan(g);
+    return launch_holds(a) ? a.workspace : 0;
 }
 
 extern "C" int nnops_hip_cache_attention_plan(const NnopsCacheAttentionArgs* g, NnopsCacheAttentionPlan* out)
@@ -306,6 +310,9 @@ extern "C" int nnops_hip_cache_attention_plan(const NnopsCacheAttentionArgs* g, 
         return rc;
     }
     const AttnPlan a = attn_plan(g);
+    if (!launch_holds(a)) {
+        return NNOPS_UNSUPPORTED;
+    }
     out->tile_rows = a.tile_rows;
     out->one_page = a.tiled && tiled_one_page(g->cache.head_dim, g->cache.page_tokens);
     out->splits = a.splits;
@@ -330,7 +337,7 @@ extern "C" int nnops_hip_cache_attention(const NnopsCacheAttentionArgs* g, void*
         return NNOPS_INVALID_ARGUMENT;
     }
     const AttnPlan a = attn_plan(g);
-    if (a.items > INT32_MAX / 512 || a.splits > 65535) {
+    if (!launch_holds(a)) {
         return NNOPS_UNSUPPORTED;
     }
     if (a.workspace > 0 && (workspace == nullptr || workspace_bytes < a.workspace || (uintptr_t)workspace % 16 != 0)) {

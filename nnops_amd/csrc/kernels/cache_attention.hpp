@@ -538,9 +538,14 @@ struct AttnPlan {
     size_t workspace;
 };
 
-// The choice for a call whose sizes check_attention_shapes lets pass (-1).
+// The choice for a call whose sizes check_attention_shapes lets pass (-1), and whether
+// a launch holds it.
 int check_attention_shapes(const NnopsCacheAttentionArgs* g);
 AttnPlan attn_plan(const NnopsCacheAttentionArgs* g);
+inline bool launch_holds(const AttnPlan& a)
+{
+    return a.items <= std::numeric_limits<int32_t>::max() / 512 && a.splits <= 65535;
+}
 
 // attention_rows_tiled's launch (cache_attention_tiled.hip): d, type and rows
 // of a workgroup that it has a kernel for.

@@ -426,7 +426,11 @@ using namespace nnops_amd;
 
 extern "C" size_t nnops_hip_prefix_attention_workspace_size(const NnopsPrefixAttentionArgs* g)
 {
-    return check_prefix(g) >= 0 ? 0 : shared_plan(g).workspace;
+    if (check_prefix(g) >= 0) {
+        return 0;
+    }
+    const SharedPlan a = shared_plan(g);
+    return a.share || launch_holds(a.own) ? a.workspace : 0;
 }
 
 extern "C" int nnops_hip_prefix_attention_plan(const NnopsPrefixAttentionArgs* g, NnopsPrefixAttentionPlan* out)
@@ -439,6 +443,9 @@ extern "C" int nnops_hip_prefix_attention_plan(const NnopsPrefixAttentionArgs* g
         return rc;
     }
     const SharedPlan a = shared_plan(g);
+    if (!a.share && !launch_holds(a.own)) {
+        return NNOPS_UNSUPPORTED;
+    }
     out->own_rows = a.own.tile_rows;
     out->own_splits = a.own.splits;
     out->workspace_bytes = a.workspace;

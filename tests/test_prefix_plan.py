@@ -63,3 +63,20 @@ def test_plan_query_and_call_agree(heads, group, d, page, columns, rows, sequenc
         w, q = whole(a), L.CacheAttentionPlan()
         assert lib.nnops_hip_cache_attention_plan(C.byref(w), C.byref(q)) == na.OK
         assert (p.own_rows, p.own_splits, p.workspace_bytes) == (q.tile_rows, q.splits, q.workspace_bytes)
+
+
+@pytest.mark.parametrize("heads,group,d,page,columns,rows,sequences,groups", [
+    (64, 4, 16, 64, 400, 1 << 16, 1 << 16, 1 << 13), (64, 1, 256, 64, 64, 1 << 16, 1 << 16, 1), (16, 1, 64, 16, 9, 1 << 18, 1 << 18, 0),
+])
+def test_sizes_that_no_launch_holds(heads, group, d, page, columns, rows, sequences, groups):
+    """2^22 workgroups: plans and calls refuse them alike, and no workspace is asked for."""
+    lib, a = na.lib(), args(heads, group, d, page, columns, rows, sequences, groups)
+    w, q = whole(a), L.CacheAttentionPlan()
+    assert plan(a)[0] == na.UNSUPPORTED and lib.nnops_hip_prefix_attention_workspace_size(C.byref(a)) == 0
+    assert lib.nnops_hip_prefix_attention(C.byref(a), C.c_void_p(99 * BASE), 1 << 50, None) == na.UNSUPPORTED
+    assert lib.nnops_hip_cache_attention_plan(C.byref(w), C.byref(q)) == na.UNSUPPORTED
+    assert lib.nnops_hip_cache_attention_workspace_size(C.byref(w)) == 0
+    assert lib.nnops_hip_cache_attention(C.byref(w), C.c_void_p(99 * BASE), 1 << 50, None) == na.UNSUPPORTED
+    # one sequence fewer
+    a = args(heads, group, d, page, columns, rows - 1, sequences - 1, groups)
+    assert plan(a)[0] == na.OK
