@@ -522,7 +522,9 @@ int nnops_hip_cache_attention(const NnopsCacheAttentionArgs* args, void* workspa
 /* Attention for sequences that share their first tokens (no counterpart in
  * nnops): the same results as nnops_hip_cache_attention without a window, up to
  * the order of the sums, with the tokens that a group of sequences shares read
- * once for the group. Group g is the sequences group_starts[g] ..
+ * once for the group. (Probabilities of f16 rows have as many bits in the second
+ * product as there, or more: two f16 where it gives a workgroup 16 rows, at least
+ * one where more.) Group g is the sequences group_starts[g] ..
  * group_starts[g + 1] - 1, whose page tables hold the same pages for the first
  * shared[g] tokens, as far as these fill whole pages (which the caller sees to;
  * a sequence may be shorter, and may bring no rows). Read as shared: the whole
@@ -532,9 +534,8 @@ int nnops_hip_cache_attention(const NnopsCacheAttentionArgs* args, void* workspa
  * are taken into [0, sequences], no group begins before the last one's end, and
  * what is shared beyond the first sequence's tokens is not.
  * Where the page table has room for so few tokens that reading them once saves
- * nothing, every sequence is looked at by itself.
- * Probabilities of f16 rows enter the second product as one f16 where a group's
- * or sequence's rows share their tiles, as two where not. The workspace holds
+ * nothing, or a call is larger than the launches for shared tokens can be, every
+ * sequence is looked at by itself. The workspace holds
  * the parts of all rows: nnops_hip_prefix_attention_workspace_size bytes, 16-byte
  * aligned, which need no initialization (0: none is needed). */
 typedef struct NnopsPrefixAttentionArgs {

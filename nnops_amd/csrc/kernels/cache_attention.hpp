@@ -395,6 +395,8 @@ __device__ __forceinline__ Scales softmax_scales(const AttnKern& p, PageScales s
 //        -> 50.5). The matrix cores bound many: a prompt of 4096 would take 196
 //        instead of 152, for an error that the output's own rounding to f16 exceeds
 //        (against 64 bits 2.6e-4 of the result, 2.1e-4 with that rounding alone).
+//        Tiles over tokens that sequences share keep what their rows have by
+//        themselves: two where these are few.
 //   f32: each value as three bf16 parts that hold it exactly (8 bits each, by
 //        truncation, the last difference having no more), codes as bf16 (7 bits
 //        and a sign: exact), three products into one f32 accumulator. Two f16
@@ -433,6 +435,27 @@ struct Operand {
             v[0][e] = (_Float16)x[e];
             v[1][e] = (_Float16)__fsub_rn(x[e], (float)v[0][e]);
         }
+    }
+    // The same values by 4 instructions a pair instead of 8 (v_fma_mix_f32 takes f16 as they
+    // lie in a register), for tiles of many rows, which vector instructions bound as well.
+    // minus_one: -1 that the compiler does not know, or it makes them two steps again.
+    static __device__ __forceinline__ void split_in_pairs(const float (&x)[8], Vec (&v)[2], float minus_one)
+    {
+#if __HIP_DEVICE_COMPILE__
+        typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            v2h h{(_Float16)x[e], (_Float16)x[e + 1]};
+            asm("" : "+v"(h));                     // (one conversion for both parts)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                v[0][e + i] = h[i];
+                v[1][e + i] = (_Float16)__builtin_fmaf((float)h[i], minus_one, x[e + i]);   // (exact before its rounding)
+            }
+        }
+#else
+        (void)x, (void)v, (void)minus_one;
+#endif
     }
     static __device__ __forceinline__ v4f mfma(Vec a, Vec b, v4f c)
     {

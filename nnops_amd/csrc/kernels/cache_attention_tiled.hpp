@@ -57,11 +57,14 @@ __device__ __forceinline__ V uniform_load(const V* p)
 
 // kOne: pages of 64 tokens and more, so that a tile lies in one: its number and
 // scales are scalars, its codes at a scalar base and fixed offsets.
-template <typename T, int DP, int NW, bool kOne, AttnMode M>
+// kFine: probabilities of f16 rows as two f16, as 16 rows a workgroup have them (shared
+// tokens of sequences with few rows each: a tile of 256 rows takes 2.5 -> 3.0 us).
+template <typename T, int DP, int NW, bool kOne, AttnMode M, bool kFine = false>
 __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const KernOf<M> p)
 {
     typedef Operand<T> Op;
     typedef typename Op::Vec Vec;
+    constexpr int kWeights = kFine && Op::kParts == 1 ? 2 : Op::kParts;   // parts of a probability
     constexpr int kThreads = 64 * NW;
     constexpr int kPieces = kTile * DP / 16;                         // 16-code pieces of a tile's side
     constexpr int kPer = (kPieces + kThreads - 1) / kThreads;        // of a thread
@@ -231,7 +234,9 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const KernOf<M> 
         return a;
     };
     v16f s[2];
-    Vec pf[4][Op::kParts];
+    Vec pf[4][kWeights];
+    float minus_one = -1.0f;
+    asm("" : "+s"(minus_one));
     const auto scores = [&](int v) {
         const uint16_t* buf = s_k[v & 1] + krow * kPitchK + 8 * hh;
         s[0] = v16f{};
@@ -318,7 +323,11 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const KernOf<M> 
                     }
                     sum += w[e];
                 }
-                Op::split(w, pf[h]);
+                if constexpr (kWeights == 2) {
+                    Op::split_in_pairs(w, pf[h], minus_one);
+                } else {
+                    Op::split(w, pf[h]);
+                }
             }
             // a page of which the row sees nothing adds nothing, whatever its scale
             l_run += !kMasked || sum != 0.0f ? sum * inv[g] : 0.0f;
@@ -484,7 +493,7 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_tiled(const KernOf<M> 
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
 #pragma unroll
-                    for (int i = 0; i < Op::kParts; ++i) {
+                    for (int i = 0; i < kWeights; ++i) {
                         pf[g][i] = Vec{};
                     }
                 }

@@ -10,12 +10,17 @@
 //
 // Which tokens are shared is found on the device: whole tiles and whole pages that
 // every row of the group sees. Rows then need no mask, and a sequence's own tokens
-// begin at a tile. Every wave finds it for few sequences (a launch less: 4 sequences of
-// 1990 16 -> 12.6 us), one workgroup before the others for more.
+// begin at a tile. Every wave finds it for few sequences (a launch less: 4 sequences over
+// 2000 shared tokens 16 -> 11.8 us), one workgroup before the others for more.
+// Probabilities of f16 rows are held in as many parts as CacheAttention has for the same
+// rows, two f16 where it gives them workgroups of 16 and one where tiles of many: results
+// differ by the order of the sums alone. With one f16 in every tile the calls below took
+// 69 and 116 us, and were off by 2.3e-4 and 2.4e-4 of the result instead of 2.1e-4, as its
+// own rounding to f16 is.
 // Measured, 32 query and 8 KV heads of 128, f16: 64 sequences of a token each, 32768
-// shared and up to 400 of their own: 70 us (each sequence by itself: 406), of which the
-// shared tokens 54 (34.4 GFLOP) and the rest with the join 17 to 22; 530 rows over 8000: 118
-// (289).
+// shared and up to 400 of their own: 78 us (each sequence by itself: 406), of which the
+// shared tokens 62 (34.4 GFLOP, and 17 for the second parts) and the rest with the join 17 to
+// 22; 530 rows over 8000: 135 (289).
 #include "cache_attention_rows.hpp"
 #include "cache_attention_tiled.hpp"
 
@@ -215,24 +220,28 @@ int check_prefix(const NnopsPrefixAttentionArgs* g)
 size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 
 // Whether what is shared is read once, or each sequence looked at by itself, which the
-// tables allow. Both read as many tokens as the table has room for, a tile of rows at
+// tables allow. Both are taken to read as many tokens as the table has room for (the host
+// sees no lengths: in a table far wider than what is in use, as a captured graph has, more
+// is shared than pays: 16 x up to 97 below, of 500 tokens in a table for 2000), a tile of rows at
 // a time, and full or not, a tile takes the same time: sharing pays where it fills tiles
 // that a sequence's rows fill in part, or makes them larger, and costs the parts of every
 // row. The rates are those of the kernels, of a row, token and channel (and 64 more for
-// the softmax). Measured, by itself / shared in us, what is taken marked *; n sequences of
-// r tokens, 32 query and 8 KV heads of 128, 500, 2000 and 8000 shared tokens:
-//   f16, 4 x 1     *10.6 / 12.3    *13.0 / 12.6    17.4 / *17.0
-//        16 x 1    *12.1 / 12.0    18.8 / *15.1    35.7 / *21.4
-//        48 x 1    15.9 / *15.6    31.1 / *20.6    77.5 / *35.4
-//        48 x 3    *17.6 / 20.4    *31.9 / 34.2    79.1 / *56.1
-//        48 x 8    *18.1 / 31.7    43.6 / *41.8    140 / *79.8
-//        48 x 33   *40.7 / 64.3    *114 / 115      403 / *308
-//        48 x 97   *71.4 / 160     *199 / 307      *703 / 791
-//        16 x up to 97 *32.7 / 55.6 88.4 / *70.5  310 / *156
-//   f32, 48 x 1    19.6 / *19.7    35.3 / *24.9    92.0 / *38.6
-//        48 x 33   *97.6 / 114     301 / *238      1099 / *651
+// the softmax; shared tiles whose probabilities are two f16 run at five sixths of it,
+// which changes none of the choices below). Measured, by itself / shared in us, what is taken
+// marked *; n sequences of r tokens, 32 query and 8 KV heads of 128, 500, 2000 and 8000
+// shared tokens:
+//   f16, 4 x 1     *9.9 / 11.0     *12.4 / 11.6    17.1 / *16.5
+//        16 x 1    *11.7 / 11.2    18.6 / *14.9    34.3 / *21.2
+//        48 x 1    15.9 / *15.2    30.2 / *20.6    77.6 / *35.0
+//        48 x 3    *17.4 / 19.9    *31.5 / 33.8    78.9 / *59.5
+//        48 x 8    *17.7 / 30.9    43.1 / *43.7    140 / *90.0
+//        48 x 33   *40.6 / 63.5    *114 / 112      402 / *303
+//        48 x 97   *71.7 / 159     *200 / 303      *709 / 776
+//        16 x up to 97 *32.4 / 54.3 88.2 / *74.6  311 / *176
+//   f32, 48 x 1    19.3 / *19.3    35.6 / *24.6    91.9 / *38.1
+//        48 x 33   *97.6 / 115     302 / *238      1101 / *648
 // Over 179 calls of such sizes and of 8 and 2 heads of 64, what is taken is 1 % slower than the
-// faster one in the mean, 14 % if it always were the one, 13 % the other.
+// faster one in the mean, 13 % if it always were the one or the other.
 bool sharing_pays(const NnopsPrefixAttentionArgs& g, const SharedPlan& a)
 {
     const double d = (double)g.cache.head_dim, seqs = (double)g.cache.sequences, groups = (double)g.groups;
@@ -283,9 +292,9 @@ SharedPlan shared_plan(const NnopsPrefixAttentionArgs* g)
     // Tiles of many rows where they fill more than a quarter and there is work enough for
     // their longer beginning and end; 16 rows a workgroup otherwise, in one launch with
     // the sequences' own tokens (us, tiled / 16 rows; n sequences of one token, 32 query
-    // and 8 KV heads of 128, f16; shared tokens 4096 and 32768): 16 27.3 / 19.2 and 50.7 /
-    // 39.7, 24 28.6 / 23.5 and 53.2 / 54.1, 32 30.4 / 23.8 and 55.9 / 64.1, 48 36.5 / 27.4 and
-    // 68.7 / 94.4; over 8192, 32 of them, d 64 26.3 / 19.1, d 256 59.3 / 64.4, f32 41.0 / 34.7.
+    // and 8 KV heads of 128, f16; shared tokens 4096 and 32768): 16 28.6 / 19.0 and 55.4 /
+    // 39.9, 24 29.7 / 23.0 and 57.9 / 54.2, 32 31.4 / 23.3 and 60.3 / 64.5, 48 37.7 / 27.7 and
+    // 74.9 / 94.7; over 8192, 32 of them, d 64 27.0 / 18.8, d 256 60.0 / 62.8, f32 41.1 / 34.4.
     const int64_t room = g->cache.table_pages * g->cache.page_tokens;
     const bool much = (double)g->rows * g->q_heads * d * room >= 0x1p31;
     const int rows = mean > 64 && much ? tiled_rows(d, g->f16, g->cache.page_tokens, mean) : 0;
@@ -332,19 +341,38 @@ SharedPlan shared_plan(const NnopsPrefixAttentionArgs* g)
     return a;
 }
 
-template <typename T, int DP, int NW, AttnMode M>
+template <typename T, int DP, int NW, AttnMode M, bool kFine>
 void launch_tiled_one(const PartKern& k, const dim3& grid, hipStream_t s)
 {
     if (DP > 128 || tiled_one_page(k.c.d, k.c.page)) {
-        NNOPS_LAUNCH((attention_rows_tiled<T, DP, NW, true, M>), grid, dim3(64 * NW), 0, s, k);
+        NNOPS_LAUNCH((attention_rows_tiled<T, DP, NW, true, M, kFine>), grid, dim3(64 * NW), 0, s, k);
     } else if constexpr (DP <= 128) {
-        NNOPS_LAUNCH((attention_rows_tiled<T, DP, NW, false, M>), grid, dim3(64 * NW), 0, s, k);
+        NNOPS_LAUNCH((attention_rows_tiled<T, DP, NW, false, M, kFine>), grid, dim3(64 * NW), 0, s, k);
     }
 }
 
-// (the kernels that tiled_rows names, and 16 rows a workgroup)
+// (the kernels that tiled_rows names)
+template <typename T, AttnMode M, bool kFine>
+void launch_tiles(const PartKern& k, const dim3& grid, hipStream_t s)
+{
+    const int d = k.c.d;
+    if constexpr (sizeof(T) == 2) {
+        if (k.tile_rows == 256) {
+            d <= 64 ? launch_tiled_one<T, 64, 8, M, kFine>(k, grid, s) : launch_tiled_one<T, 128, 8, M, kFine>(k, grid, s);
+        } else {
+            d <= 64    ? launch_tiled_one<T, 64, 4, M, kFine>(k, grid, s)
+            : d <= 128 ? launch_tiled_one<T, 128, 4, M, kFine>(k, grid, s)
+                       : launch_tiled_one<T, 256, 4, M, kFine>(k, grid, s);
+        }
+    } else if (k.tile_rows == 256) {
+        launch_tiled_one<T, 64, 8, M, kFine>(k, grid, s);
+    } else {
+        d <= 64 ? launch_tiled_one<T, 64, 4, M, kFine>(k, grid, s) : launch_tiled_one<T, 128, 4, M, kFine>(k, grid, s);
+    }
+}
+
 template <typename T, AttnMode M>
-void launch_part(const PartKern& k, const dim3& grid, hipStream_t s)
+void launch_part(const PartKern& k, bool fine, const dim3& grid, hipStream_t s)
 {
     const int d = k.c.d;
     if (k.tile_rows == kRows) {
@@ -355,18 +383,10 @@ void launch_part(const PartKern& k, const dim3& grid, hipStream_t s)
         } else {
             NNOPS_LAUNCH((attention_rows16<T, 256, M>), grid, dim3(256), 0, s, k);
         }
-    } else if constexpr (sizeof(T) == 2) {
-        if (k.tile_rows == 256) {
-            d <= 64 ? launch_tiled_one<T, 64, 8, M>(k, grid, s) : launch_tiled_one<T, 128, 8, M>(k, grid, s);
-        } else {
-            d <= 64    ? launch_tiled_one<T, 64, 4, M>(k, grid, s)
-            : d <= 128 ? launch_tiled_one<T, 128, 4, M>(k, grid, s)
-                       : launch_tiled_one<T, 256, 4, M>(k, grid, s);
-        }
-    } else if (k.tile_rows == 256) {
-        launch_tiled_one<T, 64, 8, M>(k, grid, s);
+    } else if (M == kShared && sizeof(T) == 2 && fine) {
+        launch_tiles<T, M, M == kShared && sizeof(T) == 2>(k, grid, s);
     } else {
-        d <= 64 ? launch_tiled_one<T, 64, 4, M>(k, grid, s) : launch_tiled_one<T, 128, 4, M>(k, grid, s);
+        launch_tiles<T, M, false>(k, grid, s);
     }
 }
 
@@ -410,8 +430,9 @@ void launch_prefix(const PrefixKern& p, const SharedPlan& a, int64_t blocks, hip
             NNOPS_LAUNCH((attention_both16<T, 256>), grid, dim3(256), 0, s, k, p.own, items, shared, own_items);
         }
     } else {
-        launch_part<T, kShared>(k, dim3((unsigned)a.items, (unsigned)a.splits), s);
-        launch_part<T, kOwn>(p.own, dim3((unsigned)a.own.items, (unsigned)a.own.splits), s);
+        // (probabilities in as many parts as CacheAttention has them in for the same rows)
+        launch_part<T, kShared>(k, a.own.tile_rows == kRows, dim3((unsigned)a.items, (unsigned)a.splits), s);
+        launch_part<T, kOwn>(p.own, false, dim3((unsigned)a.own.items, (unsigned)a.own.splits), s);
         if (p.own.join_here) {
             return;
         }

@@ -439,3 +439,31 @@ def test_more_rows_than_2_to_the_23():
     want, weight, spread = ref.attention(q[at], *of, [lens[b] for b in some], [n] * len(some))
     got = host(out)[at]
     assert (abs(got - want) <= ref.attention_tolerance(True, want, weight, spread, cache[3])).all()
+
+
+@pytest.mark.parametrize("d,page,heads,group,members,n", [(128, 64, 4, 4, 64, 1), (128, 16, 4, 4, 40, 1), (64, 64, 8, 8, 10, 1),
+                                                          (64, 16, 8, 8, 33, 1), (96, 128, 4, 4, 24, 3), (256, 64, 4, 4, 40, 1)])
+def test_probabilities_in_tiles_are_as_fine_as_cache_attentions(d, page, heads, group, members, n):
+    """Rows that CacheAttention gives workgroups of 16, whose probabilities are two f16:
+    in tiles over shared tokens they are as well. Few tokens have most of the weight, so
+    that where values cancel one f16 (2^-12 to 2^-11 of each weight) shows beside the
+    result's own rounding: in 0.05 to 0.9 % of the results, by numpy."""
+    import torch
+    announce(f"prefix fine d={d} page={page} heads={heads} members={members} n={n}")
+    groups, shared, scale = [0, members], [1280], 2.0 / d ** 0.5
+    lens = [1280 + n + 5 * i for i in range(members)]
+    wide = 2 ** 31 // (members * n * heads * group * d * page)
+    cache = _cache(lens, groups, shared, heads, page, d, wide=wide)
+    plan = _plan(heads, group, d, page, cache[4].shape[1], members * n, members, 1, True, False)
+    assert plan.shared_rows in (128, 256) and plan.own_rows == 16
+    q = _q(19, members * n, heads * group * d, True)
+    want, weight, spread = ref.attention(q, *cache, lens, [n] * members, scale=scale)
+    # (two f16 hold 22 bits: less than half of 2^-21; the result is rounded once)
+    tol = ref.attention_tolerance(False, want, weight, spread, cache[3]) + 1.01 * 2.0 ** -11 * abs(want) + 2.0 ** -24
+    out = torch.empty(q.shape, dtype=torch.float16, device="cuda")
+    ins = [na.tensor(dev(x)) for x in [q, *cache, np.array(lens, np.int32)]]
+    assert na.CacheAttention(scale=scale).compute([na.tensor(out)], ins) == na.OK
+    torch.cuda.synchronize()
+    assert (abs(host(out) - want) <= tol).all()
+    got = _run(q, cache, lens, [n] * members, groups, shared, ragged=False, scale=scale).astype(np.float64)
+    assert (abs(got - want) <= tol).all()
