@@ -7,9 +7,11 @@
 //   s = sum 2^y_j,  t = sum y_j 2^y_j
 //   log p_j = ln 2 (y_j - log2 s),  entropy = ln 2 (log2 s - t / s)
 // A part's s and t are brought to another's reference by d, the y of its own: s' =
-// 2^d s, t' = 2^d (t + d s). f16 rows: y = fma(x, log2(e), -r log2(e)): the rounding
-// of the second product is the same for all, and drops out. f32 rows: (x - r)
-// log2(e), which masks of the type's lowest value do not take out of f32's range.
+// 2^d s, t' = 2^d (t + d s). f16 rows: y = fma(x, log2(e), -R), R = r log2(e) rounded: one
+// instruction, and what R's rounding brings in is the same for all y: the entropy has it
+// in both terms, log p = (x - r) - (ln s - ln 2 (r log2(e) - R)), where x - r is nearly exact.
+// f32 rows: (x - r) log2(e), which masks of the type's lowest value do not take out of
+// f32's range.
 //
 // The most probable: the top-th largest of the maxima of 64 groups of 8 lanes is a
 // logit that at least `top` reach, and few more do (of random ones 64 ln(64 / (64 -
@@ -57,22 +59,25 @@ struct LogProbsKern {
     uint64_t* keys;       //   keys of [rows][splits][top], 0 where a split has fewer
 };
 
-// The reference that goes with a maximum, y against it, and y of an old one.
+// y against a reference (`base`: what its part of y is made of), y of an old one, log p.
 template <typename T>
 struct Reference;
 template <>
 struct Reference<_Float16> {
     static constexpr float kLeast = -1e38f;        // (its product is finite)
-    static __device__ __forceinline__ float of(float m) { return m * kLog2e; }
-    static __device__ __forceinline__ float y(float x, float r) { return __builtin_fmaf(x, kLog2e, -r); }
-    static __device__ __forceinline__ float step(float old, float r) { return old - r; }
-    static __device__ __forceinline__ float log_p(float x, float r, float s) { return (y(x, r) - log2f(s)) * kLn2; }
+    static __device__ __forceinline__ float base(float r) { return __fmul_rn(r, kLog2e); }
+    static __device__ __forceinline__ float y(float x, float base) { return __builtin_fmaf(x, kLog2e, -base); }
+    static __device__ __forceinline__ float step(float old, float r) { return base(old) - base(r); }
+    static __device__ __forceinline__ float log_p(float x, float r, float s)
+    {
+        return (x - r) - (logf(s) - y(r, base(r)) * kLn2);
+    }
 };
 template <>
 struct Reference<float> {
     static constexpr float kLeast = -std::numeric_limits<float>::max();
-    static __device__ __forceinline__ float of(float m) { return m; }
-    static __device__ __forceinline__ float y(float x, float r) { return (x - r) * kLog2e; }
+    static __device__ __forceinline__ float base(float r) { return r; }
+    static __device__ __forceinline__ float y(float x, float base) { return (x - base) * kLog2e; }
     static __device__ __forceinline__ float step(float old, float r) { return (old - r) * kLog2e; }
     static __device__ __forceinline__ float log_p(float x, float r, float s) { return (x - r) - logf(s); }
 };
@@ -463,7 +468,7 @@ __global__ __launch_bounds__(kThreads, 4) void log_probs(const LogProbsKern p)
     const float group = sh.group[tid % 64], high_row = row_max(group);
     const float m = fmaxf(fmaxf(lane_of(high_row, 0), lane_of(high_row, 16)),
                           fmaxf(lane_of(high_row, 32), lane_of(high_row, 48)));
-    const float r = Ref::of(fmaxf(m, Ref::kLeast));
+    const float r = fmaxf(m, Ref::kLeast), y_base = Ref::base(r);
     // (each phase converts f16 logits anew: kept as f32 they would take the registers of
     // another workgroup)
     const auto forget = [&] {
@@ -514,7 +519,7 @@ __global__ __launch_bounds__(kThreads, 4) void log_probs(const LogProbsKern p)
         if (j * kSpan < n) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float y = Ref::y((float)v[j][e], r), w = __builtin_amdgcn_exp2f(y);
+                const float y = Ref::y((float)v[j][e], y_base), w = __builtin_amdgcn_exp2f(y);
                 s += w;
                 t = __builtin_fmaf(w, fmaxf(y, -256.0f), t);   // (0 times -inf)
             }
@@ -572,7 +577,7 @@ template <typename T>
 __device__ __forceinline__ Stats join_splits(const LogProbsKern& p, int64_t row)
 {
     const int lane = threadIdx.x % 64;
-    Stats w{Reference<T>::of(Reference<T>::kLeast), 0.0f, 0.0f};
+    Stats w{Reference<T>::kLeast, 0.0f, 0.0f};
     if (lane < p.splits) {
         const float* from = p.stats + 3 * (row * p.splits + lane);
         w = Stats{from[0], from[1], from[2]};

@@ -200,6 +200,22 @@ def test_large_values():
     _check(x, np.array([[0, 77]] * 2, np.int32), 6)
 
 
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("vocab", [700, 5000, 70000])
+def test_log_probs_far_from_the_largest(vocab, f16):
+    """Whole logits: their distance from the largest is exact, so that the difference to
+    the sum's logarithm is rounded, and nothing else that counts."""
+    announce(f"log probs far vocab={vocab} f16={f16}")
+    x = np.clip(np.round(500.0 * dg.normal(vocab, (8, vocab))), -2000, 2000).astype(np.float16 if f16 else np.float32)
+    tokens = (np.arange(8 * 400).reshape(8, 400) * 7919 % vocab).astype(np.int32)
+    got = _run(x, tokens, 3)
+    lp, _, best, best_lp = ref.log_probs(x, tokens, 3)
+    # (the logarithm: of a sum of a few terms, with a few of their roundings)
+    for a, b in ((got[0], lp), (got[3], best_lp)):
+        assert (abs(a - b) <= 1.001 * 2.0 ** -24 * abs(b) + 2.0 ** -20).all()
+    assert np.array_equal(got[2], best)
+
+
 def test_given_tokens():
     """Many a row, none, negative ones (0), ones past the vocabulary (NaN)."""
     import torch
