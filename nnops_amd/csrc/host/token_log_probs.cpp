@@ -72,7 +72,9 @@ Status TokenLogProbs::validate(std::span<const TensorDesc> inputs, std::span<con
             return Status::invalid_argument;
         }
     }
-    const bool sizes = attrs_.top <= 32 && inputs[0].dims[1] <= (1 << 21);
+    const int64_t rows = inputs[0].dims[0], vocab = inputs[0].dims[1];
+    const bool sizes = attrs_.top <= 32 && vocab <= (1 << 21) && rows <= (1 << 22) &&
+                       rows * ((vocab + 32767) / 32768) < (1 << 23);
     return is_float(inputs[0].dtype) && sizes ? Status::ok : Status::unsupported;
 }
 

@@ -132,6 +132,19 @@ def test_token_log_probs_rules():
     assert na.TokenLogProbs(top=-1).validate([x, tok], outs[:2]) == INVALID
 
 
+@pytest.mark.parametrize("rows,vocab,status", [
+    (1 << 22, 100, na.OK), ((1 << 22) + 1, 100, UNSUPPORTED), ((1 << 22) - 1, 33000, na.OK), (1 << 22, 33000, UNSUPPORTED),
+    (1 << 17, 1 << 21, UNSUPPORTED), ((1 << 17) - 1, 1 << 21, na.OK),
+])
+def test_token_log_probs_rows(rows, vocab, status):
+    """validate says what the call says of rows, and of rows times parts."""
+    op, lib = na.TokenLogProbs(), na.lib()
+    ins, outs = [desc([rows, vocab], F16), desc([rows], S32)], [desc([rows], F32), desc([rows], F32)]
+    assert op.validate(ins, outs) == status
+    a = probs_args(rows=rows, vocab=vocab, ld_logits=vocab, top=0, logits=None)
+    assert lib.nnops_hip_token_log_probs(C.byref(a), None, 0, None) == (INVALID if status == na.OK else status)
+
+
 # --- the launch boundary: refusals before any launch -------------------------------
 
 BASE = 1 << 20                 # addresses that nothing is read from: 1 MB apart
