@@ -943,7 +943,7 @@ extern "C" int nnops_hip_kv_cache_compact(const NnopsKvCompactArgs* g, void* wor
                    (g->table_pages > 0 && (g->page_table == nullptr || g->new_table == nullptr))))) {
         return NNOPS_INVALID_ARGUMENT;
     }
-    if (g->page_table == g->new_table && g->ld_table != g->ld_new_table) {
+    if (b > 1 && g->page_table == g->new_table && g->ld_table != g->ld_new_table) {
         return NNOPS_INVALID_ARGUMENT;
     }
     const Range in[3] = {range_of(g->page_table, b, g->table_pages, g->ld_table), range_of(g->lengths, 1, b, b),

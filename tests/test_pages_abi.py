@@ -221,6 +221,13 @@ def test_compact_workspace():
         assert lib.nnops_hip_kv_cache_compact(C.byref(a), C.c_void_p(at), size, None) == na.NOT_INITIALIZED
 
 
+@pytest.mark.parametrize("sequences,status", [(0, na.NOT_INITIALIZED), (1, na.NOT_INITIALIZED), (2, INVALID)])
+def test_compact_in_place_pitch(sequences, status):
+    """A table of one row, or of none, has no pitch that could differ."""
+    lib, a = na.lib(), compact_args(sequences=sequences, new_table=BASE, ld_new_table=7, pages=20000)
+    assert lib.nnops_hip_kv_cache_compact(C.byref(a), None, 0, None) == status
+
+
 def copy_args(**kw):
     at = dict(k=BASE, v=2 * BASE, k_scale=3 * BASE, v_scale=4 * BASE, copies=5 * BASE, pages=9, heads=2, page_tokens=16,
               head_dim=64, count=3)
