@@ -477,9 +477,8 @@ __device__ __forceinline__ int used_before(uint32_t bits, int* s_waves)
 // j) of those, a used one at j from U on number (used before j) - (used below U).
 __global__ __launch_bounds__(256) void compact_rank(const CompactKern p)
 {
-    __shared__ int s_waves[2][4];
+    __shared__ int s_waves[4];
     __shared__ int s_sums[4][3];
-    __shared__ int s_below;
     const int tid = threadIdx.x, block = blockIdx.x;
     int all = 0, before = 0;
     for (int b = tid; b < p.blocks; b += 256) {
@@ -521,7 +520,7 @@ __global__ __launch_bounds__(256) void compact_rank(const CompactKern p)
     const int moves = u - below;
     const int at = block * kBlock + 16 * tid;
     const uint32_t bits = held_bits(p.refs, at, p.pages);
-    int rank = before + used_before(bits, s_waves[0]);
+    int rank = before + used_before(bits, s_waves);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
         const int j = at + e;
