@@ -573,7 +573,8 @@ int nnops_hip_prefix_attention(const NnopsPrefixAttentionArgs* args, void* works
  * child by child, cell by cell; where there is none left, the cell is -1 (nothing
  * is written there, and it reads as NaN). Cells past a child's pages are -1.
  * new_refs: the counts after the call; may be refs. counts: {pages that are free
- * now, cells that got none}. No other two arrays may overlap.
+ * now, cells that got none}. No other two arrays may overlap (from their first to their
+ * last element: tables may not lie between each other's rows either).
  * The contents of the arrays are not seen by the host; a page number outside
  * [0, pages) is no page, lengths are taken into what the table has room for.
  * page_tokens: a power of two from 16 to 256. children, sequences <= 16384; cells
@@ -605,7 +606,7 @@ int nnops_hip_kv_cache_fork(const NnopsKvForkArgs* args, void* workspace, size_t
  * others keep). new_table: the table with the new numbers, -1 past a sequence's
  * pages; new_refs: the counts, by new numbers. counts: {U, pages that move}.
  * new_table may be page_table (with the same ld) and new_refs refs; no other two
- * arrays may overlap. */
+ * arrays may overlap (as of fork). */
 typedef struct NnopsKvCompactArgs {
     const int32_t* page_table;  /* [sequences][ld_table], table_pages columns */
     int64_t sequences, table_pages, ld_table; /* ld: elements */

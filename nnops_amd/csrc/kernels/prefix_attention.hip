@@ -11,7 +11,7 @@
 // Which tokens are shared is found on the device: whole tiles and whole pages that
 // every row of the group sees. Rows then need no mask, and a sequence's own tokens
 // begin at a tile. Every wave finds it for few sequences (a launch less: 4 sequences over
-// 2000 shared tokens 16 -> 11.8 us), one workgroup before the others for more.
+// 2000 shared tokens 16 -> 12 us), one workgroup before the others for more.
 // Probabilities of f16 rows are held in as many parts as CacheAttention has for the same
 // rows, two f16 where it gives them workgroups of 16 and one where tiles of many: results
 // differ by the order of the sums alone. With one f16 in every tile the calls below took

@@ -8,6 +8,9 @@
 /// caller counts); 0: free. A sequence holds the pages of its first
 /// ceil(length / page_tokens) cells of page_table. A table serves all layers: the
 /// copies that fork and compact ask for are made in each layer's cache.
+///
+/// validate looks at shapes and types; how large they may be (16384 sequences and
+/// children, a new table of 2^30 cells) the call says: Status::unsupported.
 
 #include "nnops/core/op_base.hpp"
 
