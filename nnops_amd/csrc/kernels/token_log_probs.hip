@@ -20,8 +20,9 @@
 // are equal, and each counts the keys above it.
 //
 // Bound: HBM, the logits read once; few rows, the chain of a part and its join. f16,
-// 4096 x 32000, 5 alternatives 53 us, 4.9 TB/s (none 46.6; 32 60.8); f32 89 us, 5.9 TB/s;
-// 64 x 151000, 20 alternatives 15.5 us; 1 x 131072, 8 alternatives 7.6 (two launches).
+// 4096 x 32000, 5 alternatives 53 to 54 us, 4.9 TB/s (none 46.6; 32 60.7); f32 88 us, 5.9
+// TB/s; 64 x 151000, 20 alternatives 15.5 us; 1 x 131072, 8 alternatives 7.7 to 8.5 (two
+// launches).
 // A wave that read on and on, with a running maximum and a list of candidates, took
 // 174 us for the first of these: a list is thinned where nothing else is in flight.
 #include <limits>
